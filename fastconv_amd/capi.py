@@ -50,6 +50,58 @@ class IgemmPlan(C.Structure):
                 ("ws_bytes", C.c_size_t)]
 
 
+F32, BF16, F16 = 0, 1, 2                                        # fc_dtype
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3             # fc_activation
+ROTARY_AXES = 4
+
+
+class GroupNormShape(C.Structure):
+    """Strides in elements: pixel p of image n begins at n * x_image + p * x_pixel."""
+    _fields_ = [("N", C.c_int), ("P", C.c_long), ("C", C.c_int), ("G", C.c_int), ("dtype", C.c_int), ("act", C.c_int),
+                ("eps", C.c_float)] + [(n, C.c_long) for n in ("x_image", "x_pixel", "y_image", "y_pixel")]
+
+    @classmethod
+    def packed(cls, N, P, Cc, G, dtype=F32, act=ACT_NONE, eps=1e-5):
+        return cls(N, P, Cc, G, dtype, act, eps, P * Cc, Cc, P * Cc, Cc)
+
+
+class GroupNormPlan(C.Structure):
+    _fields_ = [("shape", GroupNormShape), ("span", C.c_int), ("chunks", C.c_int), ("resident", C.c_int),
+                ("resident_backward", C.c_int), ("ws_bytes", C.c_size_t), ("ws_backward_bytes", C.c_size_t)]
+
+
+class RotaryShape(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_long), ("Hq", C.c_int), ("Hk", C.c_int), ("D", C.c_int), ("axes", C.c_int),
+                ("pairs", C.c_int * ROTARY_AXES), ("interleaved", C.c_int), ("dtype", C.c_int), ("positions_batch", C.c_long)] + \
+               [(n, C.c_long) for n in ("q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head", "qo_batch", "qo_token",
+                                        "qo_head", "ko_batch", "ko_token", "ko_head")]
+
+    @classmethod
+    def packed(cls, B, T, Hq, Hk, D, pairs, dtype=F32, interleaved=False, shared_positions=False):
+        """q [B][T][Hq][D], k [B][T][Hk][D], positions [B][T][axes] (shared_positions: [T][axes]); pairs of each axis."""
+        q, k = (T * Hq * D, Hq * D, D), (T * Hk * D, Hk * D, D)
+        return cls(B, T, Hq, Hk, D, len(pairs), (C.c_int * ROTARY_AXES)(*pairs), int(interleaved), dtype,
+                   0 if shared_positions else T * len(pairs), *(q + k + q + k))
+
+
+class LinearAttentionShape(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_long), ("H", C.c_int), ("Hkv", C.c_int), ("Dk", C.c_int), ("Dv", C.c_int),
+                ("dtype", C.c_int), ("scale", C.c_float)] + \
+               [(n, C.c_long) for n in ("q_batch", "q_token", "q_head", "k_batch", "k_token", "k_head", "v_batch", "v_token",
+                                        "v_head", "o_batch", "o_token", "o_head")]
+
+    @classmethod
+    def packed(cls, B, T, H, Hkv, Dk, Dv, dtype=F32, scale=1.0):
+        """q [B][T][H][Dk], k [B][T][Hkv][Dk], v [B][T][Hkv][Dv], o [B][T][H][Dv]."""
+        return cls(B, T, H, Hkv, Dk, Dv, dtype, scale, T * H * Dk, H * Dk, Dk, T * Hkv * Dk, Hkv * Dk, Dk,
+                   T * Hkv * Dv, Hkv * Dv, Dv, T * H * Dv, H * Dv, Dv)
+
+
+class LinearAttentionPlan(C.Structure):
+    _fields_ = [("shape", LinearAttentionShape), ("chunk", C.c_int), ("segments", C.c_int), ("ws_bytes", C.c_size_t),
+                ("ws_backward_bytes", C.c_size_t)]
+
+
 class DeviceInfo(C.Structure):
     _fields_ = [("name", C.c_char * 128), ("arch", C.c_char * 32), ("compute_units", C.c_int),
                 ("clock_mhz", C.c_int), ("mem_clock_mhz", C.c_int), ("mem_bus_bits", C.c_int),
@@ -123,6 +175,13 @@ _ABI = {
     "fc_igemm_pack_filter": (C.c_int, [_vp, C.POINTER(IgemmPlan), _vp, _vp, _vp]),
     "fc_conv_implicit_gemm": (C.c_int, [_vp, C.POINTER(IgemmPlan), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp]),
     "fc_conv_implicit_gemm_static": (C.c_int, [_vp, C.POINTER(IgemmPlan), _vp, _vp, _vp, _vp, C.c_int, _vp]),
+    "fc_group_norm_make_plan": (C.c_int, [C.POINTER(GroupNormShape), C.POINTER(GroupNormPlan)]),
+    "fc_group_norm": (C.c_int, [_vp, C.POINTER(GroupNormPlan)] + [_vp] * 7),
+    "fc_group_norm_backward": (C.c_int, [_vp, C.POINTER(GroupNormPlan)] + [_vp] * 10),
+    "fc_rotary": (C.c_int, [_vp, C.POINTER(RotaryShape), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp]),
+    "fc_linear_attention_make_plan": (C.c_int, [C.POINTER(LinearAttentionShape), C.POINTER(LinearAttentionPlan)]),
+    "fc_linear_attention": (C.c_int, [_vp, C.POINTER(LinearAttentionPlan)] + [_vp] * 9),
+    "fc_linear_attention_backward": (C.c_int, [_vp, C.POINTER(LinearAttentionPlan)] + [_vp] * 13),
 }
 
 IGEMM_STATIC_WS_BYTES = 32 << 20
@@ -232,6 +291,13 @@ class Library:
 
     def upload(self, arr):
         arr = self._host_array(arr)
+        p = self.alloc(max(arr.nbytes, 4))
+        self._check(self.c.fc_upload(self.ctx, p, arr.ctypes.data_as(_vp), arr.nbytes))
+        return p
+
+    def upload_raw(self, arr):
+        """The bytes of a host array as they are (16-bit types, int32 positions and lengths)."""
+        arr = np.ascontiguousarray(arr)
         p = self.alloc(max(arr.nbytes, 4))
         self._check(self.c.fc_upload(self.ctx, p, arr.ctypes.data_as(_vp), arr.nbytes))
         return p
@@ -434,6 +500,36 @@ class Library:
     def conv_implicit_gemm_static(self, plan, x, Wp, table, y, bias=None, relu=False):
         """As conv_implicit_gemm, with the split-reduction workspace inside the library (no allocation)."""
         self._check(self.c.fc_conv_implicit_gemm_static(self.ctx, C.byref(plan), x, Wp, table, bias, int(relu), y))
+
+    # ---- operators on tokens (device pointers: ints or c_void_p; None where the call allows none)
+    def _plan(self, call, plan, shape):
+        rc = call(C.byref(shape), C.byref(plan))
+        if rc:
+            raise FastConvError(rc, self.c.fc_status_string(rc).decode())
+        return plan
+
+    def group_norm_plan(self, shape):
+        return self._plan(self.c.fc_group_norm_make_plan, GroupNormPlan(), shape)
+
+    def group_norm(self, plan, x, gamma, beta, y, mean=None, rstd=None, ws=None):
+        self._check(self.c.fc_group_norm(self.ctx, C.byref(plan), x, gamma, beta, y, mean, rstd, ws))
+
+    def group_norm_backward(self, plan, dy, x, gamma, beta, mean, rstd, dx, dgamma=None, dbeta=None, ws=None):
+        self._check(self.c.fc_group_norm_backward(self.ctx, C.byref(plan), dy, x, gamma, beta, mean, rstd, dx, dgamma, dbeta, ws))
+
+    def rotary(self, shape, q, k, positions, inv_freq, q_out, k_out, inverse=False):
+        self._check(self.c.fc_rotary(self.ctx, C.byref(shape), q, k, positions, inv_freq, int(inverse), q_out, k_out))
+
+    def linear_attention_plan(self, shape):
+        return self._plan(self.c.fc_linear_attention_make_plan, LinearAttentionPlan(), shape)
+
+    def linear_attention(self, plan, q, k, v, log_decay, o, state_in=None, state_out=None, lengths=None, ws=None):
+        self._check(self.c.fc_linear_attention(self.ctx, C.byref(plan), q, k, v, log_decay, o, state_in, state_out, lengths, ws))
+
+    def linear_attention_backward(self, plan, do, q, k, v, log_decay, dq, dk, dv, state_in=None, dstate_out=None, dstate_in=None,
+                                  lengths=None, ws=None):
+        self._check(self.c.fc_linear_attention_backward(self.ctx, C.byref(plan), do, q, k, v, log_decay, dq, dk, dv, state_in,
+                                                        dstate_out, dstate_in, lengths, ws))
 
     # ---- whole-layer helpers over host arrays (tests, smoke)
     def winograd_conv_fused(self, shape, x, w, bias=None, relu=False, config=None):

@@ -1,0 +1,579 @@
+// Group norm with an activation over channels-last pixels, forward and backward.
+//
+//   xhat = (x - mean) * rstd,  y = act(gamma * xhat + beta),  mean and variance over the P * C/G values of a group
+//   dz = dy * act'(z),  dbeta = sum dz,  dgamma = sum dz * xhat
+//   dx = rstd * (gamma dz - (s1 + xhat s2) / (P * C/G)),  s1 = sum over the group of gamma dz,  s2 = of gamma dz xhat
+//
+// Bound by memory: about 10 operations an element against 4 bytes in 16-bit types.  The first y needs the last x of its
+// group, so the pixels of an image are cut into chunks: one launch leaves each chunk's statistics, the next joins them and
+// writes the result, reading x a second time (from the 256 MB cache where x fits that).
+// A thread keeps to one column of 4 to 16 bytes of channels and walks down the pixels, so that whatever belongs to a channel
+// stays in registers; a wavefront reads whole lines.
+// Statistics are joined, never subtracted: a thread forms the mean of each batch of pixels and the squares of what differs
+// from it, and joins batches, threads, channels and chunks by
+//   n = na + nb,  mean = ma + d nb/n,  M2 = M2a + M2b + d^2 na nb/n,  d = mb - ma
+// (Chan, Golub and LeVeque, "Updating formulae and a pairwise algorithm for computing sample variances", 1979).
+#include "token_types.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxGroupChannels = 4096;
+
+struct norm_params {
+    const void *x, *dy;
+    void *y;                 // or dx
+    const float *gamma, *beta;
+    float *mean, *rstd;
+    float2 *part;            // forward: (mean, M2) [N][G][chunks]; backward: (s1, s2) likewise
+    float2 *channel_part;    // backward: (sum dz, sum dz xhat) [N][chunks][C]
+    float *dgamma, *dbeta;
+    long P, chunk;           // pixels of an image, and of a chunk
+    int N, C, G, Cg;
+    int span, spans, chunks;
+    int reduce_blocks;       // workgroups of the backward pass's second launch that add up channel_part
+    float eps;
+    long x_image, x_pixel, y_image, y_pixel;
+};
+
+template <int ACT>
+__device__ __forceinline__ float activation(float z) {
+    if (ACT == FC_ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays
+    if (ACT == FC_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    if (ACT == FC_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float activation_slope(float z) {
+    if (ACT == FC_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (ACT == FC_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        return s * (1.f + z * (1.f - s));
+    }
+    if (ACT == FC_ACT_GELU)
+        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    return 1.f;
+}
+
+// What a workgroup works on: a chunk of pixels of one image, a span of its channels.
+struct norm_place {
+    int chunk, span;
+    long n, p0, p1;
+    __device__ __forceinline__ norm_place(const norm_params &p, unsigned block) {
+        chunk = block % p.chunks;
+        const unsigned r = block / p.chunks;
+        span = r % p.spans;
+        n = r / p.spans;
+        p0 = chunk * p.chunk;
+        p1 = p0 + p.chunk < p.P ? p0 + p.chunk : p.P;
+    }
+};
+
+// Threads over a span: `cols` accesses side by side, `rows` pixels at once.
+struct norm_threads {
+    int cols, rows, tx, ty;
+    __device__ __forceinline__ norm_threads(int accesses) {
+        cols = accesses < kThreads ? accesses : kThreads;
+        rows = kThreads / cols;
+        ty = threadIdx.x / cols;
+        tx = threadIdx.x - ty * cols;
+    }
+};
+
+// Statistics of each group over a chunk.
+template <int DT, int VEC>
+__global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const norm_params p) {
+    extern __shared__ float2 entry[];      // (mean, M2) [rows][span]
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    constexpr int U = 8;                   // pixels a batch
+    const norm_place at(p, blockIdx.x);
+    const int accesses = p.span / VEC;
+    const norm_threads th(accesses);
+    const int c0 = at.span * p.span;
+    const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
+    if (th.ty < th.rows) {
+        for (int col = th.tx; col < width / VEC; col += th.cols) {
+            const E *src = (const E *)p.x + at.n * p.x_image + c0 + col * VEC;
+            float mean[VEC], m2[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; v++) mean[v] = m2[v] = 0.f;
+            float count = 0.f;
+            for (long q = at.p0 + th.ty; q < at.p1; q += (long)U * th.rows) {
+                V in[U];
+                int nb = 0;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const long r = q + (long)u * th.rows;
+                    if (r < at.p1) {
+                        in[u] = *(const V *)(src + r * p.x_pixel);
+                        nb = u + 1;
+                    }
+                }
+                const float joined = count + nb, wb = nb / joined, wm = count * wb;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; u++) s += u < nb ? in[u].get(v) : 0.f;
+                    s = nb == U ? s * (1.f / U) : s / nb;      // exact where all values are equal
+                    float sq = 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const float d = u < nb ? in[u].get(v) - s : 0.f;
+                        sq += d * d;
+                    }
+                    const float d = s - mean[v];
+                    mean[v] += d * wb;
+                    m2[v] += sq + d * d * wm;
+                }
+                count = joined;
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; v++) entry[th.ty * p.span + col * VEC + v] = make_float2(mean[v], m2[v]);
+        }
+    }
+    __syncthreads();
+    // a wavefront joins the entries of a group: count by count, the means first
+    const int lane = threadIdx.x & 63, groups = width / p.Cg, np = (int)(at.p1 - at.p0);
+    const float total = (float)np * p.Cg;
+    for (int g = threadIdx.x >> 6; g < groups; g += kThreads / 64) {
+        float s = 0.f;
+        for (int i = lane; i < p.Cg * th.rows; i += 64) {
+            const int ty = i / p.Cg, c = i - ty * p.Cg;
+            const float cnt = ty < np ? (float)((np - ty + th.rows - 1) / th.rows) : 0.f;
+            s += cnt > 0.f ? cnt * entry[ty * p.span + g * p.Cg + c].x : 0.f;
+        }
+        const float mean = fc_wave_sum(s) / total;
+        float m2 = 0.f;
+        for (int i = lane; i < p.Cg * th.rows; i += 64) {
+            const int ty = i / p.Cg, c = i - ty * p.Cg;
+            const float cnt = ty < np ? (float)((np - ty + th.rows - 1) / th.rows) : 0.f;
+            if (cnt > 0.f) {
+                const float2 e = entry[ty * p.span + g * p.Cg + c];
+                m2 += e.y + cnt * (e.x - mean) * (e.x - mean);
+            }
+        }
+        m2 = fc_wave_sum(m2);
+        if (lane == 0) p.part[(at.n * p.G + c0 / p.Cg + g) * p.chunks + at.chunk] = make_float2(mean, m2);
+    }
+}
+
+// Joins the chunks of each group and writes y.
+template <int DT, int VEC, int ACT>
+__global__ __launch_bounds__(kThreads) void fc_group_norm_apply_kernel(const norm_params p) {
+    extern __shared__ float2 stat[];      // (mean, rstd) of the span's groups
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    constexpr int U = 4;
+    const norm_place at(p, blockIdx.x);
+    const norm_threads th(p.span / VEC);
+    const int c0 = at.span * p.span;
+    const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
+    const int lane = threadIdx.x & 63, groups = width / p.Cg;
+    for (int g = threadIdx.x >> 6; g < groups; g += kThreads / 64) {
+        const long group = at.n * p.G + c0 / p.Cg + g;
+        const float2 *part = p.part + group * p.chunks;
+        float s = 0.f;
+        for (int i = lane; i < p.chunks; i += 64) {
+            const long first = i * p.chunk;
+            s += (float)(p.P - first < p.chunk ? p.P - first : p.chunk) * part[i].x;
+        }
+        const float mean = fc_wave_sum(s) / (float)p.P;
+        float m2 = 0.f;
+        for (int i = lane; i < p.chunks; i += 64) {
+            const long first = i * p.chunk;
+            const float d = part[i].x - mean;
+            m2 += part[i].y + (float)(p.P - first < p.chunk ? p.P - first : p.chunk) * p.Cg * d * d;
+        }
+        const float rstd = 1.f / sqrtf(fc_wave_sum(m2) / ((float)p.P * p.Cg) + p.eps);
+        if (lane == 0) {
+            stat[g] = make_float2(mean, rstd);
+            if (at.chunk == 0 && p.mean) {
+                p.mean[group] = mean;
+                p.rstd[group] = rstd;
+            }
+        }
+    }
+    __syncthreads();
+    if (th.ty >= th.rows) return;
+    for (int col = th.tx; col < width / VEC; col += th.cols) {
+        float mean[VEC], scale[VEC], shift[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const int c = col * VEC + v;
+            const float2 st = stat[c / p.Cg];
+            mean[v] = st.x;
+            scale[v] = st.y * (p.gamma ? p.gamma[c0 + c] : 1.f);
+            shift[v] = p.beta ? p.beta[c0 + c] : 0.f;
+        }
+        const E *src = (const E *)p.x + at.n * p.x_image + c0 + col * VEC;
+        E *dst = (E *)p.y + at.n * p.y_image + c0 + col * VEC;
+        for (long q = at.p0 + th.ty; q < at.p1; q += (long)U * th.rows) {
+            V in[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const long r = q + (long)u * th.rows;
+                if (r < at.p1) in[u] = *(const V *)(src + r * p.x_pixel);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const long r = q + (long)u * th.rows;
+                if (r >= at.p1) break;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) in[u].set(v, activation<ACT>((in[u].get(v) - mean[v]) * scale[v] + shift[v]));
+                *(V *)(dst + r * p.y_pixel) = in[u];
+            }
+        }
+    }
+}
+
+// What both launches of the backward pass keep of a column.
+template <int VEC>
+struct norm_column {
+    float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
+    __device__ __forceinline__ norm_column(const norm_params &p, long n, int c0) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const int c = c0 + v;
+            const long group = n * p.G + c / p.Cg;
+            mean[v] = p.mean[group];
+            rstd[v] = p.rstd[group];
+            gamma[v] = p.gamma ? p.gamma[c] : 1.f;
+            beta[v] = p.beta ? p.beta[c] : 0.f;
+        }
+    }
+};
+
+// Sums of dz and dz xhat of each channel over a chunk, and of both times gamma of each group.
+template <int DT, int VEC, int ACT>
+__global__ __launch_bounds__(kThreads) void fc_group_norm_sums_kernel(const norm_params p) {
+    extern __shared__ float2 entry[];      // (sum dz, sum dz xhat) [rows][span]
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    constexpr int U = 4;
+    const norm_place at(p, blockIdx.x);
+    const norm_threads th(p.span / VEC);
+    const int c0 = at.span * p.span;
+    const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
+    if (th.ty < th.rows) {
+        for (int col = th.tx; col < width / VEC; col += th.cols) {
+            const norm_column<VEC> k(p, at.n, c0 + col * VEC);
+            const E *x = (const E *)p.x + at.n * p.x_image + c0 + col * VEC;
+            const E *dy = (const E *)p.dy + at.n * p.y_image + c0 + col * VEC;
+            float a[VEC], b[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; v++) a[v] = b[v] = 0.f;
+            for (long q = at.p0 + th.ty; q < at.p1; q += (long)U * th.rows) {
+                V xs[U], ds[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const long r = q + (long)u * th.rows;
+                    if (r < at.p1) {
+                        xs[u] = *(const V *)(x + r * p.x_pixel);
+                        ds[u] = *(const V *)(dy + r * p.y_pixel);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (q + (long)u * th.rows >= at.p1) break;
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) {
+                        const float xhat = (xs[u].get(v) - k.mean[v]) * k.rstd[v];
+                        const float dz = ds[u].get(v) * activation_slope<ACT>(xhat * k.gamma[v] + k.beta[v]);
+                        a[v] += dz;
+                        b[v] += dz * xhat;
+                    }
+                }
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; v++) entry[th.ty * p.span + col * VEC + v] = make_float2(a[v], b[v]);
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += kThreads) {
+        float2 s = entry[c];
+        for (int ty = 1; ty < th.rows; ty++) {
+            s.x += entry[ty * p.span + c].x;
+            s.y += entry[ty * p.span + c].y;
+        }
+        p.channel_part[(at.n * p.chunks + at.chunk) * p.C + c0 + c] = s;
+        entry[c] = s;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < width / p.Cg; g += kThreads / 64) {
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = lane; i < p.Cg; i += 64) {
+            const float2 e = entry[g * p.Cg + i];
+            const float gamma = p.gamma ? p.gamma[c0 + g * p.Cg + i] : 1.f;
+            s1 += gamma * e.x;
+            s2 += gamma * e.y;
+        }
+        s1 = fc_wave_sum(s1);
+        s2 = fc_wave_sum(s2);
+        if (lane == 0) p.part[(at.n * p.G + c0 / p.Cg + g) * p.chunks + at.chunk] = make_float2(s1, s2);
+    }
+}
+
+// dgamma and dbeta of 32 channels: 8 threads each over the images' chunks, in a fixed order.
+__device__ __forceinline__ void reduce_channels(const norm_params &p, unsigned block, float2 *sums) {
+    const int lc = threadIdx.x & 31, row = threadIdx.x >> 5, c = block * 32 + lc;
+    float2 s = make_float2(0.f, 0.f);
+    if (c < p.C) {
+        const long rows = (long)p.N * p.chunks;
+        for (long r = row; r < rows; r += 8) {
+            const float2 e = p.channel_part[r * p.C + c];
+            s.x += e.x;
+            s.y += e.y;
+        }
+    }
+    sums[row * 32 + lc] = s;
+    __syncthreads();
+    if (row == 0 && c < p.C) {
+        for (int r = 1; r < 8; r++) {
+            s.x += sums[r * 32 + lc].x;
+            s.y += sums[r * 32 + lc].y;
+        }
+        if (p.dbeta) p.dbeta[c] = s.x;
+        if (p.dgamma) p.dgamma[c] = s.y;
+    }
+}
+
+// dx; the first workgroups add up dgamma and dbeta meanwhile.
+template <int DT, int VEC, int ACT>
+__global__ __launch_bounds__(kThreads) void fc_group_norm_gradient_kernel(const norm_params p) {
+    extern __shared__ float2 stat[];      // (s1, s2) of the span's groups over their values, or the sums of channels
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    constexpr int U = 4;
+    if ((int)blockIdx.x < p.reduce_blocks) {
+        reduce_channels(p, blockIdx.x, stat);
+        return;
+    }
+    const norm_place at(p, blockIdx.x - p.reduce_blocks);
+    const norm_threads th(p.span / VEC);
+    const int c0 = at.span * p.span;
+    const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < width / p.Cg; g += kThreads / 64) {
+        const float2 *part = p.part + (at.n * p.G + c0 / p.Cg + g) * p.chunks;
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = lane; i < p.chunks; i += 64) {
+            s1 += part[i].x;
+            s2 += part[i].y;
+        }
+        const float inv = 1.f / ((float)p.P * p.Cg);
+        s1 = fc_wave_sum(s1) * inv;
+        s2 = fc_wave_sum(s2) * inv;
+        if (lane == 0) stat[g] = make_float2(s1, s2);
+    }
+    __syncthreads();
+    if (th.ty >= th.rows) return;
+    for (int col = th.tx; col < width / VEC; col += th.cols) {
+        const norm_column<VEC> k(p, at.n, c0 + col * VEC);
+        float2 st[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) st[v] = stat[(col * VEC + v) / p.Cg];
+        const E *x = (const E *)p.x + at.n * p.x_image + c0 + col * VEC;
+        const E *dy = (const E *)p.dy + at.n * p.y_image + c0 + col * VEC;
+        E *dx = (E *)p.y + at.n * p.x_image + c0 + col * VEC;
+        for (long q = at.p0 + th.ty; q < at.p1; q += (long)U * th.rows) {
+            V xs[U], ds[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const long r = q + (long)u * th.rows;
+                if (r < at.p1) {
+                    xs[u] = *(const V *)(x + r * p.x_pixel);
+                    ds[u] = *(const V *)(dy + r * p.y_pixel);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const long r = q + (long)u * th.rows;
+                if (r >= at.p1) break;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    const float xhat = (xs[u].get(v) - k.mean[v]) * k.rstd[v];
+                    const float dz = ds[u].get(v) * activation_slope<ACT>(xhat * k.gamma[v] + k.beta[v]);
+                    xs[u].set(v, k.rstd[v] * (k.gamma[v] * dz - st[v].x - xhat * st[v].y));
+                }
+                *(V *)(dx + r * p.x_pixel) = xs[u];
+            }
+        }
+    }
+}
+
+int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
+
+long gcd(long a, long b) { return b ? gcd(b, a % b) : a; }
+
+bool shape_ok(const fc_group_norm_shape *s) {
+    if (!s || s->N < 1 || s->P < 1 || s->C < 1 || s->G < 1 || s->C % s->G || !fc_dtype_ok(s->dtype)) return false;
+    if (s->act < FC_ACT_NONE || s->act > FC_ACT_GELU || !(s->eps >= 0.f)) return false;
+    return s->x_image >= 0 && s->x_pixel >= 0 && s->y_image >= 0 && s->y_pixel >= 0;
+}
+
+bool same(const fc_group_norm_plan &a, const fc_group_norm_plan &b) {
+    const fc_group_norm_shape &s = a.shape, &t = b.shape;
+    return s.N == t.N && s.P == t.P && s.C == t.C && s.G == t.G && s.dtype == t.dtype && s.act == t.act && s.eps == t.eps &&
+           s.x_image == t.x_image && s.x_pixel == t.x_pixel && s.y_image == t.y_image && s.y_pixel == t.y_pixel && a.span == b.span &&
+           a.chunks == b.chunks && a.resident == b.resident && a.resident_backward == b.resident_backward &&
+           a.ws_bytes == b.ws_bytes && a.ws_backward_bytes == b.ws_backward_bytes;
+}
+
+// The widest access of a plan whose tensors begin at `addr`: a column lies within a span.
+int width_of(const fc_group_norm_shape &s, int span, uint64_t addr) {
+    return fc_widest(s.dtype, (uint64_t)(s.C | span | s.x_image | s.x_pixel | s.y_image | s.y_pixel), addr);
+}
+
+template <int ACT, class F>
+bool with_width(int dtype, int vec, F &&f) {
+    if (dtype == FC_F32) {
+        if (vec == 4) return f.template run<FC_F32, 4, ACT>();
+        if (vec == 2) return f.template run<FC_F32, 2, ACT>();
+        return f.template run<FC_F32, 1, ACT>();
+    }
+    if (dtype == FC_BF16) {
+        if (vec == 8) return f.template run<FC_BF16, 8, ACT>();
+        if (vec == 4) return f.template run<FC_BF16, 4, ACT>();
+        if (vec == 2) return f.template run<FC_BF16, 2, ACT>();
+        return f.template run<FC_BF16, 1, ACT>();
+    }
+    if (vec == 8) return f.template run<FC_F16, 8, ACT>();
+    if (vec == 4) return f.template run<FC_F16, 4, ACT>();
+    if (vec == 2) return f.template run<FC_F16, 2, ACT>();
+    return f.template run<FC_F16, 1, ACT>();
+}
+
+template <class F>
+bool with_kernel(const fc_group_norm_shape &s, int vec, F &&f) {
+    switch (s.act) {
+        case FC_ACT_RELU: return with_width<FC_ACT_RELU>(s.dtype, vec, f);
+        case FC_ACT_SILU: return with_width<FC_ACT_SILU>(s.dtype, vec, f);
+        case FC_ACT_GELU: return with_width<FC_ACT_GELU>(s.dtype, vec, f);
+        default: return with_width<FC_ACT_NONE>(s.dtype, vec, f);
+    }
+}
+
+struct forward_launch {
+    hipStream_t stream;
+    const norm_params &p;
+    unsigned blocks;
+    template <int DT, int VEC, int ACT>
+    bool run() {
+        const int accesses = p.span / VEC, rows = kThreads / (accesses < kThreads ? accesses : kThreads);
+        fc_group_norm_stats_kernel<DT, VEC><<<dim3(blocks), dim3(kThreads), (size_t)rows * p.span * sizeof(float2), stream>>>(p);
+        fc_group_norm_apply_kernel<DT, VEC, ACT><<<dim3(blocks), dim3(kThreads), (size_t)(p.span / p.Cg) * sizeof(float2), stream>>>(p);
+        return true;
+    }
+};
+
+struct backward_launch {
+    hipStream_t stream;
+    const norm_params &p;
+    unsigned blocks;
+    template <int DT, int VEC, int ACT>
+    bool run() {
+        const int accesses = p.span / VEC, rows = kThreads / (accesses < kThreads ? accesses : kThreads);
+        fc_group_norm_sums_kernel<DT, VEC, ACT><<<dim3(blocks), dim3(kThreads), (size_t)rows * p.span * sizeof(float2), stream>>>(p);
+        const size_t groups = (size_t)(p.span / p.Cg), need = groups > 256 ? groups : 256;
+        fc_group_norm_gradient_kernel<DT, VEC, ACT><<<dim3(blocks + p.reduce_blocks), dim3(kThreads), need * sizeof(float2), stream>>>(p);
+        return true;
+    }
+};
+
+norm_params params_of(const fc_group_norm_plan *plan) {
+    const fc_group_norm_shape &s = plan->shape;
+    norm_params p = {};
+    p.N = s.N; p.P = s.P; p.C = s.C; p.G = s.G; p.Cg = s.C / s.G; p.eps = s.eps;
+    p.span = plan->span;
+    p.spans = (s.C + plan->span - 1) / plan->span;
+    p.chunks = plan->chunks;
+    p.chunk = (s.P + plan->chunks - 1) / plan->chunks;
+    p.x_image = s.x_image; p.x_pixel = s.x_pixel; p.y_image = s.y_image; p.y_pixel = s.y_pixel;
+    return p;
+}
+
+}  // namespace
+
+extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_norm_plan *plan) {
+    if (!plan || !shape_ok(s)) return FC_ERR_INVALID;
+    const int Cg = s->C / s->G;
+    if (Cg > kMaxGroupChannels || fc_count(s->N, s->P, s->C) < 0 || fc_count(s->N, s->C) >= (1l << 31)) return FC_ERR_UNSUPPORTED;
+    *plan = {};
+    plan->shape = *s;
+    // whole groups and whole accesses, up to 4096 channels: the widest access that leaves such a span
+    long step = Cg;
+    for (int vec = fc_widest(s->dtype, (uint64_t)(s->C | s->x_image | s->x_pixel | s->y_image | s->y_pixel), 0); vec >= 1; vec >>= 1) {
+        step = Cg / gcd(Cg, vec) * vec;
+        if (step <= kMaxGroupChannels) break;
+    }
+    long span = step;
+    while (span + step <= kMaxGroupChannels && span < s->C) span += step;
+    if (span > s->C) span = s->C;
+    plan->span = (int)span;
+    const long spans = (s->C + span - 1) / span, pixels = s->P;
+    // about eight workgroups a compute unit, of 32 KB and more each
+    long chunks = 2048 / (s->N * spans);
+    const long least = 32768 / (span * (long)fc_elem_size(s->dtype)) + 1;
+    if (chunks > (pixels + least - 1) / least) chunks = (pixels + least - 1) / least;
+    if (chunks < 1) chunks = 1;
+    if (chunks > 256) chunks = 256;
+    const long chunk = (pixels + chunks - 1) / chunks;
+    chunks = (pixels + chunk - 1) / chunk;
+    if (chunk >= (1l << 30) || s->N * spans * chunks >= (1l << 31) - 65536) return FC_ERR_UNSUPPORTED;
+    plan->chunks = (int)chunks;
+    plan->ws_bytes = (size_t)s->N * s->G * chunks * sizeof(float2);
+    plan->ws_backward_bytes = plan->ws_bytes + (size_t)s->N * chunks * s->C * sizeof(float2);
+    return FC_OK;
+}
+
+static int check_plan(fc_context *ctx, const fc_group_norm_plan *plan, const char *what) {
+    fc_group_norm_plan own;
+    if (!plan || fc_group_norm_make_plan(&plan->shape, &own) != FC_OK || !same(*plan, own)) return fail(ctx, FC_ERR_INVALID, what);
+    return FC_OK;
+}
+
+extern "C" int fc_group_norm(fc_context *ctx, const fc_group_norm_plan *plan, const void *x_dev, const float *gamma_dev,
+                             const float *beta_dev, void *y_dev, float *mean_dev, float *rstd_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_group_norm: not a plan of fc_group_norm_make_plan")) return FC_ERR_INVALID;
+    if (!x_dev || !y_dev || (!ws_dev && plan->ws_bytes) || !mean_dev != !rstd_dev) return fail(ctx, FC_ERR_INVALID, "fc_group_norm: null pointer");
+    const uint64_t addr = (uint64_t)x_dev | (uint64_t)y_dev;
+    if ((addr & (fc_elem_size(plan->shape.dtype) - 1)) || ((uint64_t)ws_dev & 7) ||
+        (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_group_norm: unaligned pointer");
+    norm_params p = params_of(plan);
+    p.x = x_dev; p.y = y_dev; p.gamma = gamma_dev; p.beta = beta_dev; p.mean = mean_dev; p.rstd = rstd_dev;
+    p.part = (float2 *)ws_dev;
+    forward_launch f = {ctx->stream, p, (unsigned)((long)p.N * p.spans * p.chunks)};
+    with_kernel(plan->shape, width_of(plan->shape, plan->span, addr), f);
+    FC_LAUNCH_CHECK(ctx, "fc_group_norm");
+    return FC_OK;
+}
+
+extern "C" int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan *plan, const void *dy_dev, const void *x_dev,
+                                      const float *gamma_dev, const float *beta_dev, const float *mean_dev, const float *rstd_dev,
+                                      void *dx_dev, float *dgamma_dev, float *dbeta_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_group_norm_backward: not a plan of fc_group_norm_make_plan")) return FC_ERR_INVALID;
+    if (!dy_dev || !x_dev || !mean_dev || !rstd_dev || !dx_dev || (!ws_dev && plan->ws_backward_bytes))
+        return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: null pointer");
+    const uint64_t addr = (uint64_t)x_dev | (uint64_t)dy_dev | (uint64_t)dx_dev;
+    if ((addr & (fc_elem_size(plan->shape.dtype) - 1)) || ((uint64_t)ws_dev & 7) ||
+        (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev | (uint64_t)dgamma_dev | (uint64_t)dbeta_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: unaligned pointer");
+    norm_params p = params_of(plan);
+    p.x = x_dev; p.dy = dy_dev; p.y = dx_dev; p.gamma = gamma_dev; p.beta = beta_dev;
+    p.mean = const_cast<float *>(mean_dev); p.rstd = const_cast<float *>(rstd_dev);      // only read
+    p.part = (float2 *)ws_dev;
+    p.channel_part = p.part + (size_t)p.N * p.G * p.chunks;
+    p.dgamma = dgamma_dev; p.dbeta = dbeta_dev;
+    p.reduce_blocks = dgamma_dev || dbeta_dev ? (p.C + 31) / 32 : 0;
+    backward_launch f = {ctx->stream, p, (unsigned)((long)p.N * p.spans * p.chunks)};
+    with_kernel(plan->shape, width_of(plan->shape, plan->span, addr), f);
+    FC_LAUNCH_CHECK(ctx, "fc_group_norm_backward");
+    return FC_OK;
+}

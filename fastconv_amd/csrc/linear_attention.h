@@ -1,0 +1,54 @@
+// Linear attention with a decay for each head: what its kernels share.
+//
+//   S_t = l S_(t-1) + k_t v_t^T,   o_t = scale * S_t^T q_t,   l = exp(log_decay)
+//
+// The backward pass is made of the same recurrence.  With the gradient do of o and dS of the last state,
+//   dq_t = scale * S_t do_t:                      the forward run over (do, v, k) from S_0^T
+//   G_t = l G_(t+1) + scale * q_t do_t^T,  dk_t = G_t v_t,  dv_t = G_t^T k_t:   runs from the last token to the first over
+//                                                 (v, do, q) and (k, q, do); the state enters as dS = l G_(T+1), and l G_1
+//                                                 is the gradient of S_0
+// So one run serves all: a direction, three operands with heads and strides of their own, a state that may be read and
+// written transposed.  A forward run decays its state before it takes a token in, a backward one after it has answered.
+#pragma once
+
+#include "token_types.h"
+
+struct fc_la_operand {
+    const void *p;
+    long batch, token, head;
+    int share;               // heads that read one of this operand's heads
+};
+
+struct fc_la_run {
+    fc_la_operand q, k, v;
+    void *o;                 // in the tensors' type by strides, or
+    float *o32;              // fp32, [B][T][H][Dv], where heads are added up afterwards
+    long o_batch, o_token, o_head;
+    const float *state_in;   // element (row, column) of head bh at bh*Dk*Dv + row*state_row + column*state_col
+    float *state_out;
+    long state_row, state_col;
+    const float *log_decay;
+    const int32_t *lengths;
+    long T;
+    int H, Dk, Dv;           // of this run: rows and columns of its state
+    int reverse;
+    float scale_in, scale_out;      // of what enters the state, of what leaves it
+    float *ws;
+};
+
+__device__ __forceinline__ long fc_la_length(const fc_la_run &r, long b) {
+    if (!r.lengths) return r.T;
+    const long n = r.lengths[b];
+    return n < 0 ? 0 : n > r.T ? r.T : n;
+}
+
+// exp(n * log_decay) in two parts, n >= 0: a decay's own rounding, the same at every step, would grow with their number
+struct fc_la_power {
+    float hi, lo;
+    __device__ __forceinline__ fc_la_power(float log_decay, long n) {
+        const double l = n ? exp((double)log_decay * (double)n) : 1.0;
+        hi = (float)l;
+        lo = (float)(l - hi);
+    }
+    __device__ __forceinline__ float times(float s) const { return __builtin_fmaf(hi, s, lo * s); }
+};

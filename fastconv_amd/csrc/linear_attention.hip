@@ -1,0 +1,279 @@
+// Linear attention with a decay for each head: entry points, and the recurrence for few tokens.  See linear_attention.h for the
+// formulas.
+#include "linear_attention.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxDim = 256;
+constexpr int kStepCols = 32;      // columns of the state that a workgroup of the recurrence holds
+
+// The recurrence.  A workgroup holds 32 columns of a head's state in registers: 8 threads side by side with 4 columns each,
+// 32 threads deep with ROWS rows each.  A token costs two barriers: its q and k lie in LDS for all, its answer is summed over
+// the rows in the wavefront and then over the four wavefronts.
+// Bound by the state, which is read and written once a call, 8 bytes an element against 4 operations a token.
+template <int DT, int ROWS>
+__global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(const fc_la_run r) {
+    typedef typename fc_elem<DT>::type E;
+    __shared__ float qs[2][kMaxDim], ks[2][kMaxDim], part[2][4][kStepCols];
+    const int tid = threadIdx.x, col = tid & 7, row = tid >> 3;
+    const int slices = (r.Dv + kStepCols - 1) / kStepCols;
+    const long bh = blockIdx.x / slices, b = bh / r.H;
+    const int h = (int)(bh - b * r.H), c0 = (int)(blockIdx.x - bh * slices) * kStepCols + 4 * col;
+    const long len = fc_la_length(r, b);
+    const fc_la_power decay(r.log_decay[h], 1);
+    const bool wide = r.state_col == 1 && (r.Dv & 3) == 0 &&
+                      (((uintptr_t)r.state_in | (uintptr_t)r.state_out) & 15) == 0;      // four columns an access
+
+    float s[ROWS][4];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int rr = row + 32 * i;
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[i][j] = 0.f;
+        if (!r.state_in || rr >= r.Dk || c0 >= r.Dv) continue;
+        const float *src = r.state_in + bh * r.Dk * r.Dv + rr * r.state_row + c0 * r.state_col;
+        if (wide) {
+            const float4 x = *(const float4 *)src;
+            s[i][0] = x.x; s[i][1] = x.y; s[i][2] = x.z; s[i][3] = x.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (c0 + j < r.Dv) s[i][j] = src[j * r.state_col];
+        }
+    }
+    const E *q = (const E *)r.q.p + b * r.q.batch + (h / r.q.share) * r.q.head;
+    const E *k = (const E *)r.k.p + b * r.k.batch + (h / r.k.share) * r.k.head;
+    const E *v = (const E *)r.v.p + b * r.v.batch + (h / r.v.share) * r.v.head;
+    E *o = (E *)r.o + b * r.o_batch + h * r.o_head;
+    float *o32 = r.o32 ? r.o32 + (b * r.T * r.H + h) * r.Dv : nullptr;
+    const long o32_token = (long)r.H * r.Dv;
+
+    for (long n = 0; n < len; n++) {
+        const long t = r.reverse ? len - 1 - n : n;
+        const int buf = n & 1;
+        if (tid < r.Dk) {
+            qs[buf][tid] = (float)q[t * r.q.token + tid] * r.scale_out;
+            ks[buf][tid] = (float)k[t * r.k.token + tid] * r.scale_in;
+        }
+        float vv[4], out[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            vv[j] = c0 + j < r.Dv ? (float)v[t * r.v.token + c0 + j] : 0.f;
+            out[j] = 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            const int rr = row + 32 * i;
+            if (rr >= r.Dk) break;
+            const float kr = ks[buf][rr], qr = qs[buf][rr];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float now = __builtin_fmaf(kr, vv[j], r.reverse ? s[i][j] : decay.times(s[i][j]));
+                out[j] = __builtin_fmaf(qr, now, out[j]);
+                s[i][j] = r.reverse ? decay.times(now) : now;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int m = 8; m < 64; m <<= 1) out[j] += __shfl_xor(out[j], m);
+        }
+        if ((tid & 63) < 8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) part[buf][tid >> 6][4 * col + j] = out[j];
+        }
+        __syncthreads();
+        const int c = (int)(blockIdx.x - bh * slices) * kStepCols + tid;
+        if (tid < kStepCols && c < r.Dv) {
+            const float sum = (part[buf][0][tid] + part[buf][1][tid]) + (part[buf][2][tid] + part[buf][3][tid]);
+            if (o32) o32[t * o32_token + c] = sum;
+            else o[t * r.o_token + c] = (E)sum;
+        }
+    }
+    // tokens past the end of a shorter sequence
+    const int c = (int)(blockIdx.x - bh * slices) * kStepCols + (tid & 31);
+    if (c < r.Dv)
+        for (long t = len + (tid >> 5); t < r.T; t += kThreads / 32) {
+            if (o32) o32[t * o32_token + c] = 0.f;
+            else o[t * r.o_token + c] = (E)0.f;
+        }
+    if (!r.state_out) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const int rr = row + 32 * i;
+        if (rr >= r.Dk || c0 >= r.Dv) continue;
+        float *dst = r.state_out + bh * r.Dk * r.Dv + rr * r.state_row + c0 * r.state_col;
+        if (wide) {
+            *(float4 *)dst = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (c0 + j < r.Dv) dst[j * r.state_col] = s[i][j];
+        }
+    }
+}
+
+// Gradients of shared heads: the fp32 gradients [B][T][H][D] of the query heads, added up by key/value head.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void fc_linear_attention_shared_kernel(const float *src, void *dst, long values, long T, int Hkv, int share,
+                                                                              int D, long batch, long token, long head) {
+    typedef typename fc_elem<DT>::type E;
+    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < values; i += (long)gridDim.x * kThreads) {
+        const long row = i / D, d = i - row * D, bt = row / Hkv, hk = row - bt * Hkv, b = bt / T, t = bt - b * T;
+        const float *p = src + (bt * Hkv + hk) * share * D + d;
+        float s = 0.f;
+        for (int g = 0; g < share; g++) s += p[(long)g * D];
+        ((E *)dst)[b * batch + t * token + hk * head + d] = (E)s;
+    }
+}
+
+int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
+
+bool shape_ok(const fc_linear_attention_shape *s) {
+    if (!s || s->B < 1 || s->T < 1 || s->H < 1 || s->Hkv < 1 || s->H % s->Hkv || s->Dk < 1 || s->Dv < 1 || !fc_dtype_ok(s->dtype)) return false;
+    if (!(s->scale == s->scale) || s->scale - s->scale != 0.f) return false;
+    const long strides[12] = {s->q_batch, s->q_token, s->q_head, s->k_batch, s->k_token, s->k_head,
+                              s->v_batch, s->v_token, s->v_head, s->o_batch, s->o_token, s->o_head};
+    for (long v : strides)
+        if (v < 0) return false;
+    return true;
+}
+
+bool same(const fc_linear_attention_plan &a, const fc_linear_attention_plan &b) {
+    const fc_linear_attention_shape &s = a.shape, &t = b.shape;
+    return s.B == t.B && s.T == t.T && s.H == t.H && s.Hkv == t.Hkv && s.Dk == t.Dk && s.Dv == t.Dv && s.dtype == t.dtype && s.scale == t.scale &&
+           s.q_batch == t.q_batch && s.q_token == t.q_token && s.q_head == t.q_head && s.k_batch == t.k_batch && s.k_token == t.k_token &&
+           s.k_head == t.k_head && s.v_batch == t.v_batch && s.v_token == t.v_token && s.v_head == t.v_head && s.o_batch == t.o_batch &&
+           s.o_token == t.o_token && s.o_head == t.o_head && a.chunk == b.chunk && a.segments == b.segments && a.ws_bytes == b.ws_bytes &&
+           a.ws_backward_bytes == b.ws_backward_bytes;
+}
+
+template <int DT>
+void launch_step(fc_context *ctx, const fc_la_run &r, long B) {
+    const unsigned blocks = (unsigned)(B * r.H * ((r.Dv + kStepCols - 1) / kStepCols));
+    if (r.Dk <= 32) fc_linear_attention_step_kernel<DT, 1><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+    else if (r.Dk <= 64) fc_linear_attention_step_kernel<DT, 2><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+    else if (r.Dk <= 128) fc_linear_attention_step_kernel<DT, 4><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+    else fc_linear_attention_step_kernel<DT, 8><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+}
+
+int run(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_run &r) {
+    if (s.dtype == FC_F32) launch_step<FC_F32>(ctx, r, s.B);
+    else if (s.dtype == FC_BF16) launch_step<FC_BF16>(ctx, r, s.B);
+    else launch_step<FC_F16>(ctx, r, s.B);
+    FC_LAUNCH_CHECK(ctx, "fc_linear_attention_step_kernel");
+    return FC_OK;
+}
+
+// A gradient of a key/value operand: straight to its place, or by query head and then added up.
+int run_shared(fc_context *ctx, const fc_linear_attention_shape &s, fc_la_run &r, float *ws, void *dst, int D, long batch, long token, long head) {
+    const int share = s.H / s.Hkv;
+    r.o = dst;
+    r.o32 = share > 1 ? ws : nullptr;
+    r.o_batch = batch; r.o_token = token; r.o_head = head;
+    int rc = run(ctx, s, r);
+    if (rc || share == 1) return rc;
+    const long values = (long)s.B * s.T * s.Hkv * D;
+    const long want = (values + kThreads - 1) / kThreads;
+    const unsigned blocks = (unsigned)(want < 65536 ? want : 65536);
+    if (s.dtype == FC_F32)
+        fc_linear_attention_shared_kernel<FC_F32><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
+    else if (s.dtype == FC_BF16)
+        fc_linear_attention_shared_kernel<FC_BF16><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
+    else
+        fc_linear_attention_shared_kernel<FC_F16><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
+    FC_LAUNCH_CHECK(ctx, "fc_linear_attention_shared_kernel");
+    return FC_OK;
+}
+
+}  // namespace
+
+extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s, fc_linear_attention_plan *plan) {
+    if (!plan || !shape_ok(s)) return FC_ERR_INVALID;
+    if (s->Dk > kMaxDim || s->Dv > kMaxDim || fc_count(s->B, s->H) < 0 || fc_count(s->B, s->H) >= (1l << 31) / 8) return FC_ERR_UNSUPPORTED;
+    const int most = s->Dk > s->Dv ? s->Dk : s->Dv;
+    const long tokens = fc_count(s->B, s->T), values = tokens < 0 ? -1 : fc_count(tokens, s->H, 4 * most);
+    if (s->T >= (1l << 31) || values < 0) return FC_ERR_UNSUPPORTED;
+    *plan = {};
+    plan->shape = *s;
+    plan->chunk = 0;
+    plan->segments = 1;
+    plan->ws_bytes = 0;
+    plan->ws_backward_bytes = s->H > s->Hkv ? (size_t)values : 0;
+    return FC_OK;
+}
+
+static int check_plan(fc_context *ctx, const fc_linear_attention_plan *plan, const char *what) {
+    fc_linear_attention_plan own;
+    if (!plan || fc_linear_attention_make_plan(&plan->shape, &own) != FC_OK || !same(*plan, own)) return fail(ctx, FC_ERR_INVALID, what);
+    return FC_OK;
+}
+
+extern "C" int fc_linear_attention(fc_context *ctx, const fc_linear_attention_plan *plan, const void *q_dev, const void *k_dev,
+                                   const void *v_dev, const float *log_decay_dev, void *o_dev, const float *state_in_dev,
+                                   float *state_out_dev, const int32_t *lengths_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_linear_attention: not a plan of fc_linear_attention_make_plan")) return FC_ERR_INVALID;
+    const fc_linear_attention_shape &s = plan->shape;
+    if (!q_dev || !k_dev || !v_dev || !log_decay_dev || !o_dev || (!ws_dev && plan->ws_bytes)) return fail(ctx, FC_ERR_INVALID, "fc_linear_attention: null pointer");
+    if ((((uint64_t)q_dev | (uint64_t)k_dev | (uint64_t)v_dev | (uint64_t)o_dev) & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)ws_dev & 15) ||
+        (((uint64_t)log_decay_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev | (uint64_t)lengths_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_linear_attention: unaligned pointer");
+    const int share = s.H / s.Hkv;
+    fc_la_run r = {};
+    r.q = {q_dev, s.q_batch, s.q_token, s.q_head, 1};
+    r.k = {k_dev, s.k_batch, s.k_token, s.k_head, share};
+    r.v = {v_dev, s.v_batch, s.v_token, s.v_head, share};
+    r.o = o_dev; r.o_batch = s.o_batch; r.o_token = s.o_token; r.o_head = s.o_head;
+    r.state_in = state_in_dev; r.state_out = state_out_dev; r.state_row = s.Dv; r.state_col = 1;
+    r.log_decay = log_decay_dev; r.lengths = lengths_dev;
+    r.T = s.T; r.H = s.H; r.Dk = s.Dk; r.Dv = s.Dv;
+    r.scale_in = 1.f; r.scale_out = s.scale;
+    r.ws = (float *)ws_dev;
+    return run(ctx, s, r);
+}
+
+extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan *plan, const void *do_dev, const void *q_dev,
+                                            const void *k_dev, const void *v_dev, const float *log_decay_dev, void *dq_dev, void *dk_dev,
+                                            void *dv_dev, const float *state_in_dev, const float *dstate_out_dev, float *dstate_in_dev,
+                                            const int32_t *lengths_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_linear_attention_backward: not a plan of fc_linear_attention_make_plan")) return FC_ERR_INVALID;
+    const fc_linear_attention_shape &s = plan->shape;
+    if (!do_dev || !q_dev || !k_dev || !v_dev || !log_decay_dev || !dq_dev || !dk_dev || !dv_dev || (!ws_dev && plan->ws_backward_bytes))
+        return fail(ctx, FC_ERR_INVALID, "fc_linear_attention_backward: null pointer");
+    const uint64_t addr = (uint64_t)do_dev | (uint64_t)q_dev | (uint64_t)k_dev | (uint64_t)v_dev | (uint64_t)dq_dev | (uint64_t)dk_dev | (uint64_t)dv_dev;
+    if ((addr & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)ws_dev & 15) ||
+        (((uint64_t)log_decay_dev | (uint64_t)state_in_dev | (uint64_t)dstate_out_dev | (uint64_t)dstate_in_dev | (uint64_t)lengths_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_linear_attention_backward: unaligned pointer");
+    const int share = s.H / s.Hkv;
+    const fc_la_operand q = {q_dev, s.q_batch, s.q_token, s.q_head, 1}, k = {k_dev, s.k_batch, s.k_token, s.k_head, share},
+                        v = {v_dev, s.v_batch, s.v_token, s.v_head, share}, d = {do_dev, s.o_batch, s.o_token, s.o_head, 1};
+    float *sums = (float *)ws_dev;
+    fc_la_run r = {};
+    r.log_decay = log_decay_dev; r.lengths = lengths_dev;
+    r.T = s.T; r.H = s.H;
+    // dq, from the transposed state
+    r.q = d; r.k = v; r.v = k;
+    r.Dk = s.Dv; r.Dv = s.Dk;
+    r.state_in = state_in_dev; r.state_row = 1; r.state_col = s.Dv;
+    r.scale_in = 1.f; r.scale_out = s.scale;
+    r.o = dq_dev; r.o_batch = s.q_batch; r.o_token = s.q_token; r.o_head = s.q_head;
+    int rc = run(ctx, s, r);
+    if (rc) return rc;
+    // dk, from the last token to the first
+    r.reverse = 1;
+    r.scale_in = s.scale; r.scale_out = 1.f;
+    r.q = v; r.k = d; r.v = q;
+    r.state_in = dstate_out_dev;
+    rc = run_shared(ctx, s, r, sums, dk_dev, s.Dk, s.k_batch, s.k_token, s.k_head);
+    if (rc) return rc;
+    // dv, and the gradient of the first state
+    r.q = k; r.k = q; r.v = d;
+    r.Dk = s.Dk; r.Dv = s.Dv;
+    r.state_row = s.Dv; r.state_col = 1;
+    r.state_out = dstate_in_dev;
+    return run_shared(ctx, s, r, sums, dv_dev, s.Dv, s.v_batch, s.v_token, s.v_head);
+}

@@ -442,6 +442,133 @@ int fc_graph_destroy(fc_graph *graph);
  * without host round trips (the layer graph of layer.h:29-84). */
 int fc_maxpool2x2(fc_context *ctx, const float *x_dev, float *y_dev, int N, int C, int H, int W);
 
+/* ---- operators on tokens, channels last -------------------------------- */
+
+/* What a network runs on the pixels of a convolution trunk, or on the patches of a patch embedding, once they are tokens:
+ * channels last, so that a token's channels are neighbours.  No counterpart in the reference, which ends at the
+ * convolution.  A trunk's fp32 output of one-pixel images (N tokens of C x 1 x 1) has this layout as it is.
+ *
+ * Tensors hold fp32, bf16 or IEEE half (fc_dtype); every sum, statistic, state and angle is fp32 or wider, and a result is
+ * rounded once to the tensor's type.  Parameters (gamma, beta, log_decay, inv_freq), statistics and states are fp32 always.
+ * Strides are in elements; channels of one token (one head) are neighbours.  Pointers need the alignment of their type only:
+ * rows that begin on 16 bytes and have sizes that are multiples of 16 bytes are read fastest.  Buffers must not overlap, but
+ * where a call says so.  All calls run on the context's stream, allocate nothing and can be recorded into a graph; they are not
+ * stages and are never bracketed by timing events.  Sizes that are refused: FC_ERR_INVALID for what no such operator has,
+ * FC_ERR_UNSUPPORTED beyond the limits stated here. */
+typedef enum { FC_F32 = 0, FC_BF16 = 1, FC_F16 = 2 } fc_dtype;
+typedef enum { FC_ACT_NONE = 0, FC_ACT_RELU = 1, FC_ACT_SILU = 2, FC_ACT_GELU = 3 /* with erf */ } fc_activation;
+
+/* Group norm with an activation.  x is N images of P pixels with C channels in G groups of C/G neighbours:
+ *   xhat = (x - mean) * rstd over the P*C/G values of a group,  rstd = 1/sqrt(variance + eps)
+ *   y = act(gamma * xhat + beta)
+ * Pixel p of image n begins at n*x_image + p*x_pixel; y (and dy) likewise, dx as x.  G == 1 is a layer norm over whole images,
+ * G == C an instance norm.  Limit: C/G <= 4096. */
+typedef struct {
+    int N;
+    long P;
+    int C, G;
+    int dtype, act;
+    float eps;
+    long x_image, x_pixel, y_image, y_pixel;
+} fc_group_norm_shape;
+
+typedef struct {
+    fc_group_norm_shape shape;
+    int span;                 /* channels that one workgroup reads of a pixel: whole groups */
+    int chunks;               /* parts that the pixels of an image are cut into */
+    int resident;             /* 1: an image's groups stay in a workgroup's registers, one launch */
+    int resident_backward;
+    size_t ws_bytes;          /* workspace of the forward call, 0 if none */
+    size_t ws_backward_bytes; /* and of the backward call */
+} fc_group_norm_plan;
+
+int fc_group_norm_make_plan(const fc_group_norm_shape *shape, fc_group_norm_plan *plan);
+
+/* gamma and beta: C floats, or NULL for ones and zeros.  mean and rstd: N*G floats for the backward pass, or both NULL.
+ * y may be x where their strides are equal.  The variance is formed from differences to running means, so that a mean many
+ * times the deviation costs no accuracy. */
+int fc_group_norm(fc_context *ctx, const fc_group_norm_plan *plan, const void *x_dev, const float *gamma_dev,
+                  const float *beta_dev, void *y_dev, float *mean_dev, float *rstd_dev, void *ws_dev);
+
+/* Gradients of x (in the tensor's type), gamma and beta (fp32, overwritten; each may be NULL) from that of y.  mean and rstd are the
+ * forward call's.  Sums run in a fixed order: the same call gives the same bits.  ReLU's slope at 0 is 0. */
+int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan *plan, const void *dy_dev, const void *x_dev,
+                           const float *gamma_dev, const float *beta_dev, const float *mean_dev, const float *rstd_dev,
+                           void *dx_dev, float *dgamma_dev, float *dbeta_dev, void *ws_dev);
+
+/* Rotary positions with up to FC_ROTARY_AXES axes (time, height, width): pair j of a head is turned by the angle
+ * position[axis of j] * inv_freq[j]:  (a, b) -> (a cos - b sin, b cos + a sin).  The first pairs[0] pairs belong to axis 0, the
+ * next pairs[1] to axis 1, and so on; with R pairs in all, pair j is channels j and j + R, or 2j and 2j + 1 if `interleaved`.
+ * Channels from 2R on pass unchanged.  positions: int32 [B][T][axes], those of sequence b at b*positions_batch (0: the same
+ * ones for all); any int32 is a position, and the angle is reduced in 64 bits.  q has Hq heads and k Hk (0: no k).
+ * Token t of sequence b and head h begins at b*q_batch + t*q_token + h*q_head, and so for k and both outputs.
+ * Limits: D <= 1024. */
+#define FC_ROTARY_AXES 4
+typedef struct {
+    int B;
+    long T;
+    int Hq, Hk, D;
+    int axes;
+    int pairs[FC_ROTARY_AXES];
+    int interleaved;
+    int dtype;
+    long positions_batch;
+    long q_batch, q_token, q_head;
+    long k_batch, k_token, k_head;
+    long qo_batch, qo_token, qo_head;
+    long ko_batch, ko_token, ko_head;
+} fc_rotary_shape;
+
+/* inverse != 0 turns the other way: the backward pass (gradients in, gradients out).  q_out may be q and k_out may be k where
+ * the strides are equal.  One launch for both, one token or many. */
+int fc_rotary(fc_context *ctx, const fc_rotary_shape *shape, const void *q_dev, const void *k_dev, const int32_t *positions_dev,
+              const float *inv_freq_dev, int inverse, void *q_out_dev, void *k_out_dev);
+
+/* Linear attention with a decay for each head.  Head h has a state S of Dk x Dv floats that takes in a token at a time:
+ *   S_t = decay S_(t-1) + k_t v_t^T,   o_t = scale * S_t^T q_t,   decay = exp(log_decay[h]) in [0, 1]
+ * H query heads share Hkv key/value heads (H a multiple of Hkv; head h reads key/value head h / (H/Hkv)); every query head has
+ * its own decay and state.  Token t of sequence b and head h begins at b*q_batch + t*q_token + h*q_head, and so for k, v and o
+ * (gradients: as what they are gradients of).  States are packed [B][H][Dk][Dv].  log_decay above 0 is not checked for (the state
+ * grows); minus infinity is a decay of 0, a token that sees itself alone.
+ * lengths: B int32, or NULL when every sequence has T tokens; sequence b then ends after min(max(lengths[b], 0), T) of them: its later
+ * tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
+ * Limits: Dk, Dv <= 256. */
+typedef struct {
+    int B;
+    long T;
+    int H, Hkv, Dk, Dv;
+    int dtype;
+    float scale;
+    long q_batch, q_token, q_head;
+    long k_batch, k_token, k_head;
+    long v_batch, v_token, v_head;
+    long o_batch, o_token, o_head;
+} fc_linear_attention_shape;
+
+typedef struct {
+    fc_linear_attention_shape shape;
+    int chunk;                /* tokens that are taken in together; 0: the recurrence, a token at a time */
+    int segments;             /* parts of a sequence that run side by side, joined by their states */
+    size_t ws_bytes;          /* workspace of the forward call, 0 if none */
+    size_t ws_backward_bytes; /* and of the backward call */
+} fc_linear_attention_plan;
+
+int fc_linear_attention_make_plan(const fc_linear_attention_shape *shape, fc_linear_attention_plan *plan);
+
+/* state_in: the state before the first token (NULL: zeros).  state_out: the state after the last one (NULL: not wanted); may be
+ * state_in.  A prompt runs in chunks on the matrix cores, a few tokens through the recurrence: the same call serves both. */
+int fc_linear_attention(fc_context *ctx, const fc_linear_attention_plan *plan, const void *q_dev, const void *k_dev,
+                        const void *v_dev, const float *log_decay_dev, void *o_dev, const float *state_in_dev,
+                        float *state_out_dev, const int32_t *lengths_dev, void *ws_dev);
+
+/* Gradients of q, k, v and state_in (dstate_in; NULL: not wanted) from those of o and state_out (dstate_out; NULL: none).  The
+ * decays are constants of the model and have no gradient.  Gradients of a shared key/value head are summed over its query
+ * heads in a fixed order. */
+int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan *plan, const void *do_dev, const void *q_dev,
+                                 const void *k_dev, const void *v_dev, const float *log_decay_dev, void *dq_dev, void *dk_dev,
+                                 void *dv_dev, const float *state_in_dev, const float *dstate_out_dev, float *dstate_in_dev,
+                                 const int32_t *lengths_dev, void *ws_dev);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,280 @@
+"""Group norm with an activation, forward and backward, against the formulas in 64 bits.
+
+Tolerances: a result is rounded once to its type (ROUND); before that everything is fp32.  The joined statistics err by a few last
+places of the group's largest value, each of the dozen operations behind them by one of its result: 32 last places of
+|gamma| rstd max|x - mean| + (rstd/eps part of the mean) cover both; where the mean is many times the deviation its own last
+place counts, divided by the deviation.  No slope of an activation is above 1.13, nor its own slope above 1.1."""
+import numpy as np
+import pytest
+
+import fastconv_amd as F
+import tokens as K
+
+pytestmark = pytest.mark.gpu
+
+ACTS = {"none": F.ACT_NONE, "relu": F.ACT_RELU, "silu": F.ACT_SILU, "gelu": F.ACT_GELU}
+EPS = 1e-5
+
+
+@pytest.fixture(scope="module")
+def lib():
+    L = F.load(0, 1 << 30)
+    yield L
+    L.close()
+
+
+def inputs(rng, N, P, C):
+    x = rng.standard_normal((N, P, C)) * (0.5 + rng.random(C)) + 0.5 * rng.standard_normal(C)
+    return x, (1 + 0.2 * rng.standard_normal(C)).astype(np.float32), (0.2 * rng.standard_normal(C)).astype(np.float32)
+
+
+def forward(L, x, gamma, beta, N, P, C, G, dtype, act, gap=0, offset=0, stats=True):
+    pixel = C + gap
+    dx = K.Dev(L, (N, P, C), dtype, (P * pixel, pixel, 1), x, offset)
+    dy = K.Dev(L, (N, P, C), dtype, None, None, offset)
+    s = F.GroupNormShape(N, P, C, G, K.TYPES[dtype], ACTS[act], EPS, P * pixel, pixel, P * C, C)
+    plan = L.group_norm_plan(s)
+    m, r = (K.Dev(L, (N, G), "f32") for _ in range(2))
+    ws = L.alloc(plan.ws_bytes) if plan.ws_bytes else None
+    g, b = (None if a is None else K.floats(L, a) for a in (gamma, beta))
+    L.group_norm(plan, dx.ptr, g, b, dy.ptr, m.ptr if stats else None, r.ptr if stats else None, ws)
+    return dx, dy, plan, m, r, g, b
+
+
+def close(got, want, tol, what):
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), "%s: %d off, worst %.3g of its tolerance" % (what, bad.sum(), np.nanmax(np.abs(got - want) / tol))
+
+
+def bounds(x, gamma, beta, G, rstd, mean):
+    """fp32 error of z: 32 last places of its largest parts, and what a last place of the mean amounts to."""
+    N, P, C = x.shape
+    wide = lambda a: np.repeat(a, C // G, axis=-1)[:, None, :]  # noqa: E731
+    spread = np.abs(x.reshape(N, P, G, -1) - mean[:, None, :, None]).max(axis=(1, 3))
+    return 32 * K.EPS * (np.abs(gamma) * wide(rstd * (spread + np.abs(mean))) + np.abs(beta))
+
+
+CASES = [  # N, P, C, G, dtype, act, gap
+    (1, 1, 8, 2, "f32", "none", 0),           # one pixel
+    (2, 1, 64, 1, "bf16", "silu", 0),
+    (3, 2, 6, 3, "f32", "silu", 0),           # groups of two channels, an access that two pixels do not fill
+    (1, 196, 512, 32, "bf16", "silu", 0),
+    (2, 35, 192, 32, "f16", "gelu", 24),      # groups of six channels, a gap between pixels
+    (2, 35, 192, 32, "bf16", "relu", 5),      # a gap that no wide access fits
+    (3, 77, 63, 7, "f16", "silu", 0),         # odd channels
+    (2, 130, 64, 32, "bf16", "silu", 0),
+    (1, 1000, 40, 8, "f32", "gelu", 8),
+    (5, 33, 24, 24, "f16", "none", 0),        # instance norm
+    (2, 9, 4096, 1, "bf16", "silu", 0),       # the largest group
+    (1, 5, 4097 * 2, 4097, "f32", "relu", 0),
+    (2, 6, 4100, 2, "bf16", "none", 0),       # wide groups that no two share a workgroup
+    (1, 3, 2051 * 3, 3, "f16", "none", 0),
+    (1, 9000, 16, 4, "bf16", "silu", 0),      # many chunks
+    (2, 50176, 8, 4, "f32", "silu", 0),
+    (70, 5, 32, 8, "f32", "gelu", 0),         # many images
+    (33, 1225, 96, 32, "bf16", "gelu", 0),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)))
+def test_forward_and_backward(lib, case):
+    N, P, C, G, dtype, act, gap = case
+    rng = np.random.default_rng(sum(case[:4]))
+    x, gamma, beta = inputs(rng, N, P, C)
+    mark = lib.mark()
+    try:
+        print("group norm", case, flush=True)
+        dx, dy, plan, m, r, g, b = forward(lib, x, gamma, beta, N, P, C, G, dtype, act, gap)
+        x = dx.values
+        y, mean, rstd, xhat, z = K.group_norm(x, gamma, beta, G, EPS, act)
+        tz = bounds(x, gamma, beta, G, rstd, mean)
+        got = dy.get()
+        close(got, y, K.ROUND[dtype] * np.abs(y) + 1.2 * tz + K.TINY[dtype], "y")
+        spread = np.abs(x).reshape(N, -1).max(axis=1)[:, None]
+        close(m.get(), mean, 16 * K.EPS * spread + 1e-30, "mean")
+        close(r.get(), rstd, 32 * K.EPS * rstd * (1 + rstd ** 2 * spread ** 2 * K.EPS), "rstd")
+        # without statistics, the same bits
+        _, plain, *_ = forward(lib, x, gamma, beta, N, P, C, G, dtype, act, gap, stats=False)
+        assert np.array_equal(plain.get(), got)
+
+        grad = K.Dev(lib, (N, P, C), dtype, None, rng.standard_normal((N, P, C)))
+        out = K.Dev(lib, (N, P, C), dtype, dx.strides)
+        dgamma, dbeta = K.Dev(lib, (C,), "f32"), K.Dev(lib, (C,), "f32")
+        ws = lib.alloc(max(4, plan.ws_backward_bytes))
+        lib.group_norm_backward(plan, grad.ptr, dx.ptr, g, b, m.ptr, r.ptr, out.ptr, dgamma.ptr, dbeta.ptr, ws)
+        want, wg, wb, dz = K.group_norm_backward(grad.values, x, gamma, beta, G, EPS, act)
+        # dz errs with z (by the slope's slope) and by a few places of its own; the sums by 2 sqrt of their length at most times that
+        tdz = np.abs(grad.values) * (1.2 * tz + 8 * K.EPS)
+        if act == "relu":      # where z is within its error of the jump either slope will do
+            tdz = tdz + np.abs(grad.values) * (np.abs(z) <= tz)
+        txh = 32 * K.EPS * (np.abs(xhat) + np.repeat(rstd * (np.abs(mean) + spread), C // G, axis=-1)[:, None, :])
+        places = K.EPS * (16 + 2 * np.sqrt(N * P))
+        close(dbeta.get(), wb, tdz.sum(axis=(0, 1)) + places * np.abs(dz).sum(axis=(0, 1)) + 1e-30, "dbeta")
+        close(dgamma.get(), wg, (tdz * np.abs(xhat) + np.abs(dz) * txh).sum(axis=(0, 1)) + places * np.abs(dz * xhat).sum(axis=(0, 1)) + 1e-30,
+              "dgamma")
+        grouped = lambda a: np.repeat(a.reshape(N, P, G, -1).mean(axis=(1, 3)), C // G, axis=-1)[:, None, :]  # noqa: E731
+        rw = np.repeat(rstd, C // G, axis=-1)[:, None, :]
+        ga = np.abs(gamma)
+        h, th = ga * np.abs(dz), ga * tdz
+        ax = np.abs(xhat)
+        s1, s2 = grouped(h), grouped(h * ax)
+        ts1, ts2 = grouped(th), grouped(th * ax + h * txh)
+        tol = rw * (th + ts1 + ax * ts2 + txh * s2 + 2 * places * (h + s1 + ax * s2)) + 32 * K.EPS * np.abs(want)
+        close(out.get(), want, K.ROUND[dtype] * np.abs(want) + tol + K.TINY[dtype], "dx")
+        # again: the same bits; and without the sums
+        again, only = K.Dev(lib, (N, P, C), dtype, dx.strides), K.Dev(lib, (C,), "f32")
+        lib.group_norm_backward(plan, grad.ptr, dx.ptr, g, b, m.ptr, r.ptr, again.ptr, only.ptr, None, ws)
+        assert np.array_equal(again.get(), out.get()) and np.array_equal(only.get(), dgamma.get())
+    finally:
+        lib.release(mark)
+
+
+def test_gradient_against_differences(lib):
+    """dx, dgamma and dbeta along random directions against central differences of the forward formula in 64 bits."""
+    N, P, C, G = 2, 30, 24, 4
+    rng = np.random.default_rng(5)
+    for act in ("none", "silu", "gelu"):
+        x, gamma, beta = inputs(rng, N, P, C)
+        mark = lib.mark()
+        print("group norm, differences", act, flush=True)
+        dx, dy, plan, m, r, g, b = forward(lib, x, gamma, beta, N, P, C, G, "f32", act)
+        x = dx.values
+        w = K.Dev(lib, (N, P, C), "f32", None, rng.standard_normal((N, P, C)))
+        out, dgamma, dbeta = K.Dev(lib, (N, P, C), "f32"), K.Dev(lib, (C,), "f32"), K.Dev(lib, (C,), "f32")
+        lib.group_norm_backward(plan, w.ptr, dx.ptr, g, b, m.ptr, r.ptr, out.ptr, dgamma.ptr, dbeta.ptr, lib.alloc(plan.ws_backward_bytes))
+        loss = lambda a, c, d: (K.group_norm(a, c, d, G, EPS, act)[0] * w.values).sum()  # noqa: E731
+        e = 1e-4      # truncation is of e^2 times a third derivative of some tens
+        u, ug, ub = rng.standard_normal((N, P, C)), rng.standard_normal(C), rng.standard_normal(C)
+        gamma, beta = gamma.astype(np.float64), beta.astype(np.float64)
+        for got, d in (((out.get() * u).sum(), (loss(x + e * u, gamma, beta) - loss(x - e * u, gamma, beta)) / (2 * e)),
+                       ((dgamma.get() * ug).sum(), (loss(x, gamma + e * ug, beta) - loss(x, gamma - e * ug, beta)) / (2 * e)),
+                       ((dbeta.get() * ub).sum(), (loss(x, gamma, beta + e * ub) - loss(x, gamma, beta - e * ub)) / (2 * e))):
+            assert abs(got - d) <= 1e-4 * (1 + abs(d)), act
+        lib.release(mark)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_mean_far_above_the_deviation(lib, dtype):
+    """Values of 1000 +- 1: the variance comes from differences, not from squares."""
+    N, P, C, G = 2, 700, 16, 2
+    rng = np.random.default_rng(1)
+    x = 1000 + rng.standard_normal((N, P, C)) * (8 if dtype == "bf16" else 1)
+    x[0, 0] = 900      # and the first pixel is no typical one
+    mark = lib.mark()
+    dx, dy, *_ = forward(lib, x, None, None, N, P, C, G, dtype, "none")
+    y, mean, rstd, *_ = K.group_norm(dx.values, 1.0, 0.0, G, EPS, "none")
+    close(dy.get(), y, K.ROUND[dtype] * np.abs(y) + bounds(dx.values, np.ones(C), np.zeros(C), G, rstd, mean), "y")
+    lib.release(mark)
+
+
+def test_constant_groups_and_values_that_are_not_finite(lib):
+    N, P, C, G = 2, 40, 32, 4
+    rng = np.random.default_rng(2)
+    x, gamma, beta = inputs(rng, N, P, C)
+    x[0, :, 8:16] = 3.0
+    x[1, 7, 3], x[1, 9, 30] = np.nan, np.inf
+    mark = lib.mark()
+    dx, dy, *_ = forward(lib, x, gamma, beta, N, P, C, G, "f32", "none")
+    got = dy.get()
+    assert np.array_equal(got[0, :, 8:16], np.broadcast_to(beta[8:16].astype(np.float64), (P, 8)))
+    for n, c in ((1, slice(0, 8)), (1, slice(24, 32))):      # its own group and no other
+        assert np.isnan(got[n, :, c]).all()
+    clean = x.copy()
+    clean[1, 7, 3] = clean[1, 9, 30] = 0
+    _, ref, *_ = forward(lib, clean, gamma, beta, N, P, C, G, "f32", "none")
+    assert np.array_equal(got[0], ref.get()[0]) and np.array_equal(got[1, :, 8:24], ref.get()[1, :, 8:24])
+    lib.release(mark)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4])
+def test_tensors_that_begin_anywhere(lib, offset):
+    rng = np.random.default_rng(3)
+    x, gamma, beta = inputs(rng, 2, 50, 64)
+    mark = lib.mark()
+    _, a, *_ = forward(lib, x, gamma, beta, 2, 50, 64, 8, "bf16", "silu", gap=8)
+    _, b, *_ = forward(lib, x, gamma, beta, 2, 50, 64, 8, "bf16", "silu", gap=8, offset=offset)
+    # narrower accesses join in another order
+    assert np.abs(a.get() - b.get()).max() <= 2 * K.ROUND["bf16"] * np.abs(a.get()).max()
+    lib.release(mark)
+
+
+def test_in_place(lib):
+    rng = np.random.default_rng(4)
+    for N, P, C, G in ((2, 300, 64, 8), (1, 20000, 64, 8)):
+        x, gamma, beta = inputs(rng, N, P, C)
+        mark = lib.mark()
+        _, want, *_ = forward(lib, x, gamma, beta, N, P, C, G, "f16", "silu")
+        t = K.Dev(lib, (N, P, C), "f16", None, x)
+        plan = lib.group_norm_plan(F.GroupNormShape.packed(N, P, C, G, F.F16, F.ACT_SILU, EPS))
+        lib.group_norm(plan, t.ptr, K.floats(lib, gamma), K.floats(lib, beta), t.ptr, ws=lib.alloc(max(4, plan.ws_bytes)))
+        assert np.array_equal(t.get(), want.get())
+        lib.release(mark)
+
+
+def test_image_beyond_32_bits(lib):
+    """The second image begins 2^31 elements after the first."""
+    N, P, C, G, far = 2, 40, 32, 8, (1 << 31) + 64
+    rng = np.random.default_rng(6)
+    x, gamma, beta = inputs(rng, N, P, C)
+    raw, values = K.to_type(x, "bf16")
+    with F.load(0, 9 << 30) as L:
+        big, y = L.alloc(2 * far + 2 * P * C), K.Dev(L, (N, P, C), "bf16")
+        for n in range(N):
+            L._check(L.c.fc_upload(L.ctx, big.value + 2 * far * n, raw[n].ctypes.data, raw[n].nbytes))
+        plan = L.group_norm_plan(F.GroupNormShape(N, P, C, G, F.BF16, F.ACT_SILU, EPS, far, C, P * C, C))
+        ws = L.alloc(max(4, plan.ws_bytes))
+        L.group_norm(plan, big, K.floats(L, gamma), K.floats(L, beta), y.ptr, ws=ws)
+        want, mean, rstd, *_ = K.group_norm(values, gamma, beta, G, EPS, "silu")
+        close(y.get(), want, K.ROUND["bf16"] * np.abs(want) + 1.2 * bounds(values, gamma, beta, G, rstd, mean), "y")
+
+
+def test_replays_of_a_recorded_graph(lib):
+    N, P, C, G = 4, 500, 64, 8
+    mark = lib.mark()
+    rng = np.random.default_rng(8)
+    x, gamma, beta = inputs(rng, N, P, C)
+    dx, dy, plan, m, r, g, b = forward(lib, x, gamma, beta, N, P, C, G, "f32", "silu")
+    ws = lib.alloc(max(4, plan.ws_bytes, plan.ws_backward_bytes))
+    out, dgamma, dbeta = K.Dev(lib, (N, P, C), "f32"), K.Dev(lib, (C,), "f32"), K.Dev(lib, (C,), "f32")
+
+    def step():
+        lib.group_norm(plan, dx.ptr, g, b, dy.ptr, m.ptr, r.ptr, ws)
+        lib.group_norm_backward(plan, dy.ptr, dx.ptr, g, b, m.ptr, r.ptr, out.ptr, dgamma.ptr, dbeta.ptr, ws)
+    lib.graph_begin()
+    step()
+    graph = lib.graph_end()
+    for seed in range(3):
+        print("group norm, replay", seed, flush=True)
+        lib.upload_into(dx.base, np.concatenate([np.random.default_rng(seed).standard_normal((N * P * C,)), np.zeros(64)]))
+        step()
+        want = [lib.download(t.base, t.host.shape) for t in (dy, out, dgamma, dbeta)]
+        for t in (dy, out, dgamma, dbeta):
+            lib.fill_zero(t.base, 4 * t.count)
+        lib.graph_launch(graph)
+        for t, w in zip((dy, out, dgamma, dbeta), want):
+            n = t.count - 64
+            assert np.array_equal(lib.download(t.base, t.host.shape)[:n], w[:n])
+    lib.graph_destroy(graph)
+    lib.release(mark)
+
+
+def test_refusals_at_the_call(lib):
+    mark = lib.mark()
+    plan = lib.group_norm_plan(F.GroupNormShape.packed(2, 30000, 16, 4, F.BF16))
+    buf = lib.alloc(4 << 20)
+    p = buf.value
+    bad = F.GroupNormPlan.from_buffer_copy(plan)
+    bad.chunks += 1
+    for call in (lambda: lib.group_norm(bad, p, None, None, p, None, None, p),
+                 lambda: lib.group_norm(plan, None, None, None, p, None, None, p),
+                 lambda: lib.group_norm(plan, p, None, None, None, None, None, p),
+                 lambda: lib.group_norm(plan, p, None, None, p, p, None, p),         # one statistic of two
+                 lambda: lib.group_norm(plan, p, None, None, p, None, None, None),   # no workspace
+                 lambda: lib.group_norm(plan, p + 1, None, None, p, None, None, p),
+                 lambda: lib.group_norm(plan, p, p + 2, None, p, None, None, p),
+                 lambda: lib.group_norm_backward(plan, p, p, None, None, None, p, p, None, None, p),
+                 lambda: lib.group_norm_backward(plan, p, p, None, None, p, p, p, None, None, None)):
+        with pytest.raises(F.FastConvError) as e:
+            call()
+        assert e.value.status == -1 and "fc_group_norm" in str(e.value)
+    lib.release(mark)
