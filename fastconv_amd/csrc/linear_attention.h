@@ -33,8 +33,18 @@ struct fc_la_run {
     int H, Dk, Dv;           // of this run: rows and columns of its state
     int reverse;
     float scale_in, scale_out;      // of what enters the state, of what leaves it
-    float *ws;
+    bool wide;               // four channels of every operand lie within one access
 };
+
+// linear_attention_<type>.hip: `segments` parts of `segment` tokens of each of `heads` heads.  _state: the state that each but the
+// last adds to none, to parts [heads][segments][Dk][Dv].  _answer: the answers; each segment begins from its state in parts, or, if it is the only
+// one, from state_in.
+int fc_la_state_bf16(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
+int fc_la_state_f16(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
+int fc_la_state_f32(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
+int fc_la_answer_bf16(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
+int fc_la_answer_f16(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
+int fc_la_answer_f32(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts);
 
 __device__ __forceinline__ long fc_la_length(const fc_la_run &r, long b) {
     if (!r.lengths) return r.T;

@@ -6,6 +6,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
+constexpr long kMostSteps = 16;    // up to here the recurrence is faster
+constexpr long kWorkgroups = 512, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
+constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kStepCols = 32;      // columns of the state that a workgroup of the recurrence holds
 
 // The recurrence.  A workgroup holds 32 columns of a head's state in registers: 8 threads side by side with 4 columns each,
@@ -115,6 +118,35 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
     }
 }
 
+// The states that segments begin from: parts[s] becomes what enters segment s, for each element of a head's state.
+__global__ __launch_bounds__(kThreads) void fc_linear_attention_scan_kernel(const fc_la_run r, int segments, long segment, float *parts) {
+    constexpr int AHEAD = 8;      // segments read before the first is joined
+    const int size = r.Dk * r.Dv, blocks = (size + kThreads - 1) / kThreads;
+    const long bh = blockIdx.x / blocks, b = bh / r.H;
+    const int i = (int)(blockIdx.x - bh * blocks) * kThreads + threadIdx.x;
+    if (i >= size) return;
+    const long len = fc_la_length(r, b);
+    const float ld = r.log_decay[bh - b * r.H];
+    const fc_la_power full(ld, segment);
+    const int row = i / r.Dv, col = i - row * r.Dv;
+    float s = r.state_in ? r.state_in[bh * size + row * r.state_row + col * r.state_col] : 0.f;
+    float *p = parts + bh * segments * size + i;
+    for (int first = 0; first < segments; first += AHEAD) {
+        float add[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++)
+            add[a] = first + a < segments - 1 && (first + a) * segment < len ? p[(long)(first + a) * size] : 0.f;
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            if (first + a >= segments) break;
+            p[(long)(first + a) * size] = s;
+            const long n = len - (first + a) * segment;
+            if (n >= segment) s = full.times(s) + add[a];
+            else if (n > 0) s = fc_la_power(ld, n).times(s) + add[a];
+        }
+    }
+}
+
 // Gradients of shared heads: the fp32 gradients [B][T][H][D] of the query heads, added up by key/value head.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void fc_linear_attention_shared_kernel(const float *src, void *dst, long values, long T, int Hkv, int share,
@@ -150,6 +182,12 @@ bool same(const fc_linear_attention_plan &a, const fc_linear_attention_plan &b) 
            a.ws_backward_bytes == b.ws_backward_bytes;
 }
 
+// Tokens of a segment: whole chunks.
+long segment_of(const fc_linear_attention_shape &s, int segments) {
+    const long chunks = (s.T + kChunk - 1) / kChunk;
+    return (chunks + segments - 1) / segments * kChunk;
+}
+
 template <int DT>
 void launch_step(fc_context *ctx, const fc_la_run &r, long B) {
     const unsigned blocks = (unsigned)(B * r.H * ((r.Dv + kStepCols - 1) / kStepCols));
@@ -159,7 +197,7 @@ void launch_step(fc_context *ctx, const fc_la_run &r, long B) {
     else fc_linear_attention_step_kernel<DT, 8><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
 }
 
-int run(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_run &r) {
+int run_step(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_run &r) {
     if (s.dtype == FC_F32) launch_step<FC_F32>(ctx, r, s.B);
     else if (s.dtype == FC_BF16) launch_step<FC_BF16>(ctx, r, s.B);
     else launch_step<FC_F16>(ctx, r, s.B);
@@ -167,13 +205,38 @@ int run(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_run &r)
     return FC_OK;
 }
 
+bool wide(const fc_la_operand &x, int D, size_t es) {
+    return ((D | x.batch | x.token | x.head) & 3) == 0 && ((uintptr_t)x.p & (4 * es - 1)) == 0;
+}
+
+int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *parts) {
+    const fc_linear_attention_shape &s = plan->shape;
+    if (plan->chunk == 0) return run_step(ctx, s, r);
+    const size_t es = fc_elem_size(s.dtype);
+    r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) && wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, es);
+    const long heads = (long)s.B * s.H, segment = segment_of(s, plan->segments);
+    if (plan->segments > 1) {
+        const int rc = s.dtype == FC_F32    ? fc_la_state_f32(ctx, r, heads, plan->segments, segment, parts)
+                       : s.dtype == FC_BF16 ? fc_la_state_bf16(ctx, r, heads, plan->segments, segment, parts)
+                                            : fc_la_state_f16(ctx, r, heads, plan->segments, segment, parts);
+        if (rc) return rc;
+        const unsigned blocks = (unsigned)(heads * ((r.Dk * r.Dv + kThreads - 1) / kThreads));
+        fc_linear_attention_scan_kernel<<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r, plan->segments, segment, parts);
+        FC_LAUNCH_CHECK(ctx, "fc_linear_attention_scan_kernel");
+    }
+    return s.dtype == FC_F32    ? fc_la_answer_f32(ctx, r, heads, plan->segments, segment, parts)
+           : s.dtype == FC_BF16 ? fc_la_answer_bf16(ctx, r, heads, plan->segments, segment, parts)
+                                : fc_la_answer_f16(ctx, r, heads, plan->segments, segment, parts);
+}
+
 // A gradient of a key/value operand: straight to its place, or by query head and then added up.
-int run_shared(fc_context *ctx, const fc_linear_attention_shape &s, fc_la_run &r, float *ws, void *dst, int D, long batch, long token, long head) {
+int run_shared(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *ws, float *parts, void *dst, int D, long batch, long token, long head) {
+    const fc_linear_attention_shape &s = plan->shape;
     const int share = s.H / s.Hkv;
     r.o = dst;
     r.o32 = share > 1 ? ws : nullptr;
     r.o_batch = batch; r.o_token = token; r.o_head = head;
-    int rc = run(ctx, s, r);
+    const int rc = run(ctx, plan, r, parts);
     if (rc || share == 1) return rc;
     const long values = (long)s.B * s.T * s.Hkv * D;
     const long want = (values + kThreads - 1) / kThreads;
@@ -198,10 +261,20 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
     if (s->T >= (1l << 31) || values < 0) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    plan->chunk = 0;
     plan->segments = 1;
-    plan->ws_bytes = 0;
-    plan->ws_backward_bytes = s->H > s->Hkv ? (size_t)values : 0;
+    if (s->T > kMostSteps) {
+        plan->chunk = kChunk;
+        const long slices = (most + 127) / 128, chunks = (s->T + kChunk - 1) / kChunk;
+        long segments = kWorkgroups / (s->B * (long)s->H * slices);
+        if (segments > chunks / kLeastChunks) segments = chunks / kLeastChunks;
+        if (segments > 1) {
+            const long per = (chunks + segments - 1) / segments;
+            segments = (chunks + per - 1) / per;
+        }
+        if (segments > 1) plan->segments = (int)segments;
+        if (plan->segments > 1) plan->ws_bytes = (size_t)s->B * s->H * plan->segments * s->Dk * s->Dv * sizeof(float);
+    }
+    plan->ws_backward_bytes = plan->ws_bytes + (s->H > s->Hkv ? (size_t)values : 0);
     return FC_OK;
 }
 
@@ -231,8 +304,7 @@ extern "C" int fc_linear_attention(fc_context *ctx, const fc_linear_attention_pl
     r.log_decay = log_decay_dev; r.lengths = lengths_dev;
     r.T = s.T; r.H = s.H; r.Dk = s.Dk; r.Dv = s.Dv;
     r.scale_in = 1.f; r.scale_out = s.scale;
-    r.ws = (float *)ws_dev;
-    return run(ctx, s, r);
+    return run(ctx, plan, r, (float *)ws_dev);
 }
 
 extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan *plan, const void *do_dev, const void *q_dev,
@@ -251,7 +323,7 @@ extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_att
     const int share = s.H / s.Hkv;
     const fc_la_operand q = {q_dev, s.q_batch, s.q_token, s.q_head, 1}, k = {k_dev, s.k_batch, s.k_token, s.k_head, share},
                         v = {v_dev, s.v_batch, s.v_token, s.v_head, share}, d = {do_dev, s.o_batch, s.o_token, s.o_head, 1};
-    float *sums = (float *)ws_dev;
+    float *parts = (float *)ws_dev, *sums = parts + plan->ws_bytes / sizeof(float);
     fc_la_run r = {};
     r.log_decay = log_decay_dev; r.lengths = lengths_dev;
     r.T = s.T; r.H = s.H;
@@ -261,19 +333,19 @@ extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_att
     r.state_in = state_in_dev; r.state_row = 1; r.state_col = s.Dv;
     r.scale_in = 1.f; r.scale_out = s.scale;
     r.o = dq_dev; r.o_batch = s.q_batch; r.o_token = s.q_token; r.o_head = s.q_head;
-    int rc = run(ctx, s, r);
+    int rc = run(ctx, plan, r, parts);
     if (rc) return rc;
     // dk, from the last token to the first
     r.reverse = 1;
     r.scale_in = s.scale; r.scale_out = 1.f;
     r.q = v; r.k = d; r.v = q;
     r.state_in = dstate_out_dev;
-    rc = run_shared(ctx, s, r, sums, dk_dev, s.Dk, s.k_batch, s.k_token, s.k_head);
+    rc = run_shared(ctx, plan, r, sums, parts, dk_dev, s.Dk, s.k_batch, s.k_token, s.k_head);
     if (rc) return rc;
     // dv, and the gradient of the first state
     r.q = k; r.k = q; r.v = d;
     r.Dk = s.Dk; r.Dv = s.Dv;
     r.state_row = s.Dv; r.state_col = 1;
     r.state_out = dstate_in_dev;
-    return run_shared(ctx, s, r, sums, dv_dev, s.Dv, s.v_batch, s.v_token, s.v_head);
+    return run_shared(ctx, plan, r, sums, parts, dv_dev, s.Dv, s.v_batch, s.v_token, s.v_head);
 }

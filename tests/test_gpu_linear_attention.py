@@ -188,6 +188,28 @@ def test_a_prompt_in_two_parts_and_then_token_by_token(lib, dtype):
     lib.release(mark)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T", [9, 100])
+def test_a_later_token_reaches_no_earlier_one(lib, dtype, T):
+    """NaN or an infinity in a key or value changes no answer before its token, and no other head."""
+    mark = lib.mark()
+    want = Call(lib, 1, T, 2, 2, 40, 72, dtype, 21).forward()[0]
+    for t in (T // 2, T - 2):
+        for field, value in (("k", np.nan), ("v", np.nan), ("v", np.inf), ("q", np.inf)):
+            print("linear attention, not finite", dtype, T, t, field, value, flush=True)
+            c = Call(lib, 1, T, 2, 2, 40, 72, dtype, 21)
+            dev = getattr(c, field)
+            x = dev.values.copy()
+            x[0, t, 0, 3] = value
+            dev.__init__(lib, dev.shape, dtype, dev.strides, x)
+            got = c.forward()[0]
+            assert np.array_equal(got[0, :t], want[0, :t]) and np.array_equal(got[:, :, 1], want[:, :, 1])
+            assert not np.isfinite(got[0, t, 0]).all()
+            lib.release(mark)
+            mark = lib.mark()
+    lib.release(mark)
+
+
 def test_gradient_against_differences(lib):
     """Gradients along random directions against central differences of the recurrence in 64 bits."""
     mark = lib.mark()
@@ -223,6 +245,20 @@ def test_optional_states(lib):
         again = c.new("q", 2, 32), c.new("k", 2, 32), c.new("v", 2, 32)
         lib.linear_attention_backward(c.plan, c.do.ptr, c.q.ptr, c.k.ptr, c.v.ptr, c.gp, *(t.ptr for t in again), ws=c.ws)
         assert all(np.array_equal(a, b.get()) for a, b in zip((dq, dk, dv), again))
+    lib.release(mark)
+
+
+def test_long_memory_keeps_its_decay(lib):
+    """A decay's rounding must not build up over the tokens: a half-life of 7000 over 6000 of them, in fp32."""
+    mark = lib.mark()
+    T = 6000
+    c = Call(lib, 1, T, 1, 1, 16, 16, "f32", 8, decay=[-1e-4])
+    x = np.abs(c.k.values)      # of one sign, so that nothing cancels
+    c.k.__init__(lib, c.k.shape, "f32", None, x)
+    c.v.__init__(lib, c.v.shape, "f32", None, np.abs(c.v.values))
+    o, s = c.forward()
+    _, want = K.linear_attention(c.q.values, c.k.values, c.v.values, c.g, c.scale, c.state)
+    assert np.linalg.norm(s - want) <= 2e-6 * np.linalg.norm(want)
     lib.release(mark)
 
 
