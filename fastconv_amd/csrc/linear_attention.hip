@@ -7,7 +7,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
 constexpr long kMostSteps = 16;    // up to here the recurrence is faster
-constexpr long kWorkgroups = 512, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
+constexpr long kWavefronts = 2048, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kStepCols = 32;      // columns of the state that a workgroup of the recurrence holds
 
@@ -205,15 +205,17 @@ int run_step(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_ru
     return FC_OK;
 }
 
+// Four channels lie within one access, and a chunk's offsets within 31 bits.
 bool wide(const fc_la_operand &x, int D, size_t es) {
-    return ((D | x.batch | x.token | x.head) & 3) == 0 && ((uintptr_t)x.p & (4 * es - 1)) == 0;
+    return ((D | x.batch | x.token | x.head) & 3) == 0 && ((uintptr_t)x.p & (4 * es - 1)) == 0 && x.token < (1l << 31) / 4 / kChunk - 1024;
 }
 
 int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *parts) {
     const fc_linear_attention_shape &s = plan->shape;
     if (plan->chunk == 0) return run_step(ctx, s, r);
     const size_t es = fc_elem_size(s.dtype);
-    r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) && wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, es);
+    r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) && wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, es) &&
+             (!r.o32 || (long)r.H * r.Dv < (1l << 31) / 4 / kChunk - 1024);
     const long heads = (long)s.B * s.H, segment = segment_of(s, plan->segments);
     if (plan->segments > 1) {
         const int rc = s.dtype == FC_F32    ? fc_la_state_f32(ctx, r, heads, plan->segments, segment, parts)
@@ -264,8 +266,8 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
     plan->segments = 1;
     if (s->T > kMostSteps) {
         plan->chunk = kChunk;
-        const long slices = (most + 127) / 128, chunks = (s->T + kChunk - 1) / kChunk;
-        long segments = kWorkgroups / (s->B * (long)s->H * slices);
+        const long wavefronts = most <= 64 ? 2 : 4 * ((most + 127) / 128), chunks = (s->T + kChunk - 1) / kChunk;
+        long segments = kWavefronts / (s->B * (long)s->H * wavefronts);
         if (segments > chunks / kLeastChunks) segments = chunks / kLeastChunks;
         if (segments > 1) {
             const long per = (chunks + segments - 1) / segments;

@@ -21,12 +21,17 @@
 #include "linear_attention.h"
 
 constexpr int kLaChunk = 32;
+constexpr double kLaSettle = 1.0 / 65536;
+constexpr int kLaLoadsDone = 0x0f70;    // s_waitcnt: no load or store of global memory on its way
+constexpr int kLaOnlyVector = 0x6;      // scheduling: vector and scalar arithmetic may pass, memory and matrix instructions not
 
 typedef __bf16 la_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 la_bf16x4 __attribute__((ext_vector_type(4)));
 typedef float la_f32x16 __attribute__((ext_vector_type(16)));
 typedef float la_f32x4 __attribute__((ext_vector_type(4)));
-typedef float la_f32x8 __attribute__((ext_vector_type(8)));
+typedef float la_f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 la_bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t la_u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t la_u32x4 __attribute__((ext_vector_type(4)));
 
 // Sixteen depths of 32 rows, in LDS: UNITS 16-byte words a lane, and the products of two such operands.
@@ -57,18 +62,26 @@ struct la_math<FC_F32> {
     }
 };
 
-// PARTS parts of four values
+// PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.
 template <int PARTS>
-__device__ __forceinline__ void la_split(const float (&x)[4], la_bf16x4 (&out)[PARTS]) {
-    float r[4] = {x[0], x[1], x[2], x[3]};
+__device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[PARTS]) {
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
-        out[p] = __builtin_convertvector((la_f32x4){r[0], r[1], r[2], r[3]}, la_bf16x4);
+        out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((la_f32x2){a, b}, la_bf16x2));
         if (p + 1 < PARTS) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) r[i] -= (float)out[p][i];
+            a -= __builtin_bit_cast(float, out[p] << 16);
+            b -= __builtin_bit_cast(float, out[p] & 0xffff0000u);
         }
     }
+}
+// of four
+template <int PARTS>
+__device__ __forceinline__ void la_split(const float (&x)[4], la_bf16x4 (&out)[PARTS]) {
+    uint32_t lo[PARTS], hi[PARTS];
+    la_split_pair<PARTS>(x[0], x[1], lo);
+    la_split_pair<PARTS>(x[2], x[3], hi);
+#pragma unroll
+    for (int p = 0; p < PARTS; p++) out[p] = __builtin_bit_cast(la_bf16x4, (la_u32x2){lo[p], hi[p]});
 }
 template <int PARTS>
 __device__ __forceinline__ void la_split(const float (&x)[4], la_f32x4 (&out)[PARTS]) {
@@ -121,23 +134,53 @@ struct la_block {
     fc_vec<DT, 4> row[4];
 };
 
-// The rows of `n` that are there of four, from `src` on, `next` elements apart, of channels that are there below `channels`; zeros in
-// the place of the others.  WIDE: four channels are there or none is, and lie within one access.
+// Where a thread finds its four tokens of four channels in each chunk.
+// WIDE: four channels lie within one access.  Then a chunk is read through a buffer resource that begins at its first byte in memory (its
+// last token in a backward run); a lane whose token or channels do not exist reads past its end, which gives zeros.
 template <int DT, bool WIDE>
-__device__ __forceinline__ void la_load(la_block<DT> &b, const typename fc_elem<DT>::type *src, long next, int n, int channels) {
+struct la_source {
     typedef typename fc_elem<DT>::type E;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
+    static constexpr uint32_t NOWHERE = 0x80000000u;
+    const E *at;             // the first token of the four: of this thread, or if WIDE of the chunk, at its lowest address
+    long next;               // elements to the next token
+    uint32_t offset;
+    int token, channels;     // of the four in the chunk; that are there from the thread's first on
+
+    __device__ __forceinline__ void begin(const fc_la_operand &x, const fc_la_run &r, long b, int h, long first, int tq, int channel, int D) {
+        next = r.reverse ? -x.token : x.token;
+        token = 4 * tq;
+        channels = D - channel;
+        const E *head = (const E *)x.p + b * x.batch + (h / x.share) * x.head + first * x.token;
         if (WIDE) {
-            fc_vec<DT, 4> v = {};
-            if (i < n && channels > 0) v = *(const fc_vec<DT, 4> *)(src + i * next);
-            b.row[i] = v;
+            at = head + (r.reverse ? (kLaChunk - 1) * next : 0);
+            offset = channels > 0 ? (uint32_t)((r.reverse ? kLaChunk - 4 - token : token) * x.token + channel) * (uint32_t)sizeof(E) : NOWHERE;
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) b.row[i].v[e] = i < n && e < channels ? src[i * next + e] : (E)0.f;
+            at = head + token * next + channel;
+            offset = 0;
         }
     }
-}
+    // of a chunk of n tokens; moves on to the next one
+    __device__ __forceinline__ void load(la_block<DT> &b, int n) {
+        if (WIDE) {
+            const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<E *>(uniform_ptr(at)), 0, 0x7fffffff, 0x00020000);
+            const int step = __builtin_amdgcn_readfirstlane((int)(next * (long)sizeof(E))), lowest = step < 0 ? -3 * step : 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t there = n == kLaChunk || token + i < n ? offset : NOWHERE;
+                const int row = __builtin_amdgcn_readfirstlane(lowest + i * step);
+                if constexpr (DT == FC_F32) b.row[i] = __builtin_bit_cast(row_type, __builtin_amdgcn_raw_buffer_load_b128(res, there, row, 0));
+                else b.row[i] = __builtin_bit_cast(row_type, __builtin_amdgcn_raw_buffer_load_b64(res, there, row, 0));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) b.row[i].v[e] = token + i < n && e < channels ? at[i * next + e] : (E)0.f;
+        }
+        at += kLaChunk * next;
+    }
+    typedef fc_vec<DT, 4> row_type;
+};
 
 template <int DT, int PARTS>
 __device__ __forceinline__ void la_put(char *base, int plane, int at, const float (&x)[4]) {
@@ -162,13 +205,16 @@ __device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, typenam
 #pragma unroll
         for (int e = 0; e < 8; e++) f[0].half[e / 4][e % 4] = x[first + e];
     } else {
-        float r[8];
+        la_u32x4 w[2];
 #pragma unroll
-        for (int e = 0; e < 8; e++) r[e] = x[first + e];
-        f[0] = __builtin_convertvector((la_f32x8){r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]}, la_bf16x8);
-#pragma unroll
-        for (int e = 0; e < 8; e++) r[e] -= (float)f[0][e];
-        f[1] = __builtin_convertvector((la_f32x8){r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]}, la_bf16x8);
+        for (int i = 0; i < 4; i++) {
+            uint32_t two[2];
+            la_split_pair<2>(x[first + 2 * i], x[first + 2 * i + 1], two);
+            w[0][i] = two[0];
+            w[1][i] = two[1];
+        }
+        f[0] = __builtin_bit_cast(la_bf16x8, w[0]);
+        f[1] = __builtin_bit_cast(la_bf16x8, w[1]);
     }
 }
 
@@ -189,6 +235,9 @@ __device__ __forceinline__ uint32_t la_not_finite(const la_block<DT> &b) {
     return bad & carry;
 }
 
+// Tokens of the chunk that begins at p0.
+__device__ __forceinline__ int la_tokens(long p0, long end) { return (int)(end - p0 < kLaChunk ? end - p0 : kLaChunk); }
+
 // KT tiles of 32 rows of the state (rows past Dk are zeros), NW wavefronts of 32 columns.  FULL: answers tokens; otherwise only
 // forms the state that a segment adds.
 template <int DT, int KT, int NW, bool FULL, bool WIDE>
@@ -207,7 +256,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     int *const odd = (int *)(power + kLaChunk + 1);                 // whether a value of the chunk is not finite,
     int *const since = odd + 1;                                     // and from which token on, for each column
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5;
     unsigned block = blockIdx.x;
     const int slice = block % slices;
     block /= slices;
@@ -242,7 +291,9 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         }
         from = (float)exact[i_tok + 1 - r.reverse] * r.scale_out;
     }
-    double left = 1.0;      // what the roundings of the chunks' decays have left out so far
+    // The state is held as scale * S: what decays is the scale, one number, and what a chunk adds is divided by it, until it is small
+    // enough to be worth a pass over S.
+    double scale = 1.0;
 
     // the state: rows 32*t + 8*(e/4) + 4*g + e%4 of column col
     la_f32x16 S[KT];
@@ -256,48 +307,47 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
             S[t][e] = FULL && from_state && row < r.Dk && col < r.Dv ? from_state[row * srow + col * scol] : 0.f;
         }
 
-    // this thread's rows and channels of every operand, a chunk at a time
-    const long step = r.reverse ? -1 : 1, first = r.reverse ? len - 1 - begin : begin;
-    const E *qp[FULL ? QK_ITEMS : 1], *kp[QK_ITEMS], *vp[V_ITEMS];
-    int qk_tok[QK_ITEMS], v_tok[V_ITEMS], qk_channels[QK_ITEMS], v_channels[V_ITEMS];
+    // this thread's tokens and channels of every operand, a chunk at a time
+    const long first = r.reverse ? len - 1 - begin : begin;
+    la_source<DT, WIDE> q_from[FULL ? QK_ITEMS : 1], k_from[QK_ITEMS], v_from[V_ITEMS];
+    la_block<DT> q_in[FULL ? QK_ITEMS : 1], k_in[QK_ITEMS], v_in[V_ITEMS];
 #pragma unroll
     for (int it = 0; it < QK_ITEMS; it++) {
         const int item = tid + it * THREADS, tq = item / (DK / 4), cq = item - tq * (DK / 4);
-        qk_tok[it] = 4 * tq;
-        qk_channels[it] = r.Dk - 4 * cq;
-        if (FULL) qp[it] = (const E *)r.q.p + b * r.q.batch + (h / r.q.share) * r.q.head + (first + step * 4 * tq) * r.q.token + 4 * cq;
-        kp[it] = (const E *)r.k.p + b * r.k.batch + (h / r.k.share) * r.k.head + (first + step * 4 * tq) * r.k.token + 4 * cq;
+        if (FULL) q_from[it].begin(r.q, r, b, h, first, tq, 4 * cq, r.Dk);
+        k_from[it].begin(r.k, r, b, h, first, tq, 4 * cq, r.Dk);
     }
 #pragma unroll
     for (int it = 0; it < V_ITEMS; it++) {
         const int item = tid + it * THREADS, tq = item / (DV / 4), cq = item - tq * (DV / 4);
-        v_tok[it] = 4 * tq;
-        v_channels[it] = r.Dv - col0 - 4 * cq;
-        vp[it] = (const E *)r.v.p + b * r.v.batch + (h / r.v.share) * r.v.head + (first + step * 4 * tq) * r.v.token + col0 + 4 * cq;
+        v_from[it].begin(r.v, r, b, h, first, tq, col0 + 4 * cq, r.Dv);
     }
-    const long q_next = step * r.q.token, k_next = step * r.k.token, v_next = step * r.v.token;
-    la_block<DT> qb[FULL ? QK_ITEMS : 1], kb[QK_ITEMS], vb[V_ITEMS];
-    auto load = [&](long p0) {
-        const int n = (int)(end - p0 < kLaChunk ? end - p0 : kLaChunk);
+    // and the answers' place
+    const long o_size = r.o32 ? 4 : (long)sizeof(E), o_row = (r.o32 ? (long)r.H * r.Dv : r.o_token) * o_size;
+    const long o_step = r.reverse ? -kLaChunk * o_row : kLaChunk * o_row;
+    const uint32_t o_offset = (uint32_t)((r.reverse ? kLaChunk - 1 - i_tok : i_tok) * o_row + (32 * wave + 4 * g) * o_size);
+    char *o_at = (r.o32 ? (char *)(r.o32 + (b * r.T * r.H + h) * r.Dv + col0) : (char *)((E *)r.o + b * r.o_batch + h * r.o_head + col0)) +
+                 (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
+
+    auto load = [&](long p0) __attribute__((always_inline)) {
+        const int n = la_tokens(p0, end);
 #pragma unroll
         for (int it = 0; it < QK_ITEMS; it++) {
-            if (FULL) {
-                la_load<DT, WIDE>(qb[it], qp[it], q_next, n - qk_tok[it], qk_channels[it]);
-                qp[it] += kLaChunk * q_next;
-            }
-            la_load<DT, WIDE>(kb[it], kp[it], k_next, n - qk_tok[it], qk_channels[it]);
-            kp[it] += kLaChunk * k_next;
+            if (FULL) q_from[it].load(q_in[it], n);
+            k_from[it].load(k_in[it], n);
         }
 #pragma unroll
-        for (int it = 0; it < V_ITEMS; it++) {
-            la_load<DT, WIDE>(vb[it], vp[it], v_next, n - v_tok[it], v_channels[it]);
-            vp[it] += kLaChunk * v_next;
-        }
+        for (int it = 0; it < V_ITEMS; it++) v_from[it].load(v_in[it], n);
     };
-
-    if (begin < end) load(begin);
+    load(begin);
+    if (FULL) __builtin_amdgcn_s_waitcnt(kLaLoadsDone);
+#pragma unroll 1
     for (long p0 = begin; p0 < end; p0 += kLaChunk) {
-        const int n = (int)(end - p0 < kLaChunk ? end - p0 : kLaChunk);
+        const int n = la_tokens(p0, end);
+        const double decayed = scale * exact[n];
+        const bool settle = decayed < kLaSettle;
+        const double scale_next = settle ? 1.0 : decayed;
+        const float add = (float)(1.0 / scale_next), from_now = from * (float)scale;
         __syncthreads();      // the chunk before is read
 #pragma unroll
         for (int it = 0; it < QK_ITEMS; it++) {
@@ -307,25 +357,25 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int at = la_tile<DT>::natural(4 * tq + i, cq);
-                    la_put_raw<DT, M::PARTS>(qs, QK_PLANE, at, qb[it].row[i].v[0], qb[it].row[i].v[1], qb[it].row[i].v[2], qb[it].row[i].v[3]);
-                    la_put_raw<DT, M::PARTS>(ks, QK_PLANE, at, kb[it].row[i].v[0], kb[it].row[i].v[1], kb[it].row[i].v[2], kb[it].row[i].v[3]);
+                    la_put_raw<DT, M::PARTS>(qs, QK_PLANE, at, q_in[it].row[i].v[0], q_in[it].row[i].v[1], q_in[it].row[i].v[2], q_in[it].row[i].v[3]);
+                    la_put_raw<DT, M::PARTS>(ks, QK_PLANE, at, k_in[it].row[i].v[0], k_in[it].row[i].v[1], k_in[it].row[i].v[2], k_in[it].row[i].v[3]);
                 }
             }
             float w[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int d = n - 1 - 4 * tq - i + r.reverse;
-                w[i] = power[d < 0 ? 0 : d];      // rows past n are zeros
+                w[i] = power[d < 0 ? 0 : d] * add;      // tokens past n are zeros
             }
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 la_put<DT, M::KEPT>(kt, QK_PLANE, la_tile<DT>::turned(4 * cq + e, tq),
-                                    {kb[it].row[0].get(e) * w[0], kb[it].row[1].get(e) * w[1], kb[it].row[2].get(e) * w[2], kb[it].row[3].get(e) * w[3]});
+                                    {k_in[it].row[0].get(e) * w[0], k_in[it].row[1].get(e) * w[1], k_in[it].row[2].get(e) * w[2], k_in[it].row[3].get(e) * w[3]});
         }
 #pragma unroll
         for (int it = 0; it < V_ITEMS; it++) {
             const int item = tid + it * THREADS, tq = item / (DV / 4), cq = item - tq * (DV / 4);
-            if (FULL && la_not_finite<DT>(vb[it])) {
+            if (FULL && la_not_finite<DT>(v_in[it])) {
                 // A value that is not finite would meet the zeros of the tokens before it.  It is taken out here; its column
                 // is NaN from its token on.
                 *odd = 1;
@@ -333,120 +383,140 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                 for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float x = vb[it].row[i].get(e);
+                        const float x = v_in[it].row[i].get(e);
                         if (x - x == 0.f) continue;
                         atomicMin(&since[4 * cq + e], 4 * tq + i);
-                        vb[it].row[i].v[e] = (E)0.f;
+                        v_in[it].row[i].v[e] = (E)0.f;
                     }
             }
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                la_put_raw<DT, M::PARTS>(vt, V_PLANE, la_tile<DT>::turned(4 * cq + e, tq), vb[it].row[0].v[e], vb[it].row[1].v[e],
-                                         vb[it].row[2].v[e], vb[it].row[3].v[e]);
+                la_put_raw<DT, M::PARTS>(vt, V_PLANE, la_tile<DT>::turned(4 * cq + e, tq), v_in[it].row[0].v[e], v_in[it].row[1].v[e],
+                                         v_in[it].row[2].v[e], v_in[it].row[3].v[e]);
         }
         __syncthreads();
-        if (p0 + kLaChunk < end) load(p0 + kLaChunk);
+        load(p0 + kLaChunk);      // nothing past the last chunk
 
         frag vf[2][M::PARTS];
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int p = 0; p < M::PARTS; p++) la_tile<DT>::read_turned(vt + p * V_PLANE, wave, s, lane, vf[s][p]);
+        la_f32x16 P, O;
         if (FULL) {
-            la_f32x16 P, O;
 #pragma unroll
             for (int e = 0; e < 16; e++) P[e] = O[e] = 0.f;
-#pragma unroll
-            for (int s = 0; s < 2 * KT; s++) {
-                frag qf[M::PARTS], kf[M::PARTS], sf[M::FORMED];
+            frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
+            auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                 for (int p = 0; p < M::PARTS; p++) {
-                    la_tile<DT>::read_natural(qs + p * QK_PLANE, s, lane, qf[p]);
-                    la_tile<DT>::read_natural(ks + p * QK_PLANE, s, lane, kf[p]);
+                    la_tile<DT>::read_natural(qs + p * QK_PLANE, s, lane, qf[s & 1][p]);
+                    la_tile<DT>::read_natural(ks + p * QK_PLANE, s, lane, kf[s & 1][p]);
                 }
+            };
+            fetch(0);
+#pragma unroll
+            for (int s = 0; s < 2 * KT; s++) {
+                if (s + 1 < 2 * KT) fetch(s + 1);
+                __builtin_amdgcn_sched_barrier(kLaOnlyVector);      // reads ahead of the products that do not need them
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
                     for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 2) P = M::product(kf[a], qf[c], P);
+                        if (a + c < 2) P = M::product(kf[s & 1][a], qf[s & 1][c], P);
                 la_formed<DT>(S[s / 2], 8 * (s % 2), sf);
 #pragma unroll
                 for (int a = 0; a < M::FORMED; a++)
 #pragma unroll
                     for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 2) O = M::product(sf[a], qf[c], O);
+                        if (a + c < 2) O = M::product(sf[a], qf[s & 1][c], O);
+                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
             }
+        }
+        // the state takes the chunk in
+        if (settle) {
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) S[t][e] *= (float)decayed;
+        }
+        scale = scale_next;
+        {
+            frag kf[2][M::KEPT];
+            auto fetch = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int a = 0; a < M::KEPT; a++) la_tile<DT>::read_turned(kt + a * QK_PLANE, i / 2, i % 2, lane, kf[i & 1][a]);
+            };
+            fetch(0);
+#pragma unroll
+            for (int i = 0; i < 2 * KT; i++) {
+                if (i + 1 < 2 * KT) fetch(i + 1);
+                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
+#pragma unroll
+                for (int a = 0; a < M::KEPT; a++)
+#pragma unroll
+                    for (int c = 0; c < M::PARTS; c++)
+                        if (a + c < 3) S[i / 2] = M::product(kf[i & 1][a], vf[i % 2][c], S[i / 2]);
+                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
+            }
+        }
+        if (FULL) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                O[e] *= from;
+                O[e] *= from_now;
                 // a later token's zero leaves nothing of P, whatever that holds
                 asm("" : "+v"(near[e]));      // compared here: sixteen masks kept from chunk to chunk would not fit the scalar registers
                 P[e] = near[e] != 0.f ? P[e] * near[e] : 0.f;
             }
-            frag pf[2][M::FORMED];
 #pragma unroll
-            for (int s = 0; s < 2; s++) la_formed<DT>(P, 8 * s, pf[s]);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
+            for (int s = 0; s < 2; s++) {
+                frag pf[M::FORMED];
+                la_formed<DT>(P, 8 * s, pf);
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
                     for (int c = 0; c < M::FORMED; c++)
-                        if (a + c < 2) O = M::product(vf[s][a], pf[s][c], O);
+                        if (a + c < 2) O = M::product(vf[s][a], pf[c], O);
+            }
             if (*odd) {
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (i_tok >= since[32 * wave + 8 * (e / 4) + 4 * g + e % 4]) O[e] = __builtin_nanf("");
             }
+            // The next chunk has arrived by now; waited for here, before the answers leave, and not after, when the wait would be for them too.
+            __builtin_amdgcn_s_waitcnt(kLaLoadsDone);
             // lane: token i_tok, columns 8*(e/4) + 4*g + e%4 of the wavefront's 32
-            if (i_tok < n) {
-                const long t = r.reverse ? len - 1 - p0 - i_tok : p0 + i_tok;
+            if (WIDE) {
+                const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(o_at), 0, 0x7fffffff, 0x00020000);
+                uint32_t there[4];
 #pragma unroll
-                for (int a = 0; a < 4; a++) {
-                    const int c = col0 + 32 * wave + 8 * a + 4 * g;
-                    if (r.o32) {
-                        float *dst = r.o32 + ((b * r.T + t) * r.H + h) * r.Dv + c;
-                        if (WIDE && c < r.Dv) {
-                            *(float4 *)dst = make_float4(O[4 * a], O[4 * a + 1], O[4 * a + 2], O[4 * a + 3]);
-                        } else {
+                for (int a = 0; a < 4; a++)
+                    there[a] = i_tok < n && col0 + 32 * wave + 8 * a + 4 * g < r.Dv ? o_offset : la_source<DT, true>::NOWHERE;
+                if (DT == FC_F32 || r.o32) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (c + e < r.Dv) dst[e] = O[4 * a + e];
-                        }
-                    } else {
-                        E *dst = (E *)r.o + b * r.o_batch + t * r.o_token + h * r.o_head + c;
-                        if (WIDE && c < r.Dv) {
-                            fc_vec<DT, 4> x;
+                    for (int a = 0; a < 4; a++)
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, (la_f32x4){O[4 * a], O[4 * a + 1], O[4 * a + 2], O[4 * a + 3]}),
+                                                               res, there[a], 32 * a, 0);
+                } else if constexpr (DT != FC_F32) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) x.set(e, O[4 * a + e]);
-                            *(fc_vec<DT, 4> *)dst = x;
-                        } else {
+                    for (int a = 0; a < 4; a++) {
+                        fc_vec<DT, 4> x;
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (c + e < r.Dv) dst[e] = (E)O[4 * a + e];
-                        }
+                        for (int e = 0; e < 4; e++) x.set(e, O[4 * a + e]);
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(la_u32x2, x), res, there[a], 16 * a, 0);
                     }
                 }
-            }
-        }
-        // The decay of a chunk in fp32, rounded so that the product over the chunks keeps to the true power.
-        const double want = exact[n] * left;
-        const float decay = (float)want;
-        if (decay != 0.f) left = want / (double)decay;
+                o_at += o_step;
+            } else if (i_tok < n) {
+                const long t = r.reverse ? len - 1 - p0 - i_tok : p0 + i_tok;
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) S[t][e] *= decay;
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int a = 0; a < M::KEPT; a++) {
-                    frag kf;
-                    la_tile<DT>::read_turned(kt + a * QK_PLANE, t, s, lane, kf);
-#pragma unroll
-                    for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 3) S[t] = M::product(kf, vf[s][c], S[t]);
+                for (int e = 0; e < 16; e++) {
+                    const int c = col0 + 32 * wave + 8 * (e / 4) + 4 * g + e % 4;
+                    if (c >= r.Dv) continue;
+                    if (r.o32) r.o32[((b * r.T + t) * r.H + h) * r.Dv + c] = O[e];
+                    else ((E *)r.o)[b * r.o_batch + t * r.o_token + h * r.o_head + c] = (E)O[e];
                 }
+            }
         }
         if (FULL && *odd) {
             const bool lost = since[32 * wave + i_tok] < kLaChunk;
@@ -471,7 +541,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const int row = 32 * t + 8 * (e / 4) + 4 * g_out + e % 4;
-                if (row < r.Dk && col < r.Dv) to_state[row * orow + col * ocol] = S[t][e];
+                if (row < r.Dk && col < r.Dv) to_state[row * orow + col * ocol] = S[t][e] * (float)scale;
             }
     }
     if (!FULL) return;
