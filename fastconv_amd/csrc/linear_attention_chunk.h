@@ -62,15 +62,20 @@ struct la_math<FC_F32> {
     }
 };
 
-// PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.
+// PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  A value less its rounded
+// self is one instruction on the pair as it is packed, a - 1 * hi.lo + 0 * hi.hi, exact over the whole range of fp32 (an infinity in one makes
+// NaN of the other's second part: they are summed together anyway).  Bits that `keep` lacks are zeros in every part.
 template <int PARTS>
-__device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[PARTS]) {
+__device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[PARTS], uint32_t keep = ~0u) {
+    uint32_t low = 0x0000bf80u, high = 0xbf800000u;      // (-1, 0) and (0, -1)
+    asm("" : "+s"(low), "+s"(high));                     // from registers: as a literal the first stands for another pair
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
-        out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((la_f32x2){a, b}, la_bf16x2));
+        out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((la_f32x2){a, b}, la_bf16x2)) & keep;
         if (p + 1 < PARTS) {
-            a -= __builtin_bit_cast(float, out[p] << 16);
-            b -= __builtin_bit_cast(float, out[p] & 0xffff0000u);
+            const la_bf16x2 rounded = __builtin_bit_cast(la_bf16x2, out[p]);
+            a = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(la_bf16x2, low), a, false);
+            b = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(la_bf16x2, high), b, false);
         }
     }
 }
@@ -107,8 +112,8 @@ struct la_tile {
         return s * la_math<DT>::FRAG_BYTES + la_place<DT>(token, u, mix);
     }
     static __device__ __forceinline__ int turned(int channel, int quad) {     // quad: token / 4
-        const int td = channel >> 5;
-        return (td * 2 + (quad >> 2)) * la_math<DT>::FRAG_BYTES + la_place<DT>(channel & 31, quad & 3, td & 3);
+        const int td = channel >> 5, row = channel & 31;
+        return (td * 2 + (quad >> 2)) * la_math<DT>::FRAG_BYTES + la_place<DT>(row, quad & 3, (td & 1) | (row >> 4) << 1);
     }
     static __device__ __forceinline__ void read(const char *base, int lane, int mix0, int mix1, typename la_math<DT>::frag &f) {
         if constexpr (DT == FC_F32) {
@@ -124,9 +129,24 @@ struct la_tile {
         read(base + s * la_math<DT>::FRAG_BYTES, lane, m0, m1, f);
     }
     static __device__ __forceinline__ void read_turned(const char *base, int td, int s, int lane, typename la_math<DT>::frag &f) {
-        read(base + (td * 2 + s) * la_math<DT>::FRAG_BYTES, lane, td & 3, td & 3, f);
+        const int mix = (td & 1) | (lane >> 4 & 1) << 1;
+        read(base + (td * 2 + s) * la_math<DT>::FRAG_BYTES, lane, mix, mix, f);
     }
 };
+
+// Which four of a chunk's tokens and which four of D channels a thread has: sixteen threads side by side read 128 bytes of a token's channels,
+// the sixteen after them those of the token eight further on, which together meet every bank of LDS once when they write.
+// Threads past the last of a narrow operand have tokens past the chunk.
+template <int D>
+__device__ __forceinline__ int la_tokens_of(int item) {
+    if (D < 64 || item >= 2 * D) return item / (D / 4);
+    const int t = item >> 4 & 7;
+    return (t & 1) << 1 | (t >> 1 & 1) | (t & 4);
+}
+template <int D>
+__device__ __forceinline__ int la_channels_of(int item) {
+    return D < 64 ? item % (D / 4) : (item & 15) | item >> 7 << 4;
+}
 
 // Four tokens times four channels of an operand, on their way from global memory to LDS.
 template <int DT>
@@ -153,7 +173,7 @@ struct la_source {
         const E *head = (const E *)x.p + b * x.batch + (h / x.share) * x.head + first * x.token;
         if (WIDE) {
             at = head + (r.reverse ? (kLaChunk - 1) * next : 0);
-            offset = channels > 0 ? (uint32_t)((r.reverse ? kLaChunk - 4 - token : token) * x.token + channel) * (uint32_t)sizeof(E) : NOWHERE;
+            offset = channels > 0 && token < kLaChunk ? (uint32_t)((r.reverse ? kLaChunk - 4 - token : token) * x.token + channel) * (uint32_t)sizeof(E) : NOWHERE;
         } else {
             at = head + token * next + channel;
             offset = 0;
@@ -198,9 +218,10 @@ __device__ __forceinline__ void la_put_raw(char *base, int plane, int at, typena
     else *(typename la_math<DT>::quad *)(base + at) = (typename la_math<DT>::quad){a, b, c, d};
 }
 
-// Eight accumulators from `first` on as an operand.
+// Eight accumulators from `first` on as an operand; of 16-bit parts the bits that `keep` has, a word a pair.
 template <int DT>
-__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, typename la_math<DT>::frag (&f)[la_math<DT>::FORMED]) {
+__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, typename la_math<DT>::frag (&f)[la_math<DT>::FORMED],
+                                          const uint32_t *keep = nullptr) {
     if constexpr (DT == FC_F32) {
 #pragma unroll
         for (int e = 0; e < 8; e++) f[0].half[e / 4][e % 4] = x[first + e];
@@ -209,7 +230,7 @@ __device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, typenam
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             uint32_t two[2];
-            la_split_pair<2>(x[first + 2 * i], x[first + 2 * i + 1], two);
+            la_split_pair<2>(x[first + 2 * i], x[first + 2 * i + 1], two, keep ? keep[first / 2 + i] : ~0u);
             w[0][i] = two[0];
             w[1][i] = two[1];
         }
@@ -251,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     constexpr int QK_ITEMS = (8 * DK / 4 + THREADS - 1) / THREADS, V_ITEMS = 8 * DV / 4 / THREADS;
     extern __shared__ char lds[];
     char *const qs = lds, *const ks = qs + Q_BYTES, *const kt = ks + Q_BYTES, *const vt = kt + M::KEPT * QK_PLANE;
-    double *const exact = (double *)(vt + M::PARTS * V_PLANE);      // decay^0 .. decay^32
+    double *const exact = (double *)(vt + M::PARTS * V_PLANE + (FULL ? 0 : M::KEPT * QK_PLANE + M::PARTS * V_PLANE));      // decay^0 .. decay^32
     float *const power = (float *)(exact + kLaChunk + 1);           // the same, times what enters the state
     int *const odd = (int *)(power + kLaChunk + 1);                 // whether a value of the chunk is not finite,
     int *const since = odd + 1;                                     // and from which token on, for each column
@@ -282,12 +303,15 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     __syncthreads();
     // powers between two tokens of a chunk, zero towards an earlier one, and from the state to a token
     float near[16], from;
+    uint32_t earlier[8];
     const int i_tok = lane & 31;
     if (FULL) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const int d = i_tok - (8 * (e / 4) + 4 * g + e % 4);
             near[e] = d < 0 ? 0.f : power[d] * r.scale_out;
+            // A later token is left out of P by its bits, not multiplied by zero: it may hold anything.
+            if (e % 2 == 0) earlier[e / 2] = (d >= 0 ? 0x0000ffffu : 0u) | (d >= 1 ? 0xffff0000u : 0u);
         }
         from = (float)exact[i_tok + 1 - r.reverse] * r.scale_out;
     }
@@ -310,168 +334,271 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     // this thread's tokens and channels of every operand, a chunk at a time
     const long first = r.reverse ? len - 1 - begin : begin;
     la_source<DT, WIDE> q_from[FULL ? QK_ITEMS : 1], k_from[QK_ITEMS], v_from[V_ITEMS];
-    la_block<DT> q_in[FULL ? QK_ITEMS : 1], k_in[QK_ITEMS], v_in[V_ITEMS];
+    la_block<DT> q_in[FULL ? QK_ITEMS : 1], k_in[QK_ITEMS], k_now[QK_ITEMS], v_in[V_ITEMS];
 #pragma unroll
     for (int it = 0; it < QK_ITEMS; it++) {
-        const int item = tid + it * THREADS, tq = item / (DK / 4), cq = item - tq * (DK / 4);
+        const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
         if (FULL) q_from[it].begin(r.q, r, b, h, first, tq, 4 * cq, r.Dk);
         k_from[it].begin(r.k, r, b, h, first, tq, 4 * cq, r.Dk);
     }
 #pragma unroll
     for (int it = 0; it < V_ITEMS; it++) {
-        const int item = tid + it * THREADS, tq = item / (DV / 4), cq = item - tq * (DV / 4);
+        const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
         v_from[it].begin(r.v, r, b, h, first, tq, col0 + 4 * cq, r.Dv);
     }
-    // and the answers' place
-    const long o_size = r.o32 ? 4 : (long)sizeof(E), o_row = (r.o32 ? (long)r.H * r.Dv : r.o_token) * o_size;
-    const long o_step = r.reverse ? -kLaChunk * o_row : kLaChunk * o_row;
-    const uint32_t o_offset = (uint32_t)((r.reverse ? kLaChunk - 1 - i_tok : i_tok) * o_row + (32 * wave + 4 * g) * o_size);
-    char *o_at = (r.o32 ? (char *)(r.o32 + (b * r.T * r.H + h) * r.Dv + col0) : (char *)((E *)r.o + b * r.o_batch + h * r.o_head + col0)) +
-                 (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
-
-    auto load = [&](long p0) __attribute__((always_inline)) {
+    auto load_qk = [&](long p0) __attribute__((always_inline)) {
         const int n = la_tokens(p0, end);
 #pragma unroll
         for (int it = 0; it < QK_ITEMS; it++) {
             if (FULL) q_from[it].load(q_in[it], n);
             k_from[it].load(k_in[it], n);
         }
+    };
+    auto load_v = [&](long p0) __attribute__((always_inline)) {
+        const int n = la_tokens(p0, end);
 #pragma unroll
         for (int it = 0; it < V_ITEMS; it++) v_from[it].load(v_in[it], n);
     };
-    load(begin);
-    if (FULL) __builtin_amdgcn_s_waitcnt(kLaLoadsDone);
-#pragma unroll 1
-    for (long p0 = begin; p0 < end; p0 += kLaChunk) {
-        const int n = la_tokens(p0, end);
-        const double decayed = scale * exact[n];
-        const bool settle = decayed < kLaSettle;
-        const double scale_next = settle ? 1.0 : decayed;
-        const float add = (float)(1.0 / scale_next), from_now = from * (float)scale;
-        __syncthreads();      // the chunk before is read
+    // token i of four of q and k
+    auto put_natural = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int it = 0; it < QK_ITEMS; it++) {
-            const int item = tid + it * THREADS, tq = item / (DK / 4), cq = item - tq * (DK / 4);
-            if (tq >= 8) break;
-            if (FULL) {
+            const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
+            if (8 * DK / 4 < THREADS && tq >= 8) continue;
+            const int at = la_tile<DT>::natural(4 * tq + i, cq);
+            la_put_raw<DT, M::PARTS>(qs, QK_PLANE, at, q_in[it].row[i].v[0], q_in[it].row[i].v[1], q_in[it].row[i].v[2], q_in[it].row[i].v[3]);
+            la_put_raw<DT, M::PARTS>(ks, QK_PLANE, at, k_in[it].row[i].v[0], k_in[it].row[i].v[1], k_in[it].row[i].v[2], k_in[it].row[i].v[3]);
+        }
+    };
+    // channel e of four of what k adds to the state; w: what its four tokens are worth at the end of the chunk
+    float w[QK_ITEMS][4];
+    auto weigh = [&](int n, float add) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int at = la_tile<DT>::natural(4 * tq + i, cq);
-                    la_put_raw<DT, M::PARTS>(qs, QK_PLANE, at, q_in[it].row[i].v[0], q_in[it].row[i].v[1], q_in[it].row[i].v[2], q_in[it].row[i].v[3]);
-                    la_put_raw<DT, M::PARTS>(ks, QK_PLANE, at, k_in[it].row[i].v[0], k_in[it].row[i].v[1], k_in[it].row[i].v[2], k_in[it].row[i].v[3]);
-                }
-            }
-            float w[4];
+        for (int it = 0; it < QK_ITEMS; it++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int d = n - 1 - 4 * tq - i + r.reverse;
-                w[i] = power[d < 0 ? 0 : d] * add;      // tokens past n are zeros
+                const int d = n - 1 - 4 * la_tokens_of<DK>(tid + it * THREADS) - i + r.reverse;
+                w[it][i] = power[d < 0 ? 0 : d > kLaChunk ? kLaChunk : d] * add;      // tokens past n are zeros
             }
+    };
+    auto put_weighed = [&](char *to, int e) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                la_put<DT, M::KEPT>(kt, QK_PLANE, la_tile<DT>::turned(4 * cq + e, tq),
-                                    {k_in[it].row[0].get(e) * w[0], k_in[it].row[1].get(e) * w[1], k_in[it].row[2].get(e) * w[2], k_in[it].row[3].get(e) * w[3]});
+        for (int it = 0; it < QK_ITEMS; it++) {
+            const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
+            if (8 * DK / 4 < THREADS && tq >= 8) continue;
+            la_put<DT, M::KEPT>(to, QK_PLANE, la_tile<DT>::turned(4 * cq + e, tq),
+                                {k_now[it].row[0].get(e) * w[it][0], k_now[it].row[1].get(e) * w[it][1], k_now[it].row[2].get(e) * w[it][2],
+                                 k_now[it].row[3].get(e) * w[it][3]});
         }
+    };
+    // A value that is not finite would meet the zeros of the tokens before it.  It is taken out here; its column is NaN from its token on.
+    auto finite_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int it = 0; it < V_ITEMS; it++) {
-            const int item = tid + it * THREADS, tq = item / (DV / 4), cq = item - tq * (DV / 4);
-            if (FULL && la_not_finite<DT>(v_in[it])) {
-                // A value that is not finite would meet the zeros of the tokens before it.  It is taken out here; its column
-                // is NaN from its token on.
-                *odd = 1;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = v_in[it].row[i].get(e);
-                        if (x - x == 0.f) continue;
-                        atomicMin(&since[4 * cq + e], 4 * tq + i);
-                        v_in[it].row[i].v[e] = (E)0.f;
-                    }
-            }
+            if (!la_not_finite<DT>(v_in[it])) continue;
+            const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
+            *odd = 1;
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                la_put_raw<DT, M::PARTS>(vt, V_PLANE, la_tile<DT>::turned(4 * cq + e, tq), v_in[it].row[0].v[e], v_in[it].row[1].v[e],
-                                         v_in[it].row[2].v[e], v_in[it].row[3].v[e]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = v_in[it].row[i].get(e);
+                    if (x - x == 0.f) continue;
+                    atomicMin(&since[4 * cq + e], 4 * tq + i);
+                    v_in[it].row[i].v[e] = (E)0.f;
+                }
         }
-        __syncthreads();
-        load(p0 + kLaChunk);      // nothing past the last chunk
-
-        frag vf[2][M::PARTS];
+    };
+    // channel e of four of v
+    auto put_v = [&](char *to, int e) __attribute__((always_inline)) {
+#pragma unroll
+        for (int it = 0; it < V_ITEMS; it++) {
+            const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
+            la_put_raw<DT, M::PARTS>(to, V_PLANE, la_tile<DT>::turned(4 * cq + e, tq), v_in[it].row[0].v[e], v_in[it].row[1].v[e],
+                                     v_in[it].row[2].v[e], v_in[it].row[3].v[e]);
+        }
+    };
+    frag vf[2][M::PARTS];
+    auto read_v = [&](const char *from) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int p = 0; p < M::PARTS; p++) la_tile<DT>::read_turned(vt + p * V_PLANE, wave, s, lane, vf[s][p]);
-        la_f32x16 P, O;
-        if (FULL) {
+            for (int p = 0; p < M::PARTS; p++) la_tile<DT>::read_turned(from + p * V_PLANE, wave, s, lane, vf[s][p]);
+    };
+    // The state takes a chunk in; what(i) goes on meanwhile, in 2 * KT steps.
+    auto take_in = [&](const char *from, auto &&what) __attribute__((always_inline)) {
+        frag kf[2][M::KEPT];
+        auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) P[e] = O[e] = 0.f;
-            frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
-            auto fetch = [&](int s) __attribute__((always_inline)) {
+            for (int a = 0; a < M::KEPT; a++) la_tile<DT>::read_turned(from + a * QK_PLANE, i / 2, i % 2, lane, kf[i & 1][a]);
+        };
+        fetch(0);
 #pragma unroll
-                for (int p = 0; p < M::PARTS; p++) {
-                    la_tile<DT>::read_natural(qs + p * QK_PLANE, s, lane, qf[s & 1][p]);
-                    la_tile<DT>::read_natural(ks + p * QK_PLANE, s, lane, kf[s & 1][p]);
-                }
-            };
-            fetch(0);
+        for (int i = 0; i < 2 * KT; i++) {
+            if (i + 1 < 2 * KT) fetch(i + 1);
+            __builtin_amdgcn_sched_barrier(kLaOnlyVector);      // reads ahead of the products that do not need them
 #pragma unroll
-            for (int s = 0; s < 2 * KT; s++) {
-                if (s + 1 < 2 * KT) fetch(s + 1);
-                __builtin_amdgcn_sched_barrier(kLaOnlyVector);      // reads ahead of the products that do not need them
+            for (int a = 0; a < M::KEPT; a++)
 #pragma unroll
-                for (int a = 0; a < M::PARTS; a++)
-#pragma unroll
-                    for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 2) P = M::product(kf[s & 1][a], qf[s & 1][c], P);
-                la_formed<DT>(S[s / 2], 8 * (s % 2), sf);
-#pragma unroll
-                for (int a = 0; a < M::FORMED; a++)
-#pragma unroll
-                    for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 2) O = M::product(sf[a], qf[s & 1][c], O);
-                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
-            }
+                for (int c = 0; c < M::PARTS; c++)
+                    if (a + c < 3) S[i / 2] = M::product(kf[i & 1][a], vf[i % 2][c], S[i / 2]);
+            what(i);
+            __builtin_amdgcn_sched_barrier(kLaOnlyVector);
         }
-        // the state takes the chunk in
+    };
+    // What a chunk of n tokens does to the scale.
+    double decayed = 1.0;
+    bool settle = false;
+    float add = 1.f, from_now = 0.f;
+    auto rescale = [&](int n) __attribute__((always_inline)) {
+        from_now = from * (float)scale;
+        decayed = scale * exact[n];
+        settle = decayed < kLaSettle;
+        scale = settle ? 1.0 : decayed;
+        add = (float)(1.0 / scale);
+    };
+    auto settle_state = [&]() __attribute__((always_inline)) {
         if (settle) {
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) S[t][e] *= (float)decayed;
         }
-        scale = scale_next;
-        {
-            frag kf[2][M::KEPT];
-            auto fetch = [&](int i) __attribute__((always_inline)) {
+    };
+
+    if constexpr (!FULL) {
+        // One barrier a chunk: while the state takes in one, the next is laid out in the other half of LDS.
+        constexpr int HALF = M::KEPT * QK_PLANE + M::PARTS * V_PLANE;
+        char *const halves = kt;
+        int n = la_tokens(begin, end);
+        load_qk(begin);
+        load_v(begin);
+        rescale(n);
+        weigh(n, add);
 #pragma unroll
-                for (int a = 0; a < M::KEPT; a++) la_tile<DT>::read_turned(kt + a * QK_PLANE, i / 2, i % 2, lane, kf[i & 1][a]);
-            };
-            fetch(0);
+        for (int it = 0; it < QK_ITEMS; it++) k_now[it] = k_in[it];
 #pragma unroll
-            for (int i = 0; i < 2 * KT; i++) {
-                if (i + 1 < 2 * KT) fetch(i + 1);
-                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
-#pragma unroll
-                for (int a = 0; a < M::KEPT; a++)
-#pragma unroll
-                    for (int c = 0; c < M::PARTS; c++)
-                        if (a + c < 3) S[i / 2] = M::product(kf[i & 1][a], vf[i % 2][c], S[i / 2]);
-                __builtin_amdgcn_sched_barrier(kLaOnlyVector);
-            }
+        for (int e = 0; e < 4; e++) {
+            put_weighed(halves, e);
+            put_v(halves + M::KEPT * QK_PLANE, e);
         }
-        if (FULL) {
+        load_qk(begin + kLaChunk);
+        load_v(begin + kLaChunk);
+        bool settle_now = settle;
+        double decayed_now = decayed;
+        int half = 0;
+#pragma unroll 1
+        for (long p0 = begin; p0 < end; p0 += kLaChunk) {
+            __syncthreads();
+            const char *const now = halves + half * HALF;
+            half ^= 1;
+            char *const next = halves + half * HALF;
+            read_v(now + M::KEPT * QK_PLANE);
+            // the scale of this chunk, and then that of the next one
+            settle = settle_now;
+            decayed = decayed_now;
+            settle_state();
+            n = la_tokens(p0 + kLaChunk, end);
+            if (n > 0) {
+                rescale(n);
+                settle_now = settle;
+                decayed_now = decayed;
+                weigh(n, add);
+#pragma unroll
+                for (int it = 0; it < QK_ITEMS; it++) k_now[it] = k_in[it];
+            }
+            take_in(now, [&](int i) __attribute__((always_inline)) {
+                if (n > 0) {
+#pragma unroll
+                    for (int e = i * 4 / (2 * KT); e < (i + 1) * 4 / (2 * KT); e++) {
+                        put_weighed(next, e);
+                        put_v(next + M::KEPT * QK_PLANE, e);
+                    }
+                }
+            });
+            load_qk(p0 + 2 * kLaChunk);
+            load_v(p0 + 2 * kLaChunk);
+        }
+    } else {
+        // Two barriers a chunk.  Between the first and the second q and k are read, and what k adds and v are laid out for
+        // the state; after the second these are read, and the next chunk's q and k laid out.  So either half has work for the vector unit
+        // beside the matrix cores'.
+        const long o_size = r.o32 ? 4 : (long)sizeof(E), o_row = (r.o32 ? (long)r.H * r.Dv : r.o_token) * o_size;
+        const long o_step = r.reverse ? -kLaChunk * o_row : kLaChunk * o_row;
+        const uint32_t o_offset = (uint32_t)((r.reverse ? kLaChunk - 1 - i_tok : i_tok) * o_row + 32 * wave * o_size);
+        char *o_at = (r.o32 ? (char *)(r.o32 + (b * r.T * r.H + h) * r.Dv + col0) : (char *)((E *)r.o + b * r.o_batch + h * r.o_head + col0)) +
+                     (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
+        load_qk(begin);
+        load_v(begin);
+#pragma unroll
+        for (int i = 0; i < 4; i++) put_natural(i);
+#pragma unroll
+        for (int it = 0; it < QK_ITEMS; it++) k_now[it] = k_in[it];
+        load_qk(begin + kLaChunk);
+        __builtin_amdgcn_s_waitcnt(kLaLoadsDone);
+#pragma unroll 1
+        for (long p0 = begin; p0 < end; p0 += kLaChunk) {
+            const int n = la_tokens(p0, end);
+            rescale(n);
+            weigh(n, add);
+            __syncthreads();
+            la_f32x16 P, O;
+#pragma unroll
+            for (int e = 0; e < 16; e++) P[e] = O[e] = 0.f;
+            {
+                frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
+                auto fetch = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int p = 0; p < M::PARTS; p++) {
+                        la_tile<DT>::read_natural(qs + p * QK_PLANE, s, lane, qf[s & 1][p]);
+                        la_tile<DT>::read_natural(ks + p * QK_PLANE, s, lane, kf[s & 1][p]);
+                    }
+                };
+                finite_v();
+                fetch(0);
+#pragma unroll
+                for (int s = 0; s < 2 * KT; s++) {
+                    if (s + 1 < 2 * KT) fetch(s + 1);
+                    __builtin_amdgcn_sched_barrier(kLaOnlyVector);
+#pragma unroll
+                    for (int a = 0; a < M::PARTS; a++)
+#pragma unroll
+                        for (int c = 0; c < M::PARTS; c++)
+                            if (a + c < 2) P = M::product(kf[s & 1][a], qf[s & 1][c], P);
+                    la_formed<DT>(S[s / 2], 8 * (s % 2), sf);
+#pragma unroll
+                    for (int a = 0; a < M::FORMED; a++)
+#pragma unroll
+                        for (int c = 0; c < M::PARTS; c++)
+                            if (a + c < 2) O = M::product(sf[a], qf[s & 1][c], O);
+#pragma unroll
+                    for (int e = s * 4 / (2 * KT); e < (s + 1) * 4 / (2 * KT); e++) {
+                        put_weighed(kt, e);
+                        put_v(vt, e);
+                    }
+                    __builtin_amdgcn_sched_barrier(kLaOnlyVector);
+                }
+            }
+            load_v(p0 + kLaChunk);      // nothing past the last chunk
+            __syncthreads();
+            read_v(vt);
+            settle_state();
+            take_in(kt, [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = i * 4 / (2 * KT); e < (i + 1) * 4 / (2 * KT); e++) put_natural(e);
+            });
+#pragma unroll
+            for (int it = 0; it < QK_ITEMS; it++) k_now[it] = k_in[it];
+            load_qk(p0 + 2 * kLaChunk);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 O[e] *= from_now;
-                // a later token's zero leaves nothing of P, whatever that holds
-                asm("" : "+v"(near[e]));      // compared here: sixteen masks kept from chunk to chunk would not fit the scalar registers
-                P[e] = near[e] != 0.f ? P[e] * near[e] : 0.f;
+                P[e] = DT == FC_F32 && near[e] == 0.f ? 0.f : P[e] * near[e];
             }
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 frag pf[M::FORMED];
-                la_formed<DT>(P, 8 * s, pf);
+                la_formed<DT>(P, 8 * s, pf, earlier);
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
@@ -479,31 +606,51 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                         if (a + c < 2) O = M::product(vf[s][a], pf[c], O);
             }
             if (*odd) {
+                const bool lost = since[32 * wave + i_tok] < kLaChunk;
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) S[t][e] = lost ? __builtin_nanf("") : S[t][e];
 #pragma unroll
                 for (int e = 0; e < 16; e++)
                     if (i_tok >= since[32 * wave + 8 * (e / 4) + 4 * g + e % 4]) O[e] = __builtin_nanf("");
+                __syncthreads();
+                if (tid == 0) *odd = 0;
+                for (int c = tid; c < DV; c += THREADS) since[c] = kLaChunk;
             }
-            // The next chunk has arrived by now; waited for here, before the answers leave, and not after, when the wait would be for them too.
-            __builtin_amdgcn_s_waitcnt(kLaLoadsDone);
             // lane: token i_tok, columns 8*(e/4) + 4*g + e%4 of the wavefront's 32
             if (WIDE) {
                 const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(o_at), 0, 0x7fffffff, 0x00020000);
-                uint32_t there[4];
-#pragma unroll
-                for (int a = 0; a < 4; a++)
-                    there[a] = i_tok < n && col0 + 32 * wave + 8 * a + 4 * g < r.Dv ? o_offset : la_source<DT, true>::NOWHERE;
+                const int c = col0 + 32 * wave;
+                const uint32_t nowhere = la_source<DT, true>::NOWHERE;
                 if (DT == FC_F32 || r.o32) {
 #pragma unroll
                     for (int a = 0; a < 4; a++)
                         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, (la_f32x4){O[4 * a], O[4 * a + 1], O[4 * a + 2], O[4 * a + 3]}),
-                                                               res, there[a], 32 * a, 0);
+                                                               res, i_tok < n && c + 8 * a + 4 * g < r.Dv ? o_offset + 16 * g : nowhere, 32 * a, 0);
                 } else if constexpr (DT != FC_F32) {
+                    // 16 bytes of a token a lane: the lower half of the wavefront takes columns 0 and 8 on from both, the upper
+                    // half 16 and 24 on
+                    la_u32x2 x[4];
 #pragma unroll
                     for (int a = 0; a < 4; a++) {
-                        fc_vec<DT, 4> x;
+                        fc_vec<DT, 4> y;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x.set(e, O[4 * a + e]);
-                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(la_u32x2, x), res, there[a], 16 * a, 0);
+                        for (int e = 0; e < 4; e++) y.set(e, O[4 * a + e]);
+                        x[a] = __builtin_bit_cast(la_u32x2, y);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 2; a++) {
+                        const auto first = __builtin_amdgcn_permlane32_swap(x[a][0], x[a + 2][0], false, false);
+                        const auto second = __builtin_amdgcn_permlane32_swap(x[a][1], x[a + 2][1], false, false);
+                        const int from = c + 8 * a + 16 * g;
+                        const uint32_t there = i_tok < n && from < r.Dv ? o_offset + 32 * g : nowhere;
+                        if (r.Dv % 8 == 0)
+                            __builtin_amdgcn_raw_buffer_store_b128((la_u32x4){first[0], second[0], first[1], second[1]}, res, there, 16 * a, 0);
+                        else {      // four columns at the end
+                            __builtin_amdgcn_raw_buffer_store_b64((la_u32x2){first[0], second[0]}, res, there, 16 * a, 0);
+                            __builtin_amdgcn_raw_buffer_store_b64((la_u32x2){first[1], second[1]}, res, from + 4 < r.Dv ? there : nowhere, 16 * a + 8, 0);
+                        }
                     }
                 }
                 o_at += o_step;
@@ -517,16 +664,6 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                     else ((E *)r.o)[b * r.o_batch + t * r.o_token + h * r.o_head + c] = (E)O[e];
                 }
             }
-        }
-        if (FULL && *odd) {
-            const bool lost = since[32 * wave + i_tok] < kLaChunk;
-#pragma unroll
-            for (int t = 0; t < KT; t++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) S[t][e] = lost ? __builtin_nanf("") : S[t][e];
-            __syncthreads();
-            if (tid == 0) *odd = 0;
-            for (int c = tid; c < DV; c += THREADS) since[c] = kLaChunk;
         }
     }
 
@@ -561,7 +698,8 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 template <int DT, int KT, int NW>
 constexpr size_t la_lds_bytes(bool full) {
     typedef la_math<DT> M;
-    return (size_t)2 * KT * M::FRAG_BYTES * ((full ? 2 * M::PARTS : 0) + M::KEPT) + (size_t)2 * NW * M::FRAG_BYTES * M::PARTS + (kLaChunk + 1) * (sizeof(double) + sizeof(float)) + (1 + 32 * NW) * sizeof(int);
+    const size_t qk = (size_t)2 * KT * M::FRAG_BYTES, v = (size_t)2 * NW * M::FRAG_BYTES;
+    return (full ? 2 * M::PARTS * qk : M::KEPT * qk + M::PARTS * v) + M::KEPT * qk + M::PARTS * v + (kLaChunk + 1) * (sizeof(double) + sizeof(float)) + (1 + 32 * NW) * sizeof(int);
 }
 
 // More LDS than 64 KB has to be asked for, once for each kernel and device.
