@@ -11,9 +11,9 @@
 // All operands lie in LDS in that order, 16 bytes a lane, so that a wavefront reads 1 KB in a row.
 //
 // Roundings.  A matrix core multiplies bf16 (8 bits) and adds in fp32.  Inputs are split into as many bf16 parts as they have bits
-// for: bf16 one, half two, exactly.  What is formed between two products, P and S, goes in as two parts (16 bits, against the 8 or
-// 11 of the output); l^n k, which is summed into the state, as three (24 bits: states are fp32).  Parts whose product is below the last
-// one kept are left out.  fp32 runs on fp32 matrix instructions, one part each.
+// for: bf16 one, half two, fp32 three, exactly.  What is formed between two products, P and S, goes in as two parts for the 16-bit types
+// (16 bits, against the 8 or 11 of the output) and as three for fp32; l^n k, which is summed into the state, as three (24 bits:
+// states are fp32).  Products of parts below the last bits that are kept are left out.
 #pragma once
 
 #include <atomic>
@@ -34,33 +34,18 @@ typedef __bf16 la_bf16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t la_u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t la_u32x4 __attribute__((ext_vector_type(4)));
 
-// Sixteen depths of 32 rows, in LDS: UNITS 16-byte words a lane, and the products of two such operands.
+// Operands as bf16 parts.  PARTS: of the inputs; FORMED: of what is formed between two products; KEPT: of what enters the state.
+// Products of parts that together come ORDER or more parts late are left out (of those into the state, KEPT).
+typedef la_bf16x8 la_frag;      // sixteen depths of 32 rows
+typedef la_bf16x4 la_quad;      // four depths of a row, of four
+constexpr int kLaFrag = 1024;   // bytes
 template <int DT>
 struct la_math {
-    typedef __bf16 unit;
-    typedef la_bf16x8 frag;
-    typedef la_bf16x4 quad;      // four consecutive depths
-    static constexpr int PARTS = DT == FC_F16 ? 2 : 1, FORMED = 2, KEPT = 3;
-    static constexpr int FRAG_BYTES = 1024;
-    static __device__ __forceinline__ la_f32x16 product(const frag &a, const frag &b, la_f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
+    static constexpr int PARTS = DT == FC_F32 ? 3 : DT == FC_F16 ? 2 : 1, FORMED = DT == FC_F32 ? 3 : 2, KEPT = 3, ORDER = FORMED;
 };
-template <>
-struct la_math<FC_F32> {
-    typedef float unit;
-    struct frag {
-        la_f32x4 half[2];
-    };
-    typedef la_f32x4 quad;
-    static constexpr int PARTS = 1, FORMED = 1, KEPT = 1;
-    static constexpr int FRAG_BYTES = 2048;
-    static __device__ __forceinline__ la_f32x16 product(const frag &a, const frag &b, la_f32x16 c) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.half[e / 4][e % 4], b.half[e / 4][e % 4], c, 0, 0, 0);
-        return c;
-    }
-};
+__device__ __forceinline__ la_f32x16 la_product(const la_frag &a, const la_frag &b, la_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 
 // PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  A value less its rounded
 // self is one instruction on the pair as it is packed, a - 1 * hi.lo + 0 * hi.hi, exact over the whole range of fp32 (an infinity in one makes
@@ -88,51 +73,29 @@ __device__ __forceinline__ void la_split(const float (&x)[4], la_bf16x4 (&out)[P
 #pragma unroll
     for (int p = 0; p < PARTS; p++) out[p] = __builtin_bit_cast(la_bf16x4, (la_u32x2){lo[p], hi[p]});
 }
-template <int PARTS>
-__device__ __forceinline__ void la_split(const float (&x)[4], la_f32x4 (&out)[PARTS]) {
-    out[0] = (la_f32x4){x[0], x[1], x[2], x[3]};
-}
 
-// Byte offset of four consecutive depths (quad u of four in sixteen) of a row in a fragment.  The row's place is mixed with
-// `mix` so that lanes that write the same row of many fragments, or every fourth row, meet different banks; a wavefront that
-// reads a fragment reads all of its places whatever the mix.
-template <int DT>
-__device__ __forceinline__ int la_place(int row, int u, int mix) {
-    const int g = u & 1, half = u >> 1, slot = g * 32 + (row ^ mix);
-    return DT == FC_F32 ? half * 1024 + slot * 16 : slot * 16 + half * 8;
-}
+// Byte offset of quad u of a row in a fragment.  The row's place is mixed with `mix` so that threads that write at once meet different banks;
+// a wavefront that reads a fragment reads all of its places whatever the mix.
+__device__ __forceinline__ int la_place(int row, int u, int mix) { return ((u & 1) * 32 + (row ^ mix)) * 16 + (u >> 1) * 8; }
 
-// Fragments of an operand: PARTS planes of `frags`.
 // natural: row = token, sixteen channels a fragment.  turned: row = channel of 32, sixteen tokens a fragment.
-template <int DT>
-struct la_tile {
-    static __device__ __forceinline__ int natural(int token, int quad) {      // quad: channel / 4
-        const int s = quad >> 2, u = quad & 3;
-        const int mix = DT == FC_F32 ? (4 * s + u) & 15 : (2 * s + (u & 1)) & 15;
-        return s * la_math<DT>::FRAG_BYTES + la_place<DT>(token, u, mix);
-    }
-    static __device__ __forceinline__ int turned(int channel, int quad) {     // quad: token / 4
-        const int td = channel >> 5, row = channel & 31;
-        return (td * 2 + (quad >> 2)) * la_math<DT>::FRAG_BYTES + la_place<DT>(row, quad & 3, (td & 1) | (row >> 4) << 1);
-    }
-    static __device__ __forceinline__ void read(const char *base, int lane, int mix0, int mix1, typename la_math<DT>::frag &f) {
-        if constexpr (DT == FC_F32) {
-            f.half[0] = *(const la_f32x4 *)(base + ((lane & 32) + ((lane & 31) ^ mix0)) * 16);
-            f.half[1] = *(const la_f32x4 *)(base + 1024 + ((lane & 32) + ((lane & 31) ^ mix1)) * 16);
-        } else {
-            f = *(const la_bf16x8 *)(base + ((lane & 32) + ((lane & 31) ^ mix0)) * 16);
-        }
-    }
-    static __device__ __forceinline__ void read_natural(const char *base, int s, int lane, typename la_math<DT>::frag &f) {
-        const int g = lane >> 5;
-        const int m0 = DT == FC_F32 ? (4 * s + g) & 15 : (2 * s + g) & 15, m1 = (4 * s + 2 + g) & 15;
-        read(base + s * la_math<DT>::FRAG_BYTES, lane, m0, m1, f);
-    }
-    static __device__ __forceinline__ void read_turned(const char *base, int td, int s, int lane, typename la_math<DT>::frag &f) {
-        const int mix = (td & 1) | (lane >> 4 & 1) << 1;
-        read(base + (td * 2 + s) * la_math<DT>::FRAG_BYTES, lane, mix, mix, f);
-    }
-};
+__device__ __forceinline__ int la_natural(int token, int quad) {      // quad: channel / 4
+    const int s = quad >> 2, u = quad & 3;
+    return s * kLaFrag + la_place(token, u, (2 * s + (u & 1)) & 15);
+}
+__device__ __forceinline__ int la_turned(int channel, int quad) {     // quad: token / 4
+    const int td = channel >> 5, row = channel & 31;
+    return (td * 2 + (quad >> 2)) * kLaFrag + la_place(row, quad & 3, (td & 1) | (row >> 4) << 1);
+}
+__device__ __forceinline__ la_frag la_read(const char *frag, int lane, int mix) {
+    return *(const la_frag *)(frag + ((lane & 32) + ((lane & 31) ^ mix)) * 16);
+}
+__device__ __forceinline__ la_frag la_read_natural(const char *base, int s, int lane) {
+    return la_read(base + s * kLaFrag, lane, (2 * s + (lane >> 5)) & 15);
+}
+__device__ __forceinline__ la_frag la_read_turned(const char *base, int td, int s, int lane) {
+    return la_read(base + (td * 2 + s) * kLaFrag, lane, (td & 1) | (lane >> 4 & 1) << 1);
+}
 
 // Which four of a chunk's tokens and which four of D channels a thread has: sixteen threads side by side read 128 bytes of a token's channels,
 // the sixteen after them those of the token eight further on, which together meet every bank of LDS once when they write.
@@ -202,41 +165,34 @@ struct la_source {
     typedef fc_vec<DT, 4> row_type;
 };
 
-template <int DT, int PARTS>
+template <int PARTS>
 __device__ __forceinline__ void la_put(char *base, int plane, int at, const float (&x)[4]) {
-    typename la_math<DT>::quad q[PARTS];
+    la_quad q[PARTS];
     la_split<PARTS>(x, q);
 #pragma unroll
-    for (int p = 0; p < PARTS; p++) *(typename la_math<DT>::quad *)(base + p * plane + at) = q[p];
+    for (int p = 0; p < PARTS; p++) *(la_quad *)(base + p * plane + at) = q[p];
 }
-
-// Four values as they lie in memory, or split.
-template <int DT, int PARTS>
+// Four inputs: bf16 as they lie in memory, others split.
+template <int DT>
 __device__ __forceinline__ void la_put_raw(char *base, int plane, int at, typename fc_elem<DT>::type a, typename fc_elem<DT>::type b,
                                            typename fc_elem<DT>::type c, typename fc_elem<DT>::type d) {
-    if constexpr (DT == FC_F16) la_put<DT, PARTS>(base, plane, at, {(float)a, (float)b, (float)c, (float)d});
-    else *(typename la_math<DT>::quad *)(base + at) = (typename la_math<DT>::quad){a, b, c, d};
+    if constexpr (DT == FC_BF16) *(la_quad *)(base + at) = (la_quad){a, b, c, d};
+    else la_put<la_math<DT>::PARTS>(base, plane, at, {(float)a, (float)b, (float)c, (float)d});
 }
 
-// Eight accumulators from `first` on as an operand; of 16-bit parts the bits that `keep` has, a word a pair.
-template <int DT>
-__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, typename la_math<DT>::frag (&f)[la_math<DT>::FORMED],
-                                          const uint32_t *keep = nullptr) {
-    if constexpr (DT == FC_F32) {
+// Eight accumulators from `first` on as an operand; of each part the bits that `keep` has, a word a pair.
+template <int FORMED>
+__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, la_frag (&f)[FORMED], const uint32_t *keep = nullptr) {
+    la_u32x4 w[FORMED];
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[0].half[e / 4][e % 4] = x[first + e];
-    } else {
-        la_u32x4 w[2];
+    for (int i = 0; i < 4; i++) {
+        uint32_t two[FORMED];
+        la_split_pair<FORMED>(x[first + 2 * i], x[first + 2 * i + 1], two, keep ? keep[first / 2 + i] : ~0u);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t two[2];
-            la_split_pair<2>(x[first + 2 * i], x[first + 2 * i + 1], two, keep ? keep[first / 2 + i] : ~0u);
-            w[0][i] = two[0];
-            w[1][i] = two[1];
-        }
-        f[0] = __builtin_bit_cast(la_bf16x8, w[0]);
-        f[1] = __builtin_bit_cast(la_bf16x8, w[1]);
+        for (int p = 0; p < FORMED; p++) w[p][i] = two[p];
     }
+#pragma unroll
+    for (int p = 0; p < FORMED; p++) f[p] = __builtin_bit_cast(la_frag, w[p]);
 }
 
 // Not 0 if any element of a block is an infinity or NaN: all exponent bits set, which one more in the last of them carries over.
@@ -264,10 +220,9 @@ __device__ __forceinline__ int la_tokens(long p0, long end) { return (int)(end -
 template <int DT, int KT, int NW, bool FULL, bool WIDE>
 __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_chunk_kernel(const fc_la_run r, int segments, long segment, int slices, float *parts) {
     typedef la_math<DT> M;
-    typedef typename M::frag frag;
     typedef typename fc_elem<DT>::type E;
     constexpr int THREADS = 64 * NW, DK = 32 * KT, DV = 32 * NW;
-    constexpr int QK_PLANE = 2 * KT * M::FRAG_BYTES, V_PLANE = 2 * NW * M::FRAG_BYTES;
+    constexpr int QK_PLANE = 2 * KT * kLaFrag, V_PLANE = 2 * NW * kLaFrag;
     constexpr int Q_BYTES = FULL ? M::PARTS * QK_PLANE : 0;
     constexpr int QK_ITEMS = (8 * DK / 4 + THREADS - 1) / THREADS, V_ITEMS = 8 * DV / 4 / THREADS;
     extern __shared__ char lds[];
@@ -365,9 +320,9 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         for (int it = 0; it < QK_ITEMS; it++) {
             const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
             if (8 * DK / 4 < THREADS && tq >= 8) continue;
-            const int at = la_tile<DT>::natural(4 * tq + i, cq);
-            la_put_raw<DT, M::PARTS>(qs, QK_PLANE, at, q_in[it].row[i].v[0], q_in[it].row[i].v[1], q_in[it].row[i].v[2], q_in[it].row[i].v[3]);
-            la_put_raw<DT, M::PARTS>(ks, QK_PLANE, at, k_in[it].row[i].v[0], k_in[it].row[i].v[1], k_in[it].row[i].v[2], k_in[it].row[i].v[3]);
+            const int at = la_natural(4 * tq + i, cq);
+            la_put_raw<DT>(qs, QK_PLANE, at, q_in[it].row[i].v[0], q_in[it].row[i].v[1], q_in[it].row[i].v[2], q_in[it].row[i].v[3]);
+            la_put_raw<DT>(ks, QK_PLANE, at, k_in[it].row[i].v[0], k_in[it].row[i].v[1], k_in[it].row[i].v[2], k_in[it].row[i].v[3]);
         }
     };
     // channel e of four of what k adds to the state; w: what its four tokens are worth at the end of the chunk
@@ -386,7 +341,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         for (int it = 0; it < QK_ITEMS; it++) {
             const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
             if (8 * DK / 4 < THREADS && tq >= 8) continue;
-            la_put<DT, M::KEPT>(to, QK_PLANE, la_tile<DT>::turned(4 * cq + e, tq),
+            la_put<M::KEPT>(to, QK_PLANE, la_turned(4 * cq + e, tq),
                                 {k_now[it].row[0].get(e) * w[it][0], k_now[it].row[1].get(e) * w[it][1], k_now[it].row[2].get(e) * w[it][2],
                                  k_now[it].row[3].get(e) * w[it][3]});
         }
@@ -414,23 +369,23 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 #pragma unroll
         for (int it = 0; it < V_ITEMS; it++) {
             const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
-            la_put_raw<DT, M::PARTS>(to, V_PLANE, la_tile<DT>::turned(4 * cq + e, tq), v_in[it].row[0].v[e], v_in[it].row[1].v[e],
+            la_put_raw<DT>(to, V_PLANE, la_turned(4 * cq + e, tq), v_in[it].row[0].v[e], v_in[it].row[1].v[e],
                                      v_in[it].row[2].v[e], v_in[it].row[3].v[e]);
         }
     };
-    frag vf[2][M::PARTS];
+    la_frag vf[2][M::PARTS];
     auto read_v = [&](const char *from) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int p = 0; p < M::PARTS; p++) la_tile<DT>::read_turned(from + p * V_PLANE, wave, s, lane, vf[s][p]);
+            for (int p = 0; p < M::PARTS; p++) vf[s][p] = la_read_turned(from + p * V_PLANE, wave, s, lane);
     };
     // The state takes a chunk in; what(i) goes on meanwhile, in 2 * KT steps.
     auto take_in = [&](const char *from, auto &&what) __attribute__((always_inline)) {
-        frag kf[2][M::KEPT];
+        la_frag kf[2][M::KEPT];
         auto fetch = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int a = 0; a < M::KEPT; a++) la_tile<DT>::read_turned(from + a * QK_PLANE, i / 2, i % 2, lane, kf[i & 1][a]);
+            for (int a = 0; a < M::KEPT; a++) kf[i & 1][a] = la_read_turned(from + a * QK_PLANE, i / 2, i % 2, lane);
         };
         fetch(0);
 #pragma unroll
@@ -441,7 +396,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
             for (int a = 0; a < M::KEPT; a++)
 #pragma unroll
                 for (int c = 0; c < M::PARTS; c++)
-                    if (a + c < 3) S[i / 2] = M::product(kf[i & 1][a], vf[i % 2][c], S[i / 2]);
+                    if (a + c < M::KEPT) S[i / 2] = la_product(kf[i & 1][a], vf[i % 2][c], S[i / 2]);
             what(i);
             __builtin_amdgcn_sched_barrier(kLaOnlyVector);
         }
@@ -546,12 +501,12 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 #pragma unroll
             for (int e = 0; e < 16; e++) P[e] = O[e] = 0.f;
             {
-                frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
+                la_frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
                 auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                     for (int p = 0; p < M::PARTS; p++) {
-                        la_tile<DT>::read_natural(qs + p * QK_PLANE, s, lane, qf[s & 1][p]);
-                        la_tile<DT>::read_natural(ks + p * QK_PLANE, s, lane, kf[s & 1][p]);
+                        qf[s & 1][p] = la_read_natural(qs + p * QK_PLANE, s, lane);
+                        kf[s & 1][p] = la_read_natural(ks + p * QK_PLANE, s, lane);
                     }
                 };
                 finite_v();
@@ -564,13 +519,13 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                     for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
                         for (int c = 0; c < M::PARTS; c++)
-                            if (a + c < 2) P = M::product(kf[s & 1][a], qf[s & 1][c], P);
-                    la_formed<DT>(S[s / 2], 8 * (s % 2), sf);
+                            if (a + c < M::ORDER) P = la_product(kf[s & 1][a], qf[s & 1][c], P);
+                    la_formed<M::FORMED>(S[s / 2], 8 * (s % 2), sf);
 #pragma unroll
                     for (int a = 0; a < M::FORMED; a++)
 #pragma unroll
                         for (int c = 0; c < M::PARTS; c++)
-                            if (a + c < 2) O = M::product(sf[a], qf[s & 1][c], O);
+                            if (a + c < M::ORDER) O = la_product(sf[a], qf[s & 1][c], O);
 #pragma unroll
                     for (int e = s * 4 / (2 * KT); e < (s + 1) * 4 / (2 * KT); e++) {
                         put_weighed(kt, e);
@@ -593,17 +548,17 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 O[e] *= from_now;
-                P[e] = DT == FC_F32 && near[e] == 0.f ? 0.f : P[e] * near[e];
+                P[e] *= near[e];
             }
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                frag pf[M::FORMED];
-                la_formed<DT>(P, 8 * s, pf, earlier);
+                la_frag pf[M::FORMED];
+                la_formed<M::FORMED>(P, 8 * s, pf, earlier);
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
                     for (int c = 0; c < M::FORMED; c++)
-                        if (a + c < 2) O = M::product(vf[s][a], pf[c], O);
+                        if (a + c < M::ORDER) O = la_product(vf[s][a], pf[c], O);
             }
             if (*odd) {
                 const bool lost = since[32 * wave + i_tok] < kLaChunk;
@@ -698,7 +653,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 template <int DT, int KT, int NW>
 constexpr size_t la_lds_bytes(bool full) {
     typedef la_math<DT> M;
-    const size_t qk = (size_t)2 * KT * M::FRAG_BYTES, v = (size_t)2 * NW * M::FRAG_BYTES;
+    const size_t qk = (size_t)2 * KT * kLaFrag, v = (size_t)2 * NW * kLaFrag;
     return (full ? 2 * M::PARTS * qk : M::KEPT * qk + M::PARTS * v) + M::KEPT * qk + M::PARTS * v + (kLaChunk + 1) * (sizeof(double) + sizeof(float)) + (1 + 32 * NW) * sizeof(int);
 }
 
@@ -728,15 +683,16 @@ int la_launch_one(fc_context *ctx, const fc_la_run &r, long heads, int segments,
 
 template <int DT, bool FULL>
 int la_launch(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts) {
-    // two wavefronts where the state has no more than 64 columns
+    // Two wavefronts where the state has no more than 64 columns, and where three parts of so many rows leave no LDS for four.
+    if (r.Dk > 128 && (r.Dv <= 64 || DT == FC_F32)) return la_launch_one<DT, 8, 2, FULL>(ctx, r, heads, segments, segment, parts);
     if (r.Dv <= 64) {
         if (r.Dk <= 32) return la_launch_one<DT, 1, 2, FULL>(ctx, r, heads, segments, segment, parts);
         if (r.Dk <= 64) return la_launch_one<DT, 2, 2, FULL>(ctx, r, heads, segments, segment, parts);
-        if (r.Dk <= 128) return la_launch_one<DT, 4, 2, FULL>(ctx, r, heads, segments, segment, parts);
-        return la_launch_one<DT, 8, 2, FULL>(ctx, r, heads, segments, segment, parts);
+        return la_launch_one<DT, 4, 2, FULL>(ctx, r, heads, segments, segment, parts);
     }
     if (r.Dk <= 32) return la_launch_one<DT, 1, 4, FULL>(ctx, r, heads, segments, segment, parts);
     if (r.Dk <= 64) return la_launch_one<DT, 2, 4, FULL>(ctx, r, heads, segments, segment, parts);
     if (r.Dk <= 128) return la_launch_one<DT, 4, 4, FULL>(ctx, r, heads, segments, segment, parts);
-    return la_launch_one<DT, 8, 4, FULL>(ctx, r, heads, segments, segment, parts);
+    if constexpr (DT != FC_F32) return la_launch_one<DT, 8, 4, FULL>(ctx, r, heads, segments, segment, parts);
+    return FC_ERR_UNSUPPORTED;      // not reached
 }
