@@ -13,6 +13,8 @@
 // from it, and joins batches, threads, channels and chunks by
 //   n = na + nb,  mean = ma + d nb/n,  M2 = M2a + M2b + d^2 na nb/n,  d = mb - ma
 // (Chan, Golub and LeVeque, "Updating formulae and a pairwise algorithm for computing sample variances", 1979).
+#include <type_traits>
+
 #include "token_types.h"
 
 namespace {
@@ -73,9 +75,9 @@ struct norm_place {
 // Threads over a span: `cols` accesses side by side, `rows` pixels at once.
 struct norm_threads {
     int cols, rows, tx, ty;
-    __device__ __forceinline__ norm_threads(int accesses) {
-        cols = accesses < kThreads ? accesses : kThreads;
-        rows = kThreads / cols;
+    __device__ __forceinline__ norm_threads(int accesses, int threads = kThreads) {
+        cols = accesses < threads ? accesses : threads;
+        rows = threads / cols;
         ty = threadIdx.x / cols;
         tx = threadIdx.x - ty * cols;
     }
@@ -100,33 +102,38 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const nor
 #pragma unroll
             for (int v = 0; v < VEC; v++) mean[v] = m2[v] = 0.f;
             float count = 0.f;
-            for (long q = at.p0 + th.ty; q < at.p1; q += (long)U * th.rows) {
+            long q = at.p0 + th.ty;
+            const long whole = at.p1 - (long)(U - 1) * th.rows;
+            for (; q < whole; q += (long)U * th.rows) {
                 V in[U];
-                int nb = 0;
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const long r = q + (long)u * th.rows;
-                    if (r < at.p1) {
-                        in[u] = *(const V *)(src + r * p.x_pixel);
-                        nb = u + 1;
-                    }
-                }
-                const float joined = count + nb, wb = nb / joined, wm = count * wb;
+                for (int u = 0; u < U; u++) in[u] = *(const V *)(src + (q + (long)u * th.rows) * p.x_pixel);
+                const float joined = count + U, wb = U / joined, wm = count * wb;
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
-                    float s = 0.f;
+                    float s = 0.f, sq = 0.f;
 #pragma unroll
-                    for (int u = 0; u < U; u++) s += u < nb ? in[u].get(v) : 0.f;
-                    s = nb == U ? s * (1.f / U) : s / nb;      // exact where all values are equal
-                    float sq = 0.f;
+                    for (int u = 0; u < U; u++) s += in[u].get(v);
+                    s *= 1.f / U;
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        const float d = u < nb ? in[u].get(v) - s : 0.f;
-                        sq += d * d;
+                        const float d = in[u].get(v) - s;
+                        sq = __builtin_fmaf(d, d, sq);
                     }
                     const float d = s - mean[v];
-                    mean[v] += d * wb;
-                    m2[v] += sq + d * d * wm;
+                    mean[v] = __builtin_fmaf(d, wb, mean[v]);
+                    m2[v] += __builtin_fmaf(d * d, wm, sq);
+                }
+                count = joined;
+            }
+            for (; q < at.p1; q += th.rows) {      // what is left, a pixel at a time
+                const V in = *(const V *)(src + q * p.x_pixel);
+                const float joined = count + 1.f, wb = 1.f / joined, wm = count * wb;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    const float d = in.get(v) - mean[v];
+                    mean[v] = __builtin_fmaf(d, wb, mean[v]);
+                    m2[v] = __builtin_fmaf(d * d, wm, m2[v]);
                 }
                 count = joined;
             }
@@ -317,28 +324,44 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_sums_kernel(const norm
     }
 }
 
-// dgamma and dbeta of 32 channels: 8 threads each over the images' chunks, in a fixed order.
+// dgamma and dbeta of 8 channels: 32 threads each over the images' chunks, in a fixed order, eight loads at a time.
 __device__ __forceinline__ void reduce_channels(const norm_params &p, unsigned block, float2 *sums) {
-    const int lc = threadIdx.x & 31, row = threadIdx.x >> 5, c = block * 32 + lc;
+    const int lc = threadIdx.x & 7, row = threadIdx.x >> 3, c = block * 8 + lc;
     float2 s = make_float2(0.f, 0.f);
     if (c < p.C) {
         const long rows = (long)p.N * p.chunks;
-        for (long r = row; r < rows; r += 8) {
+        long r = row;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {
+            float2 e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) e[i] = p.channel_part[(r + 32 * i) * p.C + c];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                s.x += e[i].x;
+                s.y += e[i].y;
+            }
+        }
+        for (; r < rows; r += 32) {
             const float2 e = p.channel_part[r * p.C + c];
             s.x += e.x;
             s.y += e.y;
         }
     }
-    sums[row * 32 + lc] = s;
+    sums[row * 8 + lc] = s;
     __syncthreads();
     if (row == 0 && c < p.C) {
-        for (int r = 1; r < 8; r++) {
-            s.x += sums[r * 32 + lc].x;
-            s.y += sums[r * 32 + lc].y;
+        for (int r = 1; r < 32; r++) {
+            s.x += sums[r * 8 + lc].x;
+            s.y += sums[r * 8 + lc].y;
         }
         if (p.dbeta) p.dbeta[c] = s.x;
         if (p.dgamma) p.dgamma[c] = s.y;
     }
+}
+
+__global__ __launch_bounds__(kThreads) void fc_group_norm_channels_kernel(const norm_params p) {
+    __shared__ float2 sums[kThreads];
+    reduce_channels(p, blockIdx.x, sums);
 }
 
 // dx; the first workgroups add up dgamma and dbeta meanwhile.
@@ -405,6 +428,199 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_gradient_kernel(const 
     }
 }
 
+// ---- groups that fit a workgroup's registers: x is read once, one launch
+
+// Consecutive spans of an image share cache lines, so they go to one of the eight dies, which take workgroups in turn.
+__device__ __forceinline__ unsigned same_die(unsigned block, unsigned blocks) {
+    return blocks % 8 ? block : block % 8 * (blocks / 8) + block / 8;
+}
+
+// Sums over the pixels of each of a span's channels, from one value a thread and channel of its column.  LDS: entry [rows][span], then
+// in its place the sums of `parts` threads a channel, [parts][span].  Ends with those in LDS for all.
+template <int VEC, int THREADS>
+__device__ __forceinline__ int sum_pixels(const norm_params &p, const norm_threads &th, const float (&value)[VEC], float *entry) {
+    __syncthreads();      // what was in entry is read
+    if (th.ty < th.rows) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) entry[th.ty * p.span + th.tx * VEC + v] = value[v];
+    }
+    __syncthreads();
+    const int parts = THREADS / p.span < th.rows ? THREADS / p.span : th.rows;
+    const int part = (int)threadIdx.x / p.span, c = (int)threadIdx.x - part * p.span;
+    float s = 0.f;
+    if (part < parts)
+        for (int ty = part; ty < th.rows; ty += parts) s += entry[ty * p.span + c];
+    __syncthreads();
+    if (part < parts) entry[threadIdx.x] = s;
+    __syncthreads();
+    return parts;
+}
+
+// The same for each group, a wavefront each, left in stat.
+template <int VEC, int THREADS>
+__device__ __forceinline__ void sum_groups(const norm_params &p, const norm_threads &th, const float (&value)[VEC], float *entry, float *stat) {
+    const int parts = sum_pixels<VEC, THREADS>(p, th, value, entry);
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < p.span / p.Cg; g += THREADS / 64) {
+        float s = 0.f;
+        for (int i = lane; i < parts * p.Cg; i += 64) {
+            const int part = i / p.Cg;
+            s += entry[part * p.span + g * p.Cg + (i - part * p.Cg)];
+        }
+        s = fc_wave_sum(s);
+        if (lane == 0) stat[g] = s;
+    }
+    __syncthreads();
+}
+
+// R pixels of its column a thread.
+template <int DT, int VEC, int ACT, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const norm_params p) {
+    extern __shared__ float resident_sums[];      // [rows][span], then the groups' sums
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    const unsigned block = same_die(blockIdx.x, gridDim.x);
+    const long n = block / p.spans;
+    const int c0 = (int)(block - n * p.spans) * p.span;
+    const norm_threads th(p.span / VEC, THREADS);
+    float *const stat = resident_sums + th.rows * p.span;
+    const E *src = (const E *)p.x + n * p.x_image + c0 + th.tx * VEC;
+    const int P = th.ty < th.rows ? (int)p.P : 0;      // threads past the last row have no pixels
+    V in[R];
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int q = th.ty + k * th.rows;
+        if (q < P) in[k] = *(const V *)(src + q * p.x_pixel);
+    }
+    float sum[VEC], mean[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        sum[v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < R; k++) sum[v] += th.ty + k * th.rows < P ? in[k].get(v) : 0.f;
+    }
+    const float values = (float)p.P * p.Cg;
+    sum_groups<VEC, THREADS>(p, th, sum, resident_sums, stat);
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        mean[v] = stat[(th.tx * VEC + v) / p.Cg] / values;
+        sum[v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            const float d = th.ty + k * th.rows < P ? in[k].get(v) - mean[v] : 0.f;
+            sum[v] = __builtin_fmaf(d, d, sum[v]);
+        }
+    }
+    sum_groups<VEC, THREADS>(p, th, sum, resident_sums, stat);
+    if (th.ty >= th.rows) return;
+    float scale[VEC], shift[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        const int c = c0 + th.tx * VEC + v;
+        const float rstd = 1.f / sqrtf(stat[(th.tx * VEC + v) / p.Cg] / values + p.eps);
+        scale[v] = rstd * (p.gamma ? p.gamma[c] : 1.f);
+        shift[v] = p.beta ? p.beta[c] : 0.f;
+        if (p.mean && th.ty == 0 && c % p.Cg == 0) {
+            p.mean[n * p.G + c / p.Cg] = mean[v];
+            p.rstd[n * p.G + c / p.Cg] = rstd;
+        }
+    }
+    E *dst = (E *)p.y + n * p.y_image + c0 + th.tx * VEC;
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int q = th.ty + k * th.rows;
+        if (q >= P) break;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) in[k].set(v, activation<ACT>((in[k].get(v) - mean[v]) * scale[v] + shift[v]));
+        *(V *)(dst + q * p.y_pixel) = in[k];
+    }
+}
+
+template <int DT, int VEC, int ACT, int THREADS, int R>
+__global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kernel(const norm_params p) {
+    extern __shared__ float resident_sums[];      // [rows][span], then dbeta and dgamma of the span's channels, then s1 and s2 of its groups
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    const unsigned block = same_die(blockIdx.x, gridDim.x);
+    const long n = block / p.spans;
+    const int c0 = (int)(block - n * p.spans) * p.span;
+    const norm_threads th(p.span / VEC, THREADS);
+    float2 *const channel = (float2 *)(resident_sums + (th.rows * p.span + 1) / 2 * 2), *const stat = channel + p.span;
+    const E *x = (const E *)p.x + n * p.x_image + c0 + th.tx * VEC;
+    const E *dy = (const E *)p.dy + n * p.y_image + c0 + th.tx * VEC;
+    const int P = th.ty < th.rows ? (int)p.P : 0;
+    V xs[R], ds[R];
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int q = th.ty + k * th.rows;
+        if (q < P) {
+            xs[k] = *(const V *)(x + q * p.x_pixel);
+            ds[k] = *(const V *)(dy + q * p.y_pixel);
+        }
+    }
+    const norm_column<VEC> c(p, n, c0 + th.tx * VEC);
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) a[v] = b[v] = 0.f;
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        if (th.ty + k * th.rows >= P) break;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const float xhat = (xs[k].get(v) - c.mean[v]) * c.rstd[v];
+            const float dz = ds[k].get(v) * activation_slope<ACT>(xhat * c.gamma[v] + c.beta[v]);
+            a[v] += dz;
+            b[v] = __builtin_fmaf(dz, xhat, b[v]);
+        }
+    }
+    int parts = sum_pixels<VEC, THREADS>(p, th, a, resident_sums);
+    if ((int)threadIdx.x < p.span) {
+        float s = 0.f;
+        for (int i = 0; i < parts; i++) s += resident_sums[i * p.span + threadIdx.x];
+        channel[threadIdx.x].x = s;
+    }
+    parts = sum_pixels<VEC, THREADS>(p, th, b, resident_sums);
+    if ((int)threadIdx.x < p.span) {
+        float s = 0.f;
+        for (int i = 0; i < parts; i++) s += resident_sums[i * p.span + threadIdx.x];
+        channel[threadIdx.x].y = s;
+        if (p.channel_part) p.channel_part[n * p.C + c0 + threadIdx.x] = channel[threadIdx.x];
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < p.span / p.Cg; g += THREADS / 64) {
+        float s1 = 0.f, s2 = 0.f;
+        for (int i = lane; i < p.Cg; i += 64) {
+            const float2 e = channel[g * p.Cg + i];
+            const float gamma = p.gamma ? p.gamma[c0 + g * p.Cg + i] : 1.f;
+            s1 += gamma * e.x;
+            s2 += gamma * e.y;
+        }
+        const float inv = 1.f / ((float)p.P * p.Cg);
+        s1 = fc_wave_sum(s1) * inv;
+        s2 = fc_wave_sum(s2) * inv;
+        if (lane == 0) stat[g] = make_float2(s1, s2);
+    }
+    __syncthreads();
+    if (th.ty >= th.rows) return;
+    float2 st[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) st[v] = stat[(th.tx * VEC + v) / p.Cg];
+    E *dx = (E *)p.y + n * p.x_image + c0 + th.tx * VEC;
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        const int q = th.ty + k * th.rows;
+        if (q >= P) break;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const float xhat = (xs[k].get(v) - c.mean[v]) * c.rstd[v];
+            const float dz = ds[k].get(v) * activation_slope<ACT>(xhat * c.gamma[v] + c.beta[v]);
+            xs[k].set(v, c.rstd[v] * (c.gamma[v] * dz - st[v].x - xhat * st[v].y));
+        }
+        *(V *)(dx + q * p.x_pixel) = xs[k];
+    }
+}
+
 int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
 
 long gcd(long a, long b) { return b ? gcd(b, a % b) : a; }
@@ -429,7 +645,7 @@ int width_of(const fc_group_norm_shape &s, int span, uint64_t addr) {
 }
 
 template <int ACT, class F>
-bool with_width(int dtype, int vec, F &&f) {
+bool with_width(int dtype, int vec, F f) {
     if (dtype == FC_F32) {
         if (vec == 4) return f.template run<FC_F32, 4, ACT>();
         if (vec == 2) return f.template run<FC_F32, 2, ACT>();
@@ -448,7 +664,7 @@ bool with_width(int dtype, int vec, F &&f) {
 }
 
 template <class F>
-bool with_kernel(const fc_group_norm_shape &s, int vec, F &&f) {
+bool with_kernel(const fc_group_norm_shape &s, int vec, F f) {
     switch (s.act) {
         case FC_ACT_RELU: return with_width<FC_ACT_RELU>(s.dtype, vec, f);
         case FC_ACT_SILU: return with_width<FC_ACT_SILU>(s.dtype, vec, f);
@@ -467,6 +683,69 @@ struct forward_launch {
         fc_group_norm_stats_kernel<DT, VEC><<<dim3(blocks), dim3(kThreads), (size_t)rows * p.span * sizeof(float2), stream>>>(p);
         fc_group_norm_apply_kernel<DT, VEC, ACT><<<dim3(blocks), dim3(kThreads), (size_t)(p.span / p.Cg) * sizeof(float2), stream>>>(p);
         return true;
+    }
+};
+
+// Pixels a thread, of 256 threads or of 1024, that a resident kernel of accesses of VEC elements needs; 0 if no kernel has as many.
+int resident_pixels(long P, int span, int vec, int threads, int most) {
+    const int cols = span / vec;
+    if (cols > threads / 2 || span > threads) return 0;
+    const long need = (P + threads / cols - 1) / (threads / cols);
+    int r = 1;
+    while (r < need && r < most) r *= 2;
+    return need <= r ? r : 0;
+}
+
+// 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.
+constexpr int kResident = 16, kResidentBackward = 8;
+
+// Channels of a resident workgroup: whole groups and whole accesses of 16 bytes, and with them 64 bytes of a pixel if they fit (half a
+// cache line); 0 if not even those fit.
+int resident_span(const fc_group_norm_shape *s, int most) {
+    const int Cg = s->C / s->G, vec = 16 / (int)fc_elem_size(s->dtype);
+    if (fc_widest(s->dtype, (uint64_t)(s->C | s->x_image | s->x_pixel | s->y_image | s->y_pixel), 0) != vec) return 0;
+    const long step = Cg / gcd(Cg, vec) * vec;
+    if (step > 256) return 0;
+    int found = 0;
+    for (long span = step; span <= s->C && span <= 256; span *= 2) {
+        if (s->C % span || !resident_pixels(s->P, (int)span, vec, 1024, most)) break;
+        found = (int)span;
+        if (span * (long)fc_elem_size(s->dtype) >= 64) break;
+    }
+    return fc_count(s->N, s->C) < (1l << 31) ? found : 0;
+}
+
+template <int DT, int VEC, int ACT, bool BACKWARD, int THREADS>
+void launch_resident(hipStream_t stream, const norm_params &p, int r) {
+    const int rows = THREADS / (p.span / VEC);
+    const size_t lds = ((size_t)rows * p.span + 1) / 2 * 2 * sizeof(float) + (size_t)p.span * 2 * sizeof(float2);
+    const dim3 grid((unsigned)((long)p.N * p.spans)), threads(THREADS);
+    auto launch = [&](auto pixels) {
+        if constexpr (BACKWARD) fc_group_norm_resident_gradient_kernel<DT, VEC, ACT, THREADS, decltype(pixels)::value><<<grid, threads, lds, stream>>>(p);
+        else fc_group_norm_resident_kernel<DT, VEC, ACT, THREADS, decltype(pixels)::value><<<grid, threads, lds, stream>>>(p);
+    };
+    if (r == 1) launch(std::integral_constant<int, 1>());
+    else if (r == 2) launch(std::integral_constant<int, 2>());
+    else if constexpr (THREADS > kThreads) {
+        if (r == 4) launch(std::integral_constant<int, 4>());
+        else if (r == 8) launch(std::integral_constant<int, 8>());
+        else if constexpr (!BACKWARD) launch(std::integral_constant<int, 16>());
+    }
+}
+
+template <bool BACKWARD>
+struct resident_launch {
+    hipStream_t stream;
+    const norm_params &p;
+    template <int DT, int VEC, int ACT>
+    bool run() {
+        constexpr bool whole = VEC * sizeof(typename fc_elem<DT>::type) == 16;      // the plans' widest access
+        if constexpr (whole) {
+            const int most = BACKWARD ? kResidentBackward : kResident, few = resident_pixels(p.P, p.span, VEC, kThreads, 2);
+            if (few) launch_resident<DT, VEC, ACT, BACKWARD, kThreads>(stream, p, few);
+            else launch_resident<DT, VEC, ACT, BACKWARD, 1024>(stream, p, resident_pixels(p.P, p.span, VEC, 1024, most));
+        }
+        return whole;
     }
 };
 
@@ -525,6 +804,8 @@ extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_no
     chunks = (pixels + chunk - 1) / chunk;
     if (chunk >= (1l << 30) || s->N * spans * chunks >= (1l << 31) - 65536) return FC_ERR_UNSUPPORTED;
     plan->chunks = (int)chunks;
+    plan->resident = resident_span(s, kResident);
+    plan->resident_backward = resident_span(s, kResidentBackward);
     plan->ws_bytes = (size_t)s->N * s->G * chunks * sizeof(float2);
     plan->ws_backward_bytes = plan->ws_bytes + (size_t)s->N * chunks * s->C * sizeof(float2);
     return FC_OK;
@@ -548,6 +829,13 @@ extern "C" int fc_group_norm(fc_context *ctx, const fc_group_norm_plan *plan, co
     norm_params p = params_of(plan);
     p.x = x_dev; p.y = y_dev; p.gamma = gamma_dev; p.beta = beta_dev; p.mean = mean_dev; p.rstd = rstd_dev;
     p.part = (float2 *)ws_dev;
+    if (plan->resident && (addr & 15) == 0) {
+        p.span = plan->resident;
+        p.spans = p.C / p.span;
+        with_kernel(plan->shape, 16 / (int)fc_elem_size(plan->shape.dtype), resident_launch<false>{ctx->stream, p});
+        FC_LAUNCH_CHECK(ctx, "fc_group_norm");
+        return FC_OK;
+    }
     forward_launch f = {ctx->stream, p, (unsigned)((long)p.N * p.spans * p.chunks)};
     with_kernel(plan->shape, width_of(plan->shape, plan->span, addr), f);
     FC_LAUNCH_CHECK(ctx, "fc_group_norm");
@@ -571,7 +859,17 @@ extern "C" int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan 
     p.part = (float2 *)ws_dev;
     p.channel_part = p.part + (size_t)p.N * p.G * p.chunks;
     p.dgamma = dgamma_dev; p.dbeta = dbeta_dev;
-    p.reduce_blocks = dgamma_dev || dbeta_dev ? (p.C + 31) / 32 : 0;
+    p.reduce_blocks = dgamma_dev || dbeta_dev ? (p.C + 7) / 8 : 0;
+    if (plan->resident_backward && (addr & 15) == 0) {
+        p.span = plan->resident_backward;
+        p.spans = p.C / p.span;
+        p.chunks = 1;      // sums of channels, an image each
+        p.channel_part = p.reduce_blocks ? (float2 *)ws_dev : nullptr;
+        with_kernel(plan->shape, 16 / (int)fc_elem_size(plan->shape.dtype), resident_launch<true>{ctx->stream, p});
+        if (p.reduce_blocks) fc_group_norm_channels_kernel<<<dim3((unsigned)p.reduce_blocks), dim3(kThreads), 0, ctx->stream>>>(p);
+        FC_LAUNCH_CHECK(ctx, "fc_group_norm_backward");
+        return FC_OK;
+    }
     backward_launch f = {ctx->stream, p, (unsigned)((long)p.N * p.spans * p.chunks)};
     with_kernel(plan->shape, width_of(plan->shape, plan->span, addr), f);
     FC_LAUNCH_CHECK(ctx, "fc_group_norm_backward");

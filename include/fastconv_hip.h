@@ -476,8 +476,8 @@ typedef struct {
     fc_group_norm_shape shape;
     int span;                 /* channels that one workgroup reads of a pixel: whole groups */
     int chunks;               /* parts that the pixels of an image are cut into */
-    int resident;             /* 1: an image's groups stay in a workgroup's registers, one launch */
-    int resident_backward;
+    int resident;             /* channels whose groups stay in a workgroup's registers, so that x is read once; 0: they */
+    int resident_backward;    /* do not fit, or tensors that do not begin on 16 bytes, and x is read twice */
     size_t ws_bytes;          /* workspace of the forward call, 0 if none */
     size_t ws_backward_bytes; /* and of the backward call */
 } fc_group_norm_plan;
