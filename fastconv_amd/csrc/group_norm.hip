@@ -38,11 +38,23 @@ struct norm_params {
     long x_image, x_pixel, y_image, y_pixel;
 };
 
+// 1 - erf(|x|) = (a1 t + .. + a5 t^5) e with t = 1/(1 + 0.3275911 |x|), e = exp(-x^2), to 1.5e-7 (Hastings' formula, number 7.1.26
+// in Abramowitz and Stegun's handbook): a rounding or two of the erf(x) + 1 that it is used in, and a third of the instructions of erff.
+__device__ __forceinline__ float erf_plus_one(float x, float e) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, __builtin_fabsf(x), 1.f));
+    float s = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+    s = __builtin_fmaf(s, t, 1.421413741f);
+    s = __builtin_fmaf(s, t, -0.284496736f);
+    s = __builtin_fmaf(s, t, 0.254829592f);
+    s *= t * e;
+    return x < 0.f ? s : 2.f - s;
+}
+
 template <int ACT>
 __device__ __forceinline__ float activation(float z) {
     if (ACT == FC_ACT_RELU) return z < 0.f ? 0.f : z;      // NaN stays
     if (ACT == FC_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-    if (ACT == FC_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    if (ACT == FC_ACT_GELU) return 0.5f * z * erf_plus_one(z * 0.70710678118654752f, __expf(-0.5f * z * z));
     return z;
 }
 
@@ -53,8 +65,10 @@ __device__ __forceinline__ float activation_slope(float z) {
         const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
         return s * (1.f + z * (1.f - s));
     }
-    if (ACT == FC_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    if (ACT == FC_ACT_GELU) {
+        const float e = __expf(-0.5f * z * z);
+        return __builtin_fmaf(0.5f, erf_plus_one(z * 0.70710678118654752f, e), z * 0.39894228040143268f * e);
+    }
     return 1.f;
 }
 
@@ -83,6 +97,77 @@ struct norm_threads {
     }
 };
 
+// Sums over a workgroup by butterflies: where the accesses of a span are a power of two of threads side by side, and a group is a power of
+// two of accesses or an access holds a power of two of groups, the lanes of a wavefront that belong together differ in bits of their
+// number.  `group`: the bits that may differ among the columns of one group (0: sums of each channel).
+// Leaves in LDS [units][span] what each wavefront (each part of a wavefront's row) has; returns the number of units.
+struct norm_butterfly {
+    int cols, group;         // accesses of a span; of a group, 0 if a group is less than an access
+    bool fits;
+    __device__ __forceinline__ norm_butterfly(const norm_params &p, int vec, int threads) {
+        cols = p.span / vec;
+        group = p.Cg / vec;
+        const int within = p.Cg < vec ? p.Cg : vec;
+        fits = cols <= threads && (cols & (cols - 1)) == 0 && (within & (within - 1)) == 0 && (group & (group - 1)) == 0 &&
+               p.Cg % within == 0 && (group == 0 || p.Cg == group * vec) && group <= 64;
+    }
+};
+
+// Sums of `value` over the lanes of each column, by channel.
+template <int VEC>
+__device__ __forceinline__ void sum_lanes(float (&value)[VEC], int cols) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) {
+        if (m < cols) break;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) value[v] += __shfl_xor(value[v], m);
+    }
+}
+
+// Sums of `value` over a workgroup and each group of the span; every thread gets those of its channels' groups.
+template <int VEC, int THREADS>
+__device__ __forceinline__ void sum_groups_fast(const norm_params &p, const norm_butterfly &f, const norm_threads &th, float (&value)[VEC], float *lds) {
+    // the channels of an access that share a group
+#pragma unroll
+    for (int m = 1; m < VEC; m <<= 1) {
+        if (m >= p.Cg) break;
+        float other[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) other[v] = value[v ^ m];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) value[v] += other[v];
+    }
+    const int unit = f.cols <= 64 ? threadIdx.x >> 6 : th.ty, units = f.cols <= 64 ? THREADS / 64 : th.rows;
+    const int groups = p.span / p.Cg, first = th.tx * VEC / p.Cg;
+    if (f.group) {      // one group an access
+        float s = value[0];
+#pragma unroll
+        for (int m = 32; m; m >>= 1)
+            if (m >= f.cols || m < f.group) s += __shfl_xor(s, m);
+        __syncthreads();      // what was in lds is read
+        if (((int)threadIdx.x & 63) < f.cols && (th.tx & (f.group - 1)) == 0) lds[unit * groups + first] = s;
+        __syncthreads();
+        s = 0.f;
+        for (int u = 0; u < units; u++) s += lds[u * groups + first];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) value[v] = s;
+    } else {
+        sum_lanes<VEC>(value, f.cols);
+        __syncthreads();
+        if (((int)threadIdx.x & 63) < f.cols) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) lds[(unit * f.cols + th.tx) * VEC + v] = value[v];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < VEC; v++) value[v] = 0.f;
+        for (int u = 0; u < units; u++) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) value[v] += lds[(u * f.cols + th.tx) * VEC + v];
+        }
+    }
+}
+
 // Statistics of each group over a chunk.
 template <int DT, int VEC>
 __global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const norm_params p) {
@@ -91,8 +176,8 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const nor
     typedef typename fc_elem<DT>::type E;
     constexpr int U = 8;                   // pixels a batch
     const norm_place at(p, blockIdx.x);
-    const int accesses = p.span / VEC;
-    const norm_threads th(accesses);
+    const norm_threads th(p.span / VEC);
+    const norm_butterfly fast(p, VEC, kThreads);
     const int c0 = at.span * p.span;
     const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
     if (th.ty < th.rows) {
@@ -137,6 +222,29 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const nor
                 }
                 count = joined;
             }
+            if (fast.fits && width == p.span) {
+                const float all = (float)(at.p1 - at.p0) * p.Cg;
+                float joined[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; v++) joined[v] = count * mean[v];
+                sum_groups_fast<VEC, kThreads>(p, fast, th, joined, (float *)entry);
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    joined[v] /= all;
+                    const float d = mean[v] - joined[v];
+                    mean[v] = joined[v];
+                    m2[v] = __builtin_fmaf(count * d, d, m2[v]);
+                }
+                sum_groups_fast<VEC, kThreads>(p, fast, th, m2, (float *)entry);
+                if (th.ty == 0) {
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) {
+                        const int c = c0 + col * VEC + v;
+                        if (c % p.Cg == 0) p.part[(at.n * p.G + c / p.Cg) * p.chunks + at.chunk] = make_float2(mean[v], m2[v]);
+                    }
+                }
+                return;
+            }
 #pragma unroll
             for (int v = 0; v < VEC; v++) entry[th.ty * p.span + col * VEC + v] = make_float2(mean[v], m2[v]);
         }
@@ -178,23 +286,27 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_apply_kernel(const nor
     const norm_threads th(p.span / VEC);
     const int c0 = at.span * p.span;
     const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
-    const int lane = threadIdx.x & 63, groups = width / p.Cg;
-    for (int g = threadIdx.x >> 6; g < groups; g += kThreads / 64) {
+    const int groups = width / p.Cg;
+    // eight lanes a group where there are many, a wavefront each where there are few
+    const int lanes = groups > 4 ? 8 : 64, lane = threadIdx.x & (lanes - 1);
+    for (int g = threadIdx.x / lanes; g < groups; g += kThreads / lanes) {
         const long group = at.n * p.G + c0 / p.Cg + g;
         const float2 *part = p.part + group * p.chunks;
         float s = 0.f;
-        for (int i = lane; i < p.chunks; i += 64) {
+        for (int i = lane; i < p.chunks; i += lanes) {
             const long first = i * p.chunk;
             s += (float)(p.P - first < p.chunk ? p.P - first : p.chunk) * part[i].x;
         }
-        const float mean = fc_wave_sum(s) / (float)p.P;
+        for (int m = lanes / 2; m; m >>= 1) s += __shfl_xor(s, m);
+        const float mean = s / (float)p.P;
         float m2 = 0.f;
-        for (int i = lane; i < p.chunks; i += 64) {
+        for (int i = lane; i < p.chunks; i += lanes) {
             const long first = i * p.chunk;
             const float d = part[i].x - mean;
             m2 += part[i].y + (float)(p.P - first < p.chunk ? p.P - first : p.chunk) * p.Cg * d * d;
         }
-        const float rstd = 1.f / sqrtf(fc_wave_sum(m2) / ((float)p.P * p.Cg) + p.eps);
+        for (int m = lanes / 2; m; m >>= 1) m2 += __shfl_xor(m2, m);
+        const float rstd = 1.f / sqrtf(m2 / ((float)p.P * p.Cg) + p.eps);
         if (lane == 0) {
             stat[g] = make_float2(mean, rstd);
             if (at.chunk == 0 && p.mean) {
@@ -379,18 +491,20 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_gradient_kernel(const 
     const norm_threads th(p.span / VEC);
     const int c0 = at.span * p.span;
     const int width = (p.C - c0 < p.span ? p.C - c0 : p.span);
-    const int lane = threadIdx.x & 63;
-    for (int g = threadIdx.x >> 6; g < width / p.Cg; g += kThreads / 64) {
+    const int groups = width / p.Cg, lanes = groups > 4 ? 8 : 64, lane = threadIdx.x & (lanes - 1);
+    for (int g = threadIdx.x / lanes; g < groups; g += kThreads / lanes) {
         const float2 *part = p.part + (at.n * p.G + c0 / p.Cg + g) * p.chunks;
         float s1 = 0.f, s2 = 0.f;
-        for (int i = lane; i < p.chunks; i += 64) {
+        for (int i = lane; i < p.chunks; i += lanes) {
             s1 += part[i].x;
             s2 += part[i].y;
         }
+        for (int m = lanes / 2; m; m >>= 1) {
+            s1 += __shfl_xor(s1, m);
+            s2 += __shfl_xor(s2, m);
+        }
         const float inv = 1.f / ((float)p.P * p.Cg);
-        s1 = fc_wave_sum(s1) * inv;
-        s2 = fc_wave_sum(s2) * inv;
-        if (lane == 0) stat[g] = make_float2(s1, s2);
+        if (lane == 0) stat[g] = make_float2(s1 * inv, s2 * inv);
     }
     __syncthreads();
     if (th.ty >= th.rows) return;
@@ -456,21 +570,53 @@ __device__ __forceinline__ int sum_pixels(const norm_params &p, const norm_threa
     return parts;
 }
 
-// The same for each group, a wavefront each, left in stat.
+// Sums over the workgroup and each group of the span; every thread with pixels gets those of its channels' groups.
 template <int VEC, int THREADS>
-__device__ __forceinline__ void sum_groups(const norm_params &p, const norm_threads &th, const float (&value)[VEC], float *entry, float *stat) {
+__device__ __forceinline__ void sum_groups(const norm_params &p, const norm_butterfly &fast, const norm_threads &th, float (&value)[VEC], float *entry) {
+    if (fast.fits) {
+        sum_groups_fast<VEC, THREADS>(p, fast, th, value, entry);
+        return;
+    }
     const int parts = sum_pixels<VEC, THREADS>(p, th, value, entry);
+    float *const stat = entry + th.rows * p.span;
     const int lane = threadIdx.x & 63;
     for (int g = threadIdx.x >> 6; g < p.span / p.Cg; g += THREADS / 64) {
         float s = 0.f;
-        for (int i = lane; i < parts * p.Cg; i += 64) {
-            const int part = i / p.Cg;
-            s += entry[part * p.span + g * p.Cg + (i - part * p.Cg)];
-        }
+        for (int part = 0; part < parts; part++)
+            for (int i = lane; i < p.Cg; i += 64) s += entry[part * p.span + g * p.Cg + i];
         s = fc_wave_sum(s);
         if (lane == 0) stat[g] = s;
     }
     __syncthreads();
+    if (th.ty < th.rows) {
+#pragma unroll
+        for (int v = 0; v < VEC; v++) value[v] = stat[(th.tx * VEC + v) / p.Cg];
+    }
+}
+
+// Sums over the workgroup of each channel, left in channel[].x or .y by the first threads.
+template <int VEC, int THREADS>
+__device__ __forceinline__ void sum_channels(const norm_params &p, const norm_butterfly &fast, const norm_threads &th, float (&value)[VEC], float *entry,
+                                             float *channel) {
+    int parts;
+    if (fast.fits) {
+        sum_lanes<VEC>(value, fast.cols);
+        const int unit = fast.cols <= 64 ? threadIdx.x >> 6 : th.ty;
+        parts = fast.cols <= 64 ? THREADS / 64 : th.rows;
+        __syncthreads();
+        if (((int)threadIdx.x & 63) < fast.cols) {
+#pragma unroll
+            for (int v = 0; v < VEC; v++) entry[unit * p.span + th.tx * VEC + v] = value[v];
+        }
+        __syncthreads();
+    } else {
+        parts = sum_pixels<VEC, THREADS>(p, th, value, entry);
+    }
+    if ((int)threadIdx.x < p.span) {
+        float s = 0.f;
+        for (int i = 0; i < parts; i++) s += entry[i * p.span + threadIdx.x];
+        channel[2 * threadIdx.x] = s;
+    }
 }
 
 // R pixels of its column a thread.
@@ -483,7 +629,6 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
     const long n = block / p.spans;
     const int c0 = (int)(block - n * p.spans) * p.span;
     const norm_threads th(p.span / VEC, THREADS);
-    float *const stat = resident_sums + th.rows * p.span;
     const E *src = (const E *)p.x + n * p.x_image + c0 + th.tx * VEC;
     const int P = th.ty < th.rows ? (int)p.P : 0;      // threads past the last row have no pixels
     V in[R];
@@ -500,10 +645,11 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
         for (int k = 0; k < R; k++) sum[v] += th.ty + k * th.rows < P ? in[k].get(v) : 0.f;
     }
     const float values = (float)p.P * p.Cg;
-    sum_groups<VEC, THREADS>(p, th, sum, resident_sums, stat);
+    const norm_butterfly fast(p, VEC, THREADS);
+    sum_groups<VEC, THREADS>(p, fast, th, sum, resident_sums);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
-        mean[v] = stat[(th.tx * VEC + v) / p.Cg] / values;
+        mean[v] = sum[v] / values;
         sum[v] = 0.f;
 #pragma unroll
         for (int k = 0; k < R; k++) {
@@ -511,13 +657,13 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
             sum[v] = __builtin_fmaf(d, d, sum[v]);
         }
     }
-    sum_groups<VEC, THREADS>(p, th, sum, resident_sums, stat);
+    sum_groups<VEC, THREADS>(p, fast, th, sum, resident_sums);
     if (th.ty >= th.rows) return;
     float scale[VEC], shift[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
         const int c = c0 + th.tx * VEC + v;
-        const float rstd = 1.f / sqrtf(stat[(th.tx * VEC + v) / p.Cg] / values + p.eps);
+        const float rstd = 1.f / sqrtf(sum[v] / values + p.eps);
         scale[v] = rstd * (p.gamma ? p.gamma[c] : 1.f);
         shift[v] = p.beta ? p.beta[c] : 0.f;
         if (p.mean && th.ty == 0 && c % p.Cg == 0) {
@@ -573,19 +719,10 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kerne
             b[v] = __builtin_fmaf(dz, xhat, b[v]);
         }
     }
-    int parts = sum_pixels<VEC, THREADS>(p, th, a, resident_sums);
-    if ((int)threadIdx.x < p.span) {
-        float s = 0.f;
-        for (int i = 0; i < parts; i++) s += resident_sums[i * p.span + threadIdx.x];
-        channel[threadIdx.x].x = s;
-    }
-    parts = sum_pixels<VEC, THREADS>(p, th, b, resident_sums);
-    if ((int)threadIdx.x < p.span) {
-        float s = 0.f;
-        for (int i = 0; i < parts; i++) s += resident_sums[i * p.span + threadIdx.x];
-        channel[threadIdx.x].y = s;
-        if (p.channel_part) p.channel_part[n * p.C + c0 + threadIdx.x] = channel[threadIdx.x];
-    }
+    const norm_butterfly fast(p, VEC, THREADS);
+    sum_channels<VEC, THREADS>(p, fast, th, a, resident_sums, &channel->x);
+    sum_channels<VEC, THREADS>(p, fast, th, b, resident_sums, &channel->y);
+    if (p.channel_part && (int)threadIdx.x < p.span) p.channel_part[n * p.C + c0 + threadIdx.x] = channel[threadIdx.x];
     __syncthreads();
     const int lane = threadIdx.x & 63;
     for (int g = threadIdx.x >> 6; g < p.span / p.Cg; g += THREADS / 64) {
