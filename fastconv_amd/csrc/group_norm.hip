@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxGroupChannels = 4096;
+constexpr double kCacheBytes = 256.0 * (1 << 20);      // the last cache before HBM
 
 struct norm_params {
     const void *x, *dy;
@@ -33,6 +34,7 @@ struct norm_params {
     long P, chunk;           // pixels of an image, and of a chunk
     int N, C, G, Cg;
     int span, spans, chunks;
+    bool past_cache;
     int reduce_blocks;       // workgroups of the backward pass's second launch that add up channel_part
     float eps;
     long x_image, x_pixel, y_image, y_pixel;
@@ -70,6 +72,16 @@ __device__ __forceinline__ float activation_slope(float z) {
         return __builtin_fmaf(0.5f, erf_plus_one(z * 0.70710678118654752f, e), z * 0.39894228040143268f * e);
     }
     return 1.f;
+}
+
+template <bool PAST_CACHE, class V>
+__device__ __forceinline__ void store(void *dst, const V &x) {
+    if constexpr (PAST_CACHE && sizeof(V) == 16) {
+        typedef uint32_t words __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(words, x), (words *)dst);
+    } else {
+        *(V *)dst = x;
+    }
 }
 
 // What a workgroup works on: a chunk of pixels of one image, a span of its channels.
@@ -276,7 +288,8 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_stats_kernel(const nor
 }
 
 // Joins the chunks of each group and writes y.
-template <int DT, int VEC, int ACT>
+// PAST_CACHE: the result is stored past the caches, which then keep x for this second reading.
+template <int DT, int VEC, int ACT, bool PAST_CACHE>
 __global__ __launch_bounds__(kThreads) void fc_group_norm_apply_kernel(const norm_params p) {
     extern __shared__ float2 stat[];      // (mean, rstd) of the span's groups
     typedef fc_vec<DT, VEC> V;
@@ -342,7 +355,7 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_apply_kernel(const nor
                 if (r >= at.p1) break;
 #pragma unroll
                 for (int v = 0; v < VEC; v++) in[u].set(v, activation<ACT>((in[u].get(v) - mean[v]) * scale[v] + shift[v]));
-                *(V *)(dst + r * p.y_pixel) = in[u];
+                store<PAST_CACHE>(dst + r * p.y_pixel, in[u]);
             }
         }
     }
@@ -477,7 +490,7 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_channels_kernel(const 
 }
 
 // dx; the first workgroups add up dgamma and dbeta meanwhile.
-template <int DT, int VEC, int ACT>
+template <int DT, int VEC, int ACT, bool PAST_CACHE>
 __global__ __launch_bounds__(kThreads) void fc_group_norm_gradient_kernel(const norm_params p) {
     extern __shared__ float2 stat[];      // (s1, s2) of the span's groups over their values, or the sums of channels
     typedef fc_vec<DT, VEC> V;
@@ -536,7 +549,7 @@ __global__ __launch_bounds__(kThreads) void fc_group_norm_gradient_kernel(const 
                     const float dz = ds[u].get(v) * activation_slope<ACT>(xhat * k.gamma[v] + k.beta[v]);
                     xs[u].set(v, k.rstd[v] * (k.gamma[v] * dz - st[v].x - xhat * st[v].y));
                 }
-                *(V *)(dx + r * p.x_pixel) = xs[u];
+                store<PAST_CACHE>(dx + r * p.x_pixel, xs[u]);
             }
         }
     }
@@ -549,21 +562,20 @@ __device__ __forceinline__ unsigned same_die(unsigned block, unsigned blocks) {
     return blocks % 8 ? block : block % 8 * (blocks / 8) + block / 8;
 }
 
-// Sums over the pixels of each of a span's channels, from one value a thread and channel of its column.  LDS: entry [rows][span], then
-// in its place the sums of `parts` threads a channel, [parts][span].  Ends with those in LDS for all.
+// Sums over the pixels of each of a span's channels, from one value a thread and channel of its column.  Leaves in LDS the sums of `parts`
+// threads a channel, [parts][span].  Ends with those in LDS for all.
 template <int VEC, int THREADS>
 __device__ __forceinline__ int sum_pixels(const norm_params &p, const norm_threads &th, const float (&value)[VEC], float *entry) {
+    constexpr int PITCH = THREADS + 8;      // [VEC][THREADS], eight banks further on for each channel of an access
     __syncthreads();      // what was in entry is read
-    if (th.ty < th.rows) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) entry[th.ty * p.span + th.tx * VEC + v] = value[v];
-    }
+    for (int v = 0; v < VEC; v++) entry[v * PITCH + threadIdx.x] = value[v];
     __syncthreads();
     const int parts = THREADS / p.span < th.rows ? THREADS / p.span : th.rows;
     const int part = (int)threadIdx.x / p.span, c = (int)threadIdx.x - part * p.span;
     float s = 0.f;
     if (part < parts)
-        for (int ty = part; ty < th.rows; ty += parts) s += entry[ty * p.span + c];
+        for (int ty = part; ty < th.rows; ty += parts) s += entry[c % VEC * PITCH + ty * th.cols + c / VEC];
     __syncthreads();
     if (part < parts) entry[threadIdx.x] = s;
     __syncthreads();
@@ -578,12 +590,17 @@ __device__ __forceinline__ void sum_groups(const norm_params &p, const norm_butt
         return;
     }
     const int parts = sum_pixels<VEC, THREADS>(p, th, value, entry);
-    float *const stat = entry + th.rows * p.span;
+    float *const stat = entry + VEC * (THREADS + 8);
     const int lane = threadIdx.x & 63;
     for (int g = threadIdx.x >> 6; g < p.span / p.Cg; g += THREADS / 64) {
         float s = 0.f;
-        for (int part = 0; part < parts; part++)
-            for (int i = lane; i < p.Cg; i += 64) s += entry[part * p.span + g * p.Cg + i];
+        if (parts >= p.Cg) {
+            for (int part = lane; part < parts; part += 64)
+                for (int i = 0; i < p.Cg; i++) s += entry[part * p.span + g * p.Cg + i];
+        } else {
+            for (int part = 0; part < parts; part++)
+                for (int i = lane; i < p.Cg; i += 64) s += entry[part * p.span + g * p.Cg + i];
+        }
         s = fc_wave_sum(s);
         if (lane == 0) stat[g] = s;
     }
@@ -622,7 +639,7 @@ __device__ __forceinline__ void sum_channels(const norm_params &p, const norm_bu
 // R pixels of its column a thread.
 template <int DT, int VEC, int ACT, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const norm_params p) {
-    extern __shared__ float resident_sums[];      // [rows][span], then the groups' sums
+    extern __shared__ float resident_sums[];      // [VEC][THREADS], then the groups' sums
     typedef fc_vec<DT, VEC> V;
     typedef typename fc_elem<DT>::type E;
     const unsigned block = same_die(blockIdx.x, gridDim.x);
@@ -684,14 +701,14 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
 
 template <int DT, int VEC, int ACT, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kernel(const norm_params p) {
-    extern __shared__ float resident_sums[];      // [rows][span], then dbeta and dgamma of the span's channels, then s1 and s2 of its groups
+    extern __shared__ float resident_sums[];      // [VEC][THREADS], then dbeta and dgamma of the span's channels, then s1 and s2 of its groups
     typedef fc_vec<DT, VEC> V;
     typedef typename fc_elem<DT>::type E;
     const unsigned block = same_die(blockIdx.x, gridDim.x);
     const long n = block / p.spans;
     const int c0 = (int)(block - n * p.spans) * p.span;
     const norm_threads th(p.span / VEC, THREADS);
-    float2 *const channel = (float2 *)(resident_sums + (th.rows * p.span + 1) / 2 * 2), *const stat = channel + p.span;
+    float2 *const channel = (float2 *)(resident_sums + VEC * (THREADS + 8)), *const stat = channel + p.span;
     const E *x = (const E *)p.x + n * p.x_image + c0 + th.tx * VEC;
     const E *dy = (const E *)p.dy + n * p.y_image + c0 + th.tx * VEC;
     const int P = th.ty < th.rows ? (int)p.P : 0;
@@ -715,6 +732,7 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kerne
         for (int v = 0; v < VEC; v++) {
             const float xhat = (xs[k].get(v) - c.mean[v]) * c.rstd[v];
             const float dz = ds[k].get(v) * activation_slope<ACT>(xhat * c.gamma[v] + c.beta[v]);
+            if (DT == FC_F32) ds[k].set(v, dz);
             a[v] += dz;
             b[v] = __builtin_fmaf(dz, xhat, b[v]);
         }
@@ -751,7 +769,7 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kerne
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             const float xhat = (xs[k].get(v) - c.mean[v]) * c.rstd[v];
-            const float dz = ds[k].get(v) * activation_slope<ACT>(xhat * c.gamma[v] + c.beta[v]);
+            const float dz = DT == FC_F32 ? ds[k].get(v) : ds[k].get(v) * activation_slope<ACT>(xhat * c.gamma[v] + c.beta[v]);
             xs[k].set(v, c.rstd[v] * (c.gamma[v] * dz - st[v].x - xhat * st[v].y));
         }
         *(V *)(dx + q * p.x_pixel) = xs[k];
@@ -818,7 +836,9 @@ struct forward_launch {
     bool run() {
         const int accesses = p.span / VEC, rows = kThreads / (accesses < kThreads ? accesses : kThreads);
         fc_group_norm_stats_kernel<DT, VEC><<<dim3(blocks), dim3(kThreads), (size_t)rows * p.span * sizeof(float2), stream>>>(p);
-        fc_group_norm_apply_kernel<DT, VEC, ACT><<<dim3(blocks), dim3(kThreads), (size_t)(p.span / p.Cg) * sizeof(float2), stream>>>(p);
+        constexpr bool whole = VEC * sizeof(typename fc_elem<DT>::type) == 16;
+        const auto apply = whole && p.past_cache ? fc_group_norm_apply_kernel<DT, VEC, ACT, whole> : fc_group_norm_apply_kernel<DT, VEC, ACT, false>;
+        apply<<<dim3(blocks), dim3(kThreads), (size_t)(p.span / p.Cg) * sizeof(float2), stream>>>(p);
         return true;
     }
 };
@@ -835,6 +855,11 @@ int resident_pixels(long P, int span, int vec, int threads, int most) {
 
 // 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.
 constexpr int kResident = 16, kResidentBackward = 8;
+// Forward and backward together, resident against not: 1 image of 14x14x512 in bf16 16 and 28 us, 8 of 35x35x192 in half 32 and 37, 32 of 28x28x512 in half
+// (26 MB) 63 and 69; but 32 of 56x56x256 in fp32 (103 MB) 157 and 152, 128 of them in bf16 (206 MB) 743 and 532: the phases of two large
+// workgroups on a compute unit overlap less than those of many small ones, and the cache holds what is read twice.
+constexpr double kResidentBackwardBytes = 64e6;
+constexpr long kResidentWorkgroups = 256;      // below, a wider workgroup would leave compute units idle
 
 // Channels of a resident workgroup: whole groups and whole accesses of 16 bytes, and with them 64 bytes of a pixel if they fit (half a
 // cache line); 0 if not even those fit.
@@ -846,6 +871,7 @@ int resident_span(const fc_group_norm_shape *s, int most) {
     int found = 0;
     for (long span = step; span <= s->C && span <= 256; span *= 2) {
         if (s->C % span || !resident_pixels(s->P, (int)span, vec, 1024, most)) break;
+        if (found && s->N * (s->C / span) < kResidentWorkgroups) break;
         found = (int)span;
         if (span * (long)fc_elem_size(s->dtype) >= 64) break;
     }
@@ -854,8 +880,7 @@ int resident_span(const fc_group_norm_shape *s, int most) {
 
 template <int DT, int VEC, int ACT, bool BACKWARD, int THREADS>
 void launch_resident(hipStream_t stream, const norm_params &p, int r) {
-    const int rows = THREADS / (p.span / VEC);
-    const size_t lds = ((size_t)rows * p.span + 1) / 2 * 2 * sizeof(float) + (size_t)p.span * 2 * sizeof(float2);
+    const size_t lds = VEC * (THREADS + 8) * sizeof(float) + (size_t)p.span * 2 * sizeof(float2);
     const dim3 grid((unsigned)((long)p.N * p.spans)), threads(THREADS);
     auto launch = [&](auto pixels) {
         if constexpr (BACKWARD) fc_group_norm_resident_gradient_kernel<DT, VEC, ACT, THREADS, decltype(pixels)::value><<<grid, threads, lds, stream>>>(p);
@@ -895,7 +920,9 @@ struct backward_launch {
         const int accesses = p.span / VEC, rows = kThreads / (accesses < kThreads ? accesses : kThreads);
         fc_group_norm_sums_kernel<DT, VEC, ACT><<<dim3(blocks), dim3(kThreads), (size_t)rows * p.span * sizeof(float2), stream>>>(p);
         const size_t groups = (size_t)(p.span / p.Cg), need = groups > 256 ? groups : 256;
-        fc_group_norm_gradient_kernel<DT, VEC, ACT><<<dim3(blocks + p.reduce_blocks), dim3(kThreads), need * sizeof(float2), stream>>>(p);
+        constexpr bool whole = VEC * sizeof(typename fc_elem<DT>::type) == 16;
+        const auto gradient = whole && p.past_cache ? fc_group_norm_gradient_kernel<DT, VEC, ACT, whole> : fc_group_norm_gradient_kernel<DT, VEC, ACT, false>;
+        gradient<<<dim3(blocks + p.reduce_blocks), dim3(kThreads), need * sizeof(float2), stream>>>(p);
         return true;
     }
 };
@@ -908,6 +935,8 @@ norm_params params_of(const fc_group_norm_plan *plan) {
     p.spans = (s.C + plan->span - 1) / plan->span;
     p.chunks = plan->chunks;
     p.chunk = (s.P + plan->chunks - 1) / plan->chunks;
+    // 32 images of 224x224x64 in bf16: 147 -> 117 us.  A result that fits beside its input is left in the caches, for whoever reads it next.
+    p.past_cache = (double)s.N * s.P * s.C * fc_elem_size(s.dtype) * 2 > kCacheBytes;
     p.x_image = s.x_image; p.x_pixel = s.x_pixel; p.y_image = s.y_image; p.y_pixel = s.y_pixel;
     return p;
 }
@@ -931,8 +960,8 @@ extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_no
     if (span > s->C) span = s->C;
     plan->span = (int)span;
     const long spans = (s->C + span - 1) / span, pixels = s->P;
-    // about eight workgroups a compute unit, of 32 KB and more each
-    long chunks = 2048 / (s->N * spans);
+    // about four workgroups a compute unit, of 32 KB and more each
+    long chunks = 1024 / (s->N * spans);
     const long least = 32768 / (span * (long)fc_elem_size(s->dtype)) + 1;
     if (chunks > (pixels + least - 1) / least) chunks = (pixels + least - 1) / least;
     if (chunks < 1) chunks = 1;
@@ -940,9 +969,10 @@ extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_no
     const long chunk = (pixels + chunks - 1) / chunks;
     chunks = (pixels + chunk - 1) / chunk;
     if (chunk >= (1l << 30) || s->N * spans * chunks >= (1l << 31) - 65536) return FC_ERR_UNSUPPORTED;
+    const double values = (double)s->N * s->P * s->C;
     plan->chunks = (int)chunks;
     plan->resident = resident_span(s, kResident);
-    plan->resident_backward = resident_span(s, kResidentBackward);
+    plan->resident_backward = values * fc_elem_size(s->dtype) <= kResidentBackwardBytes ? resident_span(s, kResidentBackward) : 0;
     plan->ws_bytes = (size_t)s->N * s->G * chunks * sizeof(float2);
     plan->ws_backward_bytes = plan->ws_bytes + (size_t)s->N * chunks * s->C * sizeof(float2);
     return FC_OK;

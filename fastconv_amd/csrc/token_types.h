@@ -29,6 +29,19 @@ struct alignas(VEC * sizeof(typename fc_elem<DT>::type)) fc_vec {
     __device__ __forceinline__ void set(int i, float x) { v[i] = (typename fc_elem<DT>::type)x; }
 };
 
+// Accesses of global memory through a pointer that the compiler cannot follow to a kernel argument, and would take for one that may point
+// into LDS.
+template <class V>
+__device__ __forceinline__ V fc_load_global(const void *p) {
+    typedef __attribute__((address_space(1))) const V global;
+    return *(const V *)(global *)(uintptr_t)p;
+}
+template <class V>
+__device__ __forceinline__ void fc_store_global(void *p, const V &v) {
+    typedef __attribute__((address_space(1))) V global;
+    *(V *)(global *)(uintptr_t)p = v;
+}
+
 static inline size_t fc_elem_size(int dtype) { return dtype == FC_F32 ? 4 : 2; }
 static inline bool fc_dtype_ok(int dtype) { return dtype == FC_F32 || dtype == FC_BF16 || dtype == FC_F16; }
 
