@@ -21,12 +21,12 @@ struct fc_la_operand {
 
 struct fc_la_run {
     fc_la_operand q, k, v;
-    void *o;                 // in the tensors' type by strides, or
-    float *o32;              // fp32, [B][T][H][Dv], where heads are added up afterwards
+    void *o;                 // in the tensors' type, or
+    bool o_fp32;             // in fp32, where answers are added up afterwards
     long o_batch, o_token, o_head;
-    const float *state_in;   // element (row, column) of head bh at bh*Dk*Dv + row*state_row + column*state_col
+    const float *state_in;   // element (row, column) of head bh at bh*state_head + row*state_row + column*state_col
     float *state_out;
-    long state_row, state_col;
+    long state_head, state_row, state_col;
     const float *log_decay;
     const int32_t *lengths;
     long T;

@@ -9,6 +9,7 @@ constexpr int kMaxDim = 256;
 constexpr long kMostSteps = 16;    // up to here the recurrence is faster
 constexpr long kWavefronts = 2048, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
+constexpr int kChunkRows = 128;    // rows of a state that their kernel holds
 constexpr int kStepCols = 32;      // columns of the state that a workgroup of the recurrence holds
 
 // The recurrence.  A workgroup holds 32 columns of a head's state in registers: 8 threads side by side with 4 columns each,
@@ -35,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
 #pragma unroll
         for (int j = 0; j < 4; j++) s[i][j] = 0.f;
         if (!r.state_in || rr >= r.Dk || c0 >= r.Dv) continue;
-        const float *src = r.state_in + bh * r.Dk * r.Dv + rr * r.state_row + c0 * r.state_col;
+        const float *src = r.state_in + bh * r.state_head + rr * r.state_row + c0 * r.state_col;
         if (wide) {
             const float4 x = *(const float4 *)src;
             s[i][0] = x.x; s[i][1] = x.y; s[i][2] = x.z; s[i][3] = x.w;
@@ -48,9 +49,7 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
     const E *q = (const E *)r.q.p + b * r.q.batch + (h / r.q.share) * r.q.head;
     const E *k = (const E *)r.k.p + b * r.k.batch + (h / r.k.share) * r.k.head;
     const E *v = (const E *)r.v.p + b * r.v.batch + (h / r.v.share) * r.v.head;
-    E *o = (E *)r.o + b * r.o_batch + h * r.o_head;
-    float *o32 = r.o32 ? r.o32 + (b * r.T * r.H + h) * r.Dv : nullptr;
-    const long o32_token = (long)r.H * r.Dv;
+    const long o = b * r.o_batch + h * r.o_head;
 
     for (long n = 0; n < len; n++) {
         const long t = r.reverse ? len - 1 - n : n;
@@ -91,23 +90,23 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
         const int c = (int)(blockIdx.x - bh * slices) * kStepCols + tid;
         if (tid < kStepCols && c < r.Dv) {
             const float sum = (part[buf][0][tid] + part[buf][1][tid]) + (part[buf][2][tid] + part[buf][3][tid]);
-            if (o32) o32[t * o32_token + c] = sum;
-            else o[t * r.o_token + c] = (E)sum;
+            if (r.o_fp32) ((float *)r.o)[o + t * r.o_token + c] = sum;
+            else ((E *)r.o)[o + t * r.o_token + c] = (E)sum;
         }
     }
     // tokens past the end of a shorter sequence
     const int c = (int)(blockIdx.x - bh * slices) * kStepCols + (tid & 31);
     if (c < r.Dv)
         for (long t = len + (tid >> 5); t < r.T; t += kThreads / 32) {
-            if (o32) o32[t * o32_token + c] = 0.f;
-            else o[t * r.o_token + c] = (E)0.f;
+            if (r.o_fp32) ((float *)r.o)[o + t * r.o_token + c] = 0.f;
+            else ((E *)r.o)[o + t * r.o_token + c] = (E)0.f;
         }
     if (!r.state_out) return;
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         const int rr = row + 32 * i;
         if (rr >= r.Dk || c0 >= r.Dv) continue;
-        float *dst = r.state_out + bh * r.Dk * r.Dv + rr * r.state_row + c0 * r.state_col;
+        float *dst = r.state_out + bh * r.state_head + rr * r.state_row + c0 * r.state_col;
         if (wide) {
             *(float4 *)dst = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
         } else {
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_scan_kernel(cons
     const float ld = r.log_decay[bh - b * r.H];
     const fc_la_power full(ld, segment);
     const int row = i / r.Dv, col = i - row * r.Dv;
-    float s = r.state_in ? r.state_in[bh * size + row * r.state_row + col * r.state_col] : 0.f;
+    float s = r.state_in ? r.state_in[bh * r.state_head + row * r.state_row + col * r.state_col] : 0.f;
     float *p = parts + bh * segments * size + i;
     for (int first = 0; first < segments; first += AHEAD) {
         float add[AHEAD];
@@ -147,17 +146,17 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_scan_kernel(cons
     }
 }
 
-// Gradients of shared heads: the fp32 gradients [B][T][H][D] of the query heads, added up by key/value head.
+// Answers in fp32 that belong together, [B][T][heads][share][D], added up.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void fc_linear_attention_shared_kernel(const float *src, void *dst, long values, long T, int Hkv, int share,
-                                                                              int D, long batch, long token, long head) {
+__global__ __launch_bounds__(kThreads) void fc_linear_attention_sum_kernel(const float *src, void *dst, long values, long T, int heads, int share,
+                                                                           int D, long batch, long token, long head) {
     typedef typename fc_elem<DT>::type E;
     for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < values; i += (long)gridDim.x * kThreads) {
-        const long row = i / D, d = i - row * D, bt = row / Hkv, hk = row - bt * Hkv, b = bt / T, t = bt - b * T;
-        const float *p = src + (bt * Hkv + hk) * share * D + d;
+        const long row = i / D, d = i - row * D, bt = row / heads, h = row - bt * heads, b = bt / T, t = bt - b * T;
+        const float *p = src + row * share * D + d;
         float s = 0.f;
         for (int g = 0; g < share; g++) s += p[(long)g * D];
-        ((E *)dst)[b * batch + t * token + hk * head + d] = (E)s;
+        ((E *)dst)[b * batch + t * token + h * head + d] = (E)s;
     }
 }
 
@@ -180,6 +179,12 @@ bool same(const fc_linear_attention_plan &a, const fc_linear_attention_plan &b) 
            s.k_head == t.k_head && s.v_batch == t.v_batch && s.v_token == t.v_token && s.v_head == t.v_head && s.o_batch == t.o_batch &&
            s.o_token == t.o_token && s.o_head == t.o_head && a.chunk == b.chunk && a.segments == b.segments && a.ws_bytes == b.ws_bytes &&
            a.ws_backward_bytes == b.ws_backward_bytes;
+}
+
+// Floats of the workspace that hold the segments' states; what is added up follows.
+size_t states_of(const fc_linear_attention_plan *plan) {
+    const fc_linear_attention_shape &s = plan->shape;
+    return plan->segments > 1 ? (size_t)s.B * s.H * plan->segments * s.Dk * s.Dv : 0;
 }
 
 // Tokens of a segment: whole chunks.
@@ -210,12 +215,11 @@ bool wide(const fc_la_operand &x, int D, size_t es) {
     return ((D | x.batch | x.token | x.head) & 3) == 0 && ((uintptr_t)x.p & (4 * es - 1)) == 0 && x.token < (1l << 31) / 4 / kChunk - 1024;
 }
 
-int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *parts) {
+int run_chunks(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *parts) {
     const fc_linear_attention_shape &s = plan->shape;
-    if (plan->chunk == 0) return run_step(ctx, s, r);
     const size_t es = fc_elem_size(s.dtype);
-    r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) && wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, es) &&
-             (!r.o32 || (long)r.H * r.Dv < (1l << 31) / 4 / kChunk - 1024);
+    r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) &&
+             wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, r.o_fp32 ? sizeof(float) : es);
     const long heads = (long)s.B * s.H, segment = segment_of(s, plan->segments);
     if (plan->segments > 1) {
         const int rc = s.dtype == FC_F32    ? fc_la_state_f32(ctx, r, heads, plan->segments, segment, parts)
@@ -231,25 +235,45 @@ int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, flo
                                 : fc_la_answer_f16(ctx, r, heads, plan->segments, segment, parts);
 }
 
-// A gradient of a key/value operand: straight to its place, or by query head and then added up.
-int run_shared(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run &r, float *ws, float *parts, void *dst, int D, long batch, long token, long head) {
+// One run.  Its answers go to `dst` with the strides of r, or, where several belong together, in fp32 to `sums` and from there to dst: those
+// of the query heads that share a key/value head, if `share` of them do, and those of the two halves of a state with more rows than the
+// matrix cores' kernel holds, which is as two states that never meet.
+int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run r, float *parts, float *sums, void *dst, int share) {
     const fc_linear_attention_shape &s = plan->shape;
-    const int share = s.H / s.Hkv;
+    const int halves = plan->chunk && r.Dk > kChunkRows ? 2 : 1, together = share * halves;
+    const long batch = r.o_batch, token = r.o_token, head = r.o_head;
     r.o = dst;
-    r.o32 = share > 1 ? ws : nullptr;
-    r.o_batch = batch; r.o_token = token; r.o_head = head;
-    const int rc = run(ctx, plan, r, parts);
-    if (rc || share == 1) return rc;
-    const long values = (long)s.B * s.T * s.Hkv * D;
-    const long want = (values + kThreads - 1) / kThreads;
+    if (together > 1) {
+        r.o = sums;
+        r.o_fp32 = true;
+        r.o_head = (long)halves * r.Dv;
+        r.o_token = r.H * r.o_head;
+        r.o_batch = s.T * r.o_token;
+    }
+    const size_t es = fc_elem_size(s.dtype);
+    for (int half = 0; half < halves; half++) {
+        fc_la_run one = r;
+        if (halves > 1) {
+            const long first = half * (long)kChunkRows;
+            one.q.p = (const char *)r.q.p + first * es;
+            one.k.p = (const char *)r.k.p + first * es;
+            one.Dk = half ? r.Dk - kChunkRows : kChunkRows;
+            if (r.state_in) one.state_in = r.state_in + first * r.state_row;
+            if (r.state_out) one.state_out = r.state_out + first * r.state_row;
+            one.o = sums + half * r.Dv;
+        }
+        const int rc = plan->chunk ? run_chunks(ctx, plan, one, parts) : run_step(ctx, s, one);
+        if (rc) return rc;
+    }
+    if (together == 1) return FC_OK;
+    const int heads = r.H / share;
+    const long values = (long)s.B * s.T * heads * r.Dv, want = (values + kThreads - 1) / kThreads;
     const unsigned blocks = (unsigned)(want < 65536 ? want : 65536);
-    if (s.dtype == FC_F32)
-        fc_linear_attention_shared_kernel<FC_F32><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
-    else if (s.dtype == FC_BF16)
-        fc_linear_attention_shared_kernel<FC_BF16><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
-    else
-        fc_linear_attention_shared_kernel<FC_F16><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(ws, dst, values, s.T, s.Hkv, share, D, batch, token, head);
-    FC_LAUNCH_CHECK(ctx, "fc_linear_attention_shared_kernel");
+    const auto sum = s.dtype == FC_F32    ? fc_linear_attention_sum_kernel<FC_F32>
+                     : s.dtype == FC_BF16 ? fc_linear_attention_sum_kernel<FC_BF16>
+                                          : fc_linear_attention_sum_kernel<FC_F16>;
+    sum<<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(sums, dst, values, s.T, heads, together, r.Dv, batch, token, head);
+    FC_LAUNCH_CHECK(ctx, "fc_linear_attention_sum_kernel");
     return FC_OK;
 }
 
@@ -259,7 +283,7 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
     if (!plan || !shape_ok(s)) return FC_ERR_INVALID;
     if (s->Dk > kMaxDim || s->Dv > kMaxDim || fc_count(s->B, s->H) < 0 || fc_count(s->B, s->H) >= (1l << 31) / 8) return FC_ERR_UNSUPPORTED;
     const int most = s->Dk > s->Dv ? s->Dk : s->Dv;
-    const long tokens = fc_count(s->B, s->T), values = tokens < 0 ? -1 : fc_count(tokens, s->H, 4 * most);
+    const long tokens = fc_count(s->B, s->T), values = tokens < 0 ? -1 : fc_count(tokens, s->H, 8 * most);
     if (s->T >= (1l << 31) || values < 0) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
@@ -276,7 +300,11 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
         if (segments > 1) plan->segments = (int)segments;
         if (plan->segments > 1) plan->ws_bytes = (size_t)s->B * s->H * plan->segments * s->Dk * s->Dv * sizeof(float);
     }
-    plan->ws_backward_bytes = plan->ws_bytes + (s->H > s->Hkv ? (size_t)values : 0);
+    // Answers that are added up afterwards: of the forward run, of the largest backward one.
+    const size_t answers = (size_t)s->B * s->T * s->H * sizeof(float);
+    const bool halves = plan->chunk && most > kChunkRows;
+    plan->ws_backward_bytes = plan->ws_bytes + (halves ? 2 : s->H > s->Hkv ? 1 : 0) * answers * most;
+    if (plan->chunk && s->Dk > kChunkRows) plan->ws_bytes += 2 * answers * s->Dv;
     return FC_OK;
 }
 
@@ -301,12 +329,12 @@ extern "C" int fc_linear_attention(fc_context *ctx, const fc_linear_attention_pl
     r.q = {q_dev, s.q_batch, s.q_token, s.q_head, 1};
     r.k = {k_dev, s.k_batch, s.k_token, s.k_head, share};
     r.v = {v_dev, s.v_batch, s.v_token, s.v_head, share};
-    r.o = o_dev; r.o_batch = s.o_batch; r.o_token = s.o_token; r.o_head = s.o_head;
-    r.state_in = state_in_dev; r.state_out = state_out_dev; r.state_row = s.Dv; r.state_col = 1;
+    r.o_batch = s.o_batch; r.o_token = s.o_token; r.o_head = s.o_head;
+    r.state_in = state_in_dev; r.state_out = state_out_dev; r.state_head = (long)s.Dk * s.Dv; r.state_row = s.Dv; r.state_col = 1;
     r.log_decay = log_decay_dev; r.lengths = lengths_dev;
     r.T = s.T; r.H = s.H; r.Dk = s.Dk; r.Dv = s.Dv;
     r.scale_in = 1.f; r.scale_out = s.scale;
-    return run(ctx, plan, r, (float *)ws_dev);
+    return run(ctx, plan, r, (float *)ws_dev, (float *)ws_dev + states_of(plan), o_dev, 1);
 }
 
 extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan *plan, const void *do_dev, const void *q_dev,
@@ -325,29 +353,32 @@ extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_att
     const int share = s.H / s.Hkv;
     const fc_la_operand q = {q_dev, s.q_batch, s.q_token, s.q_head, 1}, k = {k_dev, s.k_batch, s.k_token, s.k_head, share},
                         v = {v_dev, s.v_batch, s.v_token, s.v_head, share}, d = {do_dev, s.o_batch, s.o_token, s.o_head, 1};
-    float *parts = (float *)ws_dev, *sums = parts + plan->ws_bytes / sizeof(float);
+    float *parts = (float *)ws_dev, *sums = parts + states_of(plan);
     fc_la_run r = {};
     r.log_decay = log_decay_dev; r.lengths = lengths_dev;
     r.T = s.T; r.H = s.H;
+    r.state_head = (long)s.Dk * s.Dv;
     // dq, from the transposed state
     r.q = d; r.k = v; r.v = k;
     r.Dk = s.Dv; r.Dv = s.Dk;
     r.state_in = state_in_dev; r.state_row = 1; r.state_col = s.Dv;
     r.scale_in = 1.f; r.scale_out = s.scale;
-    r.o = dq_dev; r.o_batch = s.q_batch; r.o_token = s.q_token; r.o_head = s.q_head;
-    int rc = run(ctx, plan, r, parts);
+    r.o_batch = s.q_batch; r.o_token = s.q_token; r.o_head = s.q_head;
+    int rc = run(ctx, plan, r, parts, sums, dq_dev, 1);
     if (rc) return rc;
     // dk, from the last token to the first
     r.reverse = 1;
     r.scale_in = s.scale; r.scale_out = 1.f;
     r.q = v; r.k = d; r.v = q;
     r.state_in = dstate_out_dev;
-    rc = run_shared(ctx, plan, r, sums, parts, dk_dev, s.Dk, s.k_batch, s.k_token, s.k_head);
+    r.o_batch = s.k_batch; r.o_token = s.k_token; r.o_head = s.k_head;
+    rc = run(ctx, plan, r, parts, sums, dk_dev, share);
     if (rc) return rc;
     // dv, and the gradient of the first state
     r.q = k; r.k = q; r.v = d;
     r.Dk = s.Dk; r.Dv = s.Dv;
     r.state_row = s.Dv; r.state_col = 1;
     r.state_out = dstate_in_dev;
-    return run_shared(ctx, plan, r, sums, parts, dv_dev, s.Dv, s.v_batch, s.v_token, s.v_head);
+    r.o_batch = s.v_batch; r.o_token = s.v_token; r.o_head = s.v_head;
+    return run(ctx, plan, r, parts, sums, dv_dev, share);
 }

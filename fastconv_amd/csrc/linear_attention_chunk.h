@@ -47,6 +47,10 @@ __device__ __forceinline__ la_f32x16 la_product(const la_frag &a, const la_frag 
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ la_f32x4 la_product16(const la_frag &a, const la_frag &b, la_f32x4 c) {      // 16x16, 32 depths
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
 // PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  A value less its rounded
 // self is one instruction on the pair as it is packed, a - 1 * hi.lo + 0 * hi.hi, exact over the whole range of fp32 (an infinity in one makes
 // NaN of the other's second part: they are summed together anyway).  Bits that `keep` lacks are zeros in every part.
@@ -92,6 +96,11 @@ __device__ __forceinline__ la_frag la_read(const char *frag, int lane, int mix) 
 }
 __device__ __forceinline__ la_frag la_read_natural(const char *base, int s, int lane) {
     return la_read(base + s * kLaFrag, lane, (2 * s + (lane >> 5)) & 15);
+}
+// Thirty-two depths, from two fragments, of sixteen tokens: an operand of a 16x16 product.
+__device__ __forceinline__ la_frag la_read_natural16(const char *base, int s, int first, int lane) {
+    const int f = 2 * s + (lane >> 5), g = lane >> 4 & 1;
+    return *(const la_frag *)(base + f * kLaFrag + (g * 32 + ((first + (lane & 15)) ^ ((2 * f + g) & 15))) * 16);
 }
 __device__ __forceinline__ la_frag la_read_turned(const char *base, int td, int s, int lane) {
     return la_read(base + (td * 2 + s) * kLaFrag, lane, (td & 1) | (lane >> 4 & 1) << 1);
@@ -180,14 +189,14 @@ __device__ __forceinline__ void la_put_raw(char *base, int plane, int at, typena
     else la_put<la_math<DT>::PARTS>(base, plane, at, {(float)a, (float)b, (float)c, (float)d});
 }
 
-// Eight accumulators from `first` on as an operand; of each part the bits that `keep` has, a word a pair.
+// Eight accumulators from `first` on as an operand.
 template <int FORMED>
-__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, la_frag (&f)[FORMED], const uint32_t *keep = nullptr) {
+__device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, la_frag (&f)[FORMED]) {
     la_u32x4 w[FORMED];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         uint32_t two[FORMED];
-        la_split_pair<FORMED>(x[first + 2 * i], x[first + 2 * i + 1], two, keep ? keep[first / 2 + i] : ~0u);
+        la_split_pair<FORMED>(x[first + 2 * i], x[first + 2 * i + 1], two);
 #pragma unroll
         for (int p = 0; p < FORMED; p++) w[p][i] = two[p];
     }
@@ -212,13 +221,19 @@ __device__ __forceinline__ uint32_t la_not_finite(const la_block<DT> &b) {
     return bad & carry;
 }
 
+template <int DT>
+__device__ __forceinline__ void la_answer(const fc_la_run &r, long at, float x) {
+    if (r.o_fp32) ((float *)r.o)[at] = x;
+    else ((typename fc_elem<DT>::type *)r.o)[at] = (typename fc_elem<DT>::type)x;
+}
+
 // Tokens of the chunk that begins at p0.
 __device__ __forceinline__ int la_tokens(long p0, long end) { return (int)(end - p0 < kLaChunk ? end - p0 : kLaChunk); }
 
 // KT tiles of 32 rows of the state (rows past Dk are zeros), NW wavefronts of 32 columns.  FULL: answers tokens; otherwise only
 // forms the state that a segment adds.
 template <int DT, int KT, int NW, bool FULL, bool WIDE>
-__global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_chunk_kernel(const fc_la_run r, int segments, long segment, int slices, float *parts) {
+__global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(const fc_la_run r, int segments, long segment, int slices, float *parts) {
     typedef la_math<DT> M;
     typedef typename fc_elem<DT>::type E;
     constexpr int THREADS = 64 * NW, DK = 32 * KT, DV = 32 * NW;
@@ -227,7 +242,8 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     constexpr int QK_ITEMS = (8 * DK / 4 + THREADS - 1) / THREADS, V_ITEMS = 8 * DV / 4 / THREADS;
     extern __shared__ char lds[];
     char *const qs = lds, *const ks = qs + Q_BYTES, *const kt = ks + Q_BYTES, *const vt = kt + M::KEPT * QK_PLANE;
-    double *const exact = (double *)(vt + M::PARTS * V_PLANE + (FULL ? 0 : M::KEPT * QK_PLANE + M::PARTS * V_PLANE));      // decay^0 .. decay^32
+    char *const pt = vt + M::PARTS * V_PLANE;                       // P, rows of 32 answers, if FULL
+    double *const exact = (double *)(FULL ? pt + M::FORMED * 2 * kLaFrag : pt + M::KEPT * QK_PLANE + M::PARTS * V_PLANE);      // decay^0 .. decay^32
     float *const power = (float *)(exact + kLaChunk + 1);           // the same, times what enters the state
     int *const odd = (int *)(power + kLaChunk + 1);                 // whether a value of the chunk is not finite,
     int *const since = odd + 1;                                     // and from which token on, for each column
@@ -245,6 +261,8 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
     const long begin = seg * segment, end = begin + segment < len ? begin + segment : len;
     if (!FULL && begin >= end) return;
     const float ld = r.log_decay[h];
+    if (FULL)
+        for (int i = tid; i < M::FORMED * 2 * kLaFrag / 4; i += THREADS) ((uint32_t *)pt)[i] = 0;
 
     if (tid <= kLaChunk) {
         const double l = tid ? exp((double)ld * tid) : 1.0;
@@ -256,17 +274,22 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         for (int c = tid; c < DV; c += THREADS) since[c] = kLaChunk;
     }
     __syncthreads();
-    // powers between two tokens of a chunk, zero towards an earlier one, and from the state to a token
-    float near[16], from;
-    uint32_t earlier[8];
+    // P^T in blocks of 16x16, the one above the diagonal left as zeros: this wavefront's, with the powers between their tokens.  A later
+    // token is left out of P by its bits, not multiplied by zero: it may hold anything.
+    constexpr int BLOCKS = FULL ? (3 + NW - 1) / NW : 1;
+    float near[BLOCKS][4], from = 0.f;
+    uint32_t earlier[BLOCKS][2];
     const int i_tok = lane & 31;
     if (FULL) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int d = i_tok - (8 * (e / 4) + 4 * g + e % 4);
-            near[e] = d < 0 ? 0.f : power[d] * r.scale_out;
-            // A later token is left out of P by its bits, not multiplied by zero: it may hold anything.
-            if (e % 2 == 0) earlier[e / 2] = (d >= 0 ? 0x0000ffffu : 0u) | (d >= 1 ? 0xffff0000u : 0u);
+        for (int n = 0; n < BLOCKS; n++) {
+            const int t = wave + n * NW, j0 = t == 2 ? 16 : 0, i0 = t >= 1 ? 16 : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int d = i0 + (lane & 15) - (j0 + 4 * (lane >> 4) + e);
+                near[n][e] = d < 0 ? 0.f : power[d] * r.scale_out;
+                if (e % 2 == 0) earlier[n][e / 2] = (d >= 0 ? 0x0000ffffu : 0u) | (d >= 1 ? 0xffff0000u : 0u);
+            }
         }
         from = (float)exact[i_tok + 1 - r.reverse] * r.scale_out;
     }
@@ -276,7 +299,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
 
     // the state: rows 32*t + 8*(e/4) + 4*g + e%4 of column col
     la_f32x16 S[KT];
-    const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.Dk * r.Dv : nullptr;
+    const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.state_head : nullptr;
     const long srow = segments > 1 ? r.Dv : r.state_row, scol = segments > 1 ? 1 : r.state_col;
 #pragma unroll
     for (int t = 0; t < KT; t++)
@@ -478,11 +501,10 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         // Two barriers a chunk.  Between the first and the second q and k are read, and what k adds and v are laid out for
         // the state; after the second these are read, and the next chunk's q and k laid out.  So either half has work for the vector unit
         // beside the matrix cores'.
-        const long o_size = r.o32 ? 4 : (long)sizeof(E), o_row = (r.o32 ? (long)r.H * r.Dv : r.o_token) * o_size;
+        const long o_size = r.o_fp32 ? 4 : (long)sizeof(E), o_row = r.o_token * o_size;
         const long o_step = r.reverse ? -kLaChunk * o_row : kLaChunk * o_row;
         const uint32_t o_offset = (uint32_t)((r.reverse ? kLaChunk - 1 - i_tok : i_tok) * o_row + 32 * wave * o_size);
-        char *o_at = (r.o32 ? (char *)(r.o32 + (b * r.T * r.H + h) * r.Dv + col0) : (char *)((E *)r.o + b * r.o_batch + h * r.o_head + col0)) +
-                     (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
+        char *o_at = (char *)r.o + (b * r.o_batch + h * r.o_head + col0) * o_size + (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
         load_qk(begin);
         load_v(begin);
 #pragma unroll
@@ -497,35 +519,54 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
             rescale(n);
             weigh(n, add);
             __syncthreads();
-            la_f32x16 P, O;
+            la_f32x16 O;
+            la_f32x4 P[BLOCKS];
 #pragma unroll
-            for (int e = 0; e < 16; e++) P[e] = O[e] = 0.f;
+            for (int e = 0; e < 16; e++) O[e] = 0.f;
+#pragma unroll
+            for (int n = 0; n < BLOCKS; n++) P[n] = (la_f32x4){0.f, 0.f, 0.f, 0.f};
             {
-                la_frag qf[2][M::PARTS], kf[2][M::PARTS], sf[M::FORMED];
+                la_frag qf[2][M::PARTS], sf[M::FORMED];
                 auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int p = 0; p < M::PARTS; p++) {
-                        qf[s & 1][p] = la_read_natural(qs + p * QK_PLANE, s, lane);
-                        kf[s & 1][p] = la_read_natural(ks + p * QK_PLANE, s, lane);
-                    }
+                    for (int p = 0; p < M::PARTS; p++) qf[s & 1][p] = la_read_natural(qs + p * QK_PLANE, s, lane);
                 };
                 finite_v();
                 fetch(0);
 #pragma unroll
                 for (int s = 0; s < 2 * KT; s++) {
                     if (s + 1 < 2 * KT) fetch(s + 1);
+                    la_frag qp[BLOCKS][M::PARTS], kp[BLOCKS][M::PARTS];
+                    if (s % 2 == 0) {
+#pragma unroll
+                        for (int n = 0; n < BLOCKS; n++) {
+                            const int t = wave + n * NW;
+                            if (t >= 3) continue;
+#pragma unroll
+                            for (int p = 0; p < M::PARTS; p++) {
+                                qp[n][p] = la_read_natural16(qs + p * QK_PLANE, s / 2, t >= 1 ? 16 : 0, lane);
+                                kp[n][p] = la_read_natural16(ks + p * QK_PLANE, s / 2, t == 2 ? 16 : 0, lane);
+                            }
+                        }
+                    }
                     __builtin_amdgcn_sched_barrier(kLaOnlyVector);
-#pragma unroll
-                    for (int a = 0; a < M::PARTS; a++)
-#pragma unroll
-                        for (int c = 0; c < M::PARTS; c++)
-                            if (a + c < M::ORDER) P = la_product(kf[s & 1][a], qf[s & 1][c], P);
                     la_formed<M::FORMED>(S[s / 2], 8 * (s % 2), sf);
 #pragma unroll
                     for (int a = 0; a < M::FORMED; a++)
 #pragma unroll
                         for (int c = 0; c < M::PARTS; c++)
                             if (a + c < M::ORDER) O = la_product(sf[a], qf[s & 1][c], O);
+                    if (s % 2 == 0) {
+#pragma unroll
+                        for (int n = 0; n < BLOCKS; n++) {
+                            if (wave + n * NW >= 3) continue;
+#pragma unroll
+                            for (int a = 0; a < M::PARTS; a++)
+#pragma unroll
+                                for (int c = 0; c < M::PARTS; c++)
+                                    if (a + c < M::ORDER) P[n] = la_product16(kp[n][a], qp[n][c], P[n]);
+                        }
+                    }
 #pragma unroll
                     for (int e = s * 4 / (2 * KT); e < (s + 1) * 4 / (2 * KT); e++) {
                         put_weighed(kt, e);
@@ -533,6 +574,17 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                     }
                     __builtin_amdgcn_sched_barrier(kLaOnlyVector);
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < BLOCKS; n++) {
+                const int t = wave + n * NW;
+                if (t >= 3) continue;
+                uint32_t lo[M::FORMED], hi[M::FORMED];
+                la_split_pair<M::FORMED>(P[n][0] * near[n][0], P[n][1] * near[n][1], lo, earlier[n][0]);
+                la_split_pair<M::FORMED>(P[n][2] * near[n][2], P[n][3] * near[n][3], hi, earlier[n][1]);
+                char *const to = pt + (t == 2 ? kLaFrag : 0) + la_place((t >= 1 ? 16 : 0) + (lane & 15), lane >> 4, 0);
+#pragma unroll
+                for (int p = 0; p < M::FORMED; p++) *(la_u32x2 *)(to + p * 2 * kLaFrag) = (la_u32x2){lo[p], hi[p]};
             }
             load_v(p0 + kLaChunk);      // nothing past the last chunk
             __syncthreads();
@@ -546,14 +598,12 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
             for (int it = 0; it < QK_ITEMS; it++) k_now[it] = k_in[it];
             load_qk(p0 + 2 * kLaChunk);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                O[e] *= from_now;
-                P[e] *= near[e];
-            }
+            for (int e = 0; e < 16; e++) O[e] *= from_now;
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 la_frag pf[M::FORMED];
-                la_formed<M::FORMED>(P, 8 * s, pf, earlier);
+#pragma unroll
+                for (int p = 0; p < M::FORMED; p++) pf[p] = la_read(pt + (2 * p + s) * kLaFrag, lane, 0);
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
@@ -578,7 +628,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                 const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(uniform_ptr(o_at), 0, 0x7fffffff, 0x00020000);
                 const int c = col0 + 32 * wave;
                 const uint32_t nowhere = la_source<DT, true>::NOWHERE;
-                if (DT == FC_F32 || r.o32) {
+                if (DT == FC_F32 || r.o_fp32) {
 #pragma unroll
                     for (int a = 0; a < 4; a++)
                         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(la_u32x4, (la_f32x4){O[4 * a], O[4 * a + 1], O[4 * a + 2], O[4 * a + 3]}),
@@ -615,14 +665,13 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
                 for (int e = 0; e < 16; e++) {
                     const int c = col0 + 32 * wave + 8 * (e / 4) + 4 * g + e % 4;
                     if (c >= r.Dv) continue;
-                    if (r.o32) r.o32[((b * r.T + t) * r.H + h) * r.Dv + c] = O[e];
-                    else ((E *)r.o)[b * r.o_batch + t * r.o_token + h * r.o_head + c] = (E)O[e];
+                    la_answer<DT>(r, b * r.o_batch + t * r.o_token + h * r.o_head + c, O[e]);
                 }
             }
         }
     }
 
-    float *to_state = FULL ? (seg == segments - 1 && r.state_out ? r.state_out + bh * r.Dk * r.Dv : nullptr)
+    float *to_state = FULL ? (seg == segments - 1 && r.state_out ? r.state_out + bh * r.state_head : nullptr)
                            : parts + (bh * segments + seg) * (long)r.Dk * r.Dv;
     if (to_state) {
         const long orow = FULL ? r.state_row : r.Dv, ocol = FULL ? r.state_col : 1;
@@ -644,8 +693,7 @@ __global__ __launch_bounds__(64 * NW, KT <= 4 ? 2 : 1) void fc_linear_attention_
         for (int a = 0; a < NW; a++) {
             const int c = col0 + 32 * a + (tid & 31);
             if (c >= r.Dv) continue;
-            if (r.o32) r.o32[((b * r.T + t) * r.H + h) * r.Dv + c] = 0.f;
-            else ((E *)r.o)[b * r.o_batch + t * r.o_token + h * r.o_head + c] = (E)0.f;
+            la_answer<DT>(r, b * r.o_batch + t * r.o_token + h * r.o_head + c, 0.f);
         }
     }
 }
@@ -654,7 +702,7 @@ template <int DT, int KT, int NW>
 constexpr size_t la_lds_bytes(bool full) {
     typedef la_math<DT> M;
     const size_t qk = (size_t)2 * KT * kLaFrag, v = (size_t)2 * NW * kLaFrag;
-    return (full ? 2 * M::PARTS * qk : M::KEPT * qk + M::PARTS * v) + M::KEPT * qk + M::PARTS * v + (kLaChunk + 1) * (sizeof(double) + sizeof(float)) + (1 + 32 * NW) * sizeof(int);
+    return (full ? 2 * M::PARTS * qk + M::FORMED * 2 * kLaFrag : M::KEPT * qk + M::PARTS * v) + M::KEPT * qk + M::PARTS * v + (kLaChunk + 1) * (sizeof(double) + sizeof(float)) + (1 + 32 * NW) * sizeof(int);
 }
 
 // More LDS than 64 KB has to be asked for, once for each kernel and device.
@@ -683,8 +731,7 @@ int la_launch_one(fc_context *ctx, const fc_la_run &r, long heads, int segments,
 
 template <int DT, bool FULL>
 int la_launch(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts) {
-    // Two wavefronts where the state has no more than 64 columns, and where three parts of so many rows leave no LDS for four.
-    if (r.Dk > 128 && (r.Dv <= 64 || DT == FC_F32)) return la_launch_one<DT, 8, 2, FULL>(ctx, r, heads, segments, segment, parts);
+    // up to 128 rows; two wavefronts where the state has no more than 64 columns
     if (r.Dv <= 64) {
         if (r.Dk <= 32) return la_launch_one<DT, 1, 2, FULL>(ctx, r, heads, segments, segment, parts);
         if (r.Dk <= 64) return la_launch_one<DT, 2, 2, FULL>(ctx, r, heads, segments, segment, parts);
@@ -692,7 +739,5 @@ int la_launch(fc_context *ctx, const fc_la_run &r, long heads, int segments, lon
     }
     if (r.Dk <= 32) return la_launch_one<DT, 1, 4, FULL>(ctx, r, heads, segments, segment, parts);
     if (r.Dk <= 64) return la_launch_one<DT, 2, 4, FULL>(ctx, r, heads, segments, segment, parts);
-    if (r.Dk <= 128) return la_launch_one<DT, 4, 4, FULL>(ctx, r, heads, segments, segment, parts);
-    if constexpr (DT != FC_F32) return la_launch_one<DT, 8, 4, FULL>(ctx, r, heads, segments, segment, parts);
-    return FC_ERR_UNSUPPORTED;      // not reached
+    return la_launch_one<DT, 4, 4, FULL>(ctx, r, heads, segments, segment, parts);
 }
