@@ -51,20 +51,17 @@ __device__ __forceinline__ la_f32x4 la_product16(const la_frag &a, const la_frag
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  A value less its rounded
-// self is one instruction on the pair as it is packed, a - 1 * hi.lo + 0 * hi.hi, exact over the whole range of fp32 (an infinity in one makes
-// NaN of the other's second part: they are summed together anyway).  Bits that `keep` lacks are zeros in every part.
+// PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  Bits that `keep` lacks are zeros in
+// every part.  (A value less its rounded self is one v_dot2_f32_bf16 on the pair as it is packed, too, a - 1 * hi.lo + 0 * hi.hi; with
+// it the whole kernel takes 1.13 times as long.)
 template <int PARTS>
 __device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[PARTS], uint32_t keep = ~0u) {
-    uint32_t low = 0x0000bf80u, high = 0xbf800000u;      // (-1, 0) and (0, -1)
-    asm("" : "+s"(low), "+s"(high));                     // from registers: as a literal the first stands for another pair
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
         out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((la_f32x2){a, b}, la_bf16x2)) & keep;
         if (p + 1 < PARTS) {
-            const la_bf16x2 rounded = __builtin_bit_cast(la_bf16x2, out[p]);
-            a = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(la_bf16x2, low), a, false);
-            b = __builtin_amdgcn_fdot2_f32_bf16(rounded, __builtin_bit_cast(la_bf16x2, high), b, false);
+            a -= __builtin_bit_cast(float, out[p] << 16);
+            b -= __builtin_bit_cast(float, out[p] & 0xffff0000u);
         }
     }
 }
@@ -261,6 +258,51 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
     const long begin = seg * segment, end = begin + segment < len ? begin + segment : len;
     if (!FULL && begin >= end) return;
     const float ld = r.log_decay[h];
+    // this thread's tokens and channels of every operand, a chunk at a time
+    const long first = r.reverse ? len - 1 - begin : begin;
+    la_source<DT, WIDE> q_from[FULL ? QK_ITEMS : 1], k_from[QK_ITEMS], v_from[V_ITEMS];
+    la_block<DT> q_in[FULL ? QK_ITEMS : 1], k_in[QK_ITEMS], k_now[QK_ITEMS], v_in[V_ITEMS];
+#pragma unroll
+    for (int it = 0; it < QK_ITEMS; it++) {
+        const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
+        if (FULL) q_from[it].begin(r.q, r, b, h, first, tq, 4 * cq, r.Dk);
+        k_from[it].begin(r.k, r, b, h, first, tq, 4 * cq, r.Dk);
+    }
+#pragma unroll
+    for (int it = 0; it < V_ITEMS; it++) {
+        const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
+        v_from[it].begin(r.v, r, b, h, first, tq, col0 + 4 * cq, r.Dv);
+    }
+    auto load_qk = [&](long p0) __attribute__((always_inline)) {
+        const int n = la_tokens(p0, end);
+#pragma unroll
+        for (int it = 0; it < QK_ITEMS; it++) {
+            if (FULL) q_from[it].load(q_in[it], n);
+            k_from[it].load(k_in[it], n);
+        }
+    };
+    auto load_v = [&](long p0) __attribute__((always_inline)) {
+        const int n = la_tokens(p0, end);
+#pragma unroll
+        for (int it = 0; it < V_ITEMS; it++) v_from[it].load(v_in[it], n);
+    };
+    load_qk(begin);
+    load_v(begin);
+    // the state: rows 32*t + 8*(e/4) + 4*g + e%4 of column col, zeros in place of what it does not have
+    la_f32x16 S[KT];
+    const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.state_head : nullptr;
+    {
+        const uint32_t srow = segments > 1 ? r.Dv : (uint32_t)r.state_row, scol = segments > 1 ? 1 : (uint32_t)r.state_col;
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(uniform_ptr(from_state)), 0, from_state ? 0x7fffffff : 0, 0x00020000);
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int row = 32 * t + 8 * (e / 4) + 4 * g + e % 4;
+                S[t][e] = 0.f;
+                if (FULL) S[t][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(res, row < r.Dk && col < r.Dv ? 4 * (row * srow + col * scol) : 0x80000000u, 0, 0));
+            }
+    }
     if (FULL)
         for (int i = tid; i < M::FORMED * 2 * kLaFrag / 4; i += THREADS) ((uint32_t *)pt)[i] = 0;
 
@@ -297,46 +339,6 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
     // enough to be worth a pass over S.
     double scale = 1.0;
 
-    // the state: rows 32*t + 8*(e/4) + 4*g + e%4 of column col
-    la_f32x16 S[KT];
-    const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.state_head : nullptr;
-    const long srow = segments > 1 ? r.Dv : r.state_row, scol = segments > 1 ? 1 : r.state_col;
-#pragma unroll
-    for (int t = 0; t < KT; t++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int row = 32 * t + 8 * (e / 4) + 4 * g + e % 4;
-            S[t][e] = FULL && from_state && row < r.Dk && col < r.Dv ? from_state[row * srow + col * scol] : 0.f;
-        }
-
-    // this thread's tokens and channels of every operand, a chunk at a time
-    const long first = r.reverse ? len - 1 - begin : begin;
-    la_source<DT, WIDE> q_from[FULL ? QK_ITEMS : 1], k_from[QK_ITEMS], v_from[V_ITEMS];
-    la_block<DT> q_in[FULL ? QK_ITEMS : 1], k_in[QK_ITEMS], k_now[QK_ITEMS], v_in[V_ITEMS];
-#pragma unroll
-    for (int it = 0; it < QK_ITEMS; it++) {
-        const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
-        if (FULL) q_from[it].begin(r.q, r, b, h, first, tq, 4 * cq, r.Dk);
-        k_from[it].begin(r.k, r, b, h, first, tq, 4 * cq, r.Dk);
-    }
-#pragma unroll
-    for (int it = 0; it < V_ITEMS; it++) {
-        const int tq = la_tokens_of<DV>(tid + it * THREADS), cq = la_channels_of<DV>(tid + it * THREADS);
-        v_from[it].begin(r.v, r, b, h, first, tq, col0 + 4 * cq, r.Dv);
-    }
-    auto load_qk = [&](long p0) __attribute__((always_inline)) {
-        const int n = la_tokens(p0, end);
-#pragma unroll
-        for (int it = 0; it < QK_ITEMS; it++) {
-            if (FULL) q_from[it].load(q_in[it], n);
-            k_from[it].load(k_in[it], n);
-        }
-    };
-    auto load_v = [&](long p0) __attribute__((always_inline)) {
-        const int n = la_tokens(p0, end);
-#pragma unroll
-        for (int it = 0; it < V_ITEMS; it++) v_from[it].load(v_in[it], n);
-    };
     // token i of four of q and k
     auto put_natural = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -449,8 +451,6 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
         constexpr int HALF = M::KEPT * QK_PLANE + M::PARTS * V_PLANE;
         char *const halves = kt;
         int n = la_tokens(begin, end);
-        load_qk(begin);
-        load_v(begin);
         rescale(n);
         weigh(n, add);
 #pragma unroll
@@ -505,8 +505,6 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
         const long o_step = r.reverse ? -kLaChunk * o_row : kLaChunk * o_row;
         const uint32_t o_offset = (uint32_t)((r.reverse ? kLaChunk - 1 - i_tok : i_tok) * o_row + 32 * wave * o_size);
         char *o_at = (char *)r.o + (b * r.o_batch + h * r.o_head + col0) * o_size + (r.reverse ? first - (kLaChunk - 1) : first) * o_row;
-        load_qk(begin);
-        load_v(begin);
 #pragma unroll
         for (int i = 0; i < 4; i++) put_natural(i);
 #pragma unroll
@@ -526,7 +524,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
 #pragma unroll
             for (int n = 0; n < BLOCKS; n++) P[n] = (la_f32x4){0.f, 0.f, 0.f, 0.f};
             {
-                la_frag qf[2][M::PARTS], sf[M::FORMED];
+                la_frag qf[2][M::PARTS], sf[M::FORMED], qp[BLOCKS][M::PARTS], kp[BLOCKS][M::PARTS];
                 auto fetch = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
                     for (int p = 0; p < M::PARTS; p++) qf[s & 1][p] = la_read_natural(qs + p * QK_PLANE, s, lane);
@@ -536,7 +534,6 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
 #pragma unroll
                 for (int s = 0; s < 2 * KT; s++) {
                     if (s + 1 < 2 * KT) fetch(s + 1);
-                    la_frag qp[BLOCKS][M::PARTS], kp[BLOCKS][M::PARTS];
                     if (s % 2 == 0) {
 #pragma unroll
                         for (int n = 0; n < BLOCKS; n++) {
@@ -556,7 +553,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
 #pragma unroll
                         for (int c = 0; c < M::PARTS; c++)
                             if (a + c < M::ORDER) O = la_product(sf[a], qf[s & 1][c], O);
-                    if (s % 2 == 0) {
+                    if (s % 2 == 1) {      // read a step ago
 #pragma unroll
                         for (int n = 0; n < BLOCKS; n++) {
                             if (wave + n * NW >= 3) continue;
@@ -589,6 +586,12 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
             load_v(p0 + kLaChunk);      // nothing past the last chunk
             __syncthreads();
             read_v(vt);
+            la_frag pf[2][M::FORMED];
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int p = 0; p < M::FORMED; p++) pf[s][p] = la_read(pt + (2 * p + s) * kLaFrag, lane, 0);
+            const bool any_odd = *odd;
             settle_state();
             take_in(kt, [&](int i) __attribute__((always_inline)) {
 #pragma unroll
@@ -601,16 +604,13 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
             for (int e = 0; e < 16; e++) O[e] *= from_now;
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                la_frag pf[M::FORMED];
-#pragma unroll
-                for (int p = 0; p < M::FORMED; p++) pf[p] = la_read(pt + (2 * p + s) * kLaFrag, lane, 0);
 #pragma unroll
                 for (int a = 0; a < M::PARTS; a++)
 #pragma unroll
                     for (int c = 0; c < M::FORMED; c++)
-                        if (a + c < M::ORDER) O = la_product(vf[s][a], pf[c], O);
+                        if (a + c < M::ORDER) O = la_product(vf[s][a], pf[s][c], O);
             }
-            if (*odd) {
+            if (any_odd) {
                 const bool lost = since[32 * wave + i_tok] < kLaChunk;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
