@@ -27,6 +27,8 @@ struct fc_la_run {
     const float *state_in;   // element (row, column) of head bh at bh*state_head + row*state_row + column*state_col
     float *state_out;
     long state_head, state_row, state_col;
+    long part_row, part_col; // the same of the states that segments begin from
+    bool parts_ready;        // which another run has left, transposed or not
     const float *log_decay;
     const int32_t *lengths;
     long T;

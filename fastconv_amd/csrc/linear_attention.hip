@@ -221,7 +221,11 @@ int run_chunks(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run 
     r.wide = wide(r.q, r.Dk, es) && wide(r.k, r.Dk, es) && wide(r.v, r.Dv, es) &&
              wide({r.o, r.o_batch, r.o_token, r.o_head, 1}, r.Dv, r.o_fp32 ? sizeof(float) : es);
     const long heads = (long)s.B * s.H, segment = segment_of(s, plan->segments);
-    if (plan->segments > 1) {
+    if (!r.parts_ready) {
+        r.part_row = r.Dv;
+        r.part_col = 1;
+    }
+    if (plan->segments > 1 && !r.parts_ready) {
         const int rc = s.dtype == FC_F32    ? fc_la_state_f32(ctx, r, heads, plan->segments, segment, parts)
                        : s.dtype == FC_BF16 ? fc_la_state_bf16(ctx, r, heads, plan->segments, segment, parts)
                                             : fc_la_state_f16(ctx, r, heads, plan->segments, segment, parts);
@@ -366,19 +370,21 @@ extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_att
     r.o_batch = s.q_batch; r.o_token = s.q_token; r.o_head = s.q_head;
     int rc = run(ctx, plan, r, parts, sums, dq_dev, 1);
     if (rc) return rc;
-    // dk, from the last token to the first
+    // dv, from the last token to the first, and the gradient of the first state
     r.reverse = 1;
     r.scale_in = s.scale; r.scale_out = 1.f;
-    r.q = v; r.k = d; r.v = q;
-    r.state_in = dstate_out_dev;
-    r.o_batch = s.k_batch; r.o_token = s.k_token; r.o_head = s.k_head;
-    rc = run(ctx, plan, r, parts, sums, dk_dev, share);
-    if (rc) return rc;
-    // dv, and the gradient of the first state
     r.q = k; r.k = q; r.v = d;
     r.Dk = s.Dk; r.Dv = s.Dv;
-    r.state_row = s.Dv; r.state_col = 1;
-    r.state_out = dstate_in_dev;
+    r.state_in = dstate_out_dev; r.state_out = dstate_in_dev; r.state_row = s.Dv; r.state_col = 1;
     r.o_batch = s.v_batch; r.o_token = s.v_token; r.o_head = s.v_head;
-    return run(ctx, plan, r, parts, sums, dv_dev, share);
+    rc = run(ctx, plan, r, parts, sums, dv_dev, share);
+    if (rc) return rc;
+    // dk: its segments begin from the same states, transposed
+    r.q = v; r.k = d; r.v = q;
+    r.Dk = s.Dv; r.Dv = s.Dk;
+    r.state_out = nullptr; r.state_row = 1; r.state_col = s.Dv;
+    r.parts_ready = plan->segments > 1 && s.Dk <= kChunkRows && s.Dv <= kChunkRows;
+    r.part_row = 1; r.part_col = s.Dv;
+    r.o_batch = s.k_batch; r.o_token = s.k_token; r.o_head = s.k_head;
+    return run(ctx, plan, r, parts, sums, dk_dev, share);
 }

@@ -292,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
     la_f32x16 S[KT];
     const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.state_head : nullptr;
     {
-        const uint32_t srow = segments > 1 ? r.Dv : (uint32_t)r.state_row, scol = segments > 1 ? 1 : (uint32_t)r.state_col;
+        const uint32_t srow = (uint32_t)(segments > 1 ? r.part_row : r.state_row), scol = (uint32_t)(segments > 1 ? r.part_col : r.state_col);
         const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(uniform_ptr(from_state)), 0, from_state ? 0x7fffffff : 0, 0x00020000);
 #pragma unroll
         for (int t = 0; t < KT; t++)
