@@ -6,7 +6,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 256;
-constexpr long kMostSteps = 16;    // up to here the recurrence is faster
+// Up to so many tokens run through the recurrence, about 1 us each; a chunk costs 11 to 15 us with one token or 32.  1 sequence of 16 heads of 128
+// in bf16: 4 tokens 8.3 and 11.4 us, 8 tokens 12.2 and 11.3; 8 sequences 10.1 and 12.4, 14.6 and 12.5; 64 of 16 heads of 64 16.5 and 13.5, 24.1 and 13.6;
+// 8 of 8 heads of 128 in fp32 8.3 and 15.3, 12.2 and 15.4.
+constexpr long kMostSteps = 6;
 constexpr long kWavefronts = 2048, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kChunkRows = 128;    // rows of a state that their kernel holds
@@ -25,10 +28,28 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
     const long bh = blockIdx.x / slices, b = bh / r.H;
     const int h = (int)(bh - b * r.H), c0 = (int)(blockIdx.x - bh * slices) * kStepCols + 4 * col;
     const long len = fc_la_length(r, b);
-    const fc_la_power decay(r.log_decay[h], 1);
+    const float log_decay = r.log_decay[h];
     const bool wide = r.state_col == 1 && (r.Dv & 3) == 0 &&
                       (((uintptr_t)r.state_in | (uintptr_t)r.state_out) & 15) == 0;      // four columns an access
 
+    const E *q = (const E *)r.q.p + b * r.q.batch + (h / r.q.share) * r.q.head;
+    const E *k = (const E *)r.k.p + b * r.k.batch + (h / r.k.share) * r.k.head;
+    const E *v = (const E *)r.v.p + b * r.v.batch + (h / r.v.share) * r.v.head;
+    const long o = b * r.o_batch + h * r.o_head;
+
+    // a token's values are read while the one before it is taken in
+    E q_in = (E)0.f, k_in = (E)0.f, v_in[4] = {(E)0.f, (E)0.f, (E)0.f, (E)0.f};
+    auto load = [&](long n) __attribute__((always_inline)) {
+        const long t = r.reverse ? len - 1 - n : n;
+        if (tid < r.Dk) {
+            q_in = q[t * r.q.token + tid];
+            k_in = k[t * r.k.token + tid];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (c0 + j < r.Dv) v_in[j] = v[t * r.v.token + c0 + j];
+    };
+    if (len > 0) load(0);
     float s[ROWS][4];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
@@ -46,24 +67,21 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
                 if (c0 + j < r.Dv) s[i][j] = src[j * r.state_col];
         }
     }
-    const E *q = (const E *)r.q.p + b * r.q.batch + (h / r.q.share) * r.q.head;
-    const E *k = (const E *)r.k.p + b * r.k.batch + (h / r.k.share) * r.k.head;
-    const E *v = (const E *)r.v.p + b * r.v.batch + (h / r.v.share) * r.v.head;
-    const long o = b * r.o_batch + h * r.o_head;
-
+    const fc_la_power decay(log_decay, 1);
     for (long n = 0; n < len; n++) {
         const long t = r.reverse ? len - 1 - n : n;
         const int buf = n & 1;
         if (tid < r.Dk) {
-            qs[buf][tid] = (float)q[t * r.q.token + tid] * r.scale_out;
-            ks[buf][tid] = (float)k[t * r.k.token + tid] * r.scale_in;
+            qs[buf][tid] = (float)q_in * r.scale_out;
+            ks[buf][tid] = (float)k_in * r.scale_in;
         }
         float vv[4], out[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            vv[j] = c0 + j < r.Dv ? (float)v[t * r.v.token + c0 + j] : 0.f;
+            vv[j] = (float)v_in[j];
             out[j] = 0.f;
         }
+        if (n + 1 < len) load(n + 1);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
