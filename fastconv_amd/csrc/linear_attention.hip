@@ -10,23 +10,25 @@ constexpr int kMaxDim = 256;
 // in bf16: 4 tokens 8.3 and 11.4 us, 8 tokens 12.2 and 11.3; 8 sequences 10.1 and 12.4, 14.6 and 12.5; 64 of 16 heads of 64 16.5 and 13.5, 24.1 and 13.6;
 // 8 of 8 heads of 128 in fp32 8.3 and 15.3, 12.2 and 15.4.
 constexpr long kMostSteps = 6;
+constexpr long kWholeRows = 512;   // heads from which the recurrence takes 128 columns a workgroup
 constexpr long kWavefronts = 2048, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kChunkRows = 128;    // rows of a state that their kernel holds
-constexpr int kStepCols = 32;      // columns of the state that a workgroup of the recurrence holds
 
-// The recurrence.  A workgroup holds 32 columns of a head's state in registers: 8 threads side by side with 4 columns each,
-// 32 threads deep with ROWS rows each.  A token costs two barriers: its q and k lie in LDS for all, its answer is summed over
+// The recurrence.  A workgroup holds some columns of a head's state in registers: COLS threads side by side with 4 columns each, as
+// many deep as there are, with ROWS rows each.  A token costs two barriers: its q and k lie in LDS for all, its answer is summed over
 // the rows in the wavefront and then over the four wavefronts.
-// Bound by the state, which is read and written once a call, 8 bytes an element against 4 operations a token.
-template <int DT, int ROWS>
+// Bound by the state, which is read and written once a call, 8 bytes an element against 4 operations a token.  32 columns a workgroup
+// spread one sequence's heads over the chip; 128, whole rows, read longer pieces and sum over fewer lanes.
+template <int DT, int ROWS, int COLS>
 __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(const fc_la_run r) {
     typedef typename fc_elem<DT>::type E;
-    __shared__ float qs[2][kMaxDim], ks[2][kMaxDim], part[2][4][kStepCols];
-    const int tid = threadIdx.x, col = tid & 7, row = tid >> 3;
-    const int slices = (r.Dv + kStepCols - 1) / kStepCols;
+    constexpr int DEEP = kThreads / COLS, WIDTH = 4 * COLS;
+    __shared__ float qs[2][kMaxDim], ks[2][kMaxDim], part[2][4][WIDTH];
+    const int tid = threadIdx.x, col = tid % COLS, row = tid / COLS;
+    const int slices = (r.Dv + WIDTH - 1) / WIDTH;
     const long bh = blockIdx.x / slices, b = bh / r.H;
-    const int h = (int)(bh - b * r.H), c0 = (int)(blockIdx.x - bh * slices) * kStepCols + 4 * col;
+    const int h = (int)(bh - b * r.H), c0 = (int)(blockIdx.x - bh * slices) * WIDTH + 4 * col;
     const long len = fc_la_length(r, b);
     const float log_decay = r.log_decay[h];
     const bool wide = r.state_col == 1 && (r.Dv & 3) == 0 &&
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
     float s[ROWS][4];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int rr = row + 32 * i;
+        const int rr = row + DEEP * i;
 #pragma unroll
         for (int j = 0; j < 4; j++) s[i][j] = 0.f;
         if (!r.state_in || rr >= r.Dk || c0 >= r.Dv) continue;
@@ -85,7 +87,7 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
-            const int rr = row + 32 * i;
+            const int rr = row + DEEP * i;
             if (rr >= r.Dk) break;
             const float kr = ks[buf][rr], qr = qs[buf][rr];
 #pragma unroll
@@ -98,31 +100,31 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
 #pragma unroll
         for (int j = 0; j < 4; j++) {
 #pragma unroll
-            for (int m = 8; m < 64; m <<= 1) out[j] += __shfl_xor(out[j], m);
+            for (int m = COLS; m < 64; m <<= 1) out[j] += __shfl_xor(out[j], m);
         }
-        if ((tid & 63) < 8) {
+        if ((tid & 63) < COLS) {
 #pragma unroll
             for (int j = 0; j < 4; j++) part[buf][tid >> 6][4 * col + j] = out[j];
         }
         __syncthreads();
-        const int c = (int)(blockIdx.x - bh * slices) * kStepCols + tid;
-        if (tid < kStepCols && c < r.Dv) {
+        const int c = (int)(blockIdx.x - bh * slices) * WIDTH + tid;
+        if (tid < WIDTH && c < r.Dv) {
             const float sum = (part[buf][0][tid] + part[buf][1][tid]) + (part[buf][2][tid] + part[buf][3][tid]);
             if (r.o_fp32) ((float *)r.o)[o + t * r.o_token + c] = sum;
             else ((E *)r.o)[o + t * r.o_token + c] = (E)sum;
         }
     }
     // tokens past the end of a shorter sequence
-    const int c = (int)(blockIdx.x - bh * slices) * kStepCols + (tid & 31);
+    const int c = (int)(blockIdx.x - bh * slices) * WIDTH + tid % WIDTH;
     if (c < r.Dv)
-        for (long t = len + (tid >> 5); t < r.T; t += kThreads / 32) {
+        for (long t = len + tid / WIDTH; t < r.T; t += kThreads / WIDTH) {
             if (r.o_fp32) ((float *)r.o)[o + t * r.o_token + c] = 0.f;
             else ((E *)r.o)[o + t * r.o_token + c] = (E)0.f;
         }
     if (!r.state_out) return;
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        const int rr = row + 32 * i;
+        const int rr = row + DEEP * i;
         if (rr >= r.Dk || c0 >= r.Dv) continue;
         float *dst = r.state_out + bh * r.state_head + rr * r.state_row + c0 * r.state_col;
         if (wide) {
@@ -211,19 +213,28 @@ long segment_of(const fc_linear_attention_shape &s, int segments) {
     return (chunks + segments - 1) / segments * kChunk;
 }
 
+template <int DT, int ROWS, int COLS>
+void launch_step_as(fc_context *ctx, const fc_la_run &r, long heads) {
+    const unsigned blocks = (unsigned)(heads * ((r.Dv + 4 * COLS - 1) / (4 * COLS)));
+    fc_linear_attention_step_kernel<DT, ROWS, COLS><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+}
+
 template <int DT>
-void launch_step(fc_context *ctx, const fc_la_run &r, long B) {
-    const unsigned blocks = (unsigned)(B * r.H * ((r.Dv + kStepCols - 1) / kStepCols));
-    if (r.Dk <= 32) fc_linear_attention_step_kernel<DT, 1><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
-    else if (r.Dk <= 64) fc_linear_attention_step_kernel<DT, 2><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
-    else if (r.Dk <= 128) fc_linear_attention_step_kernel<DT, 4><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
-    else fc_linear_attention_step_kernel<DT, 8><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(r);
+void launch_step(fc_context *ctx, const fc_la_run &r, long heads) {
+    if (r.Dv > 64 && r.Dk <= 128 && heads >= kWholeRows) {
+        if (r.Dk <= 64) launch_step_as<DT, 8, 32>(ctx, r, heads);
+        else launch_step_as<DT, 16, 32>(ctx, r, heads);
+    } else if (r.Dk <= 32) launch_step_as<DT, 1, 8>(ctx, r, heads);
+    else if (r.Dk <= 64) launch_step_as<DT, 2, 8>(ctx, r, heads);
+    else if (r.Dk <= 128) launch_step_as<DT, 4, 8>(ctx, r, heads);
+    else launch_step_as<DT, 8, 8>(ctx, r, heads);
 }
 
 int run_step(fc_context *ctx, const fc_linear_attention_shape &s, const fc_la_run &r) {
-    if (s.dtype == FC_F32) launch_step<FC_F32>(ctx, r, s.B);
-    else if (s.dtype == FC_BF16) launch_step<FC_BF16>(ctx, r, s.B);
-    else launch_step<FC_F16>(ctx, r, s.B);
+    const long heads = (long)s.B * s.H;
+    if (s.dtype == FC_F32) launch_step<FC_F32>(ctx, r, heads);
+    else if (s.dtype == FC_BF16) launch_step<FC_BF16>(ctx, r, heads);
+    else launch_step<FC_F16>(ctx, r, heads);
     FC_LAUNCH_CHECK(ctx, "fc_linear_attention_step_kernel");
     return FC_OK;
 }

@@ -125,6 +125,9 @@ CASES = [  # B, T, H, Hkv, Dk, Dv, dtype, layout, lengths, carry
     (1, 1500, 2, 1, 32, 48, "f16", "joined", None, False),
     (2, 1225, 2, 2, 64, 96, "f32", "packed", (1225, 640), True),
     (1, 2500, 1, 1, 128, 128, "bf16", "packed", None, True),
+    (64, 3, 8, 4, 128, 96, "bf16", "packed", None, True),         # many heads, few tokens: whole rows of the states
+    (130, 2, 4, 4, 50, 130, "f32", "odd", None, True),
+    (128, 6, 4, 2, 128, 128, "f16", "heads first", (6, 0) * 64, False),
 ]
 
 
