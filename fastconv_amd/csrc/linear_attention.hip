@@ -5,13 +5,23 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr long kMostThreads = 1l << 32;      // of a launch, not reached; a head has up to 8 workgroups
 constexpr int kMaxDim = 256;
 // Up to so many tokens run through the recurrence, about 1 us each; a chunk costs 11 to 15 us with one token or 32.  1 sequence of 16 heads of 128
 // in bf16: 4 tokens 8.3 and 11.4 us, 8 tokens 12.2 and 11.3; 8 sequences 10.1 and 12.4, 14.6 and 12.5; 64 of 16 heads of 64 16.5 and 13.5, 24.1 and 13.6;
 // 8 of 8 heads of 128 in fp32 8.3 and 15.3, 12.2 and 15.4.
 constexpr long kMostSteps = 6;
 constexpr long kWholeRows = 512;   // heads from which the recurrence takes 128 columns a workgroup
-constexpr long kWavefronts = 2048, kLeastChunks = 8;      // a sequence is cut up to fill the chip, into segments worth their states
+// A sequence is cut up to fill the chip: 16 heads of 128, 12544 tokens in bf16 140 us for 1024 wavefronts, 121 for 2048 and 145 for 4096; with a
+// backward pass, 8 x 16 heads of 64 and 3136 tokens 422, 330 and 393.
+constexpr long kWavefronts = 2048;
+// A cut costs two launches, k and v read twice, and a state a segment, written and read twice.  In two parts it loses (32 x 16 heads of 64, 4096
+// tokens: 388 us against 351 uncut; 1024 tokens 124 and 97), in three it gains (21 x 16 heads, 2048 tokens: 139 and 178).
+constexpr long kLeastSegments = 3;
+// Segments of two chunks, but where states are larger than what a segment reads and many: of four.  8 x 1225 tokens of 64x128 in fp32 with a
+// backward pass 220 us in segments of 3 chunks, 284 of 5 and 475 of 10; 16 heads of 128, 512 tokens: 29.6 in 8 segments, 35.5 in 4; 2048 tokens:
+// 42 in 16, 51 in 32.
+constexpr long kSmallState = 64 * 128, kFewSegments = 8;
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kChunkRows = 128;    // rows of a state that their kernel holds
 
@@ -314,7 +324,7 @@ int run(fc_context *ctx, const fc_linear_attention_plan *plan, fc_la_run r, floa
 
 extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s, fc_linear_attention_plan *plan) {
     if (!plan || !shape_ok(s)) return FC_ERR_INVALID;
-    if (s->Dk > kMaxDim || s->Dv > kMaxDim || fc_count(s->B, s->H) < 0 || fc_count(s->B, s->H) >= (1l << 31) / 8) return FC_ERR_UNSUPPORTED;
+    if (s->Dk > kMaxDim || s->Dv > kMaxDim || fc_count(s->B, s->H) < 0 || fc_count(s->B, s->H) >= kMostThreads / kThreads / 8) return FC_ERR_UNSUPPORTED;
     const int most = s->Dk > s->Dv ? s->Dk : s->Dv;
     const long tokens = fc_count(s->B, s->T), values = tokens < 0 ? -1 : fc_count(tokens, s->H, 8 * most);
     if (s->T >= (1l << 31) || values < 0) return FC_ERR_UNSUPPORTED;
@@ -325,12 +335,14 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
         plan->chunk = kChunk;
         const long wavefronts = most <= 64 ? 2 : 4 * ((most + 127) / 128), chunks = (s->T + kChunk - 1) / kChunk;
         long segments = kWavefronts / (s->B * (long)s->H * wavefronts);
-        if (segments > chunks / kLeastChunks) segments = chunks / kLeastChunks;
+        long worth = chunks / 2;
+        if ((long)s->Dk * s->Dv > kSmallState && worth > kFewSegments) worth = chunks / 4 > kFewSegments ? chunks / 4 : kFewSegments;
+        if (segments > worth) segments = worth;
         if (segments > 1) {
             const long per = (chunks + segments - 1) / segments;
             segments = (chunks + per - 1) / per;
         }
-        if (segments > 1) plan->segments = (int)segments;
+        if (segments >= kLeastSegments) plan->segments = (int)segments;
         if (plan->segments > 1) plan->ws_bytes = (size_t)s->B * s->H * plan->segments * s->Dk * s->Dv * sizeof(float);
     }
     // Answers that are added up afterwards: of the forward run, of the largest backward one.
