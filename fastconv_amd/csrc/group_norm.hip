@@ -5,8 +5,11 @@
 //   dx = rstd * (gamma dz - (s1 + xhat s2) / (P * C/G)),  s1 = sum over the group of gamma dz,  s2 = of gamma dz xhat
 //
 // Bound by memory: about 10 operations an element against 4 bytes in 16-bit types.  The first y needs the last x of its
-// group, so the pixels of an image are cut into chunks: one launch leaves each chunk's statistics, the next joins them and
-// writes the result, reading x a second time (from the 256 MB cache where x fits that).
+// group.  Where a few channels' pixels fit the registers of a workgroup, they wait there: one launch, x read once (1 image of 14x14x512 in bf16
+// 6.5 us, the time of a launch with three waits on memory; 32 of 56x56x256 in fp32 51 us, 4.0 TB/s).  Otherwise the pixels of an image are cut into
+// chunks: one launch leaves each chunk's statistics, the next joins them and writes the result, reading x a second time, from the 256 MB cache
+// where x fits that (32 images of 224x224x64 in bf16, 206 MB: 40 us at 5.1 TB/s and 75 at 5.5).  Backward likewise, with dy beside x (32 of 56x56x256 in
+// fp32: sums 44 us, 4.7 TB/s; gradients 52, 5.9 TB/s).
 // A thread keeps to one column of 4 to 16 bytes of channels and walks down the pixels, so that whatever belongs to a channel
 // stays in registers; a wavefront reads whole lines.
 // Statistics are joined, never subtracted: a thread forms the mean of each batch of pixels and the squares of what differs
@@ -21,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxGroupChannels = 4096;
+constexpr long kMostThreads = 1l << 32;                // of a launch, not reached
 constexpr double kCacheBytes = 256.0 * (1 << 20);      // the last cache before HBM
 
 struct norm_params {
@@ -164,19 +168,33 @@ __device__ __forceinline__ void sum_groups_fast(const norm_params &p, const norm
 #pragma unroll
         for (int v = 0; v < VEC; v++) value[v] = s;
     } else {
-        sum_lanes<VEC>(value, f.cols);
-        __syncthreads();
-        if (((int)threadIdx.x & 63) < f.cols) {
+        // one value a group of the access: 8 images of 56x56 with 128 channels in 32 groups, bf16: 18.9 -> 13.0 us
+        auto join = [&](auto channels) __attribute__((always_inline)) {
+            constexpr int STEP = decltype(channels)::value;
 #pragma unroll
-            for (int v = 0; v < VEC; v++) lds[(unit * f.cols + th.tx) * VEC + v] = value[v];
-        }
-        __syncthreads();
+            for (int m = 32; m; m >>= 1) {
+                if (m < f.cols) break;
 #pragma unroll
-        for (int v = 0; v < VEC; v++) value[v] = 0.f;
-        for (int u = 0; u < units; u++) {
+                for (int v = 0; v < VEC; v += STEP) value[v] += __shfl_xor(value[v], m);
+            }
+            __syncthreads();
+            if (((int)threadIdx.x & 63) < f.cols) {
 #pragma unroll
-            for (int v = 0; v < VEC; v++) value[v] += lds[(u * f.cols + th.tx) * VEC + v];
-        }
+                for (int v = 0; v < VEC; v += STEP) lds[(unit * f.cols + th.tx) * VEC + v] = value[v];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < VEC; v++) value[v] = 0.f;
+            for (int u = 0; u < units; u++) {
+#pragma unroll
+                for (int v = 0; v < VEC; v += STEP) value[v] += lds[(u * f.cols + th.tx) * VEC + v];
+            }
+#pragma unroll
+            for (int v = 0; v < VEC; v++) value[v] = value[v / STEP * STEP];
+        };
+        if (p.Cg == 1) join(std::integral_constant<int, 1>());
+        else if (VEC > 2 && p.Cg == 2) join(std::integral_constant<int, (VEC > 2 ? 2 : 1)>());
+        else join(std::integral_constant<int, (VEC > 1 ? VEC / 2 : 1)>());
     }
 }
 
@@ -636,6 +654,21 @@ __device__ __forceinline__ void sum_channels(const norm_params &p, const norm_bu
     }
 }
 
+// Values of 16 bits stay packed between two passes over them: the compiler would keep the unpacked ones, twice the registers (16 accesses
+// forward and 8 backward spilled 112 and 67; 32 images of 56x56x256 in bf16: forward 65 -> 35 us, backward 124 -> 69).
+template <class V, int R>
+__device__ __forceinline__ void keep_packed(V (&x)[R]) {
+    typedef unsigned __attribute__((ext_vector_type(4))) words;
+    if constexpr (sizeof(x[0].v[0]) == 2) {
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            words w = __builtin_bit_cast(words, x[k]);
+            asm("" : "+v"(w));
+            x[k] = __builtin_bit_cast(V, w);
+        }
+    }
+}
+
 // R pixels of its column a thread.
 template <int DT, int VEC, int ACT, int THREADS, int R>
 __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const norm_params p) {
@@ -663,6 +696,7 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
     }
     const float values = (float)p.P * p.Cg;
     const norm_butterfly fast(p, VEC, THREADS);
+    keep_packed(in);
     sum_groups<VEC, THREADS>(p, fast, th, sum, resident_sums);
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
@@ -674,6 +708,7 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_kernel(const n
             sum[v] = __builtin_fmaf(d, d, sum[v]);
         }
     }
+    keep_packed(in);
     sum_groups<VEC, THREADS>(p, fast, th, sum, resident_sums);
     if (th.ty >= th.rows) return;
     float scale[VEC], shift[VEC];
@@ -738,6 +773,8 @@ __global__ __launch_bounds__(THREADS) void fc_group_norm_resident_gradient_kerne
         }
     }
     const norm_butterfly fast(p, VEC, THREADS);
+    keep_packed(xs);
+    keep_packed(ds);
     sum_channels<VEC, THREADS>(p, fast, th, a, resident_sums, &channel->x);
     sum_channels<VEC, THREADS>(p, fast, th, b, resident_sums, &channel->y);
     if (p.channel_part && (int)threadIdx.x < p.span) p.channel_part[n * p.C + c0 + threadIdx.x] = channel[threadIdx.x];
@@ -853,29 +890,42 @@ int resident_pixels(long P, int span, int vec, int threads, int most) {
     return need <= r ? r : 0;
 }
 
-// 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.
+// 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.  Resident against not, 32 images of 56x56x256: forward in bf16 35 and 40 us, in
+// fp32 51 and 58; 1 of 14x14x512 in bf16 forward and backward 16 and 26; 128 of 28x28x512 in fp32 backward 196 and 232.
 constexpr int kResident = 16, kResidentBackward = 8;
-// Forward and backward together, resident against not: 1 image of 14x14x512 in bf16 16 and 28 us, 8 of 35x35x192 in half 32 and 37, 32 of 28x28x512 in half
-// (26 MB) 63 and 69; but 32 of 56x56x256 in fp32 (103 MB) 157 and 152, 128 of them in bf16 (206 MB) 743 and 532: the phases of two large
-// workgroups on a compute unit overlap less than those of many small ones, and the cache holds what is read twice.
-constexpr double kResidentBackwardBytes = 64e6;
-constexpr long kResidentWorkgroups = 256;      // below, a wider workgroup would leave compute units idle
+// With fewer, a wider workgroup leaves compute units idle: 1 image of 14x14x512 in bf16 6.5 us in 32 workgroups and 9.1 in 16, 8 of 35x35x192 in half
+// 13.9 and 17.4 in 32.
+constexpr long kResidentWorkgroups = 256;
 
-// Channels of a resident workgroup: whole groups and whole accesses of 16 bytes, and with them 64 bytes of a pixel if they fit (half a
-// cache line); 0 if not even those fit.
-int resident_span(const fc_group_norm_shape *s, int most) {
-    const int Cg = s->C / s->G, vec = 16 / (int)fc_elem_size(s->dtype);
+// Less than 64 bytes of a pixel (half a cache line) are read well by few workgroups with a short wait before their sums.  Forward, resident against
+// not, in bf16: 8 images of 8000x256 as 256 workgroups of 16 bytes 32 and 37 us; but 32 of 6272x256 as 512 of 32 bytes 77 and 74, as 1024 of 16
+// bytes 112; 4 of 12544x128 as 64 workgroups with 16 accesses a thread 36 and 24.  Backward twice as much would be read again, from the last cache
+// if it holds that: 32 of 3136x256 as 32 bytes in bf16 69 and 82, in fp32 (103 MB a tensor) 102 and 95.
+constexpr long kWhole = 64;
+constexpr int kResidentNarrow = 8;
+constexpr double kNarrowBackwardBytes = 64e6;
+
+// Channels of a resident workgroup: whole groups and whole accesses of 16 bytes, and with them kWhole bytes of a pixel if they fit; 0 if not even
+// those fit, or are read badly.
+int resident_span(const fc_group_norm_shape *s, bool backward) {
+    const int Cg = s->C / s->G, es = (int)fc_elem_size(s->dtype), vec = 16 / es, most = backward ? kResidentBackward : kResident;
     if (fc_widest(s->dtype, (uint64_t)(s->C | s->x_image | s->x_pixel | s->y_image | s->y_pixel), 0) != vec) return 0;
     const long step = Cg / gcd(Cg, vec) * vec;
     if (step > 256) return 0;
     int found = 0;
     for (long span = step; span <= s->C && span <= 256; span *= 2) {
         if (s->C % span || !resident_pixels(s->P, (int)span, vec, 1024, most)) break;
-        if (found && s->N * (s->C / span) < kResidentWorkgroups) break;
+        if (found && (long)s->N * (s->C / span) < kResidentWorkgroups) break;
         found = (int)span;
-        if (span * (long)fc_elem_size(s->dtype) >= 64) break;
+        if (span * es >= kWhole) break;
     }
-    return fc_count(s->N, s->C) < (1l << 31) ? found : 0;
+    if (!found) return 0;
+    const long blocks = (long)s->N * (s->C / found);
+    if (found * es < kWhole) {
+        if (backward && (double)s->N * s->P * s->C * es > kNarrowBackwardBytes) return 0;
+        if (!backward && (blocks > kResidentWorkgroups || !resident_pixels(s->P, found, vec, 1024, kResidentNarrow))) return 0;
+    }
+    return blocks * 1024 < kMostThreads ? found : 0;
 }
 
 template <int DT, int VEC, int ACT, bool BACKWARD, int THREADS>
@@ -960,7 +1010,8 @@ extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_no
     if (span > s->C) span = s->C;
     plan->span = (int)span;
     const long spans = (s->C + span - 1) / span, pixels = s->P;
-    // about four workgroups a compute unit, of 32 KB and more each
+    // about four workgroups a compute unit, of 32 KB and more each: 32 images of 56x56x256 in fp32 with a backward pass 145 us with 512 or 1024 of them,
+    // 151 with 2048; 4 of 112x112x128 in bf16 with a backward pass 58 in parts of 32 KB, 80 in parts of 16
     long chunks = 1024 / (s->N * spans);
     const long least = 32768 / (span * (long)fc_elem_size(s->dtype)) + 1;
     if (chunks > (pixels + least - 1) / least) chunks = (pixels + least - 1) / least;
@@ -968,11 +1019,10 @@ extern "C" int fc_group_norm_make_plan(const fc_group_norm_shape *s, fc_group_no
     if (chunks > 256) chunks = 256;
     const long chunk = (pixels + chunks - 1) / chunks;
     chunks = (pixels + chunk - 1) / chunk;
-    if (chunk >= (1l << 30) || s->N * spans * chunks >= (1l << 31) - 65536) return FC_ERR_UNSUPPORTED;
-    const double values = (double)s->N * s->P * s->C;
+    if (chunk >= (1l << 30) || (s->N * spans * chunks + s->C / 8 + 1) * kThreads >= kMostThreads) return FC_ERR_UNSUPPORTED;
     plan->chunks = (int)chunks;
-    plan->resident = resident_span(s, kResident);
-    plan->resident_backward = values * fc_elem_size(s->dtype) <= kResidentBackwardBytes ? resident_span(s, kResidentBackward) : 0;
+    plan->resident = resident_span(s, false);
+    plan->resident_backward = resident_span(s, true);
     plan->ws_bytes = (size_t)s->N * s->G * chunks * sizeof(float2);
     plan->ws_backward_bytes = plan->ws_bytes + (size_t)s->N * chunks * s->C * sizeof(float2);
     return FC_OK;

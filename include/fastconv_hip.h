@@ -462,7 +462,7 @@ typedef enum { FC_ACT_NONE = 0, FC_ACT_RELU = 1, FC_ACT_SILU = 2, FC_ACT_GELU = 
  *   xhat = (x - mean) * rstd over the P*C/G values of a group,  rstd = 1/sqrt(variance + eps)
  *   y = act(gamma * xhat + beta)
  * Pixel p of image n begins at n*x_image + p*x_pixel; y (and dy) likewise, dx as x.  G == 1 is a layer norm over whole images,
- * G == C an instance norm.  Limit: C/G <= 4096. */
+ * G == C an instance norm.  Limits: C/G <= 4096, and about 2^24 images. */
 typedef struct {
     int N;
     long P;
@@ -476,8 +476,8 @@ typedef struct {
     fc_group_norm_shape shape;
     int span;                 /* channels that one workgroup reads of a pixel: whole groups */
     int chunks;               /* parts that the pixels of an image are cut into */
-    int resident;             /* channels whose groups stay in a workgroup's registers, so that x is read once; 0: they */
-    int resident_backward;    /* do not fit, or tensors that do not begin on 16 bytes, and x is read twice */
+    int resident;             /* channels whose groups stay in a workgroup's registers, so that x is read once; 0: they do */
+    int resident_backward;    /* not fit, and x is read twice, as it is by a call whose tensors do not begin on 16 bytes */
     size_t ws_bytes;          /* workspace of the forward call, 0 if none */
     size_t ws_backward_bytes; /* and of the backward call */
 } fc_group_norm_plan;
@@ -502,7 +502,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan *plan, cons
  * Channels from 2R on pass unchanged.  positions: int32 [B][T][axes], those of sequence b at b*positions_batch (0: the same
  * ones for all); any int32 is a position, and the angle is reduced in 64 bits.  q has Hq heads and k Hk (0: no k).
  * Token t of sequence b and head h begins at b*q_batch + t*q_token + h*q_head, and so for k and both outputs.
- * Limits: D <= 1024. */
+ * Limits: D <= 1024, Hq + Hk <= 65536, fewer than 2^25 tokens in all. */
 #define FC_ROTARY_AXES 4
 typedef struct {
     int B;
@@ -532,7 +532,8 @@ int fc_rotary(fc_context *ctx, const fc_rotary_shape *shape, const void *q_dev, 
  * grows); minus infinity is a decay of 0, a token that sees itself alone.
  * lengths: B int32, or NULL when every sequence has T tokens; sequence b then ends after min(max(lengths[b], 0), T) of them: its later
  * tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
- * Limits: Dk, Dv <= 256. */
+ * A value that is not finite reaches no token before its own; in v it makes its channel of the state NaN from then on.
+ * Limits: Dk, Dv <= 256, B*H < 2^21. */
 typedef struct {
     int B;
     long T;

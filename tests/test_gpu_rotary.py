@@ -210,6 +210,7 @@ def test_refusals(lib):
     refused(-1, pairs=-1)
     refused(-1, pairs=9)                 # 33 pairs of 64 channels
     refused(-1, q_token=-1)
+    refused(-6, T=1 << 24)               # of two sequences
     for name in ("q", "k", "positions", "inv_freq", "q_out", "k_out"):
         refused(-1, **{name: None})
     refused(-1, q=p + 1)

@@ -92,3 +92,24 @@ def test_spans_are_whole_groups_that_fit():
         for dtype in (capi.F32, capi.BF16):
             rc, plan = norm(C=c, G=g, x_pixel=c, y_pixel=c, dtype=dtype)
             assert rc == 0 and 0 < plan.span <= 4096 and plan.span % (c // g) == 0 and plan.chunks >= 1
+
+
+def test_launches_stay_below_their_limit():
+    assert norm(N=1 << 24)[0] == -6
+    rc, plan = norm(N=(1 << 21) - 1)
+    assert rc == 0 and plan.resident == 32
+    rc, plan = norm(N=1 << 21)      # two resident workgroups of 1024 threads an image would be 2^32 threads
+    assert rc == 0 and plan.resident == 0
+    assert attention(B=(1 << 18) - 1, T=1)[0] == 0
+    assert attention(B=1 << 18, T=1)[0] == -6
+
+
+def test_every_norm_has_a_plan_of_whole_groups():
+    for n in (1, 7, 300):
+        for p in (1, 49, 1225, 12544, 60000):
+            for c, g in ((1, 1), (7, 7), (32, 32), (48, 6), (96, 32), (130, 13), (256, 1), (512, 32), (4096, 1), (5000, 1250)):
+                for dtype in (capi.F32, capi.BF16):
+                    rc, plan = norm(N=n, P=p, C=c, G=g, dtype=dtype, x_image=p * c, x_pixel=c, y_image=p * c, y_pixel=c)
+                    assert rc == 0 and plan.span % (c // g) == 0 and plan.chunks >= 1
+                    for span in (plan.resident, plan.resident_backward):
+                        assert span == 0 or (c % span == 0 and span % (c // g) == 0 and span % (4 if dtype == capi.F32 else 8) == 0)
