@@ -14,6 +14,14 @@
 // for: bf16 one, half two, fp32 three, exactly.  What is formed between two products, P and S, goes in as two parts for the 16-bit types
 // (16 bits, against the 8 or 11 of the output) and as three for fp32; l^n k, which is summed into the state, as three (24 bits:
 // states are fp32).  Products of parts below the last bits that are kept are left out.
+//
+// Bound by the time of a chunk in a wavefront, since a state waits for the chunk before: at D = 128 in bf16 about 50 products of 32 cycles and 480 vector
+// instructions (splits, decays, the diagonal of P) a wavefront and chunk, in two wavefronts a SIMD that overlap one another's; the registers of a
+// state, 64 of 231 at D = 128, allow no third (three spill: 330 us of training below become 450 and more).  32 tokens a chunk: with 64 P and its
+// operands would not fit beside the state, and P's products grow with the chunk.  Every wavefront of a workgroup needs the whole P, so each forms
+// a part of it for all.  Segments make up for what one wavefront waits: see the rule beside the plan.
+// 12544 tokens of 16 heads of 128 in bf16: states 37 us, their scan 14, answers 71, of 33 that a copy of as many bytes takes.  8 x 1225 tokens of 8 heads of 64x128 in fp32:
+// 67 us, of 17.  8 x 3136 tokens of 16 heads of 64 with the backward pass in bf16: 330 us, of 90, in three runs of 40 for states and four of 52 to 60 for answers.
 #pragma once
 
 #include <atomic>

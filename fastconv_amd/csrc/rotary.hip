@@ -5,6 +5,8 @@
 // Bound by memory: 6 operations a pair against 4 to 16 bytes read and written.  The cosines of a token are the same for all of
 // its heads, so a workgroup takes a few whole tokens: each thread forms a few of their angles, once, into LDS, and then all
 // threads walk over the heads of q and k, 16 bytes a lane and access.
+// 2 sequences of 16x28x28 tokens with 32 and 8 heads of 128 in bf16 (514 MB read and written): 94 us, 5.5 TB/s.  One token each of 32 sequences: 4.4 us, one
+// after another the waits for a position, its angle and the channels.
 #include "token_types.h"
 
 namespace {
