@@ -20,9 +20,9 @@ constexpr long kWavefronts = 2048;
 // A cut costs two launches, k and v read twice, and a state a segment, written and read twice.  In two parts it loses (32 x 16 heads of 64, 4096
 // tokens: 388 us against 351 uncut; 1024 tokens 124 and 97), in three it gains (21 x 16 heads, 2048 tokens: 139 and 178).
 constexpr long kLeastSegments = 3;
-// Segments of two chunks, but where states are larger than what a segment reads and many: of four.  8 x 1225 tokens of 64x128 in fp32 with a
-// backward pass 220 us in segments of 3 chunks, 284 of 5 and 475 of 10; 16 heads of 128, 512 tokens: 29.6 in 8 segments, 35.5 in 4; 2048 tokens:
-// 42 in 16, 51 in 32.
+// Segments of two chunks, but where states are larger than what a segment reads and many: of four.  8 sequences of up to 1225 tokens, 8 heads of 64x128, in fp32
+// 68 us in 8 segments of 5 chunks, 75 in 4 and 119 in 2; 16 heads of 128, 512 tokens in bf16: 29.6 in 8 segments, 35.5 in 4; 2048 tokens: 42 in 16,
+// 51 in 32.
 constexpr long kSmallState = 64 * 128, kFewSegments = 8;
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
 constexpr int kChunkRows = 128;    // rows of a state that their kernel holds
