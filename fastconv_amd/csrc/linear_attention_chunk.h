@@ -29,7 +29,10 @@
 #include "linear_attention.h"
 
 constexpr int kLaChunk = 32;
-constexpr double kLaSettle = 1.0 / 65536;
+// A state is held divided by a scale from 2 to kLaTop (2^33 where a decay above 1 lets it grow), never by less than 2: then neither it, nor what
+// a chunk adds to it, nor the first part of either comes near the largest float before the state itself does.  Divided by kLaTop a value keeps
+// its three parts down to about 1e-28, and less of them below.
+constexpr double kLaTop = 131072, kLaLeast = 2, kLaMost = kLaTop * 65536;
 constexpr int kLaLoadsDone = 0x0f70;    // s_waitcnt: no load or store of global memory on its way
 constexpr int kLaOnlyVector = 0x6;      // scheduling: vector and scalar arithmetic may pass, memory and matrix instructions not
 
@@ -300,6 +303,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
     la_f32x16 S[KT];
     const float *from_state = segments > 1 ? parts + (bh * segments + seg) * (long)r.Dk * r.Dv : r.state_in ? r.state_in + bh * r.state_head : nullptr;
     {
+        const float held = begin < end ? (float)(1.0 / kLaTop) : 1.f;
         const uint32_t srow = (uint32_t)(segments > 1 ? r.part_row : r.state_row), scol = (uint32_t)(segments > 1 ? r.part_col : r.state_col);
         const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(uniform_ptr(from_state)), 0, from_state ? 0x7fffffff : 0, 0x00020000);
 #pragma unroll
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
             for (int e = 0; e < 16; e++) {
                 const int row = 32 * t + 8 * (e / 4) + 4 * g + e % 4;
                 S[t][e] = 0.f;
-                if (FULL) S[t][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(res, row < r.Dk && col < r.Dv ? 4 * (row * srow + col * scol) : 0x80000000u, 0, 0));
+                if (FULL) S[t][e] = held * __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(res, row < r.Dk && col < r.Dv ? 4 * (row * srow + col * scol) : 0x80000000u, 0, 0));
             }
     }
     if (FULL)
@@ -343,9 +347,9 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
         }
         from = (float)exact[i_tok + 1 - r.reverse] * r.scale_out;
     }
-    // The state is held as scale * S: what decays is the scale, one number, and what a chunk adds is divided by it, until it is small
-    // enough to be worth a pass over S.
-    double scale = 1.0;
+    // The state is scale * S: what decays is the scale, one number, and what a chunk adds is divided by it, until it is small
+    // enough to be worth a pass over S.  Where no token comes it passes as it is.
+    double scale = begin < end ? kLaTop : 1.0;
 
     // token i of four of q and k
     auto put_natural = [&](int i) __attribute__((always_inline)) {
@@ -441,8 +445,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
     auto rescale = [&](int n) __attribute__((always_inline)) {
         from_now = from * (float)scale;
         decayed = scale * exact[n];
-        settle = decayed < kLaSettle;
-        scale = settle ? 1.0 : decayed;
+        settle = decayed < kLaLeast || decayed > kLaMost;
+        scale = settle ? kLaTop : decayed;
         add = (float)(1.0 / scale);
     };
     auto settle_state = [&]() __attribute__((always_inline)) {
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) S[t][e] *= (float)decayed;
+                for (int e = 0; e < 16; e++) S[t][e] *= (float)(decayed * (1.0 / kLaTop));
         }
     };
 

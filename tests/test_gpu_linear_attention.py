@@ -333,3 +333,24 @@ def test_refusals_at_the_call(lib):
             call()
         assert e.value.status == -1
     lib.release(mark)
+
+
+def scaled(c, fields, factor):
+    """The tensors of a call times a factor, in its type."""
+    for f in fields:
+        t = getattr(c, f)
+        t.__init__(c.L, t.shape, c.dtype, t.strides, t.values * factor)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("field", ["q", "k", "v", "do"])
+def test_large_values_stay_finite_whatever_the_state_has_decayed_by(lib, dtype, field):
+    """Operands of 1e35: every sum is far below the largest float, also when it is taken in by a state of which a 50000th is left."""
+    mark = lib.mark()
+    for T in (90, 200):      # in one piece, in segments
+        print("linear attention, large", dtype, field, T, flush=True)
+        c = Call(lib, 1, T, 3, 3, 64, 64, dtype, 31, decay=[-0.34, -0.05, 0.0])
+        scaled(c, [field], 1e35)
+        got = c.check()
+        assert all(np.isfinite(x).all() for x in got)
+    lib.release(mark)
