@@ -33,6 +33,7 @@ constexpr int kLaChunk = 32;
 // a chunk adds to it, nor the first part of either comes near the largest float before the state itself does.  Divided by kLaTop a value keeps
 // its three parts down to about 1e-28, and less of them below.
 constexpr double kLaTop = 131072, kLaLeast = 2, kLaMost = kLaTop * 65536;
+constexpr float kLaLargest = 0x1.fep127f;      // of bf16
 constexpr int kLaLoadsDone = 0x0f70;    // s_waitcnt: no load or store of global memory on its way
 constexpr int kLaOnlyVector = 0x6;      // scheduling: vector and scalar arithmetic may pass, memory and matrix instructions not
 
@@ -63,13 +64,16 @@ __device__ __forceinline__ la_f32x4 la_product16(const la_frag &a, const la_frag
 }
 
 // PARTS bf16 parts of two values, each pair in one word: rounded, what that leaves rounded, and so on.  Bits that `keep` lacks are zeros in
-// every part.  (A value less its rounded self is one v_dot2_f32_bf16 on the pair as it is packed, too, a - 1 * hi.lo + 0 * hi.hi; with
+// every part.  LARGE: values may lie so close to the largest float that they would round to infinity; then the first part is the largest bf16, and
+// the others hold the rest, or an infinity or NaN itself.  (A value less its rounded self is one v_dot2_f32_bf16 on the pair as it is packed, too, a - 1 * hi.lo + 0 * hi.hi; with
 // it the whole kernel takes 1.13 times as long.)
-template <int PARTS>
+template <int PARTS, bool LARGE>
 __device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[PARTS], uint32_t keep = ~0u) {
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
-        out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((la_f32x2){a, b}, la_bf16x2)) & keep;
+        la_f32x2 x = {a, b};
+        if (LARGE && p == 0) x = (la_f32x2){__builtin_amdgcn_fmed3f(a, -kLaLargest, kLaLargest), __builtin_amdgcn_fmed3f(b, -kLaLargest, kLaLargest)};
+        out[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, la_bf16x2)) & keep;
         if (p + 1 < PARTS) {
             a -= __builtin_bit_cast(float, out[p] << 16);
             b -= __builtin_bit_cast(float, out[p] & 0xffff0000u);
@@ -77,11 +81,11 @@ __device__ __forceinline__ void la_split_pair(float a, float b, uint32_t (&out)[
     }
 }
 // of four
-template <int PARTS>
+template <int PARTS, bool LARGE>
 __device__ __forceinline__ void la_split(const float (&x)[4], la_bf16x4 (&out)[PARTS]) {
     uint32_t lo[PARTS], hi[PARTS];
-    la_split_pair<PARTS>(x[0], x[1], lo);
-    la_split_pair<PARTS>(x[2], x[3], hi);
+    la_split_pair<PARTS, LARGE>(x[0], x[1], lo);
+    la_split_pair<PARTS, LARGE>(x[2], x[3], hi);
 #pragma unroll
     for (int p = 0; p < PARTS; p++) out[p] = __builtin_bit_cast(la_bf16x4, (la_u32x2){lo[p], hi[p]});
 }
@@ -182,10 +186,10 @@ struct la_source {
     typedef fc_vec<DT, 4> row_type;
 };
 
-template <int PARTS>
+template <int PARTS, bool LARGE>
 __device__ __forceinline__ void la_put(char *base, int plane, int at, const float (&x)[4]) {
     la_quad q[PARTS];
-    la_split<PARTS>(x, q);
+    la_split<PARTS, LARGE>(x, q);
 #pragma unroll
     for (int p = 0; p < PARTS; p++) *(la_quad *)(base + p * plane + at) = q[p];
 }
@@ -194,17 +198,17 @@ template <int DT>
 __device__ __forceinline__ void la_put_raw(char *base, int plane, int at, typename fc_elem<DT>::type a, typename fc_elem<DT>::type b,
                                            typename fc_elem<DT>::type c, typename fc_elem<DT>::type d) {
     if constexpr (DT == FC_BF16) *(la_quad *)(base + at) = (la_quad){a, b, c, d};
-    else la_put<la_math<DT>::PARTS>(base, plane, at, {(float)a, (float)b, (float)c, (float)d});
+    else la_put<la_math<DT>::PARTS, DT == FC_F32>(base, plane, at, {(float)a, (float)b, (float)c, (float)d});
 }
 
-// Eight accumulators from `first` on as an operand.
+// Eight accumulators of a state from `first` on as an operand: held at half the state or less.
 template <int FORMED>
 __device__ __forceinline__ void la_formed(const la_f32x16 &x, int first, la_frag (&f)[FORMED]) {
     la_u32x4 w[FORMED];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         uint32_t two[FORMED];
-        la_split_pair<FORMED>(x[first + 2 * i], x[first + 2 * i + 1], two);
+        la_split_pair<FORMED, false>(x[first + 2 * i], x[first + 2 * i + 1], two);
 #pragma unroll
         for (int p = 0; p < FORMED; p++) w[p][i] = two[p];
     }
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
         for (int it = 0; it < QK_ITEMS; it++) {
             const int tq = la_tokens_of<DK>(tid + it * THREADS), cq = la_channels_of<DK>(tid + it * THREADS);
             if (8 * DK / 4 < THREADS && tq >= 8) continue;
-            la_put<M::KEPT>(to, QK_PLANE, la_turned(4 * cq + e, tq),
+            la_put<M::KEPT, false>(to, QK_PLANE, la_turned(4 * cq + e, tq),
                                 {k_now[it].row[0].get(e) * w[it][0], k_now[it].row[1].get(e) * w[it][1], k_now[it].row[2].get(e) * w[it][2],
                                  k_now[it].row[3].get(e) * w[it][3]});
         }
@@ -589,8 +593,8 @@ __global__ __launch_bounds__(64 * NW, 2) void fc_linear_attention_chunk_kernel(c
                 const int t = wave + n * NW;
                 if (t >= 3) continue;
                 uint32_t lo[M::FORMED], hi[M::FORMED];
-                la_split_pair<M::FORMED>(P[n][0] * near[n][0], P[n][1] * near[n][1], lo, earlier[n][0]);
-                la_split_pair<M::FORMED>(P[n][2] * near[n][2], P[n][3] * near[n][3], hi, earlier[n][1]);
+                la_split_pair<M::FORMED, true>(P[n][0] * near[n][0], P[n][1] * near[n][1], lo, earlier[n][0]);
+                la_split_pair<M::FORMED, true>(P[n][2] * near[n][2], P[n][3] * near[n][3], hi, earlier[n][1]);
                 char *const to = pt + (t == 2 ? kLaFrag : 0) + la_place((t >= 1 ? 16 : 0) + (lane & 15), lane >> 4, 0);
 #pragma unroll
                 for (int p = 0; p < M::FORMED; p++) *(la_u32x2 *)(to + p * 2 * kLaFrag) = (la_u32x2){lo[p], hi[p]};

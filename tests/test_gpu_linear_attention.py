@@ -354,3 +354,31 @@ def test_large_values_stay_finite_whatever_the_state_has_decayed_by(lib, dtype, 
         got = c.check()
         assert all(np.isfinite(x).all() for x in got)
     lib.release(mark)
+
+
+@pytest.mark.parametrize("field", ["q", "k", "v", "do", "state", "dstate"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_largest_floats_are_numbers(lib, field, sign):
+    """A value of the largest size in one place, all others small enough that every sum is a number; before its token nothing changes."""
+    most, mark = float(np.finfo(np.float32).max), lib.mark()
+    for T, Dk, Dv in ((20, 24, 40), (70, 64, 64), (200, 64, 128)):
+        print("linear attention, largest", field, sign, T, flush=True)
+        calls = []
+        for value in (0.0, sign * most):
+            c = Call(lib, 1, T, 3, 3, Dk, Dv, "f32", 32, decay=[-0.34, -0.05, 0.0])
+            scaled(c, ["q", "k", "v", "do"], 1e-2)
+            c.state *= np.float32(1e-2)
+            c.dstate *= np.float32(1e-2)
+            if field in ("state", "dstate"):
+                getattr(c, field)[0, 1, 5, 7] = value
+            else:
+                t = getattr(c, field)
+                x = t.values.copy()
+                x[0, T // 2, 1, 7] = value
+                t.__init__(lib, t.shape, "f32", t.strides, x)
+            calls.append(c)
+        got = calls[1].check()
+        assert all(np.isfinite(x).all() for x in got)
+        if field in ("q", "k", "v"):
+            assert np.array_equal(got[0][0, :T // 2], calls[0].forward()[0][0, :T // 2])
+    lib.release(mark)
