@@ -4,6 +4,8 @@ Tolerances: a result is rounded once to its type (ROUND); before that everything
 places of the group's largest value, each of the dozen operations behind them by one of its result: 32 last places of
 |gamma| rstd max|x - mean| + (rstd/eps part of the mean) cover both; where the mean is many times the deviation its own last
 place counts, divided by the deviation.  No slope of an activation is above 1.13, nor its own slope above 1.1."""
+import math
+
 import numpy as np
 import pytest
 
@@ -277,4 +279,42 @@ def test_refusals_at_the_call(lib):
         with pytest.raises(F.FastConvError) as e:
             call()
         assert e.value.status == -1 and "fc_group_norm" in str(e.value)
+    lib.release(mark)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("G", [1, 32])
+def test_activations_are_exact_in_proportion(lib, act, dtype, G):
+    """gamma is 0, so that z is beta to the last bit, and one pixel makes dbeta the slope.
+
+    SiLU in fp32: exp errs through its argument's rounding by 11 last places at |z| = 12, the sum, the reciprocal and the product by one each,
+    16 allowed; 1 - s in the slope by half a last place of 1, times z.  GELU: exp(-z^2/2) takes over the roundings of its argument, z^2 last
+    places together, 2 z^2 allowed beside 32 for all else.  In 16 bits the cheap form of erf besides: 1.5e-7."""
+    C_ = 1024
+    z = np.linspace(-12, 12, C_).astype(np.float32)
+    rng = np.random.default_rng(7)
+    mark = lib.mark()
+    print("group norm, activations", act, dtype, G, flush=True)
+    x = rng.standard_normal((1, 1, C_))
+    dx, dy, plan, m, r, g, b = forward(lib, x, np.zeros(C_, np.float32), z, 1, 1, C_, G, dtype, act)
+    grad = K.Dev(lib, (1, 1, C_), dtype, None, np.ones((1, 1, C_)))
+    out, dbeta = K.Dev(lib, (1, 1, C_), dtype), K.Dev(lib, (C_,), "f32")
+    lib.group_norm_backward(plan, grad.ptr, dx.ptr, g, b, m.ptr, r.ptr, out.ptr, None, dbeta.ptr, lib.alloc(max(4, plan.ws_backward_bytes)))
+    z = z.astype(np.float64)
+    if act == "silu":
+        s, flat = 1 / (1 + np.exp(-z)), 1 / (1 + np.exp(z))      # and 1 - s
+        y, slope, size = z * s, s + z * s * flat, s + np.abs(z) * s * flat
+        ty, ts = 16 * K.EPS * np.abs(y), K.EPS * (16 * size + np.abs(z) * s)
+        more = 2 * np.abs(z) * K.EPS * size
+    else:
+        half = 0.5 * np.array([math.erfc(-v / math.sqrt(2)) for v in z])
+        bell = np.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        y, slope, size = z * half, half + z * bell, half + np.abs(z) * bell
+        ty, ts = (32 + 2 * z * z) * K.EPS * np.abs(y), (32 + 2 * z * z) * K.EPS * size
+        more = 1.5e-7 + 4 * z * z * K.EPS * size
+    if dtype != "f32":
+        ty, ts = ty + more * np.abs(z), ts + more
+    close(dy.get()[0, 0], y, K.ROUND[dtype] * np.abs(y) + ty + K.TINY[dtype], "y")
+    close(dbeta.get(), slope, ts + 1e-37, "slope")
     lib.release(mark)
