@@ -177,8 +177,11 @@ extern "C" int fc_rotary(fc_context *ctx, const fc_rotary_shape *s, const void *
     }
     if ((addr & (es - 1)) || (((uint64_t)positions_dev | (uint64_t)inv_freq_dev) & 3)) return fail(ctx, FC_ERR_INVALID, "fc_rotary: unaligned pointer");
     const long heads = (long)s->Hq + s->Hk, tokens = fc_count(s->B, s->T);
-    if (s->D > 1024 || heads > 65536 || tokens < 0 || tokens >= kMostThreads / kThreads * kMostTokens)
-        return fail(ctx, FC_ERR_UNSUPPORTED, "fc_rotary: more than 1024 channels, 65536 heads or 2^25 - 1 tokens");
+    int group = kMostTokens;
+    while (group > 1 && tokens < 1024L * group) group >>= 1;
+    // a last workgroup may have one token of two: 2^25 - 2 tokens are the most
+    if (s->D > 1024 || heads > 65536 || tokens < 0 || (tokens + group - 1) / group >= kMostThreads / kThreads)
+        return fail(ctx, FC_ERR_UNSUPPORTED, "fc_rotary: more than 1024 channels, 65536 heads or 2^25 - 2 tokens");
     const int vec = fc_widest(s->dtype, bits | (uint64_t)s->D | (uint64_t)(s->interleaved ? 2 * R : R), addr);
     rotary_params p;
     p.q = q_dev; p.k = k_dev; p.qo = q_out_dev; p.ko = k_out_dev;
@@ -197,8 +200,6 @@ extern "C" int fc_rotary(fc_context *ctx, const fc_rotary_shape *s, const void *
     p.pos_batch = s->positions_batch;
     p.qb = s->q_batch; p.qt = s->q_token; p.qh = s->q_head; p.kb = s->k_batch; p.kt = s->k_token; p.kh = s->k_head;
     p.qob = s->qo_batch; p.qot = s->qo_token; p.qoh = s->qo_head; p.kob = s->ko_batch; p.kot = s->ko_token; p.koh = s->ko_head;
-    int group = kMostTokens;
-    while (group > 1 && tokens < 1024L * group) group >>= 1;
     const unsigned blocks = (unsigned)((tokens + group - 1) / group);
     const size_t lds = (size_t)group * ((R + 1) & ~1l) * sizeof(float2);
     const bool il = s->interleaved != 0;

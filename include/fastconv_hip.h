@@ -502,7 +502,7 @@ int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan *plan, cons
  * Channels from 2R on pass unchanged.  positions: int32 [B][T][axes], those of sequence b at b*positions_batch (0: the same
  * ones for all); any int32 is a position, and the angle is reduced in 64 bits.  q has Hq heads and k Hk (0: no k).
  * Token t of sequence b and head h begins at b*q_batch + t*q_token + h*q_head, and so for k and both outputs.
- * Limits: D <= 1024, Hq + Hk <= 65536, fewer than 2^25 tokens in all. */
+ * Limits: D <= 1024, Hq + Hk <= 65536, at most 2^25 - 2 tokens in all. */
 #define FC_ROTARY_AXES 4
 typedef struct {
     int B;

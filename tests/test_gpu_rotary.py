@@ -218,3 +218,33 @@ def test_refusals(lib):
     refused(-6, D=1026)
     refused(-6, B=2 ** 20, T=2 ** 20)
     lib.release(mark)
+
+
+@pytest.mark.parametrize("B,T", [(1, 2 ** 25 - 1), (1, 2 ** 25), (31, (2 ** 25 - 1) // 31)])
+def test_tokens_that_no_launch_holds_are_refused(lib, B, T):
+    """Two tokens a workgroup, the last one with one of its own: 2^25 - 1 would be 2^32 threads, one more than a launch holds."""
+    assert B * T >= 2 ** 25 - 1
+    mark = lib.mark()
+    p = lib.alloc(1 << 10).value
+    with pytest.raises(F.FastConvError) as e:
+        lib.rotary(F.RotaryShape.packed(B, T, 1, 0, 2, (1,)), p, None, p, p, p, None)
+    assert e.value.status == -6 and "2^25 - 2" in str(e.value)
+    lib.release(mark)
+
+
+def test_as_many_tokens_as_a_launch_holds(lib):
+    """2^25 - 2 tokens of one pair, which share the positions of 2730 sequences."""
+    B, T = 2730, (2 ** 25 - 2) // 2730
+    assert B * T == 2 ** 25 - 2
+    rng = np.random.default_rng(13)
+    raw, values = K.to_type(rng.standard_normal((T, 2)), "f16")
+    mark = lib.mark()
+    print("rotary, tokens", B * T, flush=True)
+    positions = rng.integers(0, 5000, (1, T, 1)).astype(np.int32)
+    x = lib.upload_raw(np.broadcast_to(raw, (B, T, 2)))
+    s = F.RotaryShape.packed(B, T, 1, 0, 2, (1,), F.F16, shared_positions=True)
+    lib.rotary(s, x, None, lib.upload_raw(positions), K.floats(lib, ladder((1,)) * np.float32(0.01)), x, None)
+    got = lib.download(x, (B, T, 2), np.float16)
+    assert (got == got[0]).all()
+    check(values.reshape(1, T, 1, 2), got[:1].astype(np.float64).reshape(1, T, 1, 2), positions, ladder((1,)) * np.float32(0.01), (1,), False, False, "f16")
+    lib.release(mark)
