@@ -38,6 +38,14 @@ struct fc_la_run {
     bool wide;               // four channels of every operand lie within one access
 };
 
+// Wavefronts of 32 columns in a workgroup of a run with a state of Dk x Dv: two where the state has no more than 64 columns, if they have the registers to
+// lay out its rows for each other; else four, half of which idle.  With two and four, 8 x 1225 tokens of 8 heads: states of 32x32 in fp32 with the
+// backward pass 128 and 180 us; 64x64 in fp32 258 and 244 (32 x 515 tokens of 32 heads forward 250 and 197), 63x61 in half, by single elements, 91 and
+// 86 (64 x 515 tokens 627 and 447), in bf16 54 and 64; 128x64 in fp32 255 and 129, in half 118 and 69, in bf16 84 and 54.
+static inline int fc_la_wavefronts(int dtype, int Dk, int Dv, bool wide) {
+    return Dv <= 64 && (Dk <= 32 || (Dk <= 64 && (dtype == FC_BF16 || (dtype == FC_F16 && wide)))) ? 2 : 4;
+}
+
 // linear_attention_<type>.hip: `segments` parts of `segment` tokens of each of `heads` heads.  _state: the state that each but the
 // last adds to none, to parts [heads][segments][Dk][Dv].  _answer: the answers; each segment begins from its state in parts, or, if it is the only
 // one, from state_in.

@@ -15,7 +15,8 @@ constexpr long kMostSteps = 6;
 // 12.2, 1024 heads 34 and 26.
 constexpr long kWholeRows = 512;
 // A sequence is cut up to fill the chip: 16 heads of 128, 12544 tokens in bf16 140 us for 1024 wavefronts, 121 for 2048 and 145 for 4096; with a
-// backward pass, 8 x 16 heads of 64 and 3136 tokens 422, 330 and 393.
+// backward pass, 8 x 16 heads of 64 and 3136 tokens 422, 330 and 393.  In fp32, whose heads of 64 take four wavefronts, 8 heads and 11760 tokens 79 us for 1536,
+// 70 for 2048, 83 for 3072 and 86 for 4096; 32 x 8 heads and 2048 tokens 239 uncut, 252 in 3 parts, 257 in 4.
 constexpr long kWavefronts = 2048;
 // A cut costs two launches, k and v read twice, and a state a segment, written and read twice.  In two parts it loses (32 x 16 heads of 64, 4096
 // tokens: 388 us against 351 uncut; 1024 tokens 124 and 97), in three it gains (21 x 16 heads, 2048 tokens: 139 and 178).
@@ -222,6 +223,12 @@ size_t states_of(const fc_linear_attention_plan *plan) {
     return plan->segments > 1 ? (size_t)s.B * s.H * plan->segments * s.Dk * s.Dv : 0;
 }
 
+// The same but for where the tensors begin, which a plan does not know.
+bool wide_strides(const fc_linear_attention_shape &s) {
+    return ((s.Dk | s.Dv | s.q_batch | s.q_token | s.q_head | s.k_batch | s.k_token | s.k_head | s.v_batch | s.v_token | s.v_head | s.o_batch | s.o_token |
+             s.o_head) & 3) == 0;
+}
+
 // Tokens of a segment: whole chunks.
 long segment_of(const fc_linear_attention_shape &s, int segments) {
     const long chunks = (s.T + kChunk - 1) / kChunk;
@@ -338,7 +345,9 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
     plan->segments = 1;
     if (s->T > kMostSteps) {
         plan->chunk = kChunk;
-        const long wavefronts = most <= 64 ? 2 : 4 * ((most + 127) / 128), chunks = (s->T + kChunk - 1) / kChunk;
+        // of the forward run, as it is launched; the backward runs are cut where it is, since dk begins from dv's states.  More than 128 rows or
+        // columns count as two states.
+        const long wavefronts = fc_la_wavefronts(s->dtype, s->Dk, s->Dv, wide_strides(*s)) * ((most + 127) / 128), chunks = (s->T + kChunk - 1) / kChunk;
         long segments = kWavefronts / (s->B * (long)s->H * wavefronts);
         long worth = chunks / 2;
         if ((long)s->Dk * s->Dv > kSmallState && worth > kFewSegments) worth = chunks / 4 > kFewSegments ? chunks / 4 : kFewSegments;

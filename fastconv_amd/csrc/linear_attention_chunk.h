@@ -747,16 +747,10 @@ int la_launch_one(fc_context *ctx, const fc_la_run &r, long heads, int segments,
 
 template <int DT, bool FULL>
 int la_launch(fc_context *ctx, const fc_la_run &r, long heads, int segments, long segment, float *parts) {
-    // Two wavefronts where the state has no more than 64 columns, if they have the registers to lay out its rows for each other; else four, half of
-    // which idle.  With two and four, 8 x 1225 tokens of 8 heads: states of 32x32 in fp32 with the backward pass 128 and 180 us; 64x64 in fp32 258 and
-    // 244 (32 x 515 tokens of 32 heads forward 250 and 197), 63x61 in half, by single elements, 91 and 86 (64 x 515 tokens 627 and 447), in bf16 54 and
-    // 64; 128x64 in fp32 255 and 129, in half 118 and 69, in bf16 84 and 54.
-    if (r.Dv <= 64) {
+    if (fc_la_wavefronts(DT, r.Dk, r.Dv, r.wide) == 2) {
         if (r.Dk <= 32) return la_launch_one<DT, 1, 2, FULL>(ctx, r, heads, segments, segment, parts);
-        if constexpr (DT == FC_F16)
-            if (r.Dk <= 64 && r.wide) return la_launch_as<DT, 2, 2, FULL, true>(ctx, r, heads, segments, segment, parts);
-        if constexpr (DT == FC_BF16)
-            if (r.Dk <= 64) return la_launch_one<DT, 2, 2, FULL>(ctx, r, heads, segments, segment, parts);
+        if constexpr (DT == FC_F16) return la_launch_as<DT, 2, 2, FULL, true>(ctx, r, heads, segments, segment, parts);
+        if constexpr (DT == FC_BF16) return la_launch_one<DT, 2, 2, FULL>(ctx, r, heads, segments, segment, parts);
     }
     if (r.Dk <= 32) return la_launch_one<DT, 1, 4, FULL>(ctx, r, heads, segments, segment, parts);
     if (r.Dk <= 64) return la_launch_one<DT, 2, 4, FULL>(ctx, r, heads, segments, segment, parts);

@@ -113,3 +113,20 @@ def test_every_norm_has_a_plan_of_whole_groups():
                     assert rc == 0 and plan.span % (c // g) == 0 and plan.chunks >= 1
                     for span in (plan.resident, plan.resident_backward):
                         assert span == 0 or (c % span == 0 and span % (c // g) == 0 and span % (4 if dtype == capi.F32 else 8) == 0)
+
+
+def test_sequences_are_cut_for_the_wavefronts_that_are_launched():
+    """About 2048 wavefronts fill the chip.  A head of 64 takes two in 16 bits; four in fp32, and in half where four channels lie in no access."""
+    def packed(B, T, H, Dk, Dv, dtype, **change):
+        plan = capi.LinearAttentionPlan()
+        shape = capi.LinearAttentionShape.packed(B, T, H, H, Dk, Dv, dtype)
+        assert plan_of(capi.load_cdll().fc_linear_attention_make_plan, plan, shape, **change) == 0
+        return plan.segments
+    for dtype, wavefronts in ((capi.BF16, 2), (capi.F16, 2), (capi.F32, 4)):
+        for B, T, H in ((8, 2048, 32), (1, 11760, 8), (8, 1225, 8), (4, 3136, 16)):
+            segments = packed(B, T, H, 64, 64, dtype)
+            assert B * H * segments * wavefronts <= 2048 and (segments == 1 or B * H * (segments + 1) * wavefronts > 1024), (dtype, B, T, H, segments)
+    assert packed(8, 2048, 32, 64, 64, capi.F32) == 1                 # three parts or none
+    assert packed(1, 11760, 8, 32, 32, capi.F32) == packed(1, 11760, 8, 64, 64, capi.BF16) > packed(1, 11760, 8, 64, 64, capi.F32)
+    assert packed(4, 3136, 16, 63, 61, capi.F16) == packed(4, 3136, 16, 64, 64, capi.F32)
+    assert packed(4, 3136, 16, 64, 64, capi.F16, q_token=16 * 64 + 1) == packed(4, 3136, 16, 64, 64, capi.F32)
