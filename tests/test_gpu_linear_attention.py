@@ -382,3 +382,15 @@ def test_the_largest_floats_are_numbers(lib, field, sign):
         if field in ("q", "k", "v"):
             assert np.array_equal(got[0][0, :T // 2], calls[0].forward()[0][0, :T // 2])
     lib.release(mark)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("Dk,Dv", [(30, 40), (32, 61), (60, 50), (33, 64), (20, 100), (50, 120), (100, 70), (128, 128)])
+def test_single_elements_in_segments(lib, dtype, Dk, Dv):
+    """Strides or sizes that no wide access fits, through every tile of the states and of the answers."""
+    mark = lib.mark()
+    print("linear attention, single elements", dtype, Dk, Dv, flush=True)
+    c = Call(lib, 1, 225, 4, 2, Dk, Dv, dtype, Dk + Dv, "odd", None, True)
+    assert c.plan.segments >= 3
+    c.check()
+    lib.release(mark)
