@@ -318,3 +318,87 @@ def test_activations_are_exact_in_proportion(lib, act, dtype, G):
     close(dy.get()[0, 0], y, K.ROUND[dtype] * np.abs(y) + ty + K.TINY[dtype], "y")
     close(dbeta.get(), slope, ts + 1e-37, "slope")
     lib.release(mark)
+
+
+def pixels_a_thread(plan, span):
+    """What a resident kernel of 1024 threads holds, rounded up to the kernels there are."""
+    s = plan.shape
+    cols = span // (4 if s.dtype == F.F32 else 8)
+    need = -(-s.P // (1024 // cols))
+    return 1 << (need - 1).bit_length()
+
+
+RESIDENT = [  # N, P, C, G, dtype, act, pixels a thread forward, backward (0: two passes)
+    (2, 3136, 64, 4, "f32", "silu", 16, 0),
+    (1, 4096, 32, 2, "f32", "gelu", 16, 0),            # every slot taken
+    (2, 2049, 64, 2, "bf16", "silu", 16, 0),
+    (1, 3136, 64, 2, "f16", "gelu", 16, 0),
+    (2, 2047, 96, 2, "bf16", "gelu", 16, 0),           # groups of 48: no butterflies
+    (1, 2500, 48, 2, "f32", "none", 16, 0),
+    (1, 1900, 48, 1, "f16", "relu", 16, 0),
+    (2, 2000, 64, 4, "f32", "gelu", 8, 8),
+    (2, 1025, 64, 2, "bf16", "silu", 8, 8),
+    (1, 2048, 64, 2, "bf16", "gelu", 8, 8),
+    (2, 1600, 64, 2, "f16", "gelu", 8, 8),
+    (1, 1360, 96, 2, "f16", "silu", 8, 8),
+    (2, 1300, 48, 1, "bf16", "gelu", 8, 8),
+    (1, 1111, 72, 3, "f32", "silu", 8, 8),
+]
+
+
+@pytest.mark.parametrize("case", RESIDENT, ids=lambda c: "-".join(map(str, c)))
+def test_as_many_pixels_as_a_thread_holds(lib, case):
+    N, P, C_, G, dtype, act, ahead, back = case
+    plan = lib.group_norm_plan(F.GroupNormShape(N, P, C_, G, K.TYPES[dtype], ACTS[act], EPS, P * C_, C_, P * C_, C_))
+    assert plan.resident and pixels_a_thread(plan, plan.resident) == ahead
+    assert pixels_a_thread(plan, plan.resident_backward) == back if back else plan.resident_backward == 0
+    test_forward_and_backward(lib, (N, P, C_, G, dtype, act, 0))
+
+
+@pytest.mark.parametrize("dtype,N,act", [("bf16", 21, "silu"), ("f16", 21, "none"), ("f32", 12, "silu")])
+def test_tensors_beyond_the_last_cache(lib, dtype, N, act):
+    """More than 256 MB with their result, which is then stored past the caches: three images over and over, all equal to the bit to those
+    three, which are checked."""
+    P, C_, G, kinds = 224 * 224, 64, 32, 3
+    assert 2 * N * P * C_ * np.dtype(K.storage(dtype)).itemsize > 256 << 20
+    rng = np.random.default_rng(14)
+    print("group norm, beyond the cache", dtype, flush=True)
+    x, gamma, beta = inputs(rng, kinds, P, C_)
+    mark = lib.mark()
+    plan = lib.group_norm_plan(F.GroupNormShape.packed(N, P, C_, G, K.TYPES[dtype], ACTS[act], EPS))
+    assert plan.resident == 0 and plan.resident_backward == 0
+    which = np.arange(N) % kinds
+    raw, x = K.to_type(x, dtype)
+    raw_dy, dy = K.to_type(rng.standard_normal(x.shape), dtype)
+    at_x, at_dy = lib.upload_raw(raw[which]), lib.upload_raw(raw_dy[which])
+    at_y, at_dx = lib.alloc(N * raw[0].nbytes), lib.alloc(N * raw[0].nbytes)
+    m, r, dgamma, dbeta = (K.Dev(lib, n, "f32") for n in ((N, G), (N, G), (C_,), (C_,)))
+    ws, g, b = lib.alloc(max(4, plan.ws_bytes, plan.ws_backward_bytes)), K.floats(lib, gamma), K.floats(lib, beta)
+    lib.group_norm(plan, at_x, g, b, at_y, m.ptr, r.ptr, ws)
+    lib.group_norm_backward(plan, at_dy, at_x, g, b, m.ptr, r.ptr, at_dx, dgamma.ptr, dbeta.ptr, ws)
+    results = []
+    for at in (at_y, at_dx):
+        got = lib.download(at, (N, P, C_), K.storage(dtype))
+        words = got.view(np.uint32 if dtype == "f32" else np.uint16)
+        assert all(np.array_equal(words[n], words[n % kinds]) for n in range(N))
+        results.append(K.from_type(got[:kinds], dtype))
+    y, mean, rstd, xhat, z = K.group_norm(x, gamma, beta, G, EPS, act)
+    tz = bounds(x, gamma, beta, G, rstd, mean)
+    close(results[0], y, K.ROUND[dtype] * np.abs(y) + 1.2 * tz + K.TINY[dtype], "y")
+    want, _, _, dz = K.group_norm_backward(dy, x, gamma, beta, G, EPS, act)
+    # as in test_forward_and_backward
+    spread = np.abs(x).reshape(kinds, -1).max(axis=1)[:, None]
+    tdz = np.abs(dy) * (1.2 * tz + 8 * K.EPS)
+    txh = 32 * K.EPS * (np.abs(xhat) + np.repeat(rstd * (np.abs(mean) + spread), C_ // G, axis=-1)[:, None, :])
+    places = K.EPS * (16 + 2 * np.sqrt(N * P))
+    grouped = lambda a: np.repeat(a.reshape(kinds, P, G, -1).mean(axis=(1, 3)), C_ // G, axis=-1)[:, None, :]  # noqa: E731
+    rw, ga, ax = np.repeat(rstd, C_ // G, axis=-1)[:, None, :], np.abs(gamma), np.abs(xhat)
+    h, th = ga * np.abs(dz), ga * tdz
+    s1, s2 = grouped(h), grouped(h * ax)
+    tol = rw * (th + grouped(th) + ax * grouped(th * ax + h * txh) + txh * s2 + 2 * places * (h + s1 + ax * s2)) + 32 * K.EPS * np.abs(want)
+    close(results[1], want, K.ROUND[dtype] * np.abs(want) + tol + K.TINY[dtype], "dx")
+    times = np.bincount(which, minlength=kinds).astype(np.float64)
+    total = lambda a: (a.sum(axis=1) * times[:, None]).sum(axis=0)  # noqa: E731
+    close(dbeta.get(), total(dz), total(tdz) + places * total(np.abs(dz)) + 1e-30, "dbeta")
+    close(dgamma.get(), total(dz * xhat), total(tdz * ax + np.abs(dz) * txh) + places * total(np.abs(dz) * ax) + 1e-30, "dgamma")
+    lib.release(mark)
