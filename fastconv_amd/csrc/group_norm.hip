@@ -674,7 +674,7 @@ __device__ __forceinline__ void sum_channels(const norm_params &p, const norm_bu
 }
 
 // Values of 16 bits stay packed between two passes over them: the compiler would keep the unpacked ones, twice the registers (16 accesses
-// forward and 8 backward spilled 112 and 67; 32 images of 56x56x256 in bf16: forward 65 -> 35 us, backward 124 -> 69).
+// forward and 8 backward spilled 112 and 67; 32 images of 56x56x256 in bf16: forward 62 -> 36 us, backward alone 124 -> 74; backward with GELU 16 to 20 still spill).
 template <class V, int R>
 __device__ __forceinline__ void keep_packed(V (&x)[R]) {
     typedef unsigned __attribute__((ext_vector_type(4))) words;
@@ -909,8 +909,8 @@ int resident_pixels(long P, int span, int vec, int threads, int most) {
     return need <= r ? r : 0;
 }
 
-// 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.  Resident against not, 32 images of 56x56x256: forward in bf16 35 and 40 us, in
-// fp32 51 and 58; 1 of 14x14x512 in bf16 forward and backward 16 and 26; 128 of 28x28x512 in fp32 backward 196 and 232.
+// 16 accesses of 16 bytes in registers forward, 8 each of x and dy backward.  Resident against not, 32 images of 56x56x256: forward in bf16 36 and 40 us, in
+// fp32 56 and 67; 1 of 14x14x512 in bf16 forward 6.4 and 12.8, backward 9.4 and 20.4; 128 of 28x28x512 in fp32 backward 171 and 205.
 constexpr int kResident = 16, kResidentBackward = 8;
 // With fewer, a wider workgroup leaves compute units idle: 1 image of 14x14x512 in bf16 6.5 us in 32 workgroups and 9.1 in 16, 8 of 35x35x192 in half
 // 13.9 and 17.4 in 32.
@@ -919,7 +919,9 @@ constexpr long kResidentWorkgroups = 256;
 // Less than 64 bytes of a pixel (half a cache line) are read well by few workgroups with a short wait before their sums.  Forward, resident against
 // not, in bf16: 8 images of 8000x256 as 256 workgroups of 16 bytes 32 and 37 us; but 32 of 6272x256 as 512 of 32 bytes 77 and 74, as 1024 of 16
 // bytes 112; 4 of 12544x128 as 64 workgroups with 16 accesses a thread 36 and 24.  Backward twice as much would be read again, from the last cache
-// if it holds that: 32 of 3136x256 as 32 bytes in bf16 69 and 82, in fp32 (103 MB a tensor) 102 and 95.
+// if it holds that, best right after a forward pass.  Both passes, resident backward against not, 32 bytes of 3136x256: 32 images in bf16 (51 MB a tensor) 104 and 117,
+// 64 in bf16 (103 MB) 205 and 203, 20 in fp32 (64 MB) 121 and 111, 32 in fp32 (103 MB) 153 and 146, 48 in fp32 230 and 229; the backward pass alone 74 and 84,
+// 138 and 141, 79 and 72, 101 and 107, 147 and 150.
 constexpr long kWhole = 64;
 constexpr int kResidentNarrow = 8;
 constexpr double kNarrowBackwardBytes = 64e6;

@@ -39,9 +39,10 @@ struct fc_la_run {
 };
 
 // Wavefronts of 32 columns in a workgroup of a run with a state of Dk x Dv: two where the state has no more than 64 columns, if they have the registers to
-// lay out its rows for each other; else four, half of which idle.  With two and four, 8 x 1225 tokens of 8 heads: states of 32x32 in fp32 with the
-// backward pass 128 and 180 us; 64x64 in fp32 258 and 244 (32 x 515 tokens of 32 heads forward 250 and 197), 63x61 in half, by single elements, 91 and
-// 86 (64 x 515 tokens 627 and 447), in bf16 54 and 64; 128x64 in fp32 255 and 129, in half 118 and 69, in bf16 84 and 54.
+// lay out its rows for each other; else four, half of which idle.  With two and four, 8 x 1225 tokens of 8 heads, each cut for its own: states of 32x32 in fp32
+// 37 and 42 us (with the backward pass 131 and 146); 64x64 in fp32 71 and 55 (32 x 515 tokens of 32 heads 250 and 195), in bf16 36 and 39, in half 47 and 44 (212 and 266);
+// 63x61, by single elements, in half 86 and 65 (64 x 515 tokens of 32 heads 575 and 454), in bf16 55 and 53; 128x64 in fp32 290 and 131, in half 150 and 69, in
+// bf16 108 and 52.
 static inline int fc_la_wavefronts(int dtype, int Dk, int Dv, bool wide) {
     return Dv <= 64 && (Dk <= 32 || (Dk <= 64 && (dtype == FC_BF16 || (dtype == FC_F16 && wide)))) ? 2 : 4;
 }

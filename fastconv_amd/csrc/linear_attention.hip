@@ -21,8 +21,8 @@ constexpr long kWavefronts = 2048;
 // A cut costs two launches, k and v read twice, and a state a segment, written and read twice.  In two parts it loses (32 x 16 heads of 64, 4096
 // tokens: 388 us against 351 uncut; 1024 tokens 124 and 97), in three it gains (21 x 16 heads, 2048 tokens: 139 and 178).
 constexpr long kLeastSegments = 3;
-// Segments of two chunks, but where states are larger than what a segment reads and many: of four.  8 sequences of up to 1225 tokens, 8 heads of 64x128, in fp32
-// 68 us in 8 segments of 5 chunks, 75 in 4 and 119 in 2; 16 heads of 128, 512 tokens in bf16: 29.6 in 8 segments, 35.5 in 4; 2048 tokens: 42 in 16,
+// Segments of two chunks, but where states are larger than what a segment reads and many: of four.  8 sequences of 1225 tokens, 8 heads of 64x128, in fp32
+// 71 us in 8 segments of 5 chunks, 75 in 4 and 119 in 2; 16 heads of 128, 512 tokens in bf16: 29.6 in 8 segments, 35.5 in 4; 2048 tokens: 42 in 16,
 // 51 in 32.
 constexpr long kSmallState = 64 * 128, kFewSegments = 8;
 constexpr int kChunk = 32;         // tokens that the matrix cores take at once
@@ -152,8 +152,9 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
     }
 }
 
-// The states that segments begin from: parts[s] becomes what enters segment s, for each element of a head's state.  Bound by memory, what it reads
-// fresh from the caches: 16 heads of 128 in 31 segments, 65 MB read and written, 14 us.
+// The states that segments begin from: parts[s] becomes what enters segment s, for each element of a head's state.  Bound by the chain of segments, eight of
+// which are read at once: 16 heads of 128 in 31 segments, 65 MB read and written, 6 to 13 us by what the caches hold; 8 heads of 64 in 62 segments, 16 MB, 11 us,
+// and in 123 segments 21.
 __global__ __launch_bounds__(kThreads) void fc_linear_attention_scan_kernel(const fc_la_run r, int segments, long segment, float *parts) {
     constexpr int AHEAD = 8;      // segments read before the first is joined
     const int size = r.Dk * r.Dv, blocks = (size + kThreads - 1) / kThreads;

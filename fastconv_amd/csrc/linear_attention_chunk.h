@@ -3,7 +3,8 @@
 // With S the state that enters a chunk, local tokens i, j and l the decay (forward; a backward run differs by one power of l):
 //   o_i = scale * ( l^(i+1) S^T q_i + sum over j <= i of l^(i-j) (q_i . k_j) v_j )
 //   S  <- l^C S + sum over j of l^(C-1-j) k_j v_j^T
-// One pass: every q, k, v is read once, and of S nothing leaves the registers.  A wavefront owns 32 columns of S for all of its
+// Of S nothing leaves the registers between the first token of a segment and its last; q, k and v are read once by a sequence in one piece whose values have up to
+// 128 channels (q and k once more for each 128 further ones), and in segments k and v a second time.  A wavefront owns 32 columns of S for all of its
 // rows, as accumulators of 32x32 products.  What makes them fit together without a turn through LDS: lane l of an accumulator
 // holds column l % 32, rows 8*(r/4) + 4*(l/32) + r%4; lane l of an operand holds row (or column) l % 32, depths 8*(l/32) + e.
 // The order of a product's depths is free as long as both operands keep the same, so with depth 8*g + e of sixteen named
@@ -12,16 +13,20 @@
 //
 // Roundings.  A matrix core multiplies bf16 (8 bits) and adds in fp32.  Inputs are split into as many bf16 parts as they have bits
 // for: bf16 one, half two, fp32 three, exactly.  What is formed between two products, P and S, goes in as two parts for the 16-bit types
-// (16 bits, against the 8 or 11 of the output) and as three for fp32; l^n k, which is summed into the state, as three (24 bits:
-// states are fp32).  Products of parts below the last bits that are kept are left out.
+// (16 bits, against the 8 or 11 of the output, whose rounding hides it; a third would be 8 products more of 50) and as three for fp32; l^n k, which is summed into the state, as three (24 bits:
+// states are fp32).  Products of parts below the last bits that are kept are left out: for fp32 six of nine are made, which errs by 2^-24 of a product at most, 0.1 of
+// that on average.
 //
-// Bound by the time of a chunk in a wavefront, since a state waits for the chunk before: at D = 128 in bf16 about 50 products of 32 cycles and 480 vector
-// instructions (splits, decays, the diagonal of P) a wavefront and chunk, in two wavefronts a SIMD that overlap one another's; the registers of a
-// state, 64 of 231 at D = 128, allow no third (three spill: 330 us of training below become 450 and more).  32 tokens a chunk: with 64 P and its
+// Bound by the time of a chunk in a wavefront, since a state waits for the chunk before: at D = 128 in bf16 47 products of 32 cycles and 560 other vector
+// instructions (splits, decays, the diagonal of P) a wavefront and chunk, the matrix cores busy a fifth of the time, in two wavefronts a SIMD that overlap one
+// another's; the registers of a state, 64 of 231 at D = 128, allow no third (three spill: 324 us of training below become 450 and more).  fp32 with more than
+// 64 rows has one only: three parts of everything are 102 KB of LDS, one workgroup a compute unit, and 44 registers spill (104 by single elements).
+// 32 tokens a chunk: with 64 P and its
 // operands would not fit beside the state, and P's products grow with the chunk.  Every wavefront of a workgroup needs the whole P, so each forms
 // a part of it for all.  Segments make up for what one wavefront waits: see the rule beside the plan.
-// 12544 tokens of 16 heads of 128 in bf16: states 37 us, their scan 14, answers 71, of 33 that a copy of as many bytes takes.  8 x 1225 tokens of 8 heads of 64x128 in fp32:
-// 67 us, of 17.  8 x 3136 tokens of 16 heads of 64 with the backward pass in bf16: 330 us, of 90, in three runs of 40 for states and four of 52 to 60 for answers.
+// 12544 tokens of 16 heads of 128 in bf16: states 37 us, their scan 6 to 13, answers 74, 117 in all, of 33 that a copy of as many bytes takes.  8 x 1225 tokens of 8 heads
+// of 64 in fp32: 16, 5 and 36, 56 in all, of 13.  8 x 3136 tokens of 16 heads of 64 with the backward pass in bf16: 323 us, of 90, in three runs of states (25 to
+// 30 each), three scans (9 to 10) and four runs of answers (52 to 61).
 #pragma once
 
 #include <atomic>

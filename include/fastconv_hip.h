@@ -446,10 +446,13 @@ int fc_maxpool2x2(fc_context *ctx, const float *x_dev, float *y_dev, int N, int 
 
 /* What a network runs on the pixels of a convolution trunk, or on the patches of a patch embedding, once they are tokens:
  * channels last, so that a token's channels are neighbours.  No counterpart in the reference, which ends at the
- * convolution.  A trunk's fp32 output of one-pixel images (N tokens of C x 1 x 1) has this layout as it is.
+ * convolution.  The convolutions' fp32 NCHW output has this layout as it is where images have one pixel (N tokens of
+ * C x 1 x 1: a patch embedding, the projections of tokens); larger images, and 16-bit tensors, are the caller's to lay out.
  *
- * Tensors hold fp32, bf16 or IEEE half (fc_dtype); every sum, statistic, state and angle is fp32 or wider, and a result is
- * rounded once to the tensor's type.  Parameters (gamma, beta, log_decay, inv_freq), statistics and states are fp32 always.
+ * Tensors hold fp32, bf16 or IEEE half (fc_dtype); every sum, statistic, state and angle is held in fp32 or wider, and a
+ * result is rounded once to the tensor's type.  Two things have fewer bits on their way into a result of 16 bits: GELU's erf is
+ * good to 1.5e-7, and linear attention of more than six tokens multiplies q k^T and the state as 16 bits of each (bf16 products, added up in
+ * fp32; fp32 tensors have 24 bits of everything there, and every state takes in 24 bits of what is added to it).  Parameters (gamma, beta, log_decay, inv_freq), statistics and states are fp32 always.
  * Strides are in elements; channels of one token (one head) are neighbours.  Pointers need the alignment of their type only:
  * rows that begin on 16 bytes and have sizes that are multiples of 16 bytes are read fastest.  Buffers must not overlap, but
  * where a call says so.  All calls run on the context's stream, allocate nothing and can be recorded into a graph; they are not
@@ -462,7 +465,8 @@ typedef enum { FC_ACT_NONE = 0, FC_ACT_RELU = 1, FC_ACT_SILU = 2, FC_ACT_GELU = 
  *   xhat = (x - mean) * rstd over the P*C/G values of a group,  rstd = 1/sqrt(variance + eps)
  *   y = act(gamma * xhat + beta)
  * Pixel p of image n begins at n*x_image + p*x_pixel; y (and dy) likewise, dx as x.  G == 1 is a layer norm over whole images,
- * G == C an instance norm.  Limits: C/G <= 4096, and about 2^24 images. */
+ * G == C an instance norm.  Limits: C/G <= 4096, N*C < 2^31, and fewer than 2^24 - C/8 workgroups, of which an image has one for every
+ * `span` channels (of the plan: up to 4096, whole groups): about 2^24 images of up to 4096 channels, half as many of 8192. */
 typedef struct {
     int N;
     long P;
@@ -533,7 +537,7 @@ int fc_rotary(fc_context *ctx, const fc_rotary_shape *shape, const void *q_dev, 
  * lengths: B int32, or NULL when every sequence has T tokens; sequence b then ends after min(max(lengths[b], 0), T) of them: its later
  * tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
  * A value that is not finite reaches no token before its own; in v it makes its channel of the state NaN from then on.
- * Limits: Dk, Dv <= 256, B*H < 2^21. */
+ * Limits: Dk, Dv <= 256, B*H < 2^21, T < 2^31. */
 typedef struct {
     int B;
     long T;
