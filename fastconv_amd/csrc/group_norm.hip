@@ -1064,6 +1064,8 @@ extern "C" int fc_group_norm(fc_context *ctx, const fc_group_norm_plan *plan, co
     if ((addr & (fc_elem_size(plan->shape.dtype) - 1)) || ((uint64_t)ws_dev & 7) ||
         (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_group_norm: unaligned pointer");
+    const fc_group_norm_shape &s = plan->shape;
+    if (!fc_apart(s.N, s.y_image, s.C) || !fc_apart(s.P, s.y_pixel, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm: pixels of y overlap");
     norm_params p = params_of(plan);
     p.x = x_dev; p.y = y_dev; p.gamma = gamma_dev; p.beta = beta_dev; p.mean = mean_dev; p.rstd = rstd_dev;
     p.part = (float2 *)ws_dev;
@@ -1091,6 +1093,8 @@ extern "C" int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan 
     if ((addr & (fc_elem_size(plan->shape.dtype) - 1)) || ((uint64_t)ws_dev & 7) ||
         (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev | (uint64_t)dgamma_dev | (uint64_t)dbeta_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: unaligned pointer");
+    const fc_group_norm_shape &s = plan->shape;
+    if (!fc_apart(s.N, s.x_image, s.C) || !fc_apart(s.P, s.x_pixel, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: pixels of dx overlap");
     norm_params p = params_of(plan);
     p.x = x_dev; p.dy = dy_dev; p.y = dx_dev; p.gamma = gamma_dev; p.beta = beta_dev;
     p.mean = const_cast<float *>(mean_dev); p.rstd = const_cast<float *>(rstd_dev);      // only read

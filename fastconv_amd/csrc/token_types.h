@@ -60,6 +60,9 @@ static inline long fc_count(long a, long b, long c = 1) {
     return p < 0 || p > ((__int128)1 << 62) ? -1 : (long)p;
 }
 
+// Rows of so many elements, n of them a stride apart, share none.
+static inline bool fc_apart(long n, long stride, long row) { return n < 2 || stride >= row; }
+
 __device__ __forceinline__ float fc_wave_sum(float v) {
 #pragma unroll
     for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);

@@ -455,7 +455,8 @@ int fc_maxpool2x2(fc_context *ctx, const float *x_dev, float *y_dev, int N, int 
  * fp32; fp32 tensors have 24 bits of everything there, and every state takes in 24 bits of what is added to it).  Parameters (gamma, beta, log_decay, inv_freq), statistics and states are fp32 always.
  * Strides are in elements; channels of one token (one head) are neighbours.  Pointers need the alignment of their type only:
  * rows that begin on 16 bytes and have sizes that are multiples of 16 bytes are read fastest.  Buffers must not overlap, but
- * where a call says so.  All calls run on the context's stream, allocate nothing and can be recorded into a graph; they are not
+ * where a call says so.  An input may be shared along an axis (stride 0); the rows of an output may not, and a gradient has the strides of
+ * what it is the gradient of: FC_ERR_INVALID.  All calls run on the context's stream, allocate nothing and can be recorded into a graph; they are not
  * stages and are never bracketed by timing events.  Sizes that are refused: FC_ERR_INVALID for what no such operator has,
  * FC_ERR_UNSUPPORTED beyond the limits stated here. */
 typedef enum { FC_F32 = 0, FC_BF16 = 1, FC_F16 = 2 } fc_dtype;

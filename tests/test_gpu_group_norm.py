@@ -402,3 +402,29 @@ def test_tensors_beyond_the_last_cache(lib, dtype, N, act):
     close(dbeta.get(), total(dz), total(tdz) + places * total(np.abs(dz)) + 1e-30, "dbeta")
     close(dgamma.get(), total(dz * xhat), total(tdz * ax + np.abs(dz) * txh) + places * total(np.abs(dz) * ax) + 1e-30, "dgamma")
     lib.release(mark)
+
+
+def test_outputs_that_share_pixels_are_refused(lib):
+    """One image for all of a batch is an input like any other, but no output, and its gradient would be a sum."""
+    N, P, C_, G = 3, 20, 32, 4
+    rng = np.random.default_rng(15)
+    x, gamma, beta = inputs(rng, 1, P, C_)
+    mark = lib.mark()
+    dx, y = K.Dev(lib, (1, P, C_), "f32", None, x), K.Dev(lib, (N, P, C_), "f32")
+    m, r = (K.Dev(lib, (N, G), "f32") for _ in range(2))
+    plan = lib.group_norm_plan(F.GroupNormShape(N, P, C_, G, F.F32, F.ACT_SILU, EPS, 0, C_, P * C_, C_))
+    g, b, ws = K.floats(lib, gamma), K.floats(lib, beta), lib.alloc(max(4, plan.ws_bytes, plan.ws_backward_bytes))
+    lib.group_norm(plan, dx.ptr, g, b, y.ptr, m.ptr, r.ptr, ws)
+    got = y.get()
+    want, mean, rstd, *_ = K.group_norm(dx.values, gamma, beta, G, EPS, "silu")
+    close(got[:1], want, K.ROUND["f32"] * np.abs(want) + 1.2 * bounds(dx.values, gamma, beta, G, rstd, mean), "y")
+    assert np.array_equal(got[1:], got[:-1])
+    with pytest.raises(F.FastConvError) as e:
+        lib.group_norm_backward(plan, y.ptr, dx.ptr, g, b, m.ptr, r.ptr, dx.ptr, None, None, ws)
+    assert e.value.status == -1 and "overlap" in str(e.value)
+    for strides in ((P * C_, C_, 0, C_), (P * C_, C_, P * C_, C_ - 1), (P * C_, C_, P * C_, 0)):
+        bad = lib.group_norm_plan(F.GroupNormShape(N, P, C_, G, F.F32, F.ACT_SILU, EPS, *strides))
+        with pytest.raises(F.FastConvError) as e:
+            lib.group_norm(bad, y.ptr, g, b, y.ptr, None, None, ws)
+        assert e.value.status == -1 and "overlap" in str(e.value)
+    lib.release(mark)
