@@ -248,3 +248,16 @@ def test_as_many_tokens_as_a_launch_holds(lib):
     assert (got == got[0]).all()
     check(values.reshape(1, T, 1, 2), got[:1].astype(np.float64).reshape(1, T, 1, 2), positions, ladder((1,)) * np.float32(0.01), (1,), False, False, "f16")
     lib.release(mark)
+
+
+def test_outputs_that_share_heads_are_refused(lib):
+    mark = lib.mark()
+    p = lib.alloc(1 << 20).value
+    for name in ("qo_batch", "qo_token", "qo_head", "ko_batch", "ko_token", "ko_head"):
+        for value in (0, 63):
+            s = F.RotaryShape.packed(2, 8, 4, 2, 64, (8, 12, 12), F.BF16)
+            setattr(s, name, value)
+            with pytest.raises(F.FastConvError) as e:
+                lib.rotary(s, p, p, p, p, p, p)
+            assert e.value.status == -1 and "overlap" in str(e.value)
+    lib.release(mark)
