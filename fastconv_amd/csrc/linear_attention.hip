@@ -368,6 +368,10 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
     return FC_OK;
 }
 
+static bool apart(const fc_linear_attention_shape &s, long heads, long batch, long token, long head, int row) {
+    return fc_apart(s.B, batch, row) && fc_apart(s.T, token, row) && fc_apart(heads, head, row);
+}
+
 static int check_plan(fc_context *ctx, const fc_linear_attention_plan *plan, const char *what) {
     fc_linear_attention_plan own;
     if (!plan || fc_linear_attention_make_plan(&plan->shape, &own) != FC_OK || !same(*plan, own)) return fail(ctx, FC_ERR_INVALID, what);
@@ -384,6 +388,7 @@ extern "C" int fc_linear_attention(fc_context *ctx, const fc_linear_attention_pl
     if ((((uint64_t)q_dev | (uint64_t)k_dev | (uint64_t)v_dev | (uint64_t)o_dev) & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)ws_dev & 15) ||
         (((uint64_t)log_decay_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev | (uint64_t)lengths_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_linear_attention: unaligned pointer");
+    if (!apart(s, s.H, s.o_batch, s.o_token, s.o_head, s.Dv)) return fail(ctx, FC_ERR_INVALID, "fc_linear_attention: heads of o overlap");
     const int share = s.H / s.Hkv;
     fc_la_run r = {};
     r.q = {q_dev, s.q_batch, s.q_token, s.q_head, 1};
@@ -410,6 +415,9 @@ extern "C" int fc_linear_attention_backward(fc_context *ctx, const fc_linear_att
     if ((addr & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)ws_dev & 15) ||
         (((uint64_t)log_decay_dev | (uint64_t)state_in_dev | (uint64_t)dstate_out_dev | (uint64_t)dstate_in_dev | (uint64_t)lengths_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_linear_attention_backward: unaligned pointer");
+    if (!apart(s, s.H, s.q_batch, s.q_token, s.q_head, s.Dk) || !apart(s, s.Hkv, s.k_batch, s.k_token, s.k_head, s.Dk) ||
+        !apart(s, s.Hkv, s.v_batch, s.v_token, s.v_head, s.Dv))
+        return fail(ctx, FC_ERR_INVALID, "fc_linear_attention_backward: heads of a gradient overlap");
     const int share = s.H / s.Hkv;
     const fc_la_operand q = {q_dev, s.q_batch, s.q_token, s.q_head, 1}, k = {k_dev, s.k_batch, s.k_token, s.k_head, share},
                         v = {v_dev, s.v_batch, s.v_token, s.v_head, share}, d = {do_dev, s.o_batch, s.o_token, s.o_head, 1};

@@ -394,3 +394,36 @@ def test_single_elements_in_segments(lib, dtype, Dk, Dv):
     assert c.plan.segments >= 3
     c.check()
     lib.release(mark)
+
+
+@pytest.mark.parametrize("T", [4, 40])
+def test_keys_shared_by_a_batch_have_no_gradient(lib, T):
+    """Keys and values of one sequence may serve a whole batch; their gradients would be sums, and are refused, as are answers that overlap."""
+    B, H, D = 3, 2, 32
+    rng = np.random.default_rng(16)
+    mark = lib.mark()
+    q, o = K.Dev(lib, (B, T, H, D), "f32", None, rng.standard_normal((B, T, H, D))), K.Dev(lib, (B, T, H, D), "f32")
+    k, v = (K.Dev(lib, (1, T, H, D), "f32", None, rng.standard_normal((1, T, H, D))) for _ in range(2))
+    shape = F.LinearAttentionShape.packed(B, T, H, H, D, D, F.F32, 0.25)
+    shape.k_batch = shape.v_batch = 0
+    plan, g = lib.linear_attention_plan(shape), np.array([-0.05, -0.4], np.float32)
+    ws, gp = lib.alloc(max(16, plan.ws_bytes, plan.ws_backward_bytes)), K.floats(lib, g)
+    lib.linear_attention(plan, q.ptr, k.ptr, v.ptr, gp, o.ptr, ws=ws)
+    both = [np.repeat(t.values, B, axis=0) for t in (k, v)]
+    want, _ = K.linear_attention(q.values, *both, g, 0.25)
+    size, _ = K.linear_attention(np.abs(q.values), *(np.abs(t) for t in both), g, 0.25)
+    assert (np.abs(o.get() - want) <= K.EPS * (2 * T + 2 * D + 64) * size).all()
+    with pytest.raises(F.FastConvError) as e:
+        lib.linear_attention_backward(plan, o.ptr, q.ptr, k.ptr, v.ptr, gp, q.ptr, k.ptr, v.ptr, ws=ws)
+    assert e.value.status == -1 and "overlap" in str(e.value)
+    for name in ("q_batch", "q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "o_batch", "o_token", "o_head"):
+        shape = F.LinearAttentionShape.packed(B, T, H, H, D, D, F.F32, 0.25)
+        setattr(shape, name, D - 1)
+        bad = lib.linear_attention_plan(shape)
+        with pytest.raises(F.FastConvError) as e:
+            if name[0] == "o":
+                lib.linear_attention(bad, q.ptr, k.ptr, v.ptr, gp, o.ptr, ws=ws)
+            else:
+                lib.linear_attention_backward(bad, o.ptr, q.ptr, k.ptr, v.ptr, gp, q.ptr, k.ptr, v.ptr, ws=ws)
+        assert e.value.status == -1 and "overlap" in str(e.value)
+    lib.release(mark)
