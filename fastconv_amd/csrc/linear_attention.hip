@@ -153,8 +153,8 @@ __global__ __launch_bounds__(kThreads) void fc_linear_attention_step_kernel(cons
 }
 
 // The states that segments begin from: parts[s] becomes what enters segment s, for each element of a head's state.  Bound by the chain of segments, eight of
-// which are read at once: 16 heads of 128 in 31 segments, 65 MB read and written, 6 to 13 us by what the caches hold; 8 heads of 64 in 62 segments, 16 MB, 11 us,
-// and in 123 segments 21.
+// which are read at once: 16 heads of 128 in 31 segments, 65 MB read and written, 14 us; 8 heads of 64 in 62 segments, 16 MB, 12 us, and in 123
+// segments 21.
 __global__ __launch_bounds__(kThreads) void fc_linear_attention_scan_kernel(const fc_la_run r, int segments, long segment, float *parts) {
     constexpr int AHEAD = 8;      // segments read before the first is joined
     const int size = r.Dk * r.Dv, blocks = (size + kThreads - 1) / kThreads;

@@ -24,9 +24,9 @@
 // 32 tokens a chunk: with 64 P and its
 // operands would not fit beside the state, and P's products grow with the chunk.  Every wavefront of a workgroup needs the whole P, so each forms
 // a part of it for all.  Segments make up for what one wavefront waits: see the rule beside the plan.
-// 12544 tokens of 16 heads of 128 in bf16: states 37 us, their scan 6 to 13, answers 74, 117 in all, of 33 that a copy of as many bytes takes.  8 x 1225 tokens of 8 heads
-// of 64 in fp32: 16, 5 and 36, 56 in all, of 13.  8 x 3136 tokens of 16 heads of 64 with the backward pass in bf16: 323 us, of 90, in three runs of states (25 to
-// 30 each), three scans (9 to 10) and four runs of answers (52 to 61).
+// 12544 tokens of 16 heads of 128 in bf16: states 38 us, their scan 14, answers 72, 117 to 120 with the launches, of 33 that a copy of as many bytes takes.  8 x 1225 tokens of 8 heads
+// of 64 in fp32: 16, 5 and 36, 56 together, of 13.  8 x 3136 tokens of 16 heads of 64 with the backward pass in bf16: 323 us, of 90, in three runs of states (25 to
+// 30 each), three scans (9 to 10) and four runs of answers (53 to 61).
 #pragma once
 
 #include <atomic>
