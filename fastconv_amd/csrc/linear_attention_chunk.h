@@ -34,10 +34,11 @@
 #include "linear_attention.h"
 
 constexpr int kLaChunk = 32;
-// A state is held divided by a scale from 2 to kLaTop (2^33 where a decay above 1 lets it grow), never by less than 2: then neither it, nor what
-// a chunk adds to it, nor the first part of either comes near the largest float before the state itself does.  Divided by kLaTop a value keeps
-// its three parts down to about 1e-28, and less of them below.
-constexpr double kLaTop = 131072, kLaLeast = 2, kLaMost = kLaTop * 65536;
+// A state is held divided by a scale from 2 to kLaTop (kLaMost where a decay above 1 lets it grow).  Never by less than 2: then neither it, nor what
+// a chunk adds to it, nor the first part of either comes near the largest float before the state itself does.  Never by much more: the third part
+// of small values would be lost.  A wider range saves passes over the state where a head forgets within a chunk or two, 1 % at most (a top of 2^17: 12544 tokens 118 us
+// for 119, the training below 324 for 326), but with 2^17 fp32 operands of 1e-30 keep 18 bits, with 4 those of 1e-33.
+constexpr double kLaTop = 4, kLaLeast = 2, kLaMost = 65536;
 constexpr float kLaLargest = 0x1.fep127f;      // of bf16
 constexpr int kLaLoadsDone = 0x0f70;    // s_waitcnt: no load or store of global memory on its way
 constexpr int kLaOnlyVector = 0x6;      // scheduling: vector and scalar arithmetic may pass, memory and matrix instructions not

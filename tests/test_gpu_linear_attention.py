@@ -427,3 +427,22 @@ def test_keys_shared_by_a_batch_have_no_gradient(lib, T):
                 lib.linear_attention_backward(bad, o.ptr, q.ptr, k.ptr, v.ptr, gp, q.ptr, k.ptr, v.ptr, ws=ws)
         assert e.value.status == -1 and "overlap" in str(e.value)
     lib.release(mark)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("field", ["q", "k", "v", "do"])
+def test_small_values_keep_their_bits(lib, dtype, field):
+    """Operands of 1e-32, whose third parts are about 1e-37, are as exact in proportion as any: what a state is held by does not push them out of range.
+    By size: 32 last places in fp32 and in states, where a sum's roundings are independent of one another; the rounding of the result in bf16."""
+    mark = lib.mark()
+    for T in (90, 200):      # in one piece, in segments
+        print("linear attention, small", dtype, field, T, flush=True)
+        c = Call(lib, 1, T, 3, 3, 64, 64, dtype, 33, carry=False, decay=[-0.34, -0.05, 0.0])
+        scaled(c, [field], 1e-32)
+        q, k, v, do = (t.values for t in (c.q, c.k, c.v, c.do))
+        want = K.linear_attention(q, k, v, c.g, c.scale) + K.linear_attention_backward(do, q, k, v, c.g, c.scale)
+        for name, a, w in zip(("o", "state", "dq", "dk", "dv", "dstate"), c.forward() + c.backward(), want):
+            wide = dtype == "f32" or name in ("state", "dstate")
+            off = np.linalg.norm(a - w) / np.linalg.norm(w)
+            assert off <= (32 * K.EPS if wide else K.ROUND[dtype]), (name, off)
+    lib.release(mark)
