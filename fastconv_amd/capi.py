@@ -102,6 +102,64 @@ class LinearAttentionPlan(C.Structure):
                 ("ws_backward_bytes", C.c_size_t)]
 
 
+class RmsNormShape(C.Structure):
+    """Strides in elements: row i begins at i * x_row (8-bit results: i * y_row bytes)."""
+    _fields_ = [("rows", C.c_long), ("C", C.c_int), ("dtype", C.c_int), ("eps", C.c_float)] + \
+               [(n, C.c_long) for n in ("x_row", "residual_row", "sum_row", "y_row")]
+
+    @classmethod
+    def packed(cls, rows, Cc, dtype=F32, eps=1e-5):
+        return cls(rows, Cc, dtype, eps, Cc, Cc, Cc, Cc)
+
+
+class RmsNormPlan(C.Structure):
+    _fields_ = [("shape", RmsNormShape), ("parts", C.c_int), ("ws_backward_bytes", C.c_size_t)]
+
+
+class Int8ProductShape(C.Structure):
+    """x [M][K] and w [N][K] in bytes, y [M][N] of dtype."""
+    _fields_ = [("M", C.c_long), ("N", C.c_int), ("K", C.c_int), ("dtype", C.c_int)] + [(n, C.c_long) for n in ("x_row", "w_row", "y_row")]
+
+    @classmethod
+    def packed(cls, M, N, K, dtype=F32):
+        return cls(M, N, K, dtype, K, K, N)
+
+
+class Int8ProductPlan(C.Structure):
+    _fields_ = [("shape", Int8ProductShape), ("tile", C.c_int), ("ws_bytes", C.c_size_t)]
+
+
+class CausalConvShape(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_long), ("C", C.c_int), ("taps", C.c_int), ("dtype", C.c_int), ("act", C.c_int)] + \
+               [(n, C.c_long) for n in ("x_batch", "x_token", "y_batch", "y_token")]
+
+    @classmethod
+    def packed(cls, B, T, Cc, taps, dtype=F32, act=ACT_SILU):
+        """x and y [B][T][C]."""
+        return cls(B, T, Cc, taps, dtype, act, T * Cc, Cc, T * Cc, Cc)
+
+
+class CausalConvPlan(C.Structure):
+    _fields_ = [("shape", CausalConvShape), ("walks", C.c_int), ("walks_backward", C.c_int), ("ws_backward_bytes", C.c_size_t)]
+
+
+class SelectiveScanShape(C.Structure):
+    _fields_ = [("B", C.c_int), ("T", C.c_long), ("D", C.c_int), ("N", C.c_int), ("G", C.c_int), ("dtype", C.c_int), ("softplus", C.c_int)] + \
+               [(n, C.c_long) for n in ("x_batch", "x_token", "delta_batch", "delta_token", "z_batch", "z_token", "b_batch", "b_token", "b_group",
+                                        "c_batch", "c_token", "c_group", "y_batch", "y_token")]
+
+    @classmethod
+    def packed(cls, B, T, D, N, G=1, dtype=F32, softplus=True):
+        """x, delta, z, y [B][T][D], B and C [B][T][G][N]."""
+        wide, shared = (T * D, D), (T * G * N, G * N, N)
+        return cls(B, T, D, N, G, dtype, int(softplus), *(wide + wide + wide + shared + shared + wide))
+
+
+class SelectiveScanPlan(C.Structure):
+    _fields_ = [("shape", SelectiveScanShape), ("tiles", C.c_int), ("segments", C.c_int), ("walks_backward", C.c_int), ("ws_bytes", C.c_size_t),
+                ("ws_backward_bytes", C.c_size_t)]
+
+
 class DeviceInfo(C.Structure):
     _fields_ = [("name", C.c_char * 128), ("arch", C.c_char * 32), ("compute_units", C.c_int),
                 ("clock_mhz", C.c_int), ("mem_clock_mhz", C.c_int), ("mem_bus_bits", C.c_int),
@@ -110,6 +168,7 @@ class DeviceInfo(C.Structure):
 
 # every symbol include/fastconv_hip.h declares: name -> (restype, argtypes)
 _vp = C.c_void_p
+_byref = C.byref
 _ABI = {
     "fc_init": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "fc_destroy": (C.c_int, [_vp]),
@@ -182,6 +241,19 @@ _ABI = {
     "fc_linear_attention_make_plan": (C.c_int, [C.POINTER(LinearAttentionShape), C.POINTER(LinearAttentionPlan)]),
     "fc_linear_attention": (C.c_int, [_vp, C.POINTER(LinearAttentionPlan)] + [_vp] * 9),
     "fc_linear_attention_backward": (C.c_int, [_vp, C.POINTER(LinearAttentionPlan)] + [_vp] * 13),
+    "fc_rms_norm_make_plan": (C.c_int, [C.POINTER(RmsNormShape), C.POINTER(RmsNormPlan)]),
+    "fc_rms_norm": (C.c_int, [_vp, C.POINTER(RmsNormPlan)] + [_vp] * 6),
+    "fc_rms_norm_int8": (C.c_int, [_vp, C.POINTER(RmsNormPlan)] + [_vp] * 6),
+    "fc_rms_norm_backward": (C.c_int, [_vp, C.POINTER(RmsNormPlan)] + [_vp] * 8),
+    "fc_quantize_rows": (C.c_int, [_vp, C.c_long, C.c_int, C.c_int, _vp, C.c_long, _vp, C.c_long, _vp]),
+    "fc_int8_product_make_plan": (C.c_int, [C.POINTER(Int8ProductShape), C.POINTER(Int8ProductPlan)]),
+    "fc_int8_product": (C.c_int, [_vp, C.POINTER(Int8ProductPlan)] + [_vp] * 7),
+    "fc_causal_conv_make_plan": (C.c_int, [C.POINTER(CausalConvShape), C.POINTER(CausalConvPlan)]),
+    "fc_causal_conv": (C.c_int, [_vp, C.POINTER(CausalConvPlan)] + [_vp] * 7),
+    "fc_causal_conv_backward": (C.c_int, [_vp, C.POINTER(CausalConvPlan)] + [_vp] * 12),
+    "fc_selective_scan_make_plan": (C.c_int, [C.POINTER(SelectiveScanShape), C.POINTER(SelectiveScanPlan)]),
+    "fc_selective_scan": (C.c_int, [_vp, C.POINTER(SelectiveScanPlan)] + [_vp] * 13),
+    "fc_selective_scan_backward": (C.c_int, [_vp, C.POINTER(SelectiveScanPlan)] + [_vp] * 22),
 }
 
 IGEMM_STATIC_WS_BYTES = 32 << 20
@@ -530,6 +602,50 @@ class Library:
                                   lengths=None, ws=None):
         self._check(self.c.fc_linear_attention_backward(self.ctx, C.byref(plan), do, q, k, v, log_decay, dq, dk, dv, state_in,
                                                         dstate_out, dstate_in, lengths, ws))
+
+    def rms_norm_plan(self, shape):
+        return self._plan(self.c.fc_rms_norm_make_plan, RmsNormPlan(), shape)
+
+    def rms_norm(self, plan, x, gamma, y, residual=None, sum=None, rstd=None):
+        self._check(self.c.fc_rms_norm(self.ctx, C.byref(plan), x, residual, gamma, sum, y, rstd))
+
+    def rms_norm_int8(self, plan, x, gamma, q, scale, residual=None, sum=None):
+        self._check(self.c.fc_rms_norm_int8(self.ctx, C.byref(plan), x, residual, gamma, sum, q, scale))
+
+    def rms_norm_backward(self, plan, dy, sum, gamma, rstd, dx, dgamma=None, dsum=None, ws=None):
+        self._check(self.c.fc_rms_norm_backward(self.ctx, C.byref(plan), dy, sum, gamma, rstd, dsum, dx, dgamma, ws))
+
+    def quantize_rows(self, rows, Cc, dtype, x, q, scale, x_row=None, q_row=None):
+        """Strides as in a shape; packed rows if left out."""
+        self._check(self.c.fc_quantize_rows(self.ctx, rows, Cc, dtype, x, Cc if x_row is None else x_row, q, Cc if q_row is None else q_row, scale))
+
+    def int8_product_plan(self, shape):
+        return self._plan(self.c.fc_int8_product_make_plan, Int8ProductPlan(), shape)
+
+    def int8_product(self, plan, x, x_scale, w, w_scale, y, bias=None, ws=None):
+        self._check(self.c.fc_int8_product(self.ctx, C.byref(plan), x, x_scale, w, w_scale, bias, y, ws))
+
+    def causal_conv_plan(self, shape):
+        return self._plan(self.c.fc_causal_conv_make_plan, CausalConvPlan(), shape)
+
+    def causal_conv(self, plan, x, w, bias, y, state_in=None, state_out=None, lengths=None):
+        self._check(self.c.fc_causal_conv(self.ctx, C.byref(plan), x, w, bias, y, state_in, state_out, lengths))
+
+    def causal_conv_backward(self, plan, dy, x, w, bias, dx, dw=None, dbias=None, state_in=None, dstate_out=None, dstate_in=None, lengths=None,
+                             ws=None):
+        self._check(self.c.fc_causal_conv_backward(self.ctx, C.byref(plan), dy, x, w, bias, dx, dw, dbias, state_in, dstate_out, dstate_in,
+                                                   lengths, ws))
+
+    def selective_scan_plan(self, shape):
+        return self._plan(self.c.fc_selective_scan_make_plan, SelectiveScanPlan(), shape)
+
+    def selective_scan(self, plan, x, delta, A, B, C, y, D=None, z=None, delta_bias=None, state_in=None, state_out=None, lengths=None, ws=None):
+        self._check(self.c.fc_selective_scan(self.ctx, _byref(plan), x, delta, A, B, C, D, z, delta_bias, y, state_in, state_out, lengths, ws))
+
+    def selective_scan_backward(self, plan, dy, x, delta, A, B, C, dx, ddelta, dB, dC, D=None, z=None, delta_bias=None, dA=None, dD=None, dz=None,
+                                ddelta_bias=None, state_in=None, dstate_out=None, dstate_in=None, lengths=None, ws=None):
+        self._check(self.c.fc_selective_scan_backward(self.ctx, _byref(plan), dy, x, delta, A, B, C, D, z, delta_bias, dx, ddelta, dA, dB, dC, dD,
+                                                      dz, ddelta_bias, state_in, dstate_out, dstate_in, lengths, ws))
 
     # ---- whole-layer helpers over host arrays (tests, smoke)
     def winograd_conv_fused(self, shape, x, w, bias=None, relu=False, config=None):

@@ -1,0 +1,354 @@
+// Short causal convolution of each channel over the tokens of a sequence, channels last, with its activation:
+//
+//   z_t = bias + sum over j of w[j] x_(t - taps + 1 + j),   y_t = act(z_t);   rows before the first are the state
+//   dz = dy act'(z),   dx_t = sum over j of w[j] dz_(t + taps - 1 - j),   dw[j] = sum over t of dz_t x_(t - taps + 1 + j),   dbias = sum of dz
+//
+// Bound by memory: 2 * taps operations a value against 4 bytes read and written in 16-bit types.  A thread walks down the tokens of a few
+// neighbouring channels with the last rows in registers, so that every row is read once; sequences are cut into walks to fill the chip, each of
+// which reads the taps - 1 rows before its own (backward: and after) once more.
+#include <type_traits>
+
+#include "token_math.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostTaps = 8;
+constexpr int kAhead = 8, kAheadBackward = 4;      // tokens read before the first is used
+// Threads that fill the chip: a walk is cut until there are as many.
+constexpr long kFill = 2048 * 64;
+
+struct conv_params {
+    const void *x, *dy, *state_in, *dstate_out;
+    void *y, *state_out, *dstate_in;      // y: or dx
+    const float *w, *bias;
+    float *part;             // backward: [B * walks][taps + 1][C], the sums of dw and, last, dbias
+    const int32_t *lengths;
+    long T, walk;            // tokens of a sequence and of a walk
+    int B, C, taps, walks, act;
+    fc_fastdiv by_columns, by_walks;
+    long x_batch, x_token, y_batch, y_token;
+
+    __device__ __forceinline__ long length(long b) const {
+        if (!lengths) return T;
+        const long n = lengths[b];
+        return n < 0 ? 0 : n > T ? T : n;
+    }
+};
+
+// What a thread walks over: channels c.. of sequence b, tokens t0 to t1.
+struct conv_place {
+    int c, walk;
+    long b, t0, t1, len;
+    bool none;
+    __device__ __forceinline__ conv_place(const conv_params &p, int columns, int vec) {
+        const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = fc_div(i, p.by_columns);
+        none = row >= (uint32_t)(p.B * p.walks);
+        c = (int)(i - row * columns) * vec;
+        b = fc_div(row, p.by_walks);
+        walk = (int)(row - b * p.walks);
+        t0 = walk * p.walk;
+        t1 = t0 + p.walk < p.T ? t0 + p.walk : p.T;
+        len = none ? 0 : p.length(b);
+    }
+};
+
+// Weights by distance: back[m] belongs to the row m tokens back, so that the loops are the same for every number of taps up to TAPS (2, 3, 4 or 8); those that
+// a convolution lacks are left out, not multiplied by zero.
+template <int DT, int VEC, int TAPS>
+__global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_params p, int columns) {
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    const conv_place at(p, columns, VEC);
+    if (at.none) return;
+    const int taps = TAPS < 8 ? TAPS : p.taps;
+    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (taps - 1) * p.C + at.c;
+    E *y = (E *)p.y + at.b * p.y_batch + at.c;
+    float back[VEC][TAPS], bias[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        bias[v] = p.bias ? p.bias[at.c + v] : 0.f;
+#pragma unroll
+        for (int m = 0; m < TAPS; m++) back[v][m] = m < taps ? p.w[(long)(at.c + v) * taps + taps - 1 - m] : 0.f;
+    }
+    V rows[TAPS - 1 + kAhead];
+    const V zeros = {};
+    auto read = [&](long t) __attribute__((always_inline)) {      // t: of a row within the window of a token of the walk
+        if (t >= 0) return t < at.len ? *(const V *)(x + t * p.x_token) : zeros;
+        return p.state_in && t >= 1 - taps ? *(const V *)(before + (t + taps - 1) * p.C) : zeros;
+    };
+#pragma unroll
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = read(at.t0 - (TAPS - 1) + i);
+    for (long t = at.t0; t < at.t1; t += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) rows[TAPS - 1 + u] = t + u < at.t1 ? read(t + u) : zeros;
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            if (t + u >= at.t1) break;
+            V out = zeros;
+            if (t + u < at.len) {
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    float z = bias[v];
+#pragma unroll
+                    for (int m = TAPS - 1; m >= 0; m--)
+                        if (m < taps) z = __builtin_fmaf(back[v][m], rows[u + TAPS - 1 - m].get(v), z);
+                    out.set(v, p.act == FC_ACT_SILU ? fc_silu(z) : z);
+                }
+            }
+            *(V *)(y + (t + u) * p.y_token) = out;
+        }
+#pragma unroll
+        for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAhead + i];
+    }
+    // The last rows, by whoever read the first: the state may be written over the one before.  Row i lies at or before what it is read from.
+    if (at.walk == 0 && p.state_out) {
+        E *after = (E *)p.state_out + at.b * (taps - 1) * p.C + at.c;
+        for (int i = 0; i < taps - 1; i++) {
+            const V last = read(at.len - (taps - 1) + i);
+            *(V *)(after + (long)i * p.C) = last;
+        }
+    }
+}
+
+template <int DT, int VEC, int TAPS>
+__global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const conv_params p, int columns) {
+    typedef fc_vec<DT, VEC> V;
+    typedef typename fc_elem<DT>::type E;
+    const conv_place at(p, columns, VEC);
+    if (at.none) return;
+    const int taps = TAPS < 8 ? TAPS : p.taps;
+    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (taps - 1) * p.C + at.c;
+    const E *dy = (const E *)p.dy + at.b * p.y_batch + at.c, *dlast = (const E *)p.dstate_out + at.b * (taps - 1) * p.C + at.c;
+    E *dx = (E *)p.y + at.b * p.x_batch + at.c, *dfirst = (E *)p.dstate_in + at.b * (taps - 1) * p.C + at.c;
+    float back[VEC][TAPS], bias[VEC], dback[VEC][TAPS], dbias[VEC], dz[VEC][TAPS];      // dz: of the last tokens, the newest last
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+        bias[v] = p.bias ? p.bias[at.c + v] : 0.f;
+        dbias[v] = 0.f;
+#pragma unroll
+        for (int m = 0; m < TAPS; m++) {
+            back[v][m] = m < taps ? p.w[(long)(at.c + v) * taps + taps - 1 - m] : 0.f;
+            dback[v][m] = dz[v][m] = 0.f;
+        }
+    }
+    V rows[TAPS - 1 + kAheadBackward], grads[kAheadBackward];
+    const V zeros = {};
+    auto read = [&](long t) __attribute__((always_inline)) {
+        if (t >= 0) return t < at.len ? *(const V *)(x + t * p.x_token) : zeros;
+        return p.state_in && t >= 1 - taps ? *(const V *)(before + (t + taps - 1) * p.C) : zeros;
+    };
+#pragma unroll
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = read(at.t0 - (TAPS - 1) + i);
+    // the gradient of row t - TAPS + 1 is whole once dz_t is there: TAPS - 1 tokens past the walk's own
+    const long end = at.t1 + TAPS - 1;
+    for (long t = at.t0; t < end; t += kAheadBackward) {
+#pragma unroll
+        for (int u = 0; u < kAheadBackward; u++) {
+            rows[TAPS - 1 + u] = t + u < end ? read(t + u) : zeros;
+            grads[u] = t + u < end && t + u < at.len ? *(const V *)(dy + (t + u) * p.y_token) : zeros;
+        }
+#pragma unroll
+        for (int u = 0; u < kAheadBackward; u++) {
+            if (t + u >= end) break;
+            const bool there = t + u < at.len, mine = t + u < at.t1;
+            const long row = t + u - (TAPS - 1);
+            const long last = row - (at.len - (taps - 1));      // row of the state after the last token
+            V more = zeros, out;
+            const bool wanted = row >= at.t0 || (at.walk == 0 && row >= 1 - taps && p.dstate_in);
+            if (wanted && p.dstate_out && last >= 0 && last < taps - 1) more = *(const V *)(dlast + last * p.C);
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+#pragma unroll
+                for (int j = 0; j < TAPS - 1; j++) dz[v][j] = dz[v][j + 1];
+                float g = 0.f;
+                if (there) {
+                    g = grads[u].get(v);
+                    if (p.act == FC_ACT_SILU) {
+                        float z = bias[v];
+#pragma unroll
+                        for (int m = TAPS - 1; m >= 0; m--)
+                            if (m < taps) z = __builtin_fmaf(back[v][m], rows[u + TAPS - 1 - m].get(v), z);
+                        g *= fc_silu_slope(z);
+                    }
+                    if (mine) {
+                        dbias[v] += g;
+#pragma unroll
+                        for (int m = 0; m < TAPS; m++)
+                            if (m < taps) dback[v][m] = __builtin_fmaf(g, rows[u + TAPS - 1 - m].get(v), dback[v][m]);
+                    }
+                }
+                dz[v][TAPS - 1] = g;
+                float s = more.get(v);
+#pragma unroll
+                for (int m = 0; m < TAPS; m++)
+                    if (m < taps) s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz_(row + m)
+                out.set(v, row < at.len ? s : 0.f);
+            }
+            if (row >= at.t0) *(V *)(dx + row * p.x_token) = out;
+            else if (row < 0 && wanted) *(V *)(dfirst + (row + taps - 1) * p.C) = out;
+        }
+#pragma unroll
+        for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAheadBackward + i];
+    }
+    if (!p.part) return;
+    float *part = p.part + (at.b * p.walks + at.walk) * (taps + 1) * p.C + at.c;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+#pragma unroll
+        for (int m = 0; m < TAPS; m++)
+            if (m < taps) part[(long)(taps - 1 - m) * p.C + v] = dback[v][m];
+        part[(long)taps * p.C + v] = dbias[v];
+    }
+}
+
+// dw and dbias from the walks' sums, always in the same order: 64 of [taps + 1][C] a workgroup, four wavefronts that share the walks.
+__global__ __launch_bounds__(256) void fc_causal_conv_sum_kernel(const float *part, float *dw, float *dbias, int parts, int C, int taps) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long size = (long)(taps + 1) * C, i = (long)blockIdx.x * 64 + lane;
+    float s = 0.f;
+    if (i < size)
+        for (int n = wave; n < parts; n += 4) s += part[n * size + i];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || i >= size) return;
+    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    const int j = (int)(i / C), c = (int)(i - (long)j * C);
+    if (j == taps) {
+        if (dbias) dbias[c] = s;
+    } else if (dw) {
+        dw[(long)c * taps + j] = s;
+    }
+}
+
+int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
+
+bool same(const fc_causal_conv_plan &a, const fc_causal_conv_plan &b) {
+    const fc_causal_conv_shape &s = a.shape, &t = b.shape;
+    return s.B == t.B && s.T == t.T && s.C == t.C && s.taps == t.taps && s.dtype == t.dtype && s.act == t.act && s.x_batch == t.x_batch &&
+           s.x_token == t.x_token && s.y_batch == t.y_batch && s.y_token == t.y_token && a.walks == b.walks &&
+           a.walks_backward == b.walks_backward && a.ws_backward_bytes == b.ws_backward_bytes;
+}
+
+int check_plan(fc_context *ctx, const fc_causal_conv_plan *plan, const char *what) {
+    fc_causal_conv_plan own;
+    if (!plan || fc_causal_conv_make_plan(&plan->shape, &own) != FC_OK || !same(*plan, own)) return fail(ctx, FC_ERR_INVALID, what);
+    return FC_OK;
+}
+
+// Values of an access.
+int width_of(const fc_causal_conv_shape &s, uint64_t addr) {
+    const int w = fc_widest(s.dtype, (uint64_t)(s.C | s.x_batch | s.x_token | s.y_batch | s.y_token), addr), most = s.dtype == FC_F32 ? 4 : 8;
+    return w == most ? w : s.dtype != FC_F32 && w >= 2 ? 2 : 1;
+}
+
+long walks_of(const fc_causal_conv_shape *s, int vec, int least) {
+    const long columns = s->C / vec, most = (s->T + least - 1) / least;
+    long walks = (kFill + columns * s->B - 1) / (columns * s->B);
+    if (walks > most) walks = most;
+    const long walk = (s->T + walks - 1) / walks;
+    return (s->T + walk - 1) / walk;
+}
+
+template <int DT, int VEC, class F>
+void with_taps(int taps, F launch) {
+    using std::integral_constant;
+    typedef integral_constant<int, DT> dt;
+    typedef integral_constant<int, VEC> vec;
+    if (taps == 2) launch(dt(), vec(), integral_constant<int, 2>());
+    else if (taps == 3) launch(dt(), vec(), integral_constant<int, 3>());
+    else if (taps == 4) launch(dt(), vec(), integral_constant<int, 4>());
+    else launch(dt(), vec(), integral_constant<int, 8>());
+}
+
+template <class F>
+void with_kernel(int dtype, int vec, int taps, F launch) {
+    if (dtype == FC_F32) return vec == 4 ? with_taps<FC_F32, 4>(taps, launch) : with_taps<FC_F32, 1>(taps, launch);
+    if (dtype == FC_BF16) return vec == 8 ? with_taps<FC_BF16, 8>(taps, launch) : vec == 2 ? with_taps<FC_BF16, 2>(taps, launch) : with_taps<FC_BF16, 1>(taps, launch);
+    return vec == 8 ? with_taps<FC_F16, 8>(taps, launch) : vec == 2 ? with_taps<FC_F16, 2>(taps, launch) : with_taps<FC_F16, 1>(taps, launch);
+}
+
+conv_params params_of(const fc_causal_conv_shape &s, int walks, int columns) {
+    conv_params p = {};
+    p.B = s.B; p.T = s.T; p.C = s.C; p.taps = s.taps; p.act = s.act;
+    p.walks = walks;
+    p.walk = (s.T + walks - 1) / walks;
+    p.by_columns = fc_make_fastdiv((uint32_t)columns);
+    p.by_walks = fc_make_fastdiv((uint32_t)walks);
+    p.x_batch = s.x_batch; p.x_token = s.x_token; p.y_batch = s.y_batch; p.y_token = s.y_token;
+    return p;
+}
+
+}  // namespace
+
+extern "C" int fc_causal_conv_make_plan(const fc_causal_conv_shape *s, fc_causal_conv_plan *plan) {
+    if (!plan || !s || s->B < 1 || s->T < 1 || s->C < 1 || s->taps < 2 || !fc_dtype_ok(s->dtype)) return FC_ERR_INVALID;
+    if (s->act != FC_ACT_NONE && s->act != FC_ACT_SILU) return s->act < FC_ACT_NONE || s->act > FC_ACT_GELU ? FC_ERR_INVALID : FC_ERR_UNSUPPORTED;
+    if (s->x_batch < 0 || s->x_token < 0 || s->y_batch < 0 || s->y_token < 0) return FC_ERR_INVALID;
+    // a thread a value, should nothing be aligned, with room for the last workgroup's
+    if (s->taps > kMostTaps || s->T >= (1l << 31) || fc_count(s->B, s->C) < 0 || fc_count(s->B, s->C) >= (1l << 30)) return FC_ERR_UNSUPPORTED;
+    *plan = {};
+    plan->shape = *s;
+    const int vec = width_of(*s, 0);
+    plan->walks = (int)walks_of(s, vec, kAhead);
+    plan->walks_backward = (int)walks_of(s, vec, 4 * s->taps);
+    const long rows = (long)s->B * (plan->walks > plan->walks_backward ? plan->walks : plan->walks_backward);
+    if (fc_count(rows, s->C) < 0 || fc_count(rows, s->C) >= (1l << 31) - kThreads) return FC_ERR_UNSUPPORTED;
+    plan->ws_backward_bytes = (size_t)s->B * plan->walks_backward * (s->taps + 1) * s->C * sizeof(float);
+    return FC_OK;
+}
+
+extern "C" int fc_causal_conv(fc_context *ctx, const fc_causal_conv_plan *plan, const void *x_dev, const float *w_dev, const float *bias_dev,
+                              void *y_dev, const void *state_in_dev, void *state_out_dev, const int32_t *lengths_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_causal_conv: not a plan of fc_causal_conv_make_plan")) return FC_ERR_INVALID;
+    const fc_causal_conv_shape &s = plan->shape;
+    if (!x_dev || !w_dev || !y_dev) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: null pointer");
+    const uint64_t addr = (uint64_t)x_dev | (uint64_t)y_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev;
+    if ((addr & (fc_elem_size(s.dtype) - 1)) || (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)lengths_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: unaligned pointer");
+    if (!fc_apart(s.B, s.y_batch, s.C) || !fc_apart(s.T, s.y_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: tokens of y overlap");
+    const int vec = width_of(s, addr), columns = s.C / vec;
+    conv_params p = params_of(s, plan->walks, columns);
+    p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = y_dev; p.state_in = state_in_dev; p.state_out = state_out_dev; p.lengths = lengths_dev;
+    const unsigned blocks = (unsigned)(((long)s.B * p.walks * columns + kThreads - 1) / kThreads);
+    const fc_device_scope on(ctx);
+    with_kernel(s.dtype, vec, s.taps, [&](auto dt, auto v, auto taps) {
+        fc_causal_conv_kernel<decltype(dt)::value, decltype(v)::value, decltype(taps)::value><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(p, columns);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_causal_conv_kernel");
+    return FC_OK;
+}
+
+extern "C" int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_plan *plan, const void *dy_dev, const void *x_dev, const float *w_dev,
+                                       const float *bias_dev, void *dx_dev, float *dw_dev, float *dbias_dev, const void *state_in_dev,
+                                       const void *dstate_out_dev, void *dstate_in_dev, const int32_t *lengths_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_causal_conv_backward: not a plan of fc_causal_conv_make_plan")) return FC_ERR_INVALID;
+    const fc_causal_conv_shape &s = plan->shape;
+    const bool sums = dw_dev || dbias_dev;
+    if (!dy_dev || !x_dev || !w_dev || !dx_dev || (sums && !ws_dev)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: null pointer");
+    const uint64_t addr = (uint64_t)dy_dev | (uint64_t)x_dev | (uint64_t)dx_dev | (uint64_t)state_in_dev | (uint64_t)dstate_out_dev | (uint64_t)dstate_in_dev;
+    if ((addr & (fc_elem_size(s.dtype) - 1)) ||
+        (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)dw_dev | (uint64_t)dbias_dev | (uint64_t)lengths_dev | (uint64_t)ws_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: unaligned pointer");
+    if (!fc_apart(s.B, s.x_batch, s.C) || !fc_apart(s.T, s.x_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: tokens of dx overlap");
+    const int vec = width_of(s, addr), columns = s.C / vec;
+    conv_params p = params_of(s, plan->walks_backward, columns);
+    p.dy = dy_dev; p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = dx_dev; p.state_in = state_in_dev; p.dstate_out = dstate_out_dev;
+    p.dstate_in = dstate_in_dev; p.lengths = lengths_dev;
+    p.part = sums ? (float *)ws_dev : nullptr;
+    const unsigned blocks = (unsigned)(((long)s.B * p.walks * columns + kThreads - 1) / kThreads);
+    const fc_device_scope on(ctx);
+    with_kernel(s.dtype, vec, s.taps, [&](auto dt, auto v, auto taps) {
+        fc_causal_conv_gradient_kernel<decltype(dt)::value, decltype(v)::value, decltype(taps)::value>
+            <<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(p, columns);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_causal_conv_gradient_kernel");
+    if (!sums) return FC_OK;
+    const long size = (long)(s.taps + 1) * s.C;
+    fc_causal_conv_sum_kernel<<<dim3((unsigned)((size + 63) / 64)), dim3(256), 0, ctx->stream>>>(p.part, dw_dev, dbias_dev, s.B * p.walks, s.C, s.taps);
+    FC_LAUNCH_CHECK(ctx, "fc_causal_conv_sum_kernel");
+    return FC_OK;
+}

@@ -1,0 +1,259 @@
+// Selective scan: entry points, plan, and the kernels that join segments and sums.  See selective_scan.h for the formulas.
+#include "selective_scan.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr long kMostThreads = 1l << 32;      // of a launch, not reached
+constexpr int kMostStates = 64;
+// Up to so many tokens run without tiles, L lanes a channel.
+constexpr long kMostSteps = 4;
+// A sequence is cut where its channels leave the chip idle, and then into as many segments as fill it: a cut forms every state twice.
+constexpr long kEnoughWavefronts = 1536, kWavefronts = 4096;
+constexpr long kWorkgroupsBackward = 1024;
+
+// What enters each segment, from what each adds to none.  Bound by the chain of segments, eight of which are read at once.  GRADS: from the last to the
+// first, and what leaves the first is the gradient of the state before it.
+template <bool GRADS>
+__global__ __launch_bounds__(kThreads) void fc_selective_scan_join_kernel(const fc_scan_run r) {
+    constexpr int AHEAD = 8;
+    const long i = (long)blockIdx.x * kThreads + threadIdx.x, size = (long)r.channels * r.N, b = i / size, dn = i - b * size;
+    if (b >= r.B) return;
+    const long d = dn / r.N;
+    const float rate = fc_scan_rate(r.A[dn]);
+    float *p = (GRADS ? r.grads : r.parts) + b * r.segments * size + dn;
+    const float *steps = r.steps + b * r.segments * r.channels + d, *given = GRADS ? r.dstate_out : r.state_in;
+    float s = given ? given[i] : 0.f;
+    // the segment whose own part nothing follows is not asked for it
+    const int parts = GRADS ? r.segments : r.segments - 1;
+    for (int first = 0; first < r.segments; first += AHEAD) {
+        float add[AHEAD], dt[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const bool there = first + a < parts;
+            const long at = GRADS ? r.segments - 1 - first - a : first + a;
+            add[a] = there ? p[at * size] : 0.f;
+            dt[a] = there ? steps[at * r.channels] : 0.f;
+        }
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            if (first + a >= r.segments) break;
+            const long at = GRADS ? r.segments - 1 - first - a : first + a;
+            p[at * size] = s;
+            s = __builtin_fmaf(__builtin_amdgcn_exp2f(rate * dt[a]), s, add[a]);
+        }
+    }
+    if (GRADS && r.dstate_in) r.dstate_in[i] = s;
+}
+
+// dB and dC of a group from those of its workgroups, always in the same order.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void fc_selective_scan_shared_kernel(const fc_scan_run r, void *db, void *dc, long values) {
+    typedef typename fc_elem<DT>::type E;
+    const int per = r.blocks / r.G;
+    const long block = (long)r.B * r.T * 2 * r.N;
+    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < values; i += (long)gridDim.x * kThreads) {      // [B][T][G][2][N]
+        long rest = i / r.N;
+        const int n = (int)(i - rest * r.N), half = (int)(rest & 1);
+        rest >>= 1;
+        const long bt = rest / r.G, g = rest - bt * r.G, b = bt / r.T, t = bt - b * r.T;
+        const float *p = r.shared + g * per * block + (bt * 2 + half) * r.N + n;
+        float s = 0.f;
+        for (int k = 0; k < per; k++) s += p[k * block];
+        if (half) ((E *)dc)[b * r.c_batch + t * r.c_token + g * r.c_group + n] = (E)s;
+        else ((E *)db)[b * r.b_batch + t * r.b_token + g * r.b_group + n] = (E)s;
+    }
+}
+
+// dA, dD and the gradient of delta_bias from those of each walk, always in the same order: 64 of [D][N + 2] a workgroup, four wavefronts that share the walks.
+__global__ __launch_bounds__(256) void fc_selective_scan_sums_kernel(const fc_scan_run r, float *dA, float *dD, float *dbias) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long size = (long)r.channels * (r.N + 2), i = (long)blockIdx.x * 64 + lane, walks = (long)r.B * r.walks;
+    float s = 0.f;
+    if (i < size)
+        for (long n = wave; n < walks; n += 4) s += r.sums[n * size + i];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || i >= size) return;
+    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+    const long d = i / (r.N + 2);
+    const int n = (int)(i - d * (r.N + 2));
+    if (n < r.N) {
+        if (dA) dA[d * r.N + n] = s;
+    } else if (n == r.N) {
+        if (dD) dD[d] = s;
+    } else if (dbias) {
+        dbias[d] = s;
+    }
+}
+
+int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
+
+bool shape_ok(const fc_selective_scan_shape *s) {
+    if (!s || s->B < 1 || s->T < 1 || s->D < 1 || s->N < 1 || s->G < 1 || s->D % s->G || !fc_dtype_ok(s->dtype)) return false;
+    const long strides[14] = {s->x_batch, s->x_token, s->delta_batch, s->delta_token, s->z_batch, s->z_token, s->b_batch,
+                              s->b_token, s->b_group, s->c_batch, s->c_token, s->c_group, s->y_batch, s->y_token};
+    for (long v : strides)
+        if (v < 0) return false;
+    return true;
+}
+
+bool same(const fc_selective_scan_plan &a, const fc_selective_scan_plan &b) {
+    const fc_selective_scan_shape &s = a.shape, &t = b.shape;
+    return s.B == t.B && s.T == t.T && s.D == t.D && s.N == t.N && s.G == t.G && s.dtype == t.dtype && s.softplus == t.softplus && s.x_batch == t.x_batch &&
+           s.x_token == t.x_token && s.delta_batch == t.delta_batch && s.delta_token == t.delta_token && s.z_batch == t.z_batch && s.z_token == t.z_token &&
+           s.b_batch == t.b_batch && s.b_token == t.b_token && s.b_group == t.b_group && s.c_batch == t.c_batch && s.c_token == t.c_token &&
+           s.c_group == t.c_group && s.y_batch == t.y_batch && s.y_token == t.y_token && a.tiles == b.tiles && a.segments == b.segments &&
+           a.walks_backward == b.walks_backward && a.ws_bytes == b.ws_bytes && a.ws_backward_bytes == b.ws_backward_bytes;
+}
+
+int check_plan(fc_context *ctx, const fc_selective_scan_plan *plan, const char *what) {
+    fc_selective_scan_plan own;
+    if (!plan || fc_selective_scan_make_plan(&plan->shape, &own) != FC_OK || !same(*plan, own)) return fail(ctx, FC_ERR_INVALID, what);
+    return FC_OK;
+}
+
+int blocks_of(const fc_selective_scan_shape &s) {
+    const int width = fc_scan_width(fc_scan_lanes(s.N)), per_group = s.D / s.G;
+    return s.G * ((per_group + width - 1) / width);
+}
+
+size_t states_of(const fc_selective_scan_shape &s, long segments) { return (size_t)s.B * segments * s.D * s.N; }
+
+fc_scan_run run_of(const fc_selective_scan_shape &s) {
+    fc_scan_run r = {};
+    r.B = s.B; r.T = s.T; r.channels = s.D; r.N = s.N; r.G = s.G; r.per_group = s.D / s.G; r.blocks = blocks_of(s); r.softplus = s.softplus;
+    r.x_batch = s.x_batch; r.x_token = s.x_token; r.delta_batch = s.delta_batch; r.delta_token = s.delta_token;
+    r.z_batch = s.z_batch; r.z_token = s.z_token; r.y_batch = s.y_batch; r.y_token = s.y_token;
+    r.b_batch = s.b_batch; r.b_token = s.b_token; r.b_group = s.b_group; r.c_batch = s.c_batch; r.c_token = s.c_token; r.c_group = s.c_group;
+    return r;
+}
+
+int join(fc_context *ctx, const fc_scan_run &r, bool grads) {
+    const dim3 grid((unsigned)(((long)r.B * r.channels * r.N + kThreads - 1) / kThreads));
+    if (grads) fc_selective_scan_join_kernel<true><<<grid, dim3(kThreads), 0, ctx->stream>>>(r);
+    else fc_selective_scan_join_kernel<false><<<grid, dim3(kThreads), 0, ctx->stream>>>(r);
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_join_kernel");
+    return FC_OK;
+}
+
+}  // namespace
+
+#define FC_SCAN_CALL(what, dtype, ...)                                                              \
+    ((dtype) == FC_F32 ? fc_scan_##what##_f32(__VA_ARGS__) : (dtype) == FC_BF16 ? fc_scan_##what##_bf16(__VA_ARGS__) : fc_scan_##what##_f16(__VA_ARGS__))
+
+extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_selective_scan_plan *plan) {
+    if (!plan || !shape_ok(s)) return FC_ERR_INVALID;
+    if (s->N > kMostStates || s->T >= (1l << 31) || fc_count(s->B, s->D, 16 * kMostStates) < 0) return FC_ERR_UNSUPPORTED;
+    const long tiles = (s->T + kScanTile - 1) / kScanTile, workgroups = (long)blocks_of(*s) * s->B;
+    // threads of the widest launch: every tile of every channel, or every state
+    if (fc_count(workgroups, tiles) < 0 || workgroups * tiles >= kMostThreads / kThreads || fc_count(s->B, s->D) >= kMostThreads / kMostStates ||
+        fc_count(s->B * tiles, s->D, kScanTile * kMostStates) < 0)
+        return FC_ERR_UNSUPPORTED;
+    *plan = {};
+    plan->shape = *s;
+    plan->tiles = s->T > kMostSteps ? (int)tiles : 0;
+    plan->segments = 1;
+    const int lanes = fc_scan_lanes(s->N);
+    const long wavefronts = workgroups * (fc_scan_width(lanes) * lanes / 64);
+    if (plan->tiles && wavefronts < kEnoughWavefronts) {
+        long segments = kWavefronts / wavefronts;
+        if (segments > tiles / 2) segments = tiles / 2;
+        if (segments > 1) {
+            const long per = (tiles + segments - 1) / segments;
+            plan->segments = (int)((tiles + per - 1) / per);
+        }
+    }
+    if (plan->segments > 1) plan->ws_bytes = (states_of(*s, plan->segments) + (size_t)s->B * plan->segments * s->D) * sizeof(float);
+    long walks = (kWorkgroupsBackward + workgroups - 1) / workgroups;
+    if (walks > tiles) walks = tiles;
+    const long per_walk = (tiles + walks - 1) / walks;
+    plan->walks_backward = (int)((tiles + per_walk - 1) / per_walk);
+    plan->ws_backward_bytes = (2 * states_of(*s, tiles) + (size_t)s->B * tiles * s->D + (size_t)blocks_of(*s) * s->B * s->T * 2 * s->N +
+                               (size_t)s->B * plan->walks_backward * s->D * (s->N + 2)) * sizeof(float);
+    return FC_OK;
+}
+
+extern "C" int fc_selective_scan(fc_context *ctx, const fc_selective_scan_plan *plan, const void *x_dev, const void *delta_dev, const float *A_dev,
+                                 const void *B_dev, const void *C_dev, const float *D_dev, const void *z_dev, const float *delta_bias_dev, void *y_dev,
+                                 const float *state_in_dev, float *state_out_dev, const int32_t *lengths_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_selective_scan: not a plan of fc_selective_scan_make_plan")) return FC_ERR_INVALID;
+    const fc_selective_scan_shape &s = plan->shape;
+    if (!x_dev || !delta_dev || !A_dev || !B_dev || !C_dev || !y_dev || (!ws_dev && plan->ws_bytes))
+        return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: null pointer");
+    if ((((uint64_t)x_dev | (uint64_t)delta_dev | (uint64_t)B_dev | (uint64_t)C_dev | (uint64_t)z_dev | (uint64_t)y_dev) & (fc_elem_size(s.dtype) - 1)) ||
+        (((uint64_t)A_dev | (uint64_t)D_dev | (uint64_t)delta_bias_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev | (uint64_t)lengths_dev |
+          (uint64_t)ws_dev) & 3))
+        return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: unaligned pointer");
+    if (!fc_apart(s.B, s.y_batch, s.D) || !fc_apart(s.T, s.y_token, s.D)) return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: tokens of y overlap");
+    fc_scan_run r = run_of(s);
+    r.x = x_dev; r.delta = delta_dev; r.A = A_dev; r.b = B_dev; r.c = C_dev; r.D = D_dev; r.z = z_dev; r.delta_bias = delta_bias_dev; r.y = y_dev;
+    r.state_in = state_in_dev; r.state_out = state_out_dev; r.lengths = lengths_dev;
+    const fc_device_scope on(ctx);
+    if (!plan->tiles) return FC_SCAN_CALL(step, s.dtype, ctx, r);
+    const long tiles = (s.T + kScanTile - 1) / kScanTile, per = (tiles + plan->segments - 1) / plan->segments;
+    r.segments = plan->segments;
+    r.segment = per * kScanTile;
+    r.per_walk = 1;
+    if (r.segments > 1) {
+        r.parts = (float *)ws_dev;
+        r.steps = r.parts + states_of(s, r.segments);
+        r.walks = r.segments - 1;      // nothing follows the last
+        int rc = FC_SCAN_CALL(ends, s.dtype, ctx, r);
+        if (rc || (rc = join(ctx, r, false))) return rc;
+    }
+    r.walks = r.segments;
+    return FC_SCAN_CALL(answers, s.dtype, ctx, r);
+}
+
+extern "C" int fc_selective_scan_backward(fc_context *ctx, const fc_selective_scan_plan *plan, const void *dy_dev, const void *x_dev,
+                                          const void *delta_dev, const float *A_dev, const void *B_dev, const void *C_dev, const float *D_dev,
+                                          const void *z_dev, const float *delta_bias_dev, void *dx_dev, void *ddelta_dev, float *dA_dev, void *dB_dev,
+                                          void *dC_dev, float *dD_dev, void *dz_dev, float *ddelta_bias_dev, const float *state_in_dev,
+                                          const float *dstate_out_dev, float *dstate_in_dev, const int32_t *lengths_dev, void *ws_dev) {
+    if (!fc_ctx_ok(ctx)) return FC_ERR_STATE;
+    if (check_plan(ctx, plan, "fc_selective_scan_backward: not a plan of fc_selective_scan_make_plan")) return FC_ERR_INVALID;
+    const fc_selective_scan_shape &s = plan->shape;
+    if (!dy_dev || !x_dev || !delta_dev || !A_dev || !B_dev || !C_dev || !dx_dev || !ddelta_dev || !dB_dev || !dC_dev || (z_dev && !dz_dev) || !ws_dev)
+        return fail(ctx, FC_ERR_INVALID, "fc_selective_scan_backward: null pointer");
+    const uint64_t addr = (uint64_t)dy_dev | (uint64_t)x_dev | (uint64_t)delta_dev | (uint64_t)B_dev | (uint64_t)C_dev | (uint64_t)z_dev |
+                          (uint64_t)dx_dev | (uint64_t)ddelta_dev | (uint64_t)dB_dev | (uint64_t)dC_dev | (uint64_t)dz_dev;
+    const uint64_t floats = (uint64_t)A_dev | (uint64_t)D_dev | (uint64_t)delta_bias_dev | (uint64_t)dA_dev | (uint64_t)dD_dev | (uint64_t)ddelta_bias_dev |
+                            (uint64_t)state_in_dev | (uint64_t)dstate_out_dev | (uint64_t)dstate_in_dev | (uint64_t)lengths_dev | (uint64_t)ws_dev;
+    if ((addr & (fc_elem_size(s.dtype) - 1)) || (floats & 3)) return fail(ctx, FC_ERR_INVALID, "fc_selective_scan_backward: unaligned pointer");
+    if (!fc_apart(s.B, s.x_batch, s.D) || !fc_apart(s.T, s.x_token, s.D) || !fc_apart(s.B, s.delta_batch, s.D) || !fc_apart(s.T, s.delta_token, s.D) ||
+        (z_dev && (!fc_apart(s.B, s.z_batch, s.D) || !fc_apart(s.T, s.z_token, s.D))) || !fc_apart(s.B, s.b_batch, s.N) || !fc_apart(s.T, s.b_token, s.N) ||
+        !fc_apart(s.G, s.b_group, s.N) || !fc_apart(s.B, s.c_batch, s.N) || !fc_apart(s.T, s.c_token, s.N) || !fc_apart(s.G, s.c_group, s.N))
+        return fail(ctx, FC_ERR_INVALID, "fc_selective_scan_backward: tokens of a gradient overlap");
+    fc_scan_run r = run_of(s);
+    r.dy = dy_dev; r.x = x_dev; r.delta = delta_dev; r.A = A_dev; r.b = B_dev; r.c = C_dev; r.D = D_dev; r.z = z_dev; r.delta_bias = delta_bias_dev;
+    r.dx = dx_dev; r.ddelta = ddelta_dev; r.dz = dz_dev;
+    r.state_in = state_in_dev; r.dstate_out = dstate_out_dev; r.dstate_in = dstate_in_dev; r.lengths = lengths_dev;
+    const long tiles = (s.T + kScanTile - 1) / kScanTile;
+    r.segments = (int)tiles;
+    r.segment = kScanTile;
+    r.walks = plan->walks_backward;
+    r.per_walk = (int)((tiles + r.walks - 1) / r.walks);
+    r.parts = (float *)ws_dev;
+    r.grads = r.parts + states_of(s, tiles);
+    r.steps = r.grads + states_of(s, tiles);
+    r.shared = r.steps + (size_t)s.B * tiles * s.D;
+    r.sums = r.shared + (size_t)r.blocks * s.B * s.T * 2 * s.N;
+    const fc_device_scope on(ctx);
+    int rc = FC_SCAN_CALL(ends, s.dtype, ctx, r);
+    if (rc || (rc = join(ctx, r, false)) || (rc = join(ctx, r, true))) return rc;
+    rc = FC_SCAN_CALL(gradients, s.dtype, ctx, r);
+    if (rc) return rc;
+    const long values = (long)s.B * s.T * s.G * 2 * s.N, want = (values + kThreads - 1) / kThreads;
+    const auto sum = s.dtype == FC_F32    ? fc_selective_scan_shared_kernel<FC_F32>
+                     : s.dtype == FC_BF16 ? fc_selective_scan_shared_kernel<FC_BF16>
+                                          : fc_selective_scan_shared_kernel<FC_F16>;
+    sum<<<dim3((unsigned)(want < 65536 ? want : 65536)), dim3(kThreads), 0, ctx->stream>>>(r, dB_dev, dC_dev, values);
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_shared_kernel");
+    if (!dA_dev && !dD_dev && !ddelta_bias_dev) return FC_OK;
+    fc_selective_scan_sums_kernel<<<dim3((unsigned)(((long)s.D * (s.N + 2) + 63) / 64)), dim3(256), 0, ctx->stream>>>(r, dA_dev, dD_dev, ddelta_bias_dev);
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_sums_kernel");
+    return FC_OK;
+}

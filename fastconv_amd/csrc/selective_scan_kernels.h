@@ -1,0 +1,600 @@
+// Kernels of the selective scan, for one element type each (selective_scan_<type>.hip).
+#pragma once
+
+#include <type_traits>
+
+#include "selective_scan.h"
+
+namespace {
+
+// v of the lane that a cross-lane pattern of DPP names
+template <int CONTROL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CONTROL, 0xf, 0xf, true));
+}
+
+// The sum over the L neighbouring lanes of a channel, in all of them.
+template <int L>
+__device__ __forceinline__ float sum_states(float v) {
+    if (L > 1) v += dpp<0xB1>(v);       // lanes 1, 0, 3, 2
+    if (L > 2) v += dpp<0x4E>(v);       // lanes 2, 3, 0, 1
+    if (L > 4) v += dpp<0x141>(v);      // eight lanes in reverse
+    if (L > 8) v += dpp<0x140>(v);      // sixteen
+    return v;
+}
+
+template <int L>
+struct scan_form {
+    static constexpr int CH = L <= 4 ? 64 : 256 / L, THREADS = CH * L, WAVES = THREADS / 64, NP = L * kScanStates;
+    static constexpr int ROWS = THREADS / CH, EACH = kScanTile / ROWS;      // tokens at once, and of a thread, where threads lie along the channels
+    static constexpr int SHARED = (kScanTile * NP + THREADS - 1) / THREADS;      // values of B of a thread
+};
+
+// Where a workgroup is, and its threads in both of their arrangements.
+template <int L>
+struct scan_place {
+    typedef scan_form<L> F;
+    long b, len;
+    int walk, group, block;
+    int c, row;              // channel and first token of a tile, along the channels
+    int d, ds;               // channel along the channels and along the states; -1 past the last
+    int chan, sg;            // along the states: channel of the workgroup, four states of it
+    __device__ __forceinline__ scan_place(const fc_scan_run &r) {
+        unsigned i = blockIdx.x;
+        block = i % r.blocks;
+        i /= r.blocks;
+        walk = i % r.walks;
+        b = i / r.walks;
+        len = fc_scan_length(r, b);
+        const int per = r.blocks / r.G;
+        group = block / per;
+        const int first = (block - group * per) * F::CH, tid = threadIdx.x;
+        c = tid % F::CH;
+        row = tid / F::CH;
+        chan = tid / L;
+        sg = tid % L;
+        d = first + c < r.per_group ? group * r.per_group + first + c : -1;
+        ds = first + chan < r.per_group ? group * r.per_group + first + chan : -1;
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ float step_of(const fc_scan_run &r, float raw) {
+    return r.softplus ? fc_softplus(raw) : raw;
+}
+
+// What a thread has of a tile before it is laid out for the states: values of its channel, one every ROWS tokens.  Nothing past `end` is read.
+template <int DT, int L, bool GATE, bool DY>
+struct scan_tile {
+    typedef scan_form<L> F;
+    typedef typename fc_elem<DT>::type E;
+    E x[F::EACH], delta[F::EACH], z[GATE ? F::EACH : 1], dy[DY ? F::EACH : 1], b[F::SHARED], c[F::SHARED];
+
+    __device__ __forceinline__ void read(const fc_scan_run &r, const scan_place<L> &at, long t0, long end, bool with_c) {
+        if (at.d >= 0) {
+            const E *px = (const E *)r.x + at.b * r.x_batch + at.d, *pd = (const E *)r.delta + at.b * r.delta_batch + at.d;
+            const E *pz = (const E *)r.z + at.b * r.z_batch + at.d, *py = (const E *)r.dy + at.b * r.y_batch + at.d;
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) {
+                const long t = t0 + at.row + k * F::ROWS;
+                if (t < end) {
+                    x[k] = px[t * r.x_token];
+                    delta[k] = pd[t * r.delta_token];
+                    if (GATE) z[k] = pz[t * r.z_token];
+                    if (DY) dy[k] = py[t * r.y_token];
+                }
+            }
+        }
+        const E *pb = (const E *)r.b + at.b * r.b_batch + at.group * r.b_group, *pc = (const E *)r.c + at.b * r.c_batch + at.group * r.c_group;
+#pragma unroll
+        for (int k = 0; k < F::SHARED; k++) {
+            const int i = threadIdx.x + k * F::THREADS, n = i % F::NP;
+            const long t = t0 + i / F::NP;
+            b[k] = c[k] = (E)0.f;
+            if (n < r.N && t < end) {
+                b[k] = pb[t * r.b_token + n];
+                if (with_c) c[k] = pc[t * r.c_token + n];
+            }
+        }
+    }
+};
+
+// The same laid out for the states.
+template <int L>
+struct alignas(16) scan_shared {
+    typedef scan_form<L> F;
+    float2 du[kScanTile][F::CH];      // dt and dt x
+    float b[kScanTile][F::NP], c[kScanTile][F::NP];
+};
+
+template <int L, class E>
+__device__ __forceinline__ void lay_out(float (*to)[scan_form<L>::NP], const E (&v)[scan_form<L>::SHARED]) {
+    typedef scan_form<L> F;
+#pragma unroll
+    for (int k = 0; k < F::SHARED; k++) {
+        const int i = threadIdx.x + k * F::THREADS;
+        if (i < kScanTile * F::NP) to[i / F::NP][i % F::NP] = (float)v[k];
+    }
+}
+
+template <int L>
+__device__ __forceinline__ void read_rates(const fc_scan_run &r, const scan_place<L> &at, float (&rate)[kScanStates]) {
+#pragma unroll
+    for (int j = 0; j < kScanStates; j++) {
+        const int n = at.sg * kScanStates + j;
+        rate[j] = at.ds >= 0 && n < r.N ? fc_scan_rate(r.A[(long)at.ds * r.N + n]) : 0.f;
+    }
+}
+
+template <int L>
+__device__ __forceinline__ void read_states(const fc_scan_run &r, const scan_place<L> &at, const float *from, long row, float (&h)[kScanStates]) {
+#pragma unroll
+    for (int j = 0; j < kScanStates; j++) {
+        const int n = at.sg * kScanStates + j;
+        h[j] = from && at.ds >= 0 && n < r.N ? from[(row * r.channels + at.ds) * r.N + n] : 0.f;
+    }
+}
+
+template <int L>
+__device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_place<L> &at, float *to, long row, const float (&h)[kScanStates]) {
+#pragma unroll
+    for (int j = 0; j < kScanStates; j++) {
+        const int n = at.sg * kScanStates + j;
+        if (at.ds >= 0 && n < r.N) to[(row * r.channels + at.ds) * r.N + n] = h[j];
+    }
+}
+
+// Answers.  Bound by the vector ALUs: an exponential (four cycles' worth) and four operations a state, 16 states a value.
+template <int DT, int L, bool GATE>
+__global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_kernel(const fc_scan_run r) {
+    typedef scan_form<L> F;
+    typedef typename fc_elem<DT>::type E;
+    __shared__ scan_shared<L> lds;
+    __shared__ float ys[kScanTile][F::CH];
+    const scan_place<L> at(r);
+    const long t0 = at.walk * r.segment, t1 = t0 + r.segment < r.T ? t0 + r.segment : r.T, end = t1 < at.len ? t1 : at.len;
+    float rate[kScanStates], h[kScanStates];
+    read_rates<L>(r, at, rate);
+    if (r.segments > 1) read_states<L>(r, at, r.parts, at.b * r.segments + at.walk, h);
+    else read_states<L>(r, at, r.state_in, at.b, h);
+    const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
+    E *y = (E *)r.y + at.b * r.y_batch + at.d;
+    scan_tile<DT, L, GATE, false> now;
+    now.read(r, at, t0, end, true);
+    for (long t = t0; t < end; t += kScanTile) {
+        const int n = (int)(end - t < kScanTile ? end - t : kScanTile);
+        float x[F::EACH], z[GATE ? F::EACH : 1];
+#pragma unroll
+        for (int k = 0; k < F::EACH; k++) {
+            x[k] = (float)now.x[k];
+            if (GATE) z[k] = (float)now.z[k];
+            const float dt = step_of<DT>(r, (float)now.delta[k] + bias);
+            lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt, dt * x[k]);
+        }
+        lay_out<L>(lds.b, now.b);
+        lay_out<L>(lds.c, now.c);
+        __syncthreads();
+        if (t + kScanTile < end) now.read(r, at, t + kScanTile, end, true);
+        float mine = 0.f;
+        auto token = [&](int i) __attribute__((always_inline)) {
+            const float2 du = lds.du[i][at.chan];
+            const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates], c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
+            const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < kScanStates; j++) {
+                h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), h[j], du.y * bs[j]);
+                s = __builtin_fmaf(cs[j], h[j], s);
+            }
+            return sum_states<L>(s);
+        };
+        if (n == kScanTile) {
+#pragma unroll 8
+            for (int i = 0; i < kScanTile; i++) {
+                const float s = token(i);
+                mine = i % L == at.sg ? s : mine;      // each lane keeps one of L tokens
+                if (i % L == L - 1) ys[i - L + 1 + at.sg][at.chan] = mine;
+            }
+        } else {
+            for (int i = 0; i < n; i++) {
+                const float s = token(i);
+                if (at.sg == 0) ys[i][at.chan] = s;
+            }
+        }
+        __syncthreads();
+        if (at.d >= 0) {
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) {
+                const int i = at.row + k * F::ROWS;
+                if (i >= n) continue;
+                float v = __builtin_fmaf(skip, x[k], ys[i][at.c]);
+                if (GATE) v *= fc_silu(z[k]);
+                y[(t + i) * r.y_token] = (E)v;
+            }
+        }
+    }
+    // tokens past the end of a shorter sequence
+    if (at.d >= 0)
+        for (long t = (end > t0 ? end : t0) + at.row; t < t1; t += F::ROWS) y[t * r.y_token] = (E)0.f;
+    if (r.state_out && at.walk == r.segments - 1) write_states<L>(r, at, r.state_out, at.b, h);
+}
+
+// What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient.
+template <int DT, int L, bool GRADS, bool GATE>
+__global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
+    typedef scan_form<L> F;
+    __shared__ scan_shared<L> lds;
+    __shared__ float gs[GRADS ? kScanTile : 1][GRADS ? F::CH : 1];
+    const scan_place<L> at(r);
+    const long first = (long)at.walk * r.per_walk * r.segment, last = first + r.per_walk * r.segment < r.T ? first + r.per_walk * r.segment : r.T;
+    const long end = last < at.len ? last : at.len;
+    float rate[kScanStates], h[kScanStates], decay[kScanStates], grad[kScanStates], steps = 0.f;
+    read_rates<L>(r, at, rate);
+    const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f;
+    scan_tile<DT, L, GATE && GRADS, GRADS> now;
+    now.read(r, at, first, end, GRADS);
+    long segment = at.b * r.segments + (long)at.walk * r.per_walk;
+    for (long t = first; t < last; t += kScanTile) {
+        const int n = (int)(end - t < 0 ? 0 : end - t < kScanTile ? end - t : kScanTile);
+        if ((t - first) % r.segment == 0) {
+            steps = 0.f;
+#pragma unroll
+            for (int j = 0; j < kScanStates; j++) {
+                h[j] = grad[j] = 0.f;
+                decay[j] = 1.f;
+            }
+        }
+        if (n > 0) {
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) {
+                const float dt = step_of<DT>(r, (float)now.delta[k] + bias);
+                lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt, dt * (float)now.x[k]);
+                if constexpr (GRADS) {
+                    float g = (float)now.dy[k];
+                    if (GATE) g *= fc_silu((float)now.z[k]);
+                    gs[at.row + k * F::ROWS][at.c] = g;
+                }
+            }
+            lay_out<L>(lds.b, now.b);
+            if (GRADS) lay_out<L>(lds.c, now.c);
+            __syncthreads();
+            if (t + kScanTile < end) now.read(r, at, t + kScanTile, end, GRADS);
+            auto token = [&](int i) __attribute__((always_inline)) {
+                const float2 du = lds.du[i][at.chan];
+                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
+                const float bs[4] = {b.x, b.y, b.z, b.w};
+                float cs[4] = {0.f, 0.f, 0.f, 0.f}, g = 0.f;
+                if constexpr (GRADS) {
+                    const float4 c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
+                    cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+                    g = gs[i][at.chan];
+                }
+                steps += du.x;
+#pragma unroll
+                for (int j = 0; j < kScanStates; j++) {
+                    const float a = __builtin_amdgcn_exp2f(du.x * rate[j]);
+                    h[j] = __builtin_fmaf(a, h[j], du.y * bs[j]);
+                    if (GRADS) {
+                        decay[j] *= a;
+                        grad[j] = __builtin_fmaf(decay[j], cs[j] * g, grad[j]);
+                    }
+                }
+            };
+            if (n == kScanTile) {
+#pragma unroll 8
+                for (int i = 0; i < kScanTile; i++) token(i);
+            } else {
+                for (int i = 0; i < n; i++) token(i);
+            }
+            __syncthreads();
+        }
+        const long next = t + kScanTile;
+        if ((next - first) % r.segment == 0 || next >= last) {
+            write_states<L>(r, at, r.parts, segment, h);
+            if (GRADS) write_states<L>(r, at, r.grads, segment, grad);
+            if (at.sg == 0 && at.ds >= 0) r.steps[segment * r.channels + at.ds] = steps;
+            segment++;
+        }
+    }
+}
+
+// A few tokens of many sequences, L lanes a channel without LDS.  Bound by the states, read and written once a call.
+template <int DT, int L, bool GATE>
+__global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_scan_run r) {
+    typedef typename fc_elem<DT>::type E;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / L;
+    const int sg = threadIdx.x % L;
+    const long b = row / r.channels;
+    const int d = (int)(row - b * r.channels);
+    if (b >= r.B) return;
+    const int group = d / r.per_group, n0 = sg * kScanStates;
+    const long len = fc_scan_length(r, b);
+    float rate[kScanStates], h[kScanStates];
+    const bool wide = (r.N & 3) == 0 && (((uintptr_t)r.A | (uintptr_t)r.state_in | (uintptr_t)r.state_out) & 15) == 0;
+    const float *A = r.A + (long)d * r.N + n0, *from = r.state_in + row * r.N + n0;
+    float *to = r.state_out + row * r.N + n0;
+    if (wide) {
+        const bool some = n0 < r.N;
+        const float4 zeros = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = some ? *(const float4 *)A : zeros, s = some && r.state_in ? *(const float4 *)from : zeros;
+        rate[0] = a.x; rate[1] = a.y; rate[2] = a.z; rate[3] = a.w;
+        h[0] = s.x; h[1] = s.y; h[2] = s.z; h[3] = s.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kScanStates; j++) {
+            const bool some = n0 + j < r.N;
+            rate[j] = some ? A[j] : 0.f;
+            h[j] = some && r.state_in ? from[j] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kScanStates; j++) rate[j] = fc_scan_rate(rate[j]);
+    const float bias = r.delta_bias ? r.delta_bias[d] : 0.f, skip = r.D ? r.D[d] : 0.f;
+    const E *pb = (const E *)r.b + b * r.b_batch + group * r.b_group + n0, *pc = (const E *)r.c + b * r.c_batch + group * r.c_group + n0;
+    E *y = (E *)r.y + b * r.y_batch + d;
+    for (long t = 0; t < len; t++) {
+        const float x = (float)((const E *)r.x)[b * r.x_batch + t * r.x_token + d];
+        const float dt = step_of<DT>(r, (float)((const E *)r.delta)[b * r.delta_batch + t * r.delta_token + d] + bias);
+        const float u = dt * x;
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < kScanStates; j++) {
+            if (n0 + j >= r.N) continue;
+            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * rate[j]), h[j], u * (float)pb[t * r.b_token + j]);
+            s = __builtin_fmaf((float)pc[t * r.c_token + j], h[j], s);
+        }
+        s = __builtin_fmaf(skip, x, sum_states<L>(s));
+        if (GATE) s *= fc_silu((float)((const E *)r.z)[b * r.z_batch + t * r.z_token + d]);
+        if (sg == 0) y[t * r.y_token] = (E)s;
+    }
+    if (sg == 0)
+        for (long t = len; t < r.T; t++) y[t * r.y_token] = (E)0.f;
+    if (!r.state_out) return;
+    if (wide) {
+        if (n0 < r.N) *(float4 *)to = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kScanStates; j++)
+            if (n0 + j < r.N) to[j] = h[j];
+    }
+}
+
+// Sums over the channels of a wavefront (lanes with the same lane % L) of eight values a lane, v[0..3] and v[4..7]: 16 lanes are left with two
+// each.  Lanes of rows 0 and 1 (16 lanes a row) get sums of v[0..1] and v[2..3], rows 2 and 3 of v[4..5] and v[6..7].
+template <int L>
+__device__ __forceinline__ float2 sum_channels(float (&v)[8]) {
+    float w[4], o[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]), __builtin_bit_cast(unsigned, v[i + 4]), false, false);
+        const unsigned a = s[0], b = s[1];
+        w[i] = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, w[i]), __builtin_bit_cast(unsigned, w[i + 2]), false, false);
+        const unsigned a = s[0], b = s[1];
+        o[i] = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+        if (L <= 8) o[i] += dpp<0x128>(o[i]);      // lanes turned by 8 of 16
+        if (L <= 4) o[i] += dpp<0x124>(o[i]);
+        if (L <= 2) o[i] += dpp<0x122>(o[i]);
+        if (L <= 1) o[i] += dpp<0x121>(o[i]);
+    }
+    return make_float2(o[0], o[1]);
+}
+
+// Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.
+template <int DT, int L, bool GATE>
+__global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
+    typedef scan_form<L> F;
+    typedef typename fc_elem<DT>::type E;
+    __shared__ scan_shared<L> lds;
+    __shared__ float gs[kScanTile][F::CH], ys[GATE ? kScanTile : 1][GATE ? F::CH : 1];
+    __shared__ alignas(16) float waves[F::WAVES][kScanTile][2 * F::NP];      // dB and dC of each wavefront's channels
+    __shared__ float2 rows[F::ROWS][F::CH];
+    const scan_place<L> at(r);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float rate[kScanStates], dA[kScanStates] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
+    read_rates<L>(r, at, rate);
+    const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
+    const long first = (long)at.walk * r.per_walk, last = first + r.per_walk < r.segments ? first + r.per_walk : r.segments;
+    E *dx = (E *)r.dx + at.b * r.x_batch + at.d, *dd = (E *)r.ddelta + at.b * r.delta_batch + at.d, *dz = (E *)r.dz + at.b * r.z_batch + at.d;
+    constexpr bool AHEAD = F::EACH <= 8;      // the next tile's values have registers of their own
+    scan_tile<DT, L, GATE, true> now;
+    if (AHEAD) now.read(r, at, first * kScanTile, at.len, true);
+    for (long seg = first; seg < last; seg++) {
+        const long t = seg * kScanTile, end = t + kScanTile < r.T ? t + kScanTile : r.T;
+        const int n = (int)(at.len - t < 0 ? 0 : at.len - t < kScanTile ? at.len - t : kScanTile);
+        float *shared = r.shared + ((at.block * (long)r.B + at.b) * r.T + t) * 2 * r.N;
+        if (n > 0) {
+            if (!AHEAD) now.read(r, at, t, at.len, true);
+            const scan_tile<DT, L, GATE, true> here = now;
+            float steps[F::EACH];
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) {
+                const int i = at.row + k * F::ROWS;
+                const bool in = i < n && at.d >= 0;      // a token past the last moves nothing
+                const float x = in ? (float)here.x[k] : 0.f;
+                steps[k] = in ? step_of<DT>(r, (float)here.delta[k] + bias) : 0.f;
+                float g = in ? (float)here.dy[k] : 0.f;
+                if (GATE && in) g *= fc_silu((float)here.z[k]);
+                lds.du[i][at.c] = make_float2(steps[k], steps[k] * x);
+                gs[i][at.c] = g;
+            }
+            lay_out<L>(lds.b, here.b);
+            lay_out<L>(lds.c, here.c);
+            float start[kScanStates], G[kScanStates];
+            read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
+            read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
+            __syncthreads();
+            if (AHEAD && seg + 1 < last) now.read(r, at, t + kScanTile, at.len, true);
+            float hs[kScanTile][kScanStates];
+            float mine = 0.f;
+#pragma unroll
+            for (int i = 0; i < kScanTile; i++) {
+                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);      // else all tiles' reads move to the front, and registers spill
+                const float2 du = lds.du[i][at.chan];
+                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
+                const float bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int j = 0; j < kScanStates; j++)
+                    hs[i][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), i ? hs[i ? i - 1 : 0][j] : start[j], du.y * bs[j]);
+                if constexpr (GATE) {
+                    const float4 c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
+                    float s = c.x * hs[i][0];
+                    s = __builtin_fmaf(c.y, hs[i][1], s);
+                    s = __builtin_fmaf(c.z, hs[i][2], s);
+                    s = __builtin_fmaf(c.w, hs[i][3], s);
+                    s = sum_states<L>(s);
+                    mine = i % L == at.sg ? s : mine;
+                    if (i % L == L - 1) ys[i - L + 1 + at.sg][at.chan] = mine;
+                }
+            }
+            // steps and exponentials are formed again: kept from above, with the states, they would need twice the registers
+            fc_wave_sync();
+            float2 kept = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = kScanTile - 1; i >= 0; i--) {
+                if (i % 2) __builtin_amdgcn_sched_barrier(0);
+                const float2 du = lds.du[i][at.chan];
+                const float g = gs[i][at.chan];
+                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates], c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
+                const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
+                float v[8], du_sum = 0.f, dt_sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < kScanStates; j++) {
+                    G[j] = __builtin_fmaf(cs[j], g, G[j]);
+                    v[j] = G[j] * du.y;
+                    v[4 + j] = g * hs[i][j];
+                    du_sum = __builtin_fmaf(G[j], bs[j], du_sum);
+                    G[j] *= __builtin_amdgcn_exp2f(du.x * rate[j]);
+                    const float k = G[j] * (i ? hs[i ? i - 1 : 0][j] : start[j]);
+                    dt_sum = __builtin_fmaf(k, rate[j], dt_sum);
+                    dA[j] = __builtin_fmaf(k, du.x, dA[j]);
+                }
+                du_sum = sum_states<L>(du_sum);
+                dt_sum = sum_states<L>(dt_sum);
+                const float2 s = sum_channels<L>(v);
+                if (L == 16 || (lane & 15) < L)
+                    *(float2 *)&waves[wave][i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
+                if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
+                if (i % L == 0) lds.du[i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
+            }
+            __syncthreads();
+            if (at.d >= 0) {
+#pragma unroll
+                for (int k = 0; k < F::EACH; k++) {
+                    const int i = at.row + k * F::ROWS;
+                    if (i >= n) continue;
+                    const float2 s = lds.du[i][at.c];
+                    const float x = (float)here.x[k], g = gs[i][at.c];
+                    float dstep = __builtin_fmaf(x, s.x, 0.693147181f * s.y);
+                    if (r.softplus) dstep *= fc_sigmoid((float)here.delta[k] + bias);
+                    dx[(t + i) * r.x_token] = (E)__builtin_fmaf(steps[k], s.x, skip * g);
+                    dd[(t + i) * r.delta_token] = (E)dstep;
+                    if constexpr (GATE) {
+                        const float z = (float)here.z[k];
+                        dz[(t + i) * r.z_token] = (E)((float)here.dy[k] * __builtin_fmaf(skip, x, ys[i][at.c]) * fc_silu_slope(z));
+                    }
+                    dD = __builtin_fmaf(g, x, dD);
+                    dbias += dstep;
+                }
+            }
+            for (int i = threadIdx.x; i < n * 2 * F::NP; i += F::THREADS) {
+                const int token = i / (2 * F::NP), k = i % (2 * F::NP), half = k / F::NP, state = k % F::NP;
+                if (state >= r.N) continue;
+                float s = waves[0][token][k];
+#pragma unroll
+                for (int w = 1; w < F::WAVES; w++) s += waves[w][token][k];
+                shared[((long)token * 2 + half) * r.N + state] = s;
+            }
+            __syncthreads();
+        }
+        // tokens past the end of a shorter sequence
+        if (at.d >= 0)
+            for (long i = t + n + at.row; i < end; i += F::ROWS) {
+                dx[i * r.x_token] = (E)0.f;
+                dd[i * r.delta_token] = (E)0.f;
+                if (GATE) dz[i * r.z_token] = (E)0.f;
+            }
+        for (long i = (long)n * 2 * r.N + threadIdx.x; i < (end - t) * 2 * r.N; i += F::THREADS) shared[i] = 0.f;
+    }
+    // what this walk adds to the gradients of its channels
+    float *sums = r.sums + ((at.b * r.walks + at.walk) * r.channels) * (r.N + 2);
+#pragma unroll
+    for (int j = 0; j < kScanStates; j++) {
+        const int s = at.sg * kScanStates + j;
+        if (at.ds >= 0 && s < r.N) sums[(long)at.ds * (r.N + 2) + s] = dA[j];
+    }
+    rows[at.row][at.c] = make_float2(dD, dbias);
+    __syncthreads();
+    if (at.row == 0 && at.d >= 0) {
+        float2 s = rows[0][at.c];
+#pragma unroll
+        for (int k = 1; k < F::ROWS; k++) {
+            s.x += rows[k][at.c].x;
+            s.y += rows[k][at.c].y;
+        }
+        sums[(long)at.d * (r.N + 2) + r.N] = s.x;
+        sums[(long)at.d * (r.N + 2) + r.N + 1] = s.y;
+    }
+}
+
+template <class F>
+void with_lanes(int N, F launch) {
+    switch (fc_scan_lanes(N)) {
+        case 1: return launch(std::integral_constant<int, 1>());
+        case 2: return launch(std::integral_constant<int, 2>());
+        case 4: return launch(std::integral_constant<int, 4>());
+        case 8: return launch(std::integral_constant<int, 8>());
+        default: return launch(std::integral_constant<int, 16>());
+    }
+}
+
+template <int DT>
+int scan_answers(fc_context *ctx, const fc_scan_run &r) {
+    with_lanes(r.N, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        const auto kernel = r.z ? fc_selective_scan_kernel<DT, L, true> : fc_selective_scan_kernel<DT, L, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_kernel");
+    return FC_OK;
+}
+
+template <int DT>
+int scan_ends(fc_context *ctx, const fc_scan_run &r) {
+    with_lanes(r.N, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        const auto kernel = !r.dy  ? fc_selective_scan_ends_kernel<DT, L, false, false>
+                            : r.z ? fc_selective_scan_ends_kernel<DT, L, true, true>
+                                  : fc_selective_scan_ends_kernel<DT, L, true, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_ends_kernel");
+    return FC_OK;
+}
+
+template <int DT>
+int scan_step(fc_context *ctx, const fc_scan_run &r) {
+    with_lanes(r.N, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true> : fc_selective_scan_step_kernel<DT, L, false>;
+        kernel<<<dim3((unsigned)(((long)r.B * r.channels * L + 255) / 256)), dim3(256), 0, ctx->stream>>>(r);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_step_kernel");
+    return FC_OK;
+}
+
+template <int DT>
+int scan_gradients(fc_context *ctx, const fc_scan_run &r) {
+    with_lanes(r.N, [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        const auto kernel = r.z ? fc_selective_scan_gradient_kernel<DT, L, true> : fc_selective_scan_gradient_kernel<DT, L, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    });
+    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_gradient_kernel");
+    return FC_OK;
+}
+
+}  // namespace

@@ -63,6 +63,20 @@ static inline long fc_count(long a, long b, long c = 1) {
 // Rows of so many elements, n of them a stride apart, share none.
 static inline bool fc_apart(long n, long stride, long row) { return n < 2 || stride >= row; }
 
+// The context's device, for as long as a call launches on it: a stream takes launches of its own device only.
+struct fc_device_scope {
+    int before;
+    bool moved;
+    explicit fc_device_scope(const fc_context *ctx) : before(ctx->device), moved(false) {
+        if (hipGetDevice(&before) == hipSuccess && before != ctx->device) moved = hipSetDevice(ctx->device) == hipSuccess;
+    }
+    ~fc_device_scope() {
+        if (moved) (void)hipSetDevice(before);
+    }
+    fc_device_scope(const fc_device_scope &) = delete;
+    fc_device_scope &operator=(const fc_device_scope &) = delete;
+};
+
 __device__ __forceinline__ float fc_wave_sum(float v) {
 #pragma unroll
     for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);

@@ -575,6 +575,148 @@ int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan
                                  void *dv_dev, const float *state_in_dev, const float *dstate_out_dev, float *dstate_in_dev,
                                  const int32_t *lengths_dev, void *ws_dev);
 
+/* RMS norm over rows of channels, after the addition of a residual:
+ *   h = x + residual, rounded to the tensors' type;   rstd = 1/sqrt(mean of h^2 + eps);   y = h * rstd * gamma
+ * Row i of x begins at i*x_row, and so for the residual, the sum h and y (in 8 bits: strides of bytes); dy as y, dsum as the sum, dx as x.  A row whose
+ * squares overflow fp32 is normed like any other.  Limits: C <= 2^20, rows <= 2^40. */
+typedef struct {
+    long rows;
+    int C;
+    int dtype;
+    float eps;
+    long x_row, residual_row, sum_row, y_row;
+} fc_rms_norm_shape;
+
+typedef struct {
+    fc_rms_norm_shape shape;
+    int parts;                /* sums of dgamma that are formed side by side */
+    size_t ws_backward_bytes; /* workspace of the backward call, for dgamma */
+} fc_rms_norm_plan;
+
+int fc_rms_norm_make_plan(const fc_rms_norm_shape *shape, fc_rms_norm_plan *plan);
+
+/* residual and gamma (C floats): or NULL for none and ones.  sum: h, or NULL if not wanted; may be x or the residual where their strides are equal.
+ * y may be x or the residual likewise, if the sum is another.  rstd: a float a row for the backward pass, or NULL. */
+int fc_rms_norm(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x_dev, const void *residual_dev, const float *gamma_dev,
+                void *sum_dev, void *y_dev, float *rstd_dev);
+
+/* The same in 8 bits with a scale for each row: scale = max |y| / 127, q = y / scale rounded to nearest, ties to even.  A row whose largest value is below
+ * 2^-110 is zeros with a scale of 0; one with a value that is not finite is zeros with a scale of NaN, so that a product of it is NaN. */
+int fc_rms_norm_int8(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x_dev, const void *residual_dev, const float *gamma_dev,
+                     void *sum_dev, int8_t *q_dev, float *scale_dev);
+
+/* Gradient of x, which is that of the residual too (dx), and of gamma (fp32, overwritten; NULL: not wanted, and no workspace) from that of y and, where h
+ * is read elsewhere as well, of the sum (dsum; NULL: none).  sum: h of the forward call (x itself if there was no residual, with sum_row == x_row).
+ * dx may be dsum where sum_row == x_row, or dy where y_row == x_row.  Sums run in a fixed order. */
+int fc_rms_norm_backward(fc_context *ctx, const fc_rms_norm_plan *plan, const void *dy_dev, const void *sum_dev, const float *gamma_dev,
+                         const float *rstd_dev, const void *dsum_dev, void *dx_dev, float *dgamma_dev, void *ws_dev);
+
+/* Rows in 8 bits as above, without a norm: activations on their way into a product, or its matrix (a row for each output channel) once. */
+int fc_quantize_rows(fc_context *ctx, long rows, int C, int dtype, const void *x_dev, long x_row, int8_t *q_dev, long q_row, float *scale_dev);
+
+/* Product of 8-bit rows with scales for each token and channel:
+ *   y[m][n] = (sum over k of x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]
+ * Rows of x, w (bytes) and y (of `dtype`) begin x_row, w_row and y_row apart; w holds a row for each output channel.  Sums are exact, in 32-bit integers.
+ * Rows of x and w that begin on 16 bytes and have sizes that are multiples of 16 are read fastest.  Limits: K <= 131071, M < 2^31, M*N < 2^36. */
+typedef struct {
+    long M;
+    int N, K;
+    int dtype;
+    long x_row, w_row, y_row;
+} fc_int8_product_shape;
+
+typedef struct {
+    fc_int8_product_shape shape;
+    int tile;                 /* tokens and channels that a workgroup takes; 0: few tokens, w read straight into registers */
+    size_t ws_bytes;          /* workspace, 0 if none */
+} fc_int8_product_plan;
+
+int fc_int8_product_make_plan(const fc_int8_product_shape *shape, fc_int8_product_plan *plan);
+
+/* bias: N floats or NULL. */
+int fc_int8_product(fc_context *ctx, const fc_int8_product_plan *plan, const int8_t *x_dev, const float *x_scale_dev, const int8_t *w_dev,
+                    const float *w_scale_dev, const float *bias_dev, void *y_dev, void *ws_dev);
+
+/* Short causal convolution of each channel over the tokens of a sequence, with its activation (FC_ACT_NONE or FC_ACT_SILU):
+ *   y_t = act(bias + sum over j < taps of w[c][j] x_(t - taps + 1 + j))
+ * Token t of sequence b begins at b*x_batch + t*x_token, and so for y; dy as y, dx as x.  w is fp32 [C][taps], the last tap the token's own.  The inputs before
+ * the first token are a state of taps - 1 rows, packed [B][taps - 1][C] in the tensors' type, the oldest first.
+ * lengths as above: later tokens are not read, their outputs and gradients are zeros, and the state after a sequence holds its own last rows.
+ * Limits: 2 <= taps <= 8, B*C < 2^30, T < 2^31. */
+typedef struct {
+    int B;
+    long T;
+    int C, taps;
+    int dtype, act;
+    long x_batch, x_token, y_batch, y_token;
+} fc_causal_conv_shape;
+
+typedef struct {
+    fc_causal_conv_shape shape;
+    int walks, walks_backward; /* parts of a sequence that threads walk over side by side */
+    size_t ws_backward_bytes;  /* workspace of the backward call, for dw and dbias */
+} fc_causal_conv_plan;
+
+int fc_causal_conv_make_plan(const fc_causal_conv_shape *shape, fc_causal_conv_plan *plan);
+
+/* bias: C floats or NULL.  state_in: NULL for zeros.  state_out: NULL if not wanted; may be state_in.  One token or many. */
+int fc_causal_conv(fc_context *ctx, const fc_causal_conv_plan *plan, const void *x_dev, const float *w_dev, const float *bias_dev, void *y_dev,
+                   const void *state_in_dev, void *state_out_dev, const int32_t *lengths_dev);
+
+/* Gradients of x, w and bias (fp32, overwritten; each may be NULL) and state_in (dstate_in; NULL: not wanted) from those of y and state_out (dstate_out;
+ * NULL: none).  Without dw and dbias no workspace is needed.  Sums run in a fixed order. */
+int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_plan *plan, const void *dy_dev, const void *x_dev, const float *w_dev,
+                            const float *bias_dev, void *dx_dev, float *dw_dev, float *dbias_dev, const void *state_in_dev,
+                            const void *dstate_out_dev, void *dstate_in_dev, const int32_t *lengths_dev, void *ws_dev);
+
+/* Selective scan: every channel d has N states that decay and take in by what the token says:
+ *   dt = delta_t + delta_bias[d], through log(1 + e^dt) if `softplus`
+ *   h_t[n] = exp(dt * A[d][n]) h_(t-1)[n] + dt * x_t * B_t[n],   y_t = (sum over n of C_t[n] h_t[n] + D[d] x_t) * z_t / (1 + e^-z_t)
+ * x, delta, z and y: token t of sequence b begins at b*x_batch + t*x_token and so on, D channels side by side.  B and C are shared by the D/G channels of a
+ * group: N values from b*b_batch + t*b_token + group*b_group on.  A is fp32 [D][N], not its logarithm; a rate above 0 is not checked for (the state
+ * grows), one of minus infinity is a decay of 0 after a step above 0.  States are packed fp32 [B][D][N].
+ * lengths as above: later tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
+ * Limits: N <= 64, T < 2^31, B*D < 2^26, fewer than 2^24 workgroups, of which 32 tokens of 64 channels (N > 16: 32; N > 32: 16) are one. */
+typedef struct {
+    int B;
+    long T;
+    int D, N, G;
+    int dtype;
+    int softplus;
+    long x_batch, x_token;
+    long delta_batch, delta_token;
+    long z_batch, z_token;
+    long b_batch, b_token, b_group;
+    long c_batch, c_token, c_group;
+    long y_batch, y_token;
+} fc_selective_scan_shape;
+
+typedef struct {
+    fc_selective_scan_shape shape;
+    int tiles;                /* tokens are taken in tiles of 32, so many; 0: one by one */
+    int segments;             /* parts of a sequence that run side by side, joined by their states */
+    int walks_backward;       /* parts of a sequence, in whole tiles, of the backward call */
+    size_t ws_bytes;          /* workspace of the forward call, 0 if none */
+    size_t ws_backward_bytes; /* and of the backward call */
+} fc_selective_scan_plan;
+
+int fc_selective_scan_make_plan(const fc_selective_scan_shape *shape, fc_selective_scan_plan *plan);
+
+/* D, delta_bias: D floats each, or NULL for zeros.  z: NULL for no gate.  state_in: NULL for zeros.  state_out: NULL if not wanted; may be state_in.
+ * One token or many. */
+int fc_selective_scan(fc_context *ctx, const fc_selective_scan_plan *plan, const void *x_dev, const void *delta_dev, const float *A_dev,
+                      const void *B_dev, const void *C_dev, const float *D_dev, const void *z_dev, const float *delta_bias_dev, void *y_dev,
+                      const float *state_in_dev, float *state_out_dev, const int32_t *lengths_dev, void *ws_dev);
+
+/* Gradients of x, delta, B, C and, with a gate, z in the tensors' type and with the strides of what they are gradients of, of A, D and delta_bias (fp32,
+ * overwritten; each may be NULL) and of state_in (dstate_in; NULL: not wanted) from those of y and state_out (dstate_out; NULL: none; may be dstate_in).
+ * States are formed again from the inputs.  Gradients of shared values are summed in a fixed order. */
+int fc_selective_scan_backward(fc_context *ctx, const fc_selective_scan_plan *plan, const void *dy_dev, const void *x_dev, const void *delta_dev,
+                               const float *A_dev, const void *B_dev, const void *C_dev, const float *D_dev, const void *z_dev,
+                               const float *delta_bias_dev, void *dx_dev, void *ddelta_dev, float *dA_dev, void *dB_dev, void *dC_dev, float *dD_dev,
+                               void *dz_dev, float *ddelta_bias_dev, const float *state_in_dev, const float *dstate_out_dev, float *dstate_in_dev,
+                               const int32_t *lengths_dev, void *ws_dev);
+
 #ifdef __cplusplus
 }
 #endif
