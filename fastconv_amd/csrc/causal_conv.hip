@@ -14,9 +14,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTaps = 8;
+constexpr int kChannels = 4;     // of a thread, one access wherever they begin; one where there are fewer
 constexpr int kAhead = 8, kAheadBackward = 4;      // tokens read before the first is used
-// Threads that fill the chip: a walk is cut until there are as many.
-constexpr long kFill = 2048 * 64;
+// Threads that fill the chip: a sequence is cut until there are as many, into walks of some tokens at least.
+constexpr long kFill = 4096 * 64;
 
 struct conv_params {
     const void *x, *dy, *state_in, *dstate_out;
@@ -38,13 +39,15 @@ struct conv_params {
 
 // What a thread walks over: channels c.. of sequence b, tokens t0 to t1.
 struct conv_place {
-    int c, walk;
+    int c, skip, walk;       // the last thread of a row begins where its access ends with the row, and leaves out what its neighbour has
     long b, t0, t1, len;
     bool none;
     __device__ __forceinline__ conv_place(const conv_params &p, int columns, int vec) {
         const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = fc_div(i, p.by_columns);
         none = row >= (uint32_t)(p.B * p.walks);
-        c = (int)(i - row * columns) * vec;
+        const int from = (int)(i - row * columns) * vec;
+        c = from + vec <= p.C ? from : p.C - vec;
+        skip = from - c;
         b = fc_div(row, p.by_walks);
         walk = (int)(row - b * p.walks);
         t0 = walk * p.walk;
@@ -52,6 +55,37 @@ struct conv_place {
         len = none ? 0 : p.length(b);
     }
 };
+
+// The rows of a sequence's channels, from the state before the first on.  A row that is not there reads one that is, without a branch, which would
+// keep all loads before it waiting.
+template <int DT, int VEC>
+struct conv_rows {
+    typedef typename fc_elem<DT>::type E;
+    const E *x, *before;
+    long token;
+    int C, taps;
+    long len;
+    bool state;
+    __device__ __forceinline__ bool there(long t) const { return t < len && (t >= 0 || (state && t >= 1 - taps)); }
+    __device__ __forceinline__ fc_vec<DT, VEC> read(long t) const {
+        const bool early = state && t < 0;
+        const long row = early ? (t >= 1 - taps ? t + taps - 1 : 0) : t < 0 || len < 1 ? 0 : t < len ? t : len - 1;
+        fc_vec<DT, VEC> v;
+        __builtin_memcpy(&v, early ? before + row * C : x + row * token, sizeof v);
+        return v;
+    }
+};
+
+template <class V, class E>
+__device__ __forceinline__ void store(E *to, const V &v, int skip) {
+    if (!skip) {
+        __builtin_memcpy(to, &v, sizeof v);
+        return;
+    }
+#pragma unroll
+    for (int i = 1; i < (int)(sizeof(V) / sizeof(E)); i++)
+        if (i >= skip) to[i] = v.v[i];
+}
 
 // Weights by distance: back[m] belongs to the row m tokens back, so that the loops are the same for every number of taps up to TAPS (2, 3, 4 or 8); those that
 // a convolution lacks are left out, not multiplied by zero.
@@ -73,15 +107,14 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
     }
     V rows[TAPS - 1 + kAhead];
     const V zeros = {};
-    auto read = [&](long t) __attribute__((always_inline)) {      // t: of a row within the window of a token of the walk
-        if (t >= 0) return t < at.len ? *(const V *)(x + t * p.x_token) : zeros;
-        return p.state_in && t >= 1 - taps ? *(const V *)(before + (t + taps - 1) * p.C) : zeros;
-    };
+    const conv_rows<DT, VEC> in = {x, before, p.x_token, p.C, taps, at.len, p.state_in != nullptr};
 #pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = read(at.t0 - (TAPS - 1) + i);
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.read(at.t0 - (TAPS - 1) + i);
+#pragma unroll
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.there(at.t0 - (TAPS - 1) + i) ? rows[i] : zeros;
     for (long t = at.t0; t < at.t1; t += kAhead) {
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) rows[TAPS - 1 + u] = t + u < at.t1 ? read(t + u) : zeros;
+        for (int u = 0; u < kAhead; u++) rows[TAPS - 1 + u] = in.read(t + u);      // tokens past the end have no result that reads them
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
             if (t + u >= at.t1) break;
@@ -96,7 +129,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
                     out.set(v, p.act == FC_ACT_SILU ? fc_silu(z) : z);
                 }
             }
-            *(V *)(y + (t + u) * p.y_token) = out;
+            store(y + (t + u) * p.y_token, out, at.skip);
         }
 #pragma unroll
         for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAhead + i];
@@ -105,8 +138,8 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
     if (at.walk == 0 && p.state_out) {
         E *after = (E *)p.state_out + at.b * (taps - 1) * p.C + at.c;
         for (int i = 0; i < taps - 1; i++) {
-            const V last = read(at.len - (taps - 1) + i);
-            *(V *)(after + (long)i * p.C) = last;
+            const long t = at.len - (taps - 1) + i;
+            store(after + (long)i * p.C, in.there(t) ? in.read(t) : zeros, at.skip);
         }
     }
 }
@@ -134,19 +167,18 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
     }
     V rows[TAPS - 1 + kAheadBackward], grads[kAheadBackward];
     const V zeros = {};
-    auto read = [&](long t) __attribute__((always_inline)) {
-        if (t >= 0) return t < at.len ? *(const V *)(x + t * p.x_token) : zeros;
-        return p.state_in && t >= 1 - taps ? *(const V *)(before + (t + taps - 1) * p.C) : zeros;
-    };
+    const conv_rows<DT, VEC> in = {x, before, p.x_token, p.C, taps, at.len, p.state_in != nullptr}, up = {dy, dy, p.y_token, p.C, 1, at.len, false};
 #pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = read(at.t0 - (TAPS - 1) + i);
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.read(at.t0 - (TAPS - 1) + i);
+#pragma unroll
+    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.there(at.t0 - (TAPS - 1) + i) ? rows[i] : zeros;
     // the gradient of row t - TAPS + 1 is whole once dz_t is there: TAPS - 1 tokens past the walk's own
     const long end = at.t1 + TAPS - 1;
     for (long t = at.t0; t < end; t += kAheadBackward) {
 #pragma unroll
         for (int u = 0; u < kAheadBackward; u++) {
-            rows[TAPS - 1 + u] = t + u < end ? read(t + u) : zeros;
-            grads[u] = t + u < end && t + u < at.len ? *(const V *)(dy + (t + u) * p.y_token) : zeros;
+            rows[TAPS - 1 + u] = in.read(t + u);
+            grads[u] = up.read(t + u);
         }
 #pragma unroll
         for (int u = 0; u < kAheadBackward; u++) {
@@ -156,13 +188,13 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
             const long last = row - (at.len - (taps - 1));      // row of the state after the last token
             V more = zeros, out;
             const bool wanted = row >= at.t0 || (at.walk == 0 && row >= 1 - taps && p.dstate_in);
-            if (wanted && p.dstate_out && last >= 0 && last < taps - 1) more = *(const V *)(dlast + last * p.C);
+            if (wanted && p.dstate_out && last >= 0 && last < taps - 1) __builtin_memcpy(&more, dlast + last * p.C, sizeof more);
 #pragma unroll
             for (int v = 0; v < VEC; v++) {
 #pragma unroll
                 for (int j = 0; j < TAPS - 1; j++) dz[v][j] = dz[v][j + 1];
                 float g = 0.f;
-                if (there) {
+                if (there) {      // rows past the end are not zeros
                     g = grads[u].get(v);
                     if (p.act == FC_ACT_SILU) {
                         float z = bias[v];
@@ -185,8 +217,8 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
                     if (m < taps) s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz_(row + m)
                 out.set(v, row < at.len ? s : 0.f);
             }
-            if (row >= at.t0) *(V *)(dx + row * p.x_token) = out;
-            else if (row < 0 && wanted) *(V *)(dfirst + (row + taps - 1) * p.C) = out;
+            if (row >= at.t0) store(dx + row * p.x_token, out, at.skip);
+            else if (row < 0 && wanted) store(dfirst + (row + taps - 1) * p.C, out, at.skip);
         }
 #pragma unroll
         for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAheadBackward + i];
@@ -195,6 +227,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
     float *part = p.part + (at.b * p.walks + at.walk) * (taps + 1) * p.C + at.c;
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
+        if (v < at.skip) continue;
 #pragma unroll
         for (int m = 0; m < TAPS; m++)
             if (m < taps) part[(long)(taps - 1 - m) * p.C + v] = dback[v][m];
@@ -202,18 +235,11 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
     }
 }
 
-// dw and dbias from the walks' sums, always in the same order: 64 of [taps + 1][C] a workgroup, four wavefronts that share the walks.
-__global__ __launch_bounds__(256) void fc_causal_conv_sum_kernel(const float *part, float *dw, float *dbias, int parts, int C, int taps) {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long size = (long)(taps + 1) * C, i = (long)blockIdx.x * 64 + lane;
-    float s = 0.f;
-    if (i < size)
-        for (int n = wave; n < parts; n += 4) s += part[n * size + i];
-    sums[wave][lane] = s;
-    __syncthreads();
-    if (wave || i >= size) return;
-    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+// dw and dbias from the walks' sums, [taps + 1][C] each.
+__global__ __launch_bounds__(kPartThreads) void fc_causal_conv_sum_kernel(const float *part, float *dw, float *dbias, int parts, int C, int taps) {
+    long i;
+    float s;
+    if (!fc_sum_parts(part, parts, (long)(taps + 1) * C, i, s)) return;
     const int j = (int)(i / C), c = (int)(i - (long)j * C);
     if (j == taps) {
         if (dbias) dbias[c] = s;
@@ -237,15 +263,12 @@ int check_plan(fc_context *ctx, const fc_causal_conv_plan *plan, const char *wha
     return FC_OK;
 }
 
-// Values of an access.
-int width_of(const fc_causal_conv_shape &s, uint64_t addr) {
-    const int w = fc_widest(s.dtype, (uint64_t)(s.C | s.x_batch | s.x_token | s.y_batch | s.y_token), addr), most = s.dtype == FC_F32 ? 4 : 8;
-    return w == most ? w : s.dtype != FC_F32 && w >= 2 ? 2 : 1;
-}
+int channels_of(const fc_causal_conv_shape &s) { return s.C < kChannels ? 1 : kChannels; }
+int columns_of(const fc_causal_conv_shape &s) { return (s.C + channels_of(s) - 1) / channels_of(s); }
 
-long walks_of(const fc_causal_conv_shape *s, int vec, int least) {
-    const long columns = s->C / vec, most = (s->T + least - 1) / least;
-    long walks = (kFill + columns * s->B - 1) / (columns * s->B);
+long walks_of(const fc_causal_conv_shape *s, int least) {
+    const long rows = (long)columns_of(*s) * s->B, most = (s->T + least - 1) / least;
+    long walks = (kFill + rows - 1) / rows;
     if (walks > most) walks = most;
     const long walk = (s->T + walks - 1) / walks;
     return (s->T + walk - 1) / walk;
@@ -263,18 +286,19 @@ void with_taps(int taps, F launch) {
 }
 
 template <class F>
-void with_kernel(int dtype, int vec, int taps, F launch) {
-    if (dtype == FC_F32) return vec == 4 ? with_taps<FC_F32, 4>(taps, launch) : with_taps<FC_F32, 1>(taps, launch);
-    if (dtype == FC_BF16) return vec == 8 ? with_taps<FC_BF16, 8>(taps, launch) : vec == 2 ? with_taps<FC_BF16, 2>(taps, launch) : with_taps<FC_BF16, 1>(taps, launch);
-    return vec == 8 ? with_taps<FC_F16, 8>(taps, launch) : vec == 2 ? with_taps<FC_F16, 2>(taps, launch) : with_taps<FC_F16, 1>(taps, launch);
+void with_kernel(const fc_causal_conv_shape &s, F launch) {
+    const bool one = channels_of(s) == 1;
+    if (s.dtype == FC_F32) return one ? with_taps<FC_F32, 1>(s.taps, launch) : with_taps<FC_F32, kChannels>(s.taps, launch);
+    if (s.dtype == FC_BF16) return one ? with_taps<FC_BF16, 1>(s.taps, launch) : with_taps<FC_BF16, kChannels>(s.taps, launch);
+    return one ? with_taps<FC_F16, 1>(s.taps, launch) : with_taps<FC_F16, kChannels>(s.taps, launch);
 }
 
-conv_params params_of(const fc_causal_conv_shape &s, int walks, int columns) {
+conv_params params_of(const fc_causal_conv_shape &s, int walks) {
     conv_params p = {};
     p.B = s.B; p.T = s.T; p.C = s.C; p.taps = s.taps; p.act = s.act;
     p.walks = walks;
     p.walk = (s.T + walks - 1) / walks;
-    p.by_columns = fc_make_fastdiv((uint32_t)columns);
+    p.by_columns = fc_make_fastdiv((uint32_t)columns_of(s));
     p.by_walks = fc_make_fastdiv((uint32_t)walks);
     p.x_batch = s.x_batch; p.x_token = s.x_token; p.y_batch = s.y_batch; p.y_token = s.y_token;
     return p;
@@ -286,15 +310,11 @@ extern "C" int fc_causal_conv_make_plan(const fc_causal_conv_shape *s, fc_causal
     if (!plan || !s || s->B < 1 || s->T < 1 || s->C < 1 || s->taps < 2 || !fc_dtype_ok(s->dtype)) return FC_ERR_INVALID;
     if (s->act != FC_ACT_NONE && s->act != FC_ACT_SILU) return s->act < FC_ACT_NONE || s->act > FC_ACT_GELU ? FC_ERR_INVALID : FC_ERR_UNSUPPORTED;
     if (s->x_batch < 0 || s->x_token < 0 || s->y_batch < 0 || s->y_token < 0) return FC_ERR_INVALID;
-    // a thread a value, should nothing be aligned, with room for the last workgroup's
     if (s->taps > kMostTaps || s->T >= (1l << 31) || fc_count(s->B, s->C) < 0 || fc_count(s->B, s->C) >= (1l << 30)) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    const int vec = width_of(*s, 0);
-    plan->walks = (int)walks_of(s, vec, kAhead);
-    plan->walks_backward = (int)walks_of(s, vec, 4 * s->taps);
-    const long rows = (long)s->B * (plan->walks > plan->walks_backward ? plan->walks : plan->walks_backward);
-    if (fc_count(rows, s->C) < 0 || fc_count(rows, s->C) >= (1l << 31) - kThreads) return FC_ERR_UNSUPPORTED;
+    plan->walks = (int)walks_of(s, kAhead);
+    plan->walks_backward = (int)walks_of(s, 4 * s->taps);
     plan->ws_backward_bytes = (size_t)s->B * plan->walks_backward * (s->taps + 1) * s->C * sizeof(float);
     return FC_OK;
 }
@@ -309,12 +329,12 @@ extern "C" int fc_causal_conv(fc_context *ctx, const fc_causal_conv_plan *plan, 
     if ((addr & (fc_elem_size(s.dtype) - 1)) || (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)lengths_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: unaligned pointer");
     if (!fc_apart(s.B, s.y_batch, s.C) || !fc_apart(s.T, s.y_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: tokens of y overlap");
-    const int vec = width_of(s, addr), columns = s.C / vec;
-    conv_params p = params_of(s, plan->walks, columns);
+    const int columns = columns_of(s);
+    conv_params p = params_of(s, plan->walks);
     p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = y_dev; p.state_in = state_in_dev; p.state_out = state_out_dev; p.lengths = lengths_dev;
     const unsigned blocks = (unsigned)(((long)s.B * p.walks * columns + kThreads - 1) / kThreads);
     const fc_device_scope on(ctx);
-    with_kernel(s.dtype, vec, s.taps, [&](auto dt, auto v, auto taps) {
+    with_kernel(s, [&](auto dt, auto v, auto taps) {
         fc_causal_conv_kernel<decltype(dt)::value, decltype(v)::value, decltype(taps)::value><<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(p, columns);
     });
     FC_LAUNCH_CHECK(ctx, "fc_causal_conv_kernel");
@@ -334,21 +354,22 @@ extern "C" int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_pla
         (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)dw_dev | (uint64_t)dbias_dev | (uint64_t)lengths_dev | (uint64_t)ws_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: unaligned pointer");
     if (!fc_apart(s.B, s.x_batch, s.C) || !fc_apart(s.T, s.x_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: tokens of dx overlap");
-    const int vec = width_of(s, addr), columns = s.C / vec;
-    conv_params p = params_of(s, plan->walks_backward, columns);
+    const int columns = columns_of(s);
+    conv_params p = params_of(s, plan->walks_backward);
     p.dy = dy_dev; p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = dx_dev; p.state_in = state_in_dev; p.dstate_out = dstate_out_dev;
     p.dstate_in = dstate_in_dev; p.lengths = lengths_dev;
     p.part = sums ? (float *)ws_dev : nullptr;
     const unsigned blocks = (unsigned)(((long)s.B * p.walks * columns + kThreads - 1) / kThreads);
     const fc_device_scope on(ctx);
-    with_kernel(s.dtype, vec, s.taps, [&](auto dt, auto v, auto taps) {
+    with_kernel(s, [&](auto dt, auto v, auto taps) {
         fc_causal_conv_gradient_kernel<decltype(dt)::value, decltype(v)::value, decltype(taps)::value>
             <<<dim3(blocks), dim3(kThreads), 0, ctx->stream>>>(p, columns);
     });
     FC_LAUNCH_CHECK(ctx, "fc_causal_conv_gradient_kernel");
     if (!sums) return FC_OK;
     const long size = (long)(s.taps + 1) * s.C;
-    fc_causal_conv_sum_kernel<<<dim3((unsigned)((size + 63) / 64)), dim3(256), 0, ctx->stream>>>(p.part, dw_dev, dbias_dev, s.B * p.walks, s.C, s.taps);
+    fc_causal_conv_sum_kernel<<<dim3((unsigned)((size + kPartValues - 1) / kPartValues)), dim3(kPartThreads), 0, ctx->stream>>>(p.part, dw_dev, dbias_dev,
+                                                                                                                                s.B * p.walks, s.C, s.taps);
     FC_LAUNCH_CHECK(ctx, "fc_causal_conv_sum_kernel");
     return FC_OK;
 }

@@ -64,70 +64,137 @@ struct row_scale {
     __device__ __forceinline__ float whole() const { return rstd * unit; }
 };
 
-// WAVES wavefronts a row; R accesses of VEC values a thread, or any number, read twice, if R is 0.
-template <int DT, int VEC, int WAVES, int R, int TO>
-__global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kernel(const rms_params p) {
+// Values of a 16-byte access.
+template <int DT>
+constexpr int kVec = DT == FC_F32 ? 4 : 8;
+
+// A thread's share of a row: R accesses of 16 bytes in registers (any number, read again for each use, if R is 0), and one value of those that fill no
+// access.  Accesses past the row's last read that one again and count as zeros: a load behind a branch would keep the others waiting.
+template <int DT, int WAVES, int R>
+struct row_share {
+    static constexpr int VEC = kVec<DT>, PER = 64 * WAVES, KEEP = R ? R : 1;
     typedef fc_vec<DT, VEC> V;
     typedef typename fc_elem<DT>::type E;
-    struct alignas(VEC) bytes {
-        int8_t v[VEC];
-    };
-    constexpr int PER = 64 * WAVES, ROWS = WAVES > 1 ? 1 : 4, KEEP = R ? R : 1;
-    __shared__ float2 slots[2][16];
-    const int me = WAVES > 1 ? threadIdx.x : threadIdx.x & 63, accesses = p.C / VEC;
-    const int loops = R ? R : (accesses + PER - 1) / PER;
-    float g[KEEP][VEC];
-    auto read_gamma = [&](int k, float (&to)[VEC]) __attribute__((always_inline)) {
-        const int a = me + k * PER;
+    int me, full, tail;      // full: accesses of the row; tail: values that are left
+    __device__ __forceinline__ explicit row_share(int C)
+        : me(WAVES > 1 ? threadIdx.x : threadIdx.x & 63), full(C / VEC), tail(C - C / VEC * VEC) {}
+    __device__ __forceinline__ bool has(int k) const { return me + k * PER < full; }
+    __device__ __forceinline__ int at(int k) const { return (has(k) ? me + k * PER : full - 1) * VEC; }
+    __device__ __forceinline__ int last() const { return full * VEC + (me < tail ? me : 0); }      // the single value's place
+    __device__ __forceinline__ void read(V (&to)[KEEP], fc_vec<DT, 1> &one, const E *row) const {
+        if (full) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) to[v] = p.gamma && a < accesses ? p.gamma[a * VEC + v] : 1.f;
-    };
-    if constexpr (R > 0 && TO != ONLY_INT8) {
-#pragma unroll
-        for (int k = 0; k < R; k++) read_gamma(k, g[k]);
+            for (int k = 0; k < R; k++) __builtin_memcpy(&to[k], row + at(k), sizeof(V));
+        }
+        if (tail) one.v[0] = row[last()];
     }
+    __device__ __forceinline__ void clear(V (&of)[KEEP], fc_vec<DT, 1> &one) const {
+        const V zeros = {};
+#pragma unroll
+        for (int k = 0; k < R; k++)
+            if (!has(k)) of[k] = zeros;
+        if (me >= tail) one.v[0] = (E)0.f;
+    }
+    __device__ __forceinline__ void read_gamma(float (&g)[KEEP][VEC], float &one, const float *gamma) const {
+#pragma unroll
+        for (int k = 0; k < KEEP; k++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) g[k][v] = 1.f;
+        one = 1.f;
+        if (!gamma) return;
+        if (full) {
+#pragma unroll
+            for (int k = 0; k < R; k++) __builtin_memcpy(g[k], gamma + at(k), sizeof g[k]);
+        }
+        if (tail) one = gamma[last()];
+    }
+};
+
+// WAVES wavefronts a row.
+template <int DT, int WAVES, int R, int TO>
+__global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kernel(const rms_params p) {
+    typedef row_share<DT, WAVES, R> share;
+    typedef typename share::V V;
+    typedef typename share::E E;
+    typedef fc_vec<DT, 1> one;
+    constexpr int VEC = share::VEC, PER = share::PER, ROWS = WAVES > 1 ? 1 : 4, KEEP = share::KEEP;
+    __shared__ float2 slots[2][16];
+    const share of(p.C);
+    float g[KEEP][VEC], g1 = 1.f;
+    if constexpr (TO != ONLY_INT8) of.read_gamma(g, g1, p.gamma);
     int turn = 0;
     for (long row = (long)blockIdx.x * ROWS + (WAVES > 1 ? 0 : threadIdx.x >> 6); row < p.rows; row += (long)gridDim.x * ROWS) {
         const E *x = (const E *)p.x + row * p.x_row, *res = (const E *)p.residual + row * p.residual_row;
         E *sum = (E *)p.sum + row * p.sum_row;
         V h[KEEP];
-        // x + residual; again: where it is stored, from there
-        auto read = [&](int k, V &to, bool again) __attribute__((always_inline)) {
-            const int a = me + k * PER;
-            if (a >= accesses) return;
-            if (again && p.sum) {
-                to = *(const V *)(sum + a * VEC);
-                return;
-            }
-            to = *(const V *)(x + a * VEC);
-            if (p.residual) {
-                const V r = *(const V *)(res + a * VEC);
+        one h1;
+        h1.v[0] = (E)0.f;
+        auto add = [](auto &a, const auto &b, int n) __attribute__((always_inline)) {
 #pragma unroll
-                for (int v = 0; v < VEC; v++) to.set(v, to.get(v) + r.get(v));
+            for (int v = 0; v < n; v++) a.set(v, a.get(v) + b.get(v));
+        };
+        if constexpr (R > 0) {
+            of.read(h, h1, x);
+            if (p.residual) {
+                V r[KEEP];
+                one r1 = h1;
+                of.read(r, r1, res);
+#pragma unroll
+                for (int k = 0; k < R; k++) add(h[k], r[k], VEC);
+                add(h1, r1, 1);
             }
-            if (p.sum && !again) *(V *)(sum + a * VEC) = to;
+            of.clear(h, h1);
+            if (p.sum) {
+#pragma unroll
+                for (int k = 0; k < R; k++)
+                    if (of.has(k)) __builtin_memcpy(sum + of.at(k), &h[k], sizeof(V));
+                if (of.me < of.tail) sum[of.last()] = h1.v[0];
+            }
+        }
+        // f(values of h, of gamma, how many, where): what the thread has of the row.  Where it is not kept it is read, and the sum written the first time.
+        auto visit = [&](bool again, auto f) __attribute__((always_inline)) {
+            if constexpr (R > 0) {
+#pragma unroll
+                for (int k = 0; k < R; k++) f(h[k], g[k], std::integral_constant<int, VEC>(), of.at(k), of.has(k));
+                f(h1, &g1, std::integral_constant<int, 1>(), of.last(), of.me < of.tail);
+            } else {
+                auto part = [&](auto &t, auto &r, const float *gamma, auto n, int at) __attribute__((always_inline)) {
+                    const bool stored = again && p.sum;
+                    __builtin_memcpy(&t, (stored ? sum : x) + at, sizeof t);
+                    if (p.residual && !stored) {
+                        __builtin_memcpy(&r, res + at, sizeof r);
+                        add(t, r, n);
+                    }
+                    if (p.sum && !again) __builtin_memcpy(sum + at, &t, sizeof t);
+                    f(t, gamma, n, at, true);
+                };
+                for (int a = of.me; a < of.full; a += PER) {
+                    V t, r;
+                    if (TO != ONLY_INT8 && p.gamma) __builtin_memcpy(g[0], p.gamma + a * VEC, sizeof g[0]);
+                    part(t, r, g[0], std::integral_constant<int, VEC>(), a * VEC);
+                }
+                if (of.me < of.tail) {
+                    one t, r;
+                    part(t, r, &g1, std::integral_constant<int, 1>(), of.last());
+                }
+            }
         };
         // the sum of squares and the largest |h gamma|, of h times unit
         auto measure = [&](bool again, float unit) __attribute__((always_inline)) {
             float2 m = make_float2(0.f, 0.f);
             bool bad = false;
+            visit(again, [&](const auto &t, const float *gamma, auto n, int, bool) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < loops; k++) {
-                V &t = h[R ? k : 0];
-                if (!R || !again) read(k, t, again);
-                if constexpr (R == 0 && TO == TO_INT8) read_gamma(k, g[0]);
-                if (me + k * PER >= accesses) continue;
-#pragma unroll
-                for (int v = 0; v < VEC; v++) {
+                for (int v = 0; v < n; v++) {
                     const float s = t.get(v) * unit;
                     if (TO != ONLY_INT8) m.x = __builtin_fmaf(s, s, m.x);
                     if (TO != TO_TYPE) {
-                        const float w = TO == ONLY_INT8 ? s : s * g[R ? k : 0][v];
+                        const float w = TO == ONLY_INT8 ? s : s * gamma[v];
                         m.y = fmaxf(m.y, __builtin_fabsf(w));
                         bad |= !(__builtin_fabsf(w) < __builtin_inff());
                     }
                 }
-            }
+            });
             if (TO != TO_TYPE && bad) m.y = __builtin_inff();      // also where it is NaN, which fmaxf drops
             return join<WAVES>(m, slots, turn++);
         };
@@ -138,14 +205,10 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kern
             // Squares that overflow, or vanish beside no eps to speak of: again, of values near 1.
             if (!(m.x < 1e36f) || !(m.y < 1e36f) || (m.x < 1e-20f && eps < 1e-20f)) {
                 float2 top = make_float2(0.f, 0.f);
+                visit(true, [&](const auto &t, const float *, auto n, int, bool) __attribute__((always_inline)) {
 #pragma unroll
-                for (int k = 0; k < loops; k++) {
-                    V &t = h[R ? k : 0];
-                    if (!R) read(k, t, true);
-                    if (me + k * PER >= accesses) continue;
-#pragma unroll
-                    for (int v = 0; v < VEC; v++) top.y = fmaxf(top.y, __builtin_fabsf(t.get(v)));
-                }
+                    for (int v = 0; v < n; v++) top.y = fmaxf(top.y, __builtin_fabsf(t.get(v)));
+                });
                 top = join<WAVES>(top, slots, turn++);
                 if (top.y > 0.f && top.y < __builtin_inff()) {
                     int e = ilogbf(top.y);
@@ -157,7 +220,7 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kern
                 }
             }
             s.rstd = 1.f / sqrtf(m.x / (float)p.C + eps);
-            if (p.rstd && me == 0) p.rstd[row] = s.whole();
+            if (p.rstd && of.me == 0) p.rstd[row] = s.whole();
         }
         float inv = 0.f;
         if constexpr (TO != TO_TYPE) {
@@ -165,144 +228,154 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kern
             const float top = m.y * s.rstd;
             const bool number = top < __builtin_inff();
             if (top >= kLeastTop && number) inv = 127.f / m.y;
-            if (me == 0) p.scale[row] = !number ? __builtin_nanf("") : top >= kLeastTop ? top / 127.f : 0.f;
+            if (of.me == 0) p.scale[row] = !number ? __builtin_nanf("") : top >= kLeastTop ? top / 127.f : 0.f;
         }
-#pragma unroll
-        for (int k = 0; k < loops; k++) {
-            V &t = h[R ? k : 0];
-            if (!R) read(k, t, true);
-            if constexpr (R == 0 && TO != ONLY_INT8) read_gamma(k, g[0]);
-            const int a = me + k * PER;
-            if (a >= accesses) continue;
+        visit(true, [&](const auto &t, const float *gamma, auto n, int at, bool there) __attribute__((always_inline)) {
             if constexpr (TO == TO_TYPE) {
+                auto y = t;
 #pragma unroll
-                for (int v = 0; v < VEC; v++) t.set(v, t.get(v) * s.unit * s.rstd * g[R ? k : 0][v]);
-                *(V *)((E *)p.y + row * p.y_row + a * VEC) = t;
+                for (int v = 0; v < n; v++) y.set(v, t.get(v) * s.unit * s.rstd * gamma[v]);
+                if (there) __builtin_memcpy((E *)p.y + row * p.y_row + at, &y, sizeof y);
             } else {
-                bytes q;
+                int8_t q[n];
 #pragma unroll
-                for (int v = 0; v < VEC; v++) {
-                    const float w = TO == ONLY_INT8 ? t.get(v) : t.get(v) * s.unit * g[R ? k : 0][v];
-                    q.v[v] = inv > 0.f ? (int8_t)(int)rintf(w * inv) : (int8_t)0;
+                for (int v = 0; v < n; v++) {
+                    const float w = TO == ONLY_INT8 ? t.get(v) : t.get(v) * s.unit * gamma[v];
+                    q[v] = inv > 0.f ? (int8_t)(int)rintf(w * inv) : (int8_t)0;
                 }
-                *(bytes *)((int8_t *)p.y + row * p.y_row + a * VEC) = q;
+                if (there) __builtin_memcpy((int8_t *)p.y + row * p.y_row + at, q, n);
             }
-        }
+        });
     }
 }
 
-// dx, and what each workgroup's rows add to dgamma: part[workgroup][C] (WAVES == 1: [wavefront][C]).
-template <int DT, int VEC, int WAVES, int R>
+// dx, and what each workgroup's rows add to dgamma: part[workgroup][C].
+template <int DT, int WAVES, int R>
 __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_gradient_kernel(const rms_params p) {
-    typedef fc_vec<DT, VEC> V;
-    typedef typename fc_elem<DT>::type E;
-    constexpr int PER = 64 * WAVES, ROWS = WAVES > 1 ? 1 : 4, KEEP = R ? R : 1;
+    typedef row_share<DT, WAVES, R> share;
+    typedef typename share::V V;
+    typedef typename share::E E;
+    typedef fc_vec<DT, 1> one;
+    constexpr int VEC = share::VEC, PER = share::PER, ROWS = WAVES > 1 ? 1 : 4, KEEP = share::KEEP;
     __shared__ float2 slots[2][16];
-    const int me = WAVES > 1 ? threadIdx.x : threadIdx.x & 63, accesses = p.C / VEC;
-    const int loops = R ? R : (accesses + PER - 1) / PER;
-    const long first = (long)blockIdx.x * ROWS + (WAVES > 1 ? 0 : threadIdx.x >> 6);
-    float *part = p.part ? p.part + first * p.C : nullptr;
-    float g[KEEP][VEC], dg[KEEP][VEC];
-    auto read_gamma = [&](int k, float (&to)[VEC]) __attribute__((always_inline)) {
-        const int a = me + k * PER;
+    const share of(p.C);
+    const int wave = threadIdx.x >> 6;
+    const long first = (long)blockIdx.x * ROWS + (WAVES > 1 ? 0 : wave);
+    float *part = p.part ? p.part + (long)blockIdx.x * p.C : nullptr;
+    float g[KEEP][VEC], dg[KEEP][VEC], g1 = 1.f, dg1 = 0.f;
+    of.read_gamma(g, g1, p.gamma);
 #pragma unroll
-        for (int v = 0; v < VEC; v++) to[v] = p.gamma && a < accesses ? p.gamma[a * VEC + v] : 1.f;
-    };
-#pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-        if constexpr (R > 0) read_gamma(k, g[k]);
+    for (int k = 0; k < KEEP; k++)
 #pragma unroll
         for (int v = 0; v < VEC; v++) dg[k][v] = 0.f;
-    }
     int turn = 0;
     for (long row = first; row < p.rows; row += (long)gridDim.x * ROWS) {
-        const E *hr = (const E *)p.h + row * p.sum_row, *dr = (const E *)p.dy + row * p.dy_row;
+        const E *hr = (const E *)p.h + row * p.sum_row, *dr = (const E *)p.dy + row * p.dy_row, *more = (const E *)p.dsum + row * p.sum_row;
+        E *dx = (E *)p.y + row * p.x_row;
         const float rstd = p.rstd[row];
-        V h[KEEP], d[KEEP];
-        float2 along = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < loops; k++) {
-            const int a = me + k * PER, i = R ? k : 0;
-            if (a >= accesses) continue;
-            h[i] = *(const V *)(hr + a * VEC);
-            d[i] = *(const V *)(dr + a * VEC);
-            if constexpr (R == 0) read_gamma(k, g[0]);
-#pragma unroll
-            for (int v = 0; v < VEC; v++) along.x = __builtin_fmaf(g[i][v] * d[i].get(v), h[i].get(v) * rstd, along.x);
+        V h[KEEP], d[KEEP], m[KEEP];
+        one h1, d1, m1;
+        h1.v[0] = d1.v[0] = m1.v[0] = (E)0.f;
+        if constexpr (R > 0) {
+            of.read(h, h1, hr);
+            of.read(d, d1, dr);
+            if (p.dsum) of.read(m, m1, more);
+            of.clear(h, h1);
+            of.clear(d, d1);
         }
+        // f(h, dy, dsum, gamma, its gradient, how many, where): what the thread has of the row
+        auto visit = [&](auto f) __attribute__((always_inline)) {
+            if constexpr (R > 0) {
+#pragma unroll
+                for (int k = 0; k < R; k++) f(h[k], d[k], m[k], g[k], dg[k], std::integral_constant<int, VEC>(), of.at(k), of.has(k));
+                f(h1, d1, m1, &g1, &dg1, std::integral_constant<int, 1>(), of.last(), of.me < of.tail);
+            } else {
+                auto some = [&](auto &a, auto &b, auto &c, float *gamma, auto n, int at) __attribute__((always_inline)) {
+                    __builtin_memcpy(&a, hr + at, sizeof a);
+                    __builtin_memcpy(&b, dr + at, sizeof b);
+                    if (p.dsum) __builtin_memcpy(&c, more + at, sizeof c);
+                    if (p.gamma) __builtin_memcpy(gamma, p.gamma + at, n * sizeof(float));
+                    f(a, b, c, gamma, part ? part + at : nullptr, n, at, true);
+                };
+                for (int a = of.me; a < of.full; a += PER) some(h[0], d[0], m[0], g[0], std::integral_constant<int, VEC>(), a * VEC);
+                if (of.me < of.tail) some(h1, d1, m1, &g1, std::integral_constant<int, 1>(), of.last());
+            }
+        };
+        float2 along = make_float2(0.f, 0.f);
+        visit([&](const auto &a, const auto &b, const auto &, const float *gamma, float *, auto n, int, bool) __attribute__((always_inline)) {
+#pragma unroll
+            for (int v = 0; v < n; v++) along.x = __builtin_fmaf(gamma[v] * b.get(v), a.get(v) * rstd, along.x);
+        });
         along = join<WAVES>(along, slots, turn++);
         const float mean = along.x / (float)p.C;
+        visit([&](const auto &a, const auto &b, const auto &c, const float *gamma, float *dgamma, auto n, int at, bool there) __attribute__((always_inline)) {
+            auto out = a;
 #pragma unroll
-        for (int k = 0; k < loops; k++) {
-            const int a = me + k * PER, i = R ? k : 0;
-            if (a >= accesses) continue;
-            if constexpr (R == 0) {
-                h[0] = *(const V *)(hr + a * VEC);
-                d[0] = *(const V *)(dr + a * VEC);
-                read_gamma(k, g[0]);
+            for (int v = 0; v < n; v++) {
+                const float xhat = a.get(v) * rstd, dy = b.get(v);
+                if constexpr (R > 0) dgamma[v] = __builtin_fmaf(dy, xhat, dgamma[v]);
+                else if (dgamma) dgamma[v] = row == first ? dy * xhat : __builtin_fmaf(dy, xhat, dgamma[v]);      // a thread's own place, from row to row
+                const float dh = rstd * __builtin_fmaf(-xhat, mean, gamma[v] * dy);
+                out.set(v, p.dsum ? dh + c.get(v) : dh);
             }
-            V more;
-            if (p.dsum) more = *(const V *)((const E *)p.dsum + row * p.sum_row + a * VEC);
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                const float xhat = h[i].get(v) * rstd, dy = d[i].get(v);
-                if constexpr (R > 0) dg[i][v] = __builtin_fmaf(dy, xhat, dg[i][v]);
-                else if (part) {      // a thread's own place, from row to row
-                    float *to = part + a * VEC + v;
-                    *to = row == first ? dy * xhat : __builtin_fmaf(dy, xhat, *to);
-                }
-                const float dh = rstd * __builtin_fmaf(-xhat, mean, g[i][v] * dy);
-                h[i].set(v, p.dsum ? dh + more.get(v) : dh);
-            }
-            *(V *)((E *)p.y + row * p.x_row + a * VEC) = h[i];
-        }
+            if (there) __builtin_memcpy(dx + at, &out, sizeof out);
+        });
     }
     if constexpr (R > 0) {
         if (!part) return;
+        constexpr int WIDTH = 64 * (R * VEC + 1);
+        __shared__ float others[WAVES > 1 ? 1 : 3][WAVES > 1 ? 1 : WIDTH];      // four rows at once: their wavefronts' sums
+        if constexpr (WAVES == 1) {
+            if (wave) {
 #pragma unroll
-        for (int k = 0; k < R; k++) {
-            const int a = me + k * PER;
-            if (a >= accesses) continue;
+                for (int k = 0; k < R; k++)
 #pragma unroll
-            for (int v = 0; v < VEC; v++) part[a * VEC + v] = dg[k][v];
+                    for (int v = 0; v < VEC; v++) others[wave - 1][(k * VEC + v) * 64 + of.me] = dg[k][v];
+                others[wave - 1][R * VEC * 64 + of.me] = dg1;
+            }
+            __syncthreads();
+            if (wave) return;
+#pragma unroll
+            for (int k = 0; k < R; k++)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) {
+                    const int i = (k * VEC + v) * 64 + of.me;
+                    dg[k][v] = (dg[k][v] + others[0][i]) + (others[1][i] + others[2][i]);
+                }
+            const int i = R * VEC * 64 + of.me;
+            dg1 = (dg1 + others[0][i]) + (others[1][i] + others[2][i]);
         }
+#pragma unroll
+        for (int k = 0; k < R; k++)
+            if (of.has(k)) __builtin_memcpy(part + of.at(k), dg[k], sizeof dg[k]);
+        if (of.me < of.tail) part[of.last()] = dg1;
     }
 }
 
-// dgamma from its parts, always in the same order: 64 channels a workgroup, four wavefronts that share the parts.
-__global__ __launch_bounds__(256) void fc_rms_norm_dgamma_kernel(const float *part, float *dgamma, int parts, int C) {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    float s = 0.f;
-    if (c < C) {
-        for (int i = wave; i < parts; i += 4) s += part[(long)i * C + c];
-    }
-    sums[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && c < C) dgamma[c] = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+__global__ __launch_bounds__(kPartThreads) void fc_rms_norm_dgamma_kernel(const float *part, float *dgamma, int parts, int C) {
+    long c;
+    float s;
+    if (fc_sum_parts(part, parts, C, c, s)) dgamma[c] = s;
 }
 
 int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
-
-// Accesses are 16 bytes wide, two 16-bit values, or single values.
-int width_of(int dtype, uint64_t bits, uint64_t addr) {
-    const int w = fc_widest(dtype, bits, addr), most = 16 / (int)fc_elem_size(dtype);
-    return w == most ? w : dtype != FC_F32 && w >= 2 ? 2 : 1;
-}
 
 // Wavefronts of a row: one, four or sixteen, and whether the row stays in their registers.
 struct row_form {
     int waves;
     bool kept;
-    long blocks(long rows) const {
-        const long want = waves > 1 ? rows : (rows + 3) / 4, most = waves > 4 ? 512 : 2048;
+    // workgroups, each of which takes rows until there are none
+    long blocks(long rows, long most) const {
+        const long want = waves > 1 ? rows : (rows + 3) / 4;
+        if (waves > 4) most /= 4;
         return want < most ? want : most;
     }
 };
 
+constexpr long kBlocks = 2048, kBlocksBackward = 768;
 constexpr int kAccesses = 4;      // of a thread
-row_form form_of(long rows, int C, int vec) {
-    const int accesses = C / vec;
+row_form form_of(long rows, int C, int dtype) {
+    const int vec = dtype == FC_F32 ? 4 : 8, accesses = (C + vec - 1) / vec;
     // few rows: as many wavefronts as there are accesses for, a wait for one access each; many: as few as hold the row
     const int least = rows < 1024 ? 1 : kAccesses;
     if (accesses <= 64 * least) return {1, true};
@@ -310,32 +383,31 @@ row_form form_of(long rows, int C, int vec) {
     return {16, accesses <= 1024 * kAccesses};
 }
 
-template <int DT, int VEC, class F>
+template <int DT, class F>
 void with_rows(const row_form &f, F launch) {
     using std::integral_constant;
     typedef integral_constant<int, DT> dt;
-    typedef integral_constant<int, VEC> vec;
-    if (f.waves == 1) launch(dt(), vec(), integral_constant<int, 1>(), integral_constant<int, kAccesses>());
-    else if (f.waves == 4) launch(dt(), vec(), integral_constant<int, 4>(), integral_constant<int, kAccesses>());
-    else if (f.kept) launch(dt(), vec(), integral_constant<int, 16>(), integral_constant<int, kAccesses>());
-    else launch(dt(), vec(), integral_constant<int, 16>(), integral_constant<int, 0>());
+    if (f.waves == 1) launch(dt(), integral_constant<int, 1>(), integral_constant<int, kAccesses>());
+    else if (f.waves == 4) launch(dt(), integral_constant<int, 4>(), integral_constant<int, kAccesses>());
+    else if (f.kept) launch(dt(), integral_constant<int, 16>(), integral_constant<int, kAccesses>());
+    else launch(dt(), integral_constant<int, 16>(), integral_constant<int, 0>());
 }
 
 template <class F>
-void with_kernel(int dtype, int vec, const row_form &f, F launch) {
-    if (dtype == FC_F32) return vec == 4 ? with_rows<FC_F32, 4>(f, launch) : with_rows<FC_F32, 1>(f, launch);
-    if (dtype == FC_BF16) return vec == 8 ? with_rows<FC_BF16, 8>(f, launch) : vec == 2 ? with_rows<FC_BF16, 2>(f, launch) : with_rows<FC_BF16, 1>(f, launch);
-    return vec == 8 ? with_rows<FC_F16, 8>(f, launch) : vec == 2 ? with_rows<FC_F16, 2>(f, launch) : with_rows<FC_F16, 1>(f, launch);
+void with_kernel(int dtype, const row_form &f, F launch) {
+    if (dtype == FC_F32) return with_rows<FC_F32>(f, launch);
+    if (dtype == FC_BF16) return with_rows<FC_BF16>(f, launch);
+    return with_rows<FC_F16>(f, launch);
 }
 
 template <int TO>
-int run(fc_context *ctx, const rms_params &p, int dtype, uint64_t bits, uint64_t addr, const char *name) {
-    const int vec = width_of(dtype, bits | (uint64_t)p.C, addr);
-    const row_form f = form_of(p.rows, p.C, vec);
-    with_kernel(dtype, vec, f, [&](auto dt, auto v, auto waves, auto r) {
+int run(fc_context *ctx, const rms_params &p, int dtype, const char *name) {
+    const row_form f = form_of(p.rows, p.C, dtype);
+    const fc_device_scope on(ctx);
+    with_kernel(dtype, f, [&](auto dt, auto waves, auto r) {
         constexpr int W = decltype(waves)::value;
-        fc_rms_norm_kernel<decltype(dt)::value, decltype(v)::value, W, decltype(r)::value, TO>
-            <<<dim3((unsigned)f.blocks(p.rows)), dim3(W > 4 ? 64 * W : 256), 0, ctx->stream>>>(p);
+        fc_rms_norm_kernel<decltype(dt)::value, W, decltype(r)::value, TO>
+            <<<dim3((unsigned)f.blocks(p.rows, kBlocks)), dim3(W > 4 ? 64 * W : 256), 0, ctx->stream>>>(p);
     });
     FC_LAUNCH_CHECK(ctx, name);
     return FC_OK;
@@ -354,21 +426,11 @@ int check_plan(fc_context *ctx, const fc_rms_norm_plan *plan, const char *what) 
 }
 
 // What both forward calls check and set.
-int forward_params(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x, const void *residual, const float *gamma, void *sum, rms_params &p,
-                   uint64_t &bits, uint64_t &addr) {
+int forward_params(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x, const void *residual, const float *gamma, void *sum, rms_params &p) {
     const fc_rms_norm_shape &s = plan->shape;
     if (!x) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: null pointer");
     if (sum && !fc_apart(s.rows, s.sum_row, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: rows of the sum overlap");
-    bits = (uint64_t)s.x_row;
-    addr = (uint64_t)x;
-    if (residual) {
-        bits |= (uint64_t)s.residual_row;
-        addr |= (uint64_t)residual;
-    }
-    if (sum) {
-        bits |= (uint64_t)s.sum_row;
-        addr |= (uint64_t)sum;
-    }
+    const uint64_t addr = (uint64_t)x | (uint64_t)residual | (uint64_t)sum;
     if ((addr & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)gamma & 3)) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: unaligned pointer");
     p.x = x; p.residual = residual; p.sum = sum; p.gamma = gamma;
     p.rows = s.rows; p.C = s.C; p.eps = s.eps;
@@ -384,13 +446,7 @@ extern "C" int fc_rms_norm_make_plan(const fc_rms_norm_shape *s, fc_rms_norm_pla
     if (s->rows > kMostRows || s->C > kMostChannels) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    // wherever the tensors begin: the most parts that any access width leads to
-    const int widths[3] = {16 / (int)fc_elem_size(s->dtype), 2, 1};
-    for (int w : widths) {
-        const row_form f = form_of(s->rows, s->C, w);
-        const long parts = f.blocks(s->rows) * (f.waves == 1 ? 4 : 1);
-        if (parts > plan->parts) plan->parts = (int)parts;
-    }
+    plan->parts = (int)form_of(s->rows, s->C, s->dtype).blocks(s->rows, kBlocksBackward);
     plan->ws_backward_bytes = (size_t)plan->parts * s->C * sizeof(float);
     return FC_OK;
 }
@@ -401,22 +457,14 @@ extern "C" int fc_rms_norm(fc_context *ctx, const fc_rms_norm_plan *plan, const 
     if (check_plan(ctx, plan, "fc_rms_norm: not a plan of fc_rms_norm_make_plan")) return FC_ERR_INVALID;
     const fc_rms_norm_shape &s = plan->shape;
     rms_params p = {};
-    uint64_t bits, addr;
-    const int rc = forward_params(ctx, plan, x_dev, residual_dev, gamma_dev, sum_dev, p, bits, addr);
+    const int rc = forward_params(ctx, plan, x_dev, residual_dev, gamma_dev, sum_dev, p);
     if (rc) return rc;
     if (!y_dev) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: null pointer");
     if (((uint64_t)y_dev & (fc_elem_size(s.dtype) - 1)) || ((uint64_t)rstd_dev & 3)) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: unaligned pointer");
     if (!fc_apart(s.rows, s.y_row, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm: rows of y overlap");
     p.y = y_dev;
     p.rstd = rstd_dev;
-    const fc_device_scope on(ctx);
-    return run<TO_TYPE>(ctx, p, s.dtype, bits | (uint64_t)s.y_row, addr | (uint64_t)y_dev, "fc_rms_norm");
-}
-
-// Rows of bytes: an access of n values writes n of them.
-static void add_bytes(int dtype, long row, const void *q, uint64_t &bits, uint64_t &addr) {
-    bits |= (uint64_t)row;
-    addr |= (uint64_t)q * fc_elem_size(dtype);
+    return run<TO_TYPE>(ctx, p, s.dtype, "fc_rms_norm");
 }
 
 extern "C" int fc_rms_norm_int8(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x_dev, const void *residual_dev, const float *gamma_dev,
@@ -425,17 +473,14 @@ extern "C" int fc_rms_norm_int8(fc_context *ctx, const fc_rms_norm_plan *plan, c
     if (check_plan(ctx, plan, "fc_rms_norm_int8: not a plan of fc_rms_norm_make_plan")) return FC_ERR_INVALID;
     const fc_rms_norm_shape &s = plan->shape;
     rms_params p = {};
-    uint64_t bits, addr;
-    const int rc = forward_params(ctx, plan, x_dev, residual_dev, gamma_dev, sum_dev, p, bits, addr);
+    const int rc = forward_params(ctx, plan, x_dev, residual_dev, gamma_dev, sum_dev, p);
     if (rc) return rc;
     if (!q_dev || !scale_dev) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm_int8: null pointer");
     if ((uint64_t)scale_dev & 3) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm_int8: unaligned pointer");
     if (!fc_apart(s.rows, s.y_row, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_rms_norm_int8: rows of q overlap");
     p.y = q_dev;
     p.scale = scale_dev;
-    add_bytes(s.dtype, s.y_row, q_dev, bits, addr);
-    const fc_device_scope on(ctx);
-    return run<TO_INT8>(ctx, p, s.dtype, bits, addr, "fc_rms_norm_int8");
+    return run<TO_INT8>(ctx, p, s.dtype, "fc_rms_norm_int8");
 }
 
 extern "C" int fc_quantize_rows(fc_context *ctx, long rows, int C, int dtype, const void *x_dev, long x_row, int8_t *q_dev, long q_row,
@@ -449,10 +494,7 @@ extern "C" int fc_quantize_rows(fc_context *ctx, long rows, int C, int dtype, co
     rms_params p = {};
     p.x = x_dev; p.y = q_dev; p.scale = scale_dev;
     p.rows = rows; p.C = C; p.x_row = x_row; p.y_row = q_row;
-    uint64_t bits = (uint64_t)x_row, addr = (uint64_t)x_dev;
-    add_bytes(dtype, q_row, q_dev, bits, addr);
-    const fc_device_scope on(ctx);
-    return run<ONLY_INT8>(ctx, p, dtype, bits, addr, "fc_quantize_rows");
+    return run<ONLY_INT8>(ctx, p, dtype, "fc_quantize_rows");
 }
 
 extern "C" int fc_rms_norm_backward(fc_context *ctx, const fc_rms_norm_plan *plan, const void *dy_dev, const void *sum_dev, const float *gamma_dev,
@@ -471,20 +513,15 @@ extern "C" int fc_rms_norm_backward(fc_context *ctx, const fc_rms_norm_plan *pla
     p.part = dgamma_dev ? (float *)ws_dev : nullptr;
     p.rows = s.rows; p.C = s.C;
     p.x_row = s.x_row; p.sum_row = s.sum_row; p.dy_row = s.y_row;
-    const int vec = width_of(s.dtype, (uint64_t)s.C | (uint64_t)s.x_row | (uint64_t)s.sum_row | (uint64_t)s.y_row, addr);
-    const row_form f = form_of(s.rows, s.C, vec);
-    const long blocks = f.blocks(s.rows);
+    const row_form f = form_of(s.rows, s.C, s.dtype);
     const fc_device_scope on(ctx);
-    with_kernel(s.dtype, vec, f, [&](auto dt, auto v, auto waves, auto r) {
+    with_kernel(s.dtype, f, [&](auto dt, auto waves, auto r) {
         constexpr int W = decltype(waves)::value;
-        fc_rms_norm_gradient_kernel<decltype(dt)::value, decltype(v)::value, W, decltype(r)::value>
-            <<<dim3((unsigned)blocks), dim3(W > 4 ? 64 * W : 256), 0, ctx->stream>>>(p);
+        fc_rms_norm_gradient_kernel<decltype(dt)::value, W, decltype(r)::value><<<dim3((unsigned)plan->parts), dim3(W > 4 ? 64 * W : 256), 0, ctx->stream>>>(p);
     });
     FC_LAUNCH_CHECK(ctx, "fc_rms_norm_gradient_kernel");
     if (!dgamma_dev) return FC_OK;
-    // rows past the last have no wavefront: parts of wavefronts that had none are not written
-    const long parts = f.waves > 1 ? blocks : blocks * 4 < s.rows ? blocks * 4 : s.rows;
-    fc_rms_norm_dgamma_kernel<<<dim3((unsigned)((s.C + 63) / 64)), dim3(256), 0, ctx->stream>>>(p.part, dgamma_dev, (int)parts, s.C);
+    fc_rms_norm_dgamma_kernel<<<dim3((unsigned)((s.C + kPartValues - 1) / kPartValues)), dim3(kPartThreads), 0, ctx->stream>>>(p.part, dgamma_dev, plan->parts, s.C);
     FC_LAUNCH_CHECK(ctx, "fc_rms_norm_dgamma_kernel");
     return FC_OK;
 }

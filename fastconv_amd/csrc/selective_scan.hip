@@ -65,18 +65,11 @@ __global__ __launch_bounds__(kThreads) void fc_selective_scan_shared_kernel(cons
     }
 }
 
-// dA, dD and the gradient of delta_bias from those of each walk, always in the same order: 64 of [D][N + 2] a workgroup, four wavefronts that share the walks.
-__global__ __launch_bounds__(256) void fc_selective_scan_sums_kernel(const fc_scan_run r, float *dA, float *dD, float *dbias) {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long size = (long)r.channels * (r.N + 2), i = (long)blockIdx.x * 64 + lane, walks = (long)r.B * r.walks;
-    float s = 0.f;
-    if (i < size)
-        for (long n = wave; n < walks; n += 4) s += r.sums[n * size + i];
-    sums[wave][lane] = s;
-    __syncthreads();
-    if (wave || i >= size) return;
-    s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+// dA, dD and the gradient of delta_bias from those of each walk, [D][N + 2] each.
+__global__ __launch_bounds__(kPartThreads) void fc_selective_scan_sums_kernel(const fc_scan_run r, float *dA, float *dD, float *dbias) {
+    long i;
+    float s;
+    if (!fc_sum_parts(r.sums, (long)r.B * r.walks, (long)r.channels * (r.N + 2), i, s)) return;
     const long d = i / (r.N + 2);
     const int n = (int)(i - d * (r.N + 2));
     if (n < r.N) {
@@ -151,6 +144,9 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     if (fc_count(workgroups, tiles) < 0 || workgroups * tiles >= kMostThreads / kThreads || fc_count(s->B, s->D) >= kMostThreads / kMostStates ||
         fc_count(s->B * tiles, s->D, kScanTile * kMostStates) < 0)
         return FC_ERR_UNSUPPORTED;
+    // a tile's offsets are 31 bits
+    const long far = s->x_token | s->delta_token | s->z_token | s->b_token | s->c_token | s->y_token;
+    if (s->T > kMostSteps && far >= (1l << 24)) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
     plan->tiles = s->T > kMostSteps ? (int)tiles : 0;
@@ -253,7 +249,8 @@ extern "C" int fc_selective_scan_backward(fc_context *ctx, const fc_selective_sc
     sum<<<dim3((unsigned)(want < 65536 ? want : 65536)), dim3(kThreads), 0, ctx->stream>>>(r, dB_dev, dC_dev, values);
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_shared_kernel");
     if (!dA_dev && !dD_dev && !ddelta_bias_dev) return FC_OK;
-    fc_selective_scan_sums_kernel<<<dim3((unsigned)(((long)s.D * (s.N + 2) + 63) / 64)), dim3(256), 0, ctx->stream>>>(r, dA_dev, dD_dev, ddelta_bias_dev);
+    fc_selective_scan_sums_kernel<<<dim3((unsigned)(((long)s.D * (s.N + 2) + kPartValues - 1) / kPartValues)), dim3(kPartThreads), 0, ctx->stream>>>(r, dA_dev, dD_dev,
+                                                                                                                                           ddelta_bias_dev);
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_sums_kernel");
     return FC_OK;
 }

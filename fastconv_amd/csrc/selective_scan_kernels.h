@@ -36,6 +36,7 @@ struct scan_place {
     typedef scan_form<L> F;
     long b, len;
     int walk, group, block;
+    long first;              // channel of the tensors that the workgroup begins with
     int c, row;              // channel and first token of a tile, along the channels
     int d, ds;               // channel along the channels and along the states; -1 past the last
     int chan, sg;            // along the states: channel of the workgroup, four states of it
@@ -48,13 +49,41 @@ struct scan_place {
         len = fc_scan_length(r, b);
         const int per = r.blocks / r.G;
         group = block / per;
-        const int first = (block - group * per) * F::CH, tid = threadIdx.x;
+        const int from = (block - group * per) * F::CH, tid = threadIdx.x;
+        first = group * (long)r.per_group + from;
         c = tid % F::CH;
         row = tid / F::CH;
         chan = tid / L;
         sg = tid % L;
-        d = first + c < r.per_group ? group * r.per_group + first + c : -1;
-        ds = first + chan < r.per_group ? group * r.per_group + first + chan : -1;
+        d = from + c < r.per_group ? group * r.per_group + from + c : -1;
+        ds = from + chan < r.per_group ? group * r.per_group + from + chan : -1;
+    }
+};
+
+constexpr uint32_t kNowhere = 0x80000000u;
+
+// A thread's offsets in bytes into tiles of the tensors, and the tokens' distances.
+struct scan_offsets {
+    uint32_t x, delta, z, y, b, c;
+    uint32_t x_token, delta_token, z_token, y_token, b_token, c_token;
+    template <int L>
+    __device__ __forceinline__ scan_offsets(const fc_scan_run &r, const scan_place<L> &at, uint32_t es) {
+        typedef scan_form<L> F;
+        x_token = (uint32_t)r.x_token * es;
+        delta_token = (uint32_t)r.delta_token * es;
+        z_token = (uint32_t)r.z_token * es;
+        y_token = (uint32_t)r.y_token * es;
+        b_token = (uint32_t)r.b_token * es;
+        c_token = (uint32_t)r.c_token * es;
+        const uint32_t none = at.d >= 0 ? 0 : kNowhere, lane = at.c * es | none, row = at.row;
+        x = lane + row * x_token;
+        delta = lane + row * delta_token;
+        z = lane + row * z_token;
+        y = lane + row * y_token;
+        const int n = threadIdx.x % F::NP;
+        const uint32_t state = n < r.N ? n * es : kNowhere, token = threadIdx.x / F::NP;
+        b = state + token * b_token;
+        c = state + token * c_token;
     }
 };
 
@@ -63,38 +92,67 @@ __device__ __forceinline__ float step_of(const fc_scan_run &r, float raw) {
     return r.softplus ? fc_softplus(raw) : raw;
 }
 
-// What a thread has of a tile before it is laid out for the states: values of its channel, one every ROWS tokens.  Nothing past `end` is read.
+// A tensor's tokens from t0 of a tile on, through a buffer resource: a thread has one 32-bit offset for all its tokens, whose distances are scalars, and an
+// offset past 2^31 reads zeros and writes nothing.
+template <int DT>
+struct scan_window {
+    typedef typename fc_elem<DT>::type E;
+    static constexpr int ES = (int)sizeof(E);
+    __amdgpu_buffer_rsrc_t res;
+    __device__ __forceinline__ scan_window(const void *base, long offset)
+        : res(__builtin_amdgcn_make_buffer_rsrc(uniform_ptr((E *)base + offset), 0, 0x7fffffff, 0x00020000)) {}
+    __device__ __forceinline__ E get(uint32_t at, uint32_t further) const {
+        if constexpr (ES == 4) return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(res, at, further, 0));
+        else return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(res, at, further, 0));
+    }
+    __device__ __forceinline__ void put(float v, uint32_t at, uint32_t further) const {
+        const E e = (E)v;
+        if constexpr (ES == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), res, at, further, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, e), res, at, further, 0);
+    }
+};
+
+// What a thread has of a tile before it is laid out for the states: values of its channel, one every ROWS tokens.  `n` tokens are there, the others zeros.
 template <int DT, int L, bool GATE, bool DY>
 struct scan_tile {
     typedef scan_form<L> F;
     typedef typename fc_elem<DT>::type E;
+    typedef scan_window<DT> W;
     E x[F::EACH], delta[F::EACH], z[GATE ? F::EACH : 1], dy[DY ? F::EACH : 1], b[F::SHARED], c[F::SHARED];
 
-    __device__ __forceinline__ void read(const fc_scan_run &r, const scan_place<L> &at, long t0, long end, bool with_c) {
-        if (at.d >= 0) {
-            const E *px = (const E *)r.x + at.b * r.x_batch + at.d, *pd = (const E *)r.delta + at.b * r.delta_batch + at.d;
-            const E *pz = (const E *)r.z + at.b * r.z_batch + at.d, *py = (const E *)r.dy + at.b * r.y_batch + at.d;
+    // channels: x, delta, z, dy; states: B, and C if asked for
+    __device__ __forceinline__ void read(const fc_scan_run &r, const scan_place<L> &at, const scan_offsets &off, long t0, long end, bool channels, bool states,
+                                         bool with_c) {
+        const int n = (int)(end - t0 < kScanTile ? end - t0 : kScanTile);
+        const W wx(r.x, at.b * r.x_batch + t0 * r.x_token + at.first), wd(r.delta, at.b * r.delta_batch + t0 * r.delta_token + at.first);
+        const W wz(r.z, at.b * r.z_batch + t0 * r.z_token + at.first), wy(r.dy, at.b * r.y_batch + t0 * r.y_token + at.first);
+        const W wb(r.b, at.b * r.b_batch + t0 * r.b_token + at.group * r.b_group), wc(r.c, at.b * r.c_batch + t0 * r.c_token + at.group * r.c_group);
+        constexpr int BC = F::THREADS / F::NP;      // tokens of B and C at once
+        auto all = [&](auto each, auto several) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < F::EACH; k++) {
-                const long t = t0 + at.row + k * F::ROWS;
-                if (t < end) {
-                    x[k] = px[t * r.x_token];
-                    delta[k] = pd[t * r.delta_token];
-                    if (GATE) z[k] = pz[t * r.z_token];
-                    if (DY) dy[k] = py[t * r.y_token];
-                }
+            for (int k = 0; k < F::EACH && channels; k++) {
+                x[k] = each(wx, off.x, off.x_token, k);
+                delta[k] = each(wd, off.delta, off.delta_token, k);
+                if (GATE) z[k] = each(wz, off.z, off.z_token, k);
+                if (DY) dy[k] = each(wy, off.y, off.y_token, k);
             }
-        }
-        const E *pb = (const E *)r.b + at.b * r.b_batch + at.group * r.b_group, *pc = (const E *)r.c + at.b * r.c_batch + at.group * r.c_group;
 #pragma unroll
-        for (int k = 0; k < F::SHARED; k++) {
-            const int i = threadIdx.x + k * F::THREADS, n = i % F::NP;
-            const long t = t0 + i / F::NP;
-            b[k] = c[k] = (E)0.f;
-            if (n < r.N && t < end) {
-                b[k] = pb[t * r.b_token + n];
-                if (with_c) c[k] = pc[t * r.c_token + n];
+            for (int k = 0; k < F::SHARED && states; k++) {
+                b[k] = several(wb, off.b, off.b_token, k);
+                if (with_c) c[k] = several(wc, off.c, off.c_token, k);
             }
+        };
+        if (n == kScanTile) {
+            all([&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) { return w.get(lane, k * F::ROWS * token); },
+                [&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) { return w.get(lane, k * BC * token); });
+        } else {
+            const int row = threadIdx.x / F::NP;
+            all([&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) {
+                    return w.get(at.row + k * F::ROWS < n ? lane + k * F::ROWS * token : kNowhere, 0);
+                },
+                [&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) {
+                    return w.get(row + k * BC < n ? lane + k * BC * token : kNowhere, 0);
+                });
         }
     }
 };
@@ -146,7 +204,7 @@ __device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_pl
 
 // Answers.  Bound by the vector ALUs: an exponential (four cycles' worth) and four operations a state, 16 states a value.
 template <int DT, int L, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_kernel(const fc_scan_run r) {
+__global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_selective_scan_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
     typedef typename fc_elem<DT>::type E;
     __shared__ scan_shared<L> lds;
@@ -158,9 +216,9 @@ __global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_kerne
     if (r.segments > 1) read_states<L>(r, at, r.parts, at.b * r.segments + at.walk, h);
     else read_states<L>(r, at, r.state_in, at.b, h);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
-    E *y = (E *)r.y + at.b * r.y_batch + at.d;
+    const scan_offsets off(r, at, sizeof(E));
     scan_tile<DT, L, GATE, false> now;
-    now.read(r, at, t0, end, true);
+    if (t0 < end) now.read(r, at, off, t0, end, true, true, true);
     for (long t = t0; t < end; t += kScanTile) {
         const int n = (int)(end - t < kScanTile ? end - t : kScanTile);
         float x[F::EACH], z[GATE ? F::EACH : 1];
@@ -174,7 +232,7 @@ __global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_kerne
         lay_out<L>(lds.b, now.b);
         lay_out<L>(lds.c, now.c);
         __syncthreads();
-        if (t + kScanTile < end) now.read(r, at, t + kScanTile, end, true);
+        if (t + kScanTile < end) now.read(r, at, off, t + kScanTile, end, true, true, true);
         float mine = 0.f;
         auto token = [&](int i) __attribute__((always_inline)) {
             const float2 du = lds.du[i][at.chan];
@@ -202,26 +260,25 @@ __global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_kerne
             }
         }
         __syncthreads();
-        if (at.d >= 0) {
+        const scan_window<DT> y(r.y, at.b * r.y_batch + t * r.y_token + at.first);
 #pragma unroll
-            for (int k = 0; k < F::EACH; k++) {
-                const int i = at.row + k * F::ROWS;
-                if (i >= n) continue;
-                float v = __builtin_fmaf(skip, x[k], ys[i][at.c]);
-                if (GATE) v *= fc_silu(z[k]);
-                y[(t + i) * r.y_token] = (E)v;
-            }
+        for (int k = 0; k < F::EACH; k++) {
+            const int i = at.row + k * F::ROWS;
+            float v = __builtin_fmaf(skip, x[k], ys[i][at.c]);
+            if (GATE) v *= fc_silu(z[k]);
+            if (n == kScanTile) y.put(v, off.y, k * F::ROWS * off.y_token);
+            else y.put(v, i < n ? off.y + k * F::ROWS * off.y_token : kNowhere, 0);
         }
     }
     // tokens past the end of a shorter sequence
     if (at.d >= 0)
-        for (long t = (end > t0 ? end : t0) + at.row; t < t1; t += F::ROWS) y[t * r.y_token] = (E)0.f;
+        for (long t = (end > t0 ? end : t0) + at.row; t < t1; t += F::ROWS) ((E *)r.y)[at.b * r.y_batch + t * r.y_token + at.d] = (E)0.f;
     if (r.state_out && at.walk == r.segments - 1) write_states<L>(r, at, r.state_out, at.b, h);
 }
 
 // What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient.
 template <int DT, int L, bool GRADS, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
+__global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
     __shared__ scan_shared<L> lds;
     __shared__ float gs[GRADS ? kScanTile : 1][GRADS ? F::CH : 1];
@@ -231,8 +288,9 @@ __global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_ends_
     float rate[kScanStates], h[kScanStates], decay[kScanStates], grad[kScanStates], steps = 0.f;
     read_rates<L>(r, at, rate);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f;
+    const scan_offsets off(r, at, sizeof(typename fc_elem<DT>::type));
     scan_tile<DT, L, GATE && GRADS, GRADS> now;
-    now.read(r, at, first, end, GRADS);
+    if (first < end) now.read(r, at, off, first, end, true, true, GRADS);
     long segment = at.b * r.segments + (long)at.walk * r.per_walk;
     for (long t = first; t < last; t += kScanTile) {
         const int n = (int)(end - t < 0 ? 0 : end - t < kScanTile ? end - t : kScanTile);
@@ -258,7 +316,7 @@ __global__ __launch_bounds__(scan_form<L>::THREADS) void fc_selective_scan_ends_
             lay_out<L>(lds.b, now.b);
             if (GRADS) lay_out<L>(lds.c, now.c);
             __syncthreads();
-            if (t + kScanTile < end) now.read(r, at, t + kScanTile, end, GRADS);
+            if (t + kScanTile < end) now.read(r, at, off, t + kScanTile, end, true, true, GRADS);
             auto token = [&](int i) __attribute__((always_inline)) {
                 const float2 du = lds.du[i][at.chan];
                 const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
@@ -398,108 +456,100 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gr
     read_rates<L>(r, at, rate);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
     const long first = (long)at.walk * r.per_walk, last = first + r.per_walk < r.segments ? first + r.per_walk : r.segments;
-    E *dx = (E *)r.dx + at.b * r.x_batch + at.d, *dd = (E *)r.ddelta + at.b * r.delta_batch + at.d, *dz = (E *)r.dz + at.b * r.z_batch + at.d;
-    constexpr bool AHEAD = F::EACH <= 8;      // the next tile's values have registers of their own
+    const scan_offsets off(r, at, sizeof(E));
     scan_tile<DT, L, GATE, true> now;
-    if (AHEAD) now.read(r, at, first * kScanTile, at.len, true);
+    if (first * kScanTile < at.len) now.read(r, at, off, first * kScanTile, at.len, true, true, true);
     for (long seg = first; seg < last; seg++) {
         const long t = seg * kScanTile, end = t + kScanTile < r.T ? t + kScanTile : r.T;
         const int n = (int)(at.len - t < 0 ? 0 : at.len - t < kScanTile ? at.len - t : kScanTile);
         float *shared = r.shared + ((at.block * (long)r.B + at.b) * r.T + t) * 2 * r.N;
         if (n > 0) {
-            if (!AHEAD) now.read(r, at, t, at.len, true);
-            const scan_tile<DT, L, GATE, true> here = now;
             float steps[F::EACH];
 #pragma unroll
             for (int k = 0; k < F::EACH; k++) {
                 const int i = at.row + k * F::ROWS;
                 const bool in = i < n && at.d >= 0;      // a token past the last moves nothing
-                const float x = in ? (float)here.x[k] : 0.f;
-                steps[k] = in ? step_of<DT>(r, (float)here.delta[k] + bias) : 0.f;
-                float g = in ? (float)here.dy[k] : 0.f;
-                if (GATE && in) g *= fc_silu((float)here.z[k]);
+                const float x = in ? (float)now.x[k] : 0.f;
+                steps[k] = in ? step_of<DT>(r, (float)now.delta[k] + bias) : 0.f;
+                float g = in ? (float)now.dy[k] : 0.f;
+                if (GATE && in) g *= fc_silu((float)now.z[k]);
                 lds.du[i][at.c] = make_float2(steps[k], steps[k] * x);
                 gs[i][at.c] = g;
             }
-            lay_out<L>(lds.b, here.b);
-            lay_out<L>(lds.c, here.c);
+            lay_out<L>(lds.b, now.b);
+            lay_out<L>(lds.c, now.c);
             float start[kScanStates], G[kScanStates];
             read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
             read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
             __syncthreads();
-            if (AHEAD && seg + 1 < last) now.read(r, at, t + kScanTile, at.len, true);
-            float hs[kScanTile][kScanStates];
-            float mine = 0.f;
-#pragma unroll
-            for (int i = 0; i < kScanTile; i++) {
-                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);      // else all tiles' reads move to the front, and registers spill
+            // Half a tile's states are kept at a time: with all of them there are no registers left for what comes next.
+            constexpr int HALF = kScanTile / 2;
+            float mid[kScanStates] = {start[0], start[1], start[2], start[3]};
+#pragma unroll 8
+            for (int i = 0; i < HALF; i++) {
                 const float2 du = lds.du[i][at.chan];
                 const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
                 const float bs[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-                for (int j = 0; j < kScanStates; j++)
-                    hs[i][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), i ? hs[i ? i - 1 : 0][j] : start[j], du.y * bs[j]);
-                if constexpr (GATE) {
-                    const float4 c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
-                    float s = c.x * hs[i][0];
-                    s = __builtin_fmaf(c.y, hs[i][1], s);
-                    s = __builtin_fmaf(c.z, hs[i][2], s);
-                    s = __builtin_fmaf(c.w, hs[i][3], s);
-                    s = sum_states<L>(s);
-                    mine = i % L == at.sg ? s : mine;
-                    if (i % L == L - 1) ys[i - L + 1 + at.sg][at.chan] = mine;
-                }
+                for (int j = 0; j < kScanStates; j++) mid[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), mid[j], du.y * bs[j]);
             }
-            // steps and exponentials are formed again: kept from above, with the states, they would need twice the registers
-            fc_wave_sync();
-            float2 kept = make_float2(0.f, 0.f);
+#pragma unroll 1
+            for (int half = HALF; half >= 0; half -= HALF) {
+                float hs[HALF][kScanStates], enters[kScanStates];
 #pragma unroll
-            for (int i = kScanTile - 1; i >= 0; i--) {
-                if (i % 2) __builtin_amdgcn_sched_barrier(0);
-                const float2 du = lds.du[i][at.chan];
-                const float g = gs[i][at.chan];
-                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates], c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
-                const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
-                float v[8], du_sum = 0.f, dt_sum = 0.f;
+                for (int j = 0; j < kScanStates; j++) enters[j] = half ? mid[j] : start[j];
 #pragma unroll
-                for (int j = 0; j < kScanStates; j++) {
-                    G[j] = __builtin_fmaf(cs[j], g, G[j]);
-                    v[j] = G[j] * du.y;
-                    v[4 + j] = g * hs[i][j];
-                    du_sum = __builtin_fmaf(G[j], bs[j], du_sum);
-                    G[j] *= __builtin_amdgcn_exp2f(du.x * rate[j]);
-                    const float k = G[j] * (i ? hs[i ? i - 1 : 0][j] : start[j]);
-                    dt_sum = __builtin_fmaf(k, rate[j], dt_sum);
-                    dA[j] = __builtin_fmaf(k, du.x, dA[j]);
+                for (int i = 0; i < HALF; i++) {
+                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);      // else all reads move to the front, and registers spill
+                    const float2 du = lds.du[half + i][at.chan];
+                    const float4 b = *(const float4 *)&lds.b[half + i][at.sg * kScanStates];
+                    const float bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int j = 0; j < kScanStates; j++)
+                        hs[i][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), i ? hs[i ? i - 1 : 0][j] : enters[j], du.y * bs[j]);
                 }
-                du_sum = sum_states<L>(du_sum);
-                dt_sum = sum_states<L>(dt_sum);
-                const float2 s = sum_channels<L>(v);
-                if (L == 16 || (lane & 15) < L)
-                    *(float2 *)&waves[wave][i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
-                if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
-                if (i % L == 0) lds.du[i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
-            }
-            __syncthreads();
-            if (at.d >= 0) {
+                fc_wave_sync();      // steps and exponentials are formed again: kept, they would need twice the registers
+                float2 kept = make_float2(0.f, 0.f);
+                float mine = 0.f;
 #pragma unroll
-                for (int k = 0; k < F::EACH; k++) {
-                    const int i = at.row + k * F::ROWS;
-                    if (i >= n) continue;
-                    const float2 s = lds.du[i][at.c];
-                    const float x = (float)here.x[k], g = gs[i][at.c];
-                    float dstep = __builtin_fmaf(x, s.x, 0.693147181f * s.y);
-                    if (r.softplus) dstep *= fc_sigmoid((float)here.delta[k] + bias);
-                    dx[(t + i) * r.x_token] = (E)__builtin_fmaf(steps[k], s.x, skip * g);
-                    dd[(t + i) * r.delta_token] = (E)dstep;
-                    if constexpr (GATE) {
-                        const float z = (float)here.z[k];
-                        dz[(t + i) * r.z_token] = (E)((float)here.dy[k] * __builtin_fmaf(skip, x, ys[i][at.c]) * fc_silu_slope(z));
+                for (int i = HALF - 1; i >= 0; i--) {
+                    if (i % 2) __builtin_amdgcn_sched_barrier(0);
+                    const float2 du = lds.du[half + i][at.chan];
+                    const float g = gs[half + i][at.chan];
+                    const float4 b = *(const float4 *)&lds.b[half + i][at.sg * kScanStates], c = *(const float4 *)&lds.c[half + i][at.sg * kScanStates];
+                    const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
+                    float v[8], du_sum = 0.f, dt_sum = 0.f, y = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kScanStates; j++) {
+                        G[j] = __builtin_fmaf(cs[j], g, G[j]);
+                        v[j] = G[j] * du.y;
+                        v[4 + j] = g * hs[i][j];
+                        if (GATE) y = __builtin_fmaf(cs[j], hs[i][j], y);
+                        du_sum = __builtin_fmaf(G[j], bs[j], du_sum);
+                        G[j] *= __builtin_amdgcn_exp2f(du.x * rate[j]);
+                        const float k = G[j] * (i ? hs[i ? i - 1 : 0][j] : enters[j]);
+                        dt_sum = __builtin_fmaf(k, rate[j], dt_sum);
+                        dA[j] = __builtin_fmaf(k, du.x, dA[j]);
                     }
-                    dD = __builtin_fmaf(g, x, dD);
-                    dbias += dstep;
+                    du_sum = sum_states<L>(du_sum);
+                    dt_sum = sum_states<L>(dt_sum);
+                    const float2 s = sum_channels<L>(v);
+                    if (L == 16 || (lane & 15) < L)
+                        *(float2 *)&waves[wave][half + i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
+                    // each lane keeps one of L tokens
+                    if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
+                    if (i % L == 0) lds.du[half + i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
+                    if constexpr (GATE) {
+                        y = sum_states<L>(y);
+                        mine = i % L == at.sg ? y : mine;
+                        if (i % L == 0) ys[half + i + at.sg][at.chan] = mine;
+                    }
                 }
             }
+            scan_tile<DT, L, GATE, true> here;
+            // this tile's values once more: kept, they would leave the states no registers
+            here.read(r, at, off, t, at.len, true, false, false);
+            __syncthreads();
             for (int i = threadIdx.x; i < n * 2 * F::NP; i += F::THREADS) {
                 const int token = i / (2 * F::NP), k = i % (2 * F::NP), half = k / F::NP, state = k % F::NP;
                 if (state >= r.N) continue;
@@ -508,14 +558,35 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gr
                 for (int w = 1; w < F::WAVES; w++) s += waves[w][token][k];
                 shared[((long)token * 2 + half) * r.N + state] = s;
             }
+            if (seg + 1 < last && t + kScanTile < at.len) now.read(r, at, off, t + kScanTile, at.len, true, true, true);
+            const scan_window<DT> dx(r.dx, at.b * r.x_batch + t * r.x_token + at.first), dd(r.ddelta, at.b * r.delta_batch + t * r.delta_token + at.first);
+            const scan_window<DT> dz(r.dz, at.b * r.z_batch + t * r.z_token + at.first);
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) {
+                const int i = at.row + k * F::ROWS;
+                const bool in = i < n;      // channels past the last are zeros and nowhere
+                const float2 s = lds.du[i][at.c];
+                const float x = (float)here.x[k], g = gs[i][at.c];
+                float dstep = __builtin_fmaf(x, s.x, 0.693147181f * s.y);
+                if (r.softplus) dstep *= fc_sigmoid((float)here.delta[k] + bias);
+                auto put = [&](const scan_window<DT> &w, float v, uint32_t lane, uint32_t token) __attribute__((always_inline)) {
+                    if (n == kScanTile) w.put(v, lane, k * F::ROWS * token);
+                    else w.put(v, in ? lane + k * F::ROWS * token : kNowhere, 0);
+                };
+                put(dx, __builtin_fmaf(steps[k], s.x, skip * g), off.x, off.x_token);
+                put(dd, dstep, off.delta, off.delta_token);
+                if constexpr (GATE) put(dz, (float)here.dy[k] * __builtin_fmaf(skip, x, ys[i][at.c]) * fc_silu_slope((float)here.z[k]), off.z, off.z_token);
+                dD = in ? __builtin_fmaf(g, x, dD) : dD;
+                dbias = in ? dbias + dstep : dbias;
+            }
             __syncthreads();
         }
         // tokens past the end of a shorter sequence
         if (at.d >= 0)
             for (long i = t + n + at.row; i < end; i += F::ROWS) {
-                dx[i * r.x_token] = (E)0.f;
-                dd[i * r.delta_token] = (E)0.f;
-                if (GATE) dz[i * r.z_token] = (E)0.f;
+                ((E *)r.dx)[at.b * r.x_batch + i * r.x_token + at.d] = (E)0.f;
+                ((E *)r.ddelta)[at.b * r.delta_batch + i * r.delta_token + at.d] = (E)0.f;
+                if (GATE) ((E *)r.dz)[at.b * r.z_batch + i * r.z_token + at.d] = (E)0.f;
             }
         for (long i = (long)n * 2 * r.N + threadIdx.x; i < (end - t) * 2 * r.N; i += F::THREADS) shared[i] = 0.f;
     }

@@ -18,17 +18,13 @@ __device__ __forceinline__ float fc_exp(float v) {
 }
 
 // log(1 + e^v), exact in proportion down to e^v itself: max(v, 0) + log(1 + e), e = e^-|v| <= 1, and with s = e / (2 + e) <= 1/3
-//   log(1 + e) = 2 (s + s^3/3 + s^5/5 + ...),
-// eight terms of which leave out less than s^16/17 / (1 - s^2) < 2e-9 of it.
+//   log(1 + e) = 2 atanh(s) = 2 s P(s^2),
+// P fitted to atanh(s)/s over s^2 <= 1/9 so that the largest relative error is least: 8e-9 with these five terms.
 __device__ __forceinline__ float fc_softplus(float v) {
     const float e = fc_exp(-__builtin_fabsf(v)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float r = 1.f / 15.f;
-    r = __builtin_fmaf(r, q, 1.f / 13.f);
-    r = __builtin_fmaf(r, q, 1.f / 11.f);
-    r = __builtin_fmaf(r, q, 1.f / 9.f);
-    r = __builtin_fmaf(r, q, 1.f / 7.f);
-    r = __builtin_fmaf(r, q, 1.f / 5.f);
-    r = __builtin_fmaf(r, q, 1.f / 3.f);
+    float r = __builtin_fmaf(0.140891671f, q, 0.139803007f);
+    r = __builtin_fmaf(r, q, 0.200124547f);
+    r = __builtin_fmaf(r, q, 0.333331585f);
     r = __builtin_fmaf(r, q, 1.f);
     return __builtin_fmaf(2.f * s, r, fmaxf(v, 0.f));      // NaN comes through s
 }

@@ -42,6 +42,34 @@ __device__ __forceinline__ void fc_store_global(void *p, const V &v) {
     *(V *)(global *)(uintptr_t)p = v;
 }
 
+// Sums of values that lie in `parts` rows of `size`, in an order that depends on their number alone: a workgroup of 1024 threads sums 32 of a row,
+// 32 threads a value, each every 32nd part.  In the first 32 threads, where true, `i` is the value's place and `sum` the sum.
+constexpr int kPartThreads = 1024, kPartValues = 32;
+__device__ __forceinline__ bool fc_sum_parts(const float *part, long parts, long size, long &i, float &sum) {
+    __shared__ float sums[32][kPartValues];
+    const int at = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    i = (long)blockIdx.x * kPartValues + at;
+    float s = 0.f;
+    if (i < size) {
+        const float *p = part + i;
+        long n = slice;
+        for (; n + 7 * 32 < parts; n += 8 * 32) {      // eight on their way at once
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = p[(n + k * 32) * size];
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += v[k];
+        }
+        for (; n < parts; n += 32) s += p[n * size];
+    }
+    sums[slice][at] = s;
+    __syncthreads();
+    if (slice || i >= size) return false;
+    sum = 0.f;
+    for (int k = 0; k < 32; k++) sum += sums[k][at];
+    return true;
+}
+
 static inline size_t fc_elem_size(int dtype) { return dtype == FC_F32 ? 4 : 2; }
 static inline bool fc_dtype_ok(int dtype) { return dtype == FC_F32 || dtype == FC_BF16 || dtype == FC_F16; }
 
