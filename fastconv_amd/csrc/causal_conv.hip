@@ -14,8 +14,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMostTaps = 8;
-constexpr int kChannels = 4;     // of a thread, one access wherever they begin; one where there are fewer
-constexpr int kAhead = 8, kAheadBackward = 4;      // tokens read before the first is used
+constexpr int kChannels = 2;     // of a thread, one access wherever they begin; one where there are fewer
+constexpr int kAhead = 4, kAheadBackward = 4;      // tokens read before the first is used
 // Threads that fill the chip: a sequence is cut until there are as many, into walks of some tokens at least.
 constexpr long kFill = 4096 * 64;
 
@@ -30,17 +30,17 @@ struct conv_params {
     fc_fastdiv by_columns, by_walks;
     long x_batch, x_token, y_batch, y_token;
 
-    __device__ __forceinline__ long length(long b) const {
-        if (!lengths) return T;
-        const long n = lengths[b];
-        return n < 0 ? 0 : n > T ? T : n;
+    __device__ __forceinline__ int length(long b) const {
+        const int n = lengths ? lengths[b] : (int)T;
+        return n < 0 ? 0 : n > T ? (int)T : n;
     }
 };
 
 // What a thread walks over: channels c.. of sequence b, tokens t0 to t1.
 struct conv_place {
     int c, skip, walk;       // the last thread of a row begins where its access ends with the row, and leaves out what its neighbour has
-    long b, t0, t1, len;
+    long b;
+    int t0, t1, len;
     bool none;
     __device__ __forceinline__ conv_place(const conv_params &p, int columns, int vec) {
         const uint32_t i = blockIdx.x * kThreads + threadIdx.x, row = fc_div(i, p.by_columns);
@@ -50,31 +50,37 @@ struct conv_place {
         skip = from - c;
         b = fc_div(row, p.by_walks);
         walk = (int)(row - b * p.walks);
-        t0 = walk * p.walk;
-        t1 = t0 + p.walk < p.T ? t0 + p.walk : p.T;
+        t0 = (int)(walk * p.walk);
+        t1 = (int)(t0 + p.walk < p.T ? t0 + p.walk : p.T);
         len = none ? 0 : p.length(b);
     }
 };
 
-// The rows of a sequence's channels, from the state before the first on.  A row that is not there reads one that is, without a branch, which would
-// keep all loads before it waiting.
-template <int DT, int VEC>
-struct conv_rows {
-    typedef typename fc_elem<DT>::type E;
-    const E *x, *before;
-    long token;
-    int C, taps;
-    long len;
-    bool state;
-    __device__ __forceinline__ bool there(long t) const { return t < len && (t >= 0 || (state && t >= 1 - taps)); }
-    __device__ __forceinline__ fc_vec<DT, VEC> read(long t) const {
-        const bool early = state && t < 0;
-        const long row = early ? (t >= 1 - taps ? t + taps - 1 : 0) : t < 0 || len < 1 ? 0 : t < len ? t : len - 1;
-        fc_vec<DT, VEC> v;
-        __builtin_memcpy(&v, early ? before + row * C : x + row * token, sizeof v);
-        return v;
+// Some rows from token t on: N of them, or as many as there are tokens.  A row that is not there reads the first, without a branch of its own, which would keep
+// all loads before it waiting.
+template <int N, class V, class E>
+__device__ __forceinline__ void read_rows(V (&to)[N], const E *first, const E *row, long token, int t, int len) {
+    if (t + N <= len) {
+#pragma unroll
+        for (int u = 0; u < N; u++) __builtin_memcpy(&to[u], row + u * token, sizeof(V));
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; u++) __builtin_memcpy(&to[u], t + u < len ? row + u * token : first, sizeof(V));
     }
-};
+}
+
+// The rows before token t of a window: those of the state, or zeros, before the first token.
+template <int N, class V, class E>
+__device__ __forceinline__ void read_before(V (&to)[N], const E *first, const E *state, long token, int C, int taps, int t, int len) {
+    const V zeros = {};
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int row = t - N + i;
+        const bool early = row < 0 && state && row >= 1 - taps, there = early || (row >= 0 && row < len);
+        __builtin_memcpy(&to[i], early ? state + (long)(row + taps - 1) * C : first + (there ? row * token : 0), sizeof(V));
+        if (!there) to[i] = zeros;
+    }
+}
 
 template <class V, class E>
 __device__ __forceinline__ void store(E *to, const V &v, int skip) {
@@ -105,41 +111,45 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
 #pragma unroll
         for (int m = 0; m < TAPS; m++) back[v][m] = m < taps ? p.w[(long)(at.c + v) * taps + taps - 1 - m] : 0.f;
     }
-    V rows[TAPS - 1 + kAhead];
-    const V zeros = {};
-    const conv_rows<DT, VEC> in = {x, before, p.x_token, p.C, taps, at.len, p.state_in != nullptr};
+    V window[TAPS - 1], now[kAhead], next[kAhead];
+    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.t0, at.len);
+    const E *row = x + at.t0 * p.x_token;
+    E *to = y + at.t0 * p.y_token;
+    read_rows(next, x, row, p.x_token, at.t0, at.len);
+    for (int t = at.t0; t < at.t1; t += kAhead) {
 #pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.read(at.t0 - (TAPS - 1) + i);
+        for (int u = 0; u < kAhead; u++) now[u] = next[u];
+        row += kAhead * p.x_token;
+        if (t + kAhead < at.t1) read_rows(next, x, row, p.x_token, t + kAhead, at.len);
+        auto results = [&](auto edge) __attribute__((always_inline)) {      // edge: some of the tokens are not there, or another walk's
 #pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.there(at.t0 - (TAPS - 1) + i) ? rows[i] : zeros;
-    for (long t = at.t0; t < at.t1; t += kAhead) {
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) rows[TAPS - 1 + u] = in.read(t + u);      // tokens past the end have no result that reads them
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            if (t + u >= at.t1) break;
-            V out = zeros;
-            if (t + u < at.len) {
+            for (int u = 0; u < kAhead; u++) {
+                V out;
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
                     float z = bias[v];
 #pragma unroll
                     for (int m = TAPS - 1; m >= 0; m--)
-                        if (m < taps) z = __builtin_fmaf(back[v][m], rows[u + TAPS - 1 - m].get(v), z);
-                    out.set(v, p.act == FC_ACT_SILU ? fc_silu(z) : z);
+                        if (m < taps) z = __builtin_fmaf(back[v][m], u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v), z);
+                    if (p.act == FC_ACT_SILU) z = fc_silu(z);
+                    out.set(v, edge && t + u >= at.len ? 0.f : z);
                 }
+                if (!edge || t + u < at.t1) store(to + u * p.y_token, out, at.skip);
             }
-            store(y + (t + u) * p.y_token, out, at.skip);
-        }
+        };
+        if (t + kAhead <= (at.len < at.t1 ? at.len : at.t1)) results(std::false_type());
+        else results(std::true_type());
+        to += kAhead * p.y_token;
 #pragma unroll
-        for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAhead + i];
+        for (int i = 0; i < TAPS - 1; i++) window[i] = now[kAhead - (TAPS - 1) + i];
     }
     // The last rows, by whoever read the first: the state may be written over the one before.  Row i lies at or before what it is read from.
     if (at.walk == 0 && p.state_out) {
         E *after = (E *)p.state_out + at.b * (taps - 1) * p.C + at.c;
         for (int i = 0; i < taps - 1; i++) {
-            const long t = at.len - (taps - 1) + i;
-            store(after + (long)i * p.C, in.there(t) ? in.read(t) : zeros, at.skip);
+            V last[1];
+            read_before(last, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.len - (taps - 1) + i + 1, at.len);
+            store(after + (long)i * p.C, last[0], at.skip);
         }
     }
 }
@@ -165,63 +175,75 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
             dback[v][m] = dz[v][m] = 0.f;
         }
     }
-    V rows[TAPS - 1 + kAheadBackward], grads[kAheadBackward];
+    constexpr int AHEAD = kAheadBackward;
+    V window[TAPS - 1], now[AHEAD], grads[AHEAD], next[AHEAD], more_grads[AHEAD];
     const V zeros = {};
-    const conv_rows<DT, VEC> in = {x, before, p.x_token, p.C, taps, at.len, p.state_in != nullptr}, up = {dy, dy, p.y_token, p.C, 1, at.len, false};
+    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.t0, at.len);
+    const E *row = x + at.t0 * p.x_token, *from = dy + at.t0 * p.y_token;
+    E *to = dx + ((long)at.t0 - (TAPS - 1)) * p.x_token;      // of row t - (TAPS - 1), whose gradient is whole once dz_t is there:
+    const int end = at.t1 + TAPS - 1;                         // TAPS - 1 tokens past the walk's own
+    read_rows(next, x, row, p.x_token, at.t0, at.len);
+    read_rows(more_grads, dy, from, p.y_token, at.t0, at.len);
+    for (int t = at.t0; t < end; t += AHEAD) {
 #pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.read(at.t0 - (TAPS - 1) + i);
-#pragma unroll
-    for (int i = 0; i < TAPS - 1; i++) rows[i] = in.there(at.t0 - (TAPS - 1) + i) ? rows[i] : zeros;
-    // the gradient of row t - TAPS + 1 is whole once dz_t is there: TAPS - 1 tokens past the walk's own
-    const long end = at.t1 + TAPS - 1;
-    for (long t = at.t0; t < end; t += kAheadBackward) {
-#pragma unroll
-        for (int u = 0; u < kAheadBackward; u++) {
-            rows[TAPS - 1 + u] = in.read(t + u);
-            grads[u] = up.read(t + u);
+        for (int u = 0; u < AHEAD; u++) {
+            now[u] = next[u];
+            grads[u] = more_grads[u];
         }
+        row += AHEAD * p.x_token;
+        from += AHEAD * p.y_token;
+        if (t + AHEAD < end) {
+            read_rows(next, x, row, p.x_token, t + AHEAD, at.len);
+            read_rows(more_grads, dy, from, p.y_token, t + AHEAD, at.len);
+        }
+        auto results = [&](auto edge) __attribute__((always_inline)) {      // edge: some of the tokens or rows are not there, or another walk's, or in the state
 #pragma unroll
-        for (int u = 0; u < kAheadBackward; u++) {
-            if (t + u >= end) break;
-            const bool there = t + u < at.len, mine = t + u < at.t1;
-            const long row = t + u - (TAPS - 1);
-            const long last = row - (at.len - (taps - 1));      // row of the state after the last token
-            V more = zeros, out;
-            const bool wanted = row >= at.t0 || (at.walk == 0 && row >= 1 - taps && p.dstate_in);
-            if (wanted && p.dstate_out && last >= 0 && last < taps - 1) __builtin_memcpy(&more, dlast + last * p.C, sizeof more);
+            for (int u = 0; u < AHEAD; u++) {
+                const bool there = !edge || t + u < at.len, mine = !edge || (there && t + u < at.t1);
+                const int r = t + u - (TAPS - 1), last = r - (at.len - (taps - 1));      // last: row of the state after the last token
+                V more = zeros, out;
+                const bool wanted = !edge || r >= at.t0 || (at.walk == 0 && r >= 1 - taps && p.dstate_in);
+                if (edge && p.dstate_out && wanted && last >= 0 && last < taps - 1) __builtin_memcpy(&more, dlast + (long)last * p.C, sizeof more);
 #pragma unroll
-            for (int v = 0; v < VEC; v++) {
+                for (int v = 0; v < VEC; v++) {
+                    auto x_back = [&](int m) __attribute__((always_inline)) { return u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v); };
 #pragma unroll
-                for (int j = 0; j < TAPS - 1; j++) dz[v][j] = dz[v][j + 1];
-                float g = 0.f;
-                if (there) {      // rows past the end are not zeros
-                    g = grads[u].get(v);
+                    for (int j = 0; j < TAPS - 1; j++) dz[v][j] = dz[v][j + 1];
+                    float g = grads[u].get(v);
                     if (p.act == FC_ACT_SILU) {
                         float z = bias[v];
 #pragma unroll
                         for (int m = TAPS - 1; m >= 0; m--)
-                            if (m < taps) z = __builtin_fmaf(back[v][m], rows[u + TAPS - 1 - m].get(v), z);
+                            if (m < taps) z = __builtin_fmaf(back[v][m], x_back(m), z);
                         g *= fc_silu_slope(z);
                     }
+                    if (!there) g = 0.f;      // what was read in place of rows that are not there may be anything
+                    dz[v][TAPS - 1] = g;
                     if (mine) {
                         dbias[v] += g;
 #pragma unroll
                         for (int m = 0; m < TAPS; m++)
-                            if (m < taps) dback[v][m] = __builtin_fmaf(g, rows[u + TAPS - 1 - m].get(v), dback[v][m]);
+                            if (m < taps) dback[v][m] = __builtin_fmaf(g, x_back(m), dback[v][m]);
                     }
+                    float s = edge ? more.get(v) : 0.f;
+#pragma unroll
+                    for (int m = 0; m < TAPS; m++)
+                        if (m < taps) s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz of row r + m
+                    out.set(v, edge && r >= at.len ? 0.f : s);
                 }
-                dz[v][TAPS - 1] = g;
-                float s = more.get(v);
-#pragma unroll
-                for (int m = 0; m < TAPS; m++)
-                    if (m < taps) s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz_(row + m)
-                out.set(v, row < at.len ? s : 0.f);
+                if (!edge || (t + u < end && r >= at.t0)) store(to + u * p.x_token, out, at.skip);
+                else if (t + u < end && r < 0 && wanted) store(dfirst + (long)(r + taps - 1) * p.C, out, at.skip);
             }
-            if (row >= at.t0) store(dx + row * p.x_token, out, at.skip);
-            else if (row < 0 && wanted) store(dfirst + (row + taps - 1) * p.C, out, at.skip);
-        }
+        };
+        const int inside = at.len < at.t1 ? at.len : at.t1;      // rows of the state after the last token come later
+        if (t + AHEAD <= inside && t - (TAPS - 1) >= at.t0) results(std::false_type());
+        else results(std::true_type());
+        to += AHEAD * p.x_token;
 #pragma unroll
-        for (int i = 0; i < TAPS - 1; i++) rows[i] = rows[kAheadBackward + i];
+        for (int i = 0; i < TAPS - 1; i++) {
+            if constexpr (TAPS - 1 <= AHEAD) window[i] = now[AHEAD - (TAPS - 1) + i];
+            else window[i] = i + AHEAD < TAPS - 1 ? window[i + AHEAD < TAPS - 1 ? i + AHEAD : 0] : now[i + AHEAD < TAPS - 1 ? 0 : i + AHEAD - (TAPS - 1)];
+        }
     }
     if (!p.part) return;
     float *part = p.part + (at.b * p.walks + at.walk) * (taps + 1) * p.C + at.c;

@@ -15,7 +15,8 @@ typedef int intx4 __attribute__((ext_vector_type(4)));
 typedef int intx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMostTerms = 131071;      // of 128 * 128 each: 2^31 - 2^14
-constexpr int kStage = 128;             // bytes of a row that a tile takes at once: 8 words of 16
+constexpr int kStage = 64;              // bytes of a row that a tile takes at once: 4 words of 16
+constexpr int kFewStage = 128;          // bytes of a row that a wavefront takes at once where tokens are few
 
 __device__ const intx4 kZeroWord = {0, 0, 0, 0};
 
@@ -27,7 +28,6 @@ struct product_params {
     int N, K;
     long x_row, w_row, y_row;
     int tiles_m, tiles_n;
-    bool wide;               // four neighbouring channels of y lie within one access
 };
 
 // 16 bytes of a row from k on, wherever they begin; zeros past its end.
@@ -48,16 +48,19 @@ template <int DT>
 __device__ __forceinline__ void put(const product_params &p, long m, int n, const int (&sum)[4], float xs) {
     typedef typename fc_elem<DT>::type E;
     E *y = (E *)p.y + m * p.y_row + n;
-    if (p.wide && n + 4 <= p.N) {
+    if (n + 4 <= p.N) {
+        float ws[4], bias[4] = {0.f, 0.f, 0.f, 0.f};
+        __builtin_memcpy(ws, p.w_scale + n, sizeof ws);
+        if (p.bias) __builtin_memcpy(bias, p.bias + n, sizeof bias);
         fc_vec<DT, 4> out;
 #pragma unroll
-        for (int i = 0; i < 4; i++) out.set(i, __builtin_fmaf((float)sum[i] * xs, p.w_scale[n + i], p.bias ? p.bias[n + i] : 0.f));
-        *(fc_vec<DT, 4> *)y = out;
+        for (int i = 0; i < 4; i++) out.set(i, p.bias ? __builtin_fmaf((float)sum[i] * xs, ws[i], bias[i]) : (float)sum[i] * xs * ws[i]);
+        __builtin_memcpy(y, &out, sizeof out);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (n + i < p.N) y[i] = (E)__builtin_fmaf((float)sum[i] * xs, p.w_scale[n + i], p.bias ? p.bias[n + i] : 0.f);
+        if (n + i < p.N) y[i] = (E)(p.bias ? __builtin_fmaf((float)sum[i] * xs, p.w_scale[n + i], p.bias[n + i]) : (float)sum[i] * xs * p.w_scale[n + i]);
 }
 
 // Few tokens.  Bound by w, read once: a workgroup takes 16 * NF channels and up to 16 * MF tokens, its wavefronts take 128 bytes of the rows
@@ -78,8 +81,8 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_few_kernel(const p
     for (int i = 0; i < MF; i++)
 #pragma unroll
         for (int j = 0; j < NF; j++) sum[i][j] = intx4{0, 0, 0, 0};
-    int k = wave * kStage;
-    for (; k + kStage <= p.K; k += WAVES * kStage) {
+    int k = wave * kFewStage;
+    for (; k + kFewStage <= p.K; k += WAVES * kFewStage) {
         intx4 a[2][NF], b[2][MF];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -125,14 +128,15 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_few_kernel(const p
     }
 }
 
-// Many tokens: tiles of BM tokens x BN channels, WM x WN wavefronts, stages of 128 bytes of the rows in LDS, two of them in turn.  Word c of a
-// stage's row lies at place c ^ (row / 2 % 8), so that 16 neighbouring rows' words of one k cover all banks.  DIRECT: rows begin on and are multiples of 16
-// bytes, which go to LDS without passing registers.
-template <int DT, int BM, int BN, int WM, int WN, bool DIRECT>
-__global__ __launch_bounds__(64 * WM * WN) void fc_int8_product_kernel(const product_params p) {
-    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MI = BM / WM / 32, NI = BN / WN / 32, WORDS = (BM + BN) * 8, EACH = WORDS / THREADS;
-    extern __shared__ intx4 lds[];      // [2][BN + BM rows][8]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Many tokens: tiles of BM tokens x BN channels, WM x WN wavefronts, stages of 64 bytes of the rows in LDS, read two stages before they are ready and one
+// more before they are used, so that a wavefront's first operands of a stage arrive under the products of the one before.  Word c of a stage's row lies
+// at place c ^ (row / 4 % 4): 16 neighbouring rows' words of one k cover all banks.  DIRECT: rows begin on and are multiples of 16 bytes, which go to
+// LDS without passing registers.
+template <int DT, int BM, int BN, int WM, int WN, int BUFFERS, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) void fc_int8_product_kernel(const product_params p) {
+    constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MI = BM / WM / 32, NI = BN / WN / 32, WORDS = (BM + BN) * 4, EACH = WORDS / THREADS;
+    extern __shared__ intx4 lds[];      // [BUFFERS][BN + BM rows][4]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // tiles in bands of eight rows of tiles, column by column, each XCD (workgroups are dealt to eight in turn) a contiguous part of them
     const unsigned tiles = gridDim.x, per = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8;
     const unsigned id = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
@@ -141,90 +145,187 @@ __global__ __launch_bounds__(64 * WM * WN) void fc_int8_product_kernel(const pro
     const long m0 = (long)(band * 8 + in_band % height) * BM;
     const int n0 = (int)(in_band / height) * BN;
 
-    // word i of a stage: row i / 8 (those of w first), place i % 8
-    const int8_t *from[EACH];
-    int k_of[EACH];
+    // word i of a stage: row i / 4 (those of w first), place i % 4.  DIRECT: 32-bit offsets from where the tile begins, which moves on with the stages.
+    const int k_of = ((lane & 3) ^ (lane >> 4 & 3)) * 16;      // rows of an access begin at a multiple of 16
+    const int8_t *const w_tile = p.w + n0 * p.w_row, *const x_tile = p.x + m0 * p.x_row;
+    uint32_t off[DIRECT ? EACH : 1];
+    const int8_t *from[DIRECT ? 1 : EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
-        const int i = (e * WAVES + wave) * 64 + lane, row = i >> 3;
-        k_of[e] = ((i & 7) ^ (row >> 1 & 7)) * 16;
-        if (row < BN) from[e] = p.w + (n0 + row < p.N ? n0 + row : p.N - 1) * p.w_row + k_of[e];
-        else from[e] = p.x + (m0 + row - BN < p.M ? m0 + row - BN : p.M - 1) * p.x_row + k_of[e];
+        const int row = ((e * WAVES + wave) * 64 + lane) >> 2;
+        const bool of_w = e * WAVES * 16 < BN;      // of the whole access: BN is a multiple of its rows
+        const long at = of_w ? n0 + row < p.N ? row : p.N - 1 - n0 : m0 + row - BN < p.M ? row - BN : p.M - 1 - m0;
+        if constexpr (DIRECT) off[e] = (uint32_t)(at * (of_w ? p.w_row : p.x_row)) + k_of;
+        else from[e] = (of_w ? w_tile + at * p.w_row : x_tile + at * p.x_row) + k_of;
     }
+    static_assert(BN % (16 * WAVES) == 0);
+    const int stages = (p.K + kStage - 1) / kStage;
     intx4 held[DIRECT ? 1 : EACH];
-    auto fetch = [&](int k, int buf) __attribute__((always_inline)) {
+    auto fetch = [&](int s, auto whole) __attribute__((always_inline)) {      // whole: the stage is known to be there, all of it
+        const int k = s * kStage;
+        if constexpr (DIRECT) {
+            intx4 *to = lds + (s % BUFFERS) * WORDS + wave * 64;
+            const int8_t *w = uniform_ptr(w_tile + k), *x = uniform_ptr(x_tile + k);
 #pragma unroll
-        for (int e = 0; e < EACH; e++) {
-            if constexpr (DIRECT) {
-                const void *at = k + k_of[e] < p.K ? (const void *)(from[e] + k) : (const void *)&kZeroWord;
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at,
-                                                 (__attribute__((address_space(3))) void *)(lds + buf * WORDS + (e * WAVES + wave) * 64), 16, 0, 0);
-            } else {
-                held[e] = row_word(from[e] - k_of[e], k + k_of[e], p.K);
+            for (int e = 0; e < EACH; e++) {
+                const void *at = (e * WAVES * 16 < BN ? w : x) + off[e];
+                if (!whole && k + k_of >= p.K) at = &kZeroWord;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at, (__attribute__((address_space(3))) void *)(to + e * THREADS),
+                                                 16, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                if (whole || k + kStage <= p.K) __builtin_memcpy(&held[e], from[e] + k, 16);
+                else held[e] = row_word(from[e] - k_of, k + k_of, p.K);
             }
         }
     };
-    auto store = [&](int buf) __attribute__((always_inline)) {
+    auto store = [&](int s) __attribute__((always_inline)) {
         if constexpr (!DIRECT) {
 #pragma unroll
-            for (int e = 0; e < EACH; e++) lds[buf * WORDS + (e * WAVES + wave) * 64 + lane] = held[e];
+            for (int e = 0; e < EACH; e++) lds[(s % BUFFERS) * WORDS + e * THREADS + wave * 64 + lane] = held[e];
         }
+    };
+    // This wavefront's words are in LDS but for those of `later` stages; then everybody's are, and everybody has read the stage before the last.  In one block of
+    // assembly: a fence would wait for all loads on their way.
+    auto ready = [&](bool later) __attribute__((always_inline)) {
+        if (DIRECT && BUFFERS > 3 && later) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((BUFFERS - 3) * EACH) : "memory");
+        else if (DIRECT) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
     intx16 sum[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; i++)
 #pragma unroll
         for (int j = 0; j < NI; j++) sum[i][j] = intx16{};
-    const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5, turn = r >> 1 & 7;
-    const int a_row = wn * (BN / WN) + r, b_row = BN + wm * (BM / WM) + r;
-    fetch(0, 0);
+    const int wm = wave / WN, wn = wave % WN, r = lane & 31, half = lane >> 5, turn = r >> 2 & 3;
+    const int a_row = (wn * (BN / WN) + r) * 4, b_row = (BN + wm * (BM / WM) + r) * 4;
+    intx4 a[2][NI], b[2][MI];
+    auto operands = [&](int s, int kk) __attribute__((always_inline)) {
+        const intx4 *at = lds + (s % BUFFERS) * WORDS + ((2 * kk + half) ^ turn);
+#pragma unroll
+        for (int j = 0; j < NI; j++) a[kk][j] = at[a_row + 128 * j];
+#pragma unroll
+        for (int i = 0; i < MI; i++) b[kk][i] = at[b_row + 128 * i];
+    };
+    auto products = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+            for (int j = 0; j < NI; j++) sum[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[kk][j], b[kk][i], sum[i][j], 0, 0, 0);
+    };
+    // stage s is in use, s + 1 ready, the others on their way; without DIRECT, s + 2 in registers
+    constexpr int AHEAD = DIRECT ? BUFFERS - 1 : 2;
+    const std::false_type some;
+    const std::true_type all;
+    fetch(0, some);
     store(0);
-    const int stages = (p.K + kStage - 1) / kStage;
-    for (int s = 0; s < stages; s++) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this wavefront's words of the stage are in LDS
-        __syncthreads();
-        if (s + 1 < stages) fetch((s + 1) * kStage, (s + 1) & 1);
-        const intx4 *at = lds + (s & 1) * WORDS;
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            const int place = (2 * kk + half) ^ turn;
-            intx4 a[NI], b[MI];
-#pragma unroll
-            for (int j = 0; j < NI; j++) a[j] = at[(a_row + 32 * j) * 8 + place];
-#pragma unroll
-            for (int i = 0; i < MI; i++) b[i] = at[(b_row + 32 * i) * 8 + place];
-#pragma unroll
-            for (int i = 0; i < MI; i++)
-#pragma unroll
-                for (int j = 0; j < NI; j++) sum[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[j], b[i], sum[i][j], 0, 0, 0);
-        }
-        if (s + 1 < stages) store((s + 1) & 1);
+    if (1 < stages) fetch(1, some);
+    if (1 < stages) store(1);
+    if (AHEAD > 2 || !DIRECT)
+        if (2 < stages) fetch(2, some);
+    ready(false);
+    operands(0, 0);
+    int s = 0;
+    if (AHEAD < stages && DIRECT) fetch(AHEAD, some);
+    operands(0, 1);
+    products(0);
+    if (1 < stages) operands(1, 0);
+    products(1);
+    for (s = 1; s + AHEAD < stages - 1; s++) {      // the last stage may not be whole
+        store(s + 1);
+        ready(true);      // stage s + 1
+        fetch(s + AHEAD, all);
+        operands(s, 1);
+        products(0);
+        operands(s + 1, 0);
+        products(1);
     }
+    for (; s < stages; s++) {
+        if (s + 1 < stages) store(s + 1);
+        ready(s + 2 < stages);
+        if (s + AHEAD < stages) fetch(s + AHEAD, some);
+        operands(s, 1);
+        products(0);
+        if (s + 1 < stages) operands(s + 1, 0);
+        products(1);
+    }
+    // A lane has one token and, of every eight channels, four neighbours.  They are laid out as rows in LDS, 32 tokens of the wavefront at a time, and leave in
+    // whole lines.
+    typedef typename fc_elem<DT>::type E;
+    constexpr int VEC = 16 / (int)sizeof(E), COLS = BN / WN, PITCH = COLS * (int)sizeof(E) + 16, PER_ROW = COLS / VEC, AT_ONCE = 64 / PER_ROW;
+    static_assert(WAVES * 32 * PITCH <= BUFFERS * WORDS * 16);
+    const int n_wave = n0 + wn * COLS;
+    float ws[NI][4][4], bias[NI][4][4];
+#pragma unroll
+    for (int j = 0; j < NI; j++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int n = n_wave + 32 * j + 8 * g + 4 * half;
+            if (n0 + BN <= p.N) {
+                __builtin_memcpy(ws[j][g], p.w_scale + n, 16);
+                if (p.bias) __builtin_memcpy(bias[j][g], p.bias + n, 16);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const int at = n + v < p.N ? n + v : p.N - 1;
+                    ws[j][g][v] = p.w_scale[at];
+                    if (p.bias) bias[j][g][v] = p.bias[at];
+                }
+            }
+        }
+    float xs[MI];
 #pragma unroll
     for (int i = 0; i < MI; i++) {
         const long m = m0 + wm * (BM / WM) + 32 * i + r;
-        if (m >= p.M) continue;
-        const float xs = p.x_scale[m];
+        xs[i] = p.x_scale[m < p.M ? m : p.M - 1];
+    }
+    __syncthreads();      // everybody's operands are read
+    char *mine = (char *)lds + wave * 32 * PITCH;
+    const int row = lane / PER_ROW, col = lane % PER_ROW * VEC;
+#pragma unroll
+    for (int i = 0; i < MI; i++) {
 #pragma unroll
         for (int j = 0; j < NI; j++)
 #pragma unroll
             for (int g = 0; g < 4; g++) {
-                const int n = n0 + wn * (BN / WN) + 32 * j + 8 * g + 4 * half;
-                const int four[4] = {sum[i][j][4 * g], sum[i][j][4 * g + 1], sum[i][j][4 * g + 2], sum[i][j][4 * g + 3]};
-                if (n < p.N) put<DT>(p, m, n, four, xs);
+                fc_vec<DT, 4> out;
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const float product = (float)sum[i][j][4 * g + v] * xs[i];
+                    out.set(v, p.bias ? __builtin_fmaf(product, ws[j][g][v], bias[j][g][v]) : product * ws[j][g][v]);
+                }
+                *(fc_vec<DT, 4> *)(mine + r * PITCH + (32 * j + 8 * g + 4 * half) * sizeof(E)) = out;
             }
+        fc_wave_sync();
+#pragma unroll
+        for (int k = 0; k < 32 / AT_ONCE; k++) {
+            const fc_vec<DT, VEC> out = *(const fc_vec<DT, VEC> *)(mine + (row + k * AT_ONCE) * PITCH + col * sizeof(E));
+            const long m = m0 + wm * (BM / WM) + 32 * i + row + k * AT_ONCE;
+            if (m >= p.M) continue;
+            E *to = (E *)p.y + m * p.y_row + n_wave + col;
+            if (n_wave + col + VEC <= p.N) {
+                __builtin_memcpy(to, &out, 16);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VEC; v++)
+                    if (n_wave + col + v < p.N) to[v] = out.v[v];
+            }
+        }
+        fc_wave_sync();
     }
 }
 
 int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
 
-template <int DT, int BM, int BN, int WM, int WN>
-int run_tiles(fc_context *ctx, product_params &p, bool direct) {
+template <int DT, int BM, int BN, int WM, int WN, int BUFFERS>
+int run_tiles(fc_context *ctx, product_params p, bool direct) {
     p.tiles_m = (int)((p.M + BM - 1) / BM);
     p.tiles_n = (p.N + BN - 1) / BN;
-    constexpr size_t lds = 2 * (BM + BN) * kStage;
+    constexpr size_t lds = BUFFERS * (BM + BN) * kStage;
     const dim3 grid((unsigned)((long)p.tiles_m * p.tiles_n)), threads(64 * WM * WN);
-    const auto kernel = direct ? fc_int8_product_kernel<DT, BM, BN, WM, WN, true> : fc_int8_product_kernel<DT, BM, BN, WM, WN, false>;
+    const auto kernel = direct ? fc_int8_product_kernel<DT, BM, BN, WM, WN, BUFFERS, true> : fc_int8_product_kernel<DT, BM, BN, WM, WN, BUFFERS, false>;
     if (lds > 65536) FC_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     kernel<<<grid, threads, lds, ctx->stream>>>(p);
     FC_LAUNCH_CHECK(ctx, "fc_int8_product_kernel");
@@ -247,9 +348,9 @@ int run(fc_context *ctx, product_params &p, int tile, bool direct) {
         if (p.M <= 32) return run_few<DT, 2>(ctx, p);
         return run_few<DT, 4>(ctx, p);
     }
-    if (tile == 256) return run_tiles<DT, 256, 256, 2, 4>(ctx, p, direct);
-    if (tile == 128) return run_tiles<DT, 128, 128, 2, 2>(ctx, p, direct);
-    return run_tiles<DT, 64, 64, 2, 2>(ctx, p, direct);
+    if (tile == 256) return run_tiles<DT, 256, 256, 2, 4, 4>(ctx, p, direct);
+    if (tile == 128) return run_tiles<DT, 128, 128, 2, 2, 4>(ctx, p, direct);
+    return run_tiles<DT, 64, 64, 2, 2, 4>(ctx, p, direct);
 }
 
 bool same(const fc_int8_product_plan &a, const fc_int8_product_plan &b) {
@@ -284,8 +385,8 @@ extern "C" int fc_int8_product(fc_context *ctx, const fc_int8_product_plan *plan
     product_params p = {};
     p.x = x_dev; p.w = w_dev; p.x_scale = x_scale_dev; p.w_scale = w_scale_dev; p.bias = bias_dev; p.y = y_dev;
     p.M = s.M; p.N = s.N; p.K = s.K; p.x_row = s.x_row; p.w_row = s.w_row; p.y_row = s.y_row;
-    p.wide = ((s.N | s.y_row) & 3) == 0 && ((uint64_t)y_dev & (4 * fc_elem_size(s.dtype) - 1)) == 0;
-    const bool direct = ((s.K | s.x_row | s.w_row) & 15) == 0 && (((uint64_t)x_dev | (uint64_t)w_dev) & 15) == 0;
+    // a tile's offsets are 32 bits
+    const bool direct = ((s.K | s.x_row | s.w_row) & 15) == 0 && (((uint64_t)x_dev | (uint64_t)w_dev) & 15) == 0 && (s.x_row | s.w_row) < (1l << 23);
     const fc_device_scope on(ctx);
     if (s.dtype == FC_F32) return run<FC_F32>(ctx, p, plan->tile, direct);
     if (s.dtype == FC_BF16) return run<FC_BF16>(ctx, p, plan->tile, direct);
