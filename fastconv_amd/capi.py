@@ -126,7 +126,7 @@ class Int8ProductShape(C.Structure):
 
 
 class Int8ProductPlan(C.Structure):
-    _fields_ = [("shape", Int8ProductShape), ("tile", C.c_int), ("ws_bytes", C.c_size_t)]
+    _fields_ = [("shape", Int8ProductShape), ("tile", C.c_int), ("parts", C.c_int), ("ws_bytes", C.c_size_t)]
 
 
 class CausalConvShape(C.Structure):

@@ -5,6 +5,8 @@
 // Sums are 32-bit integers, exact up to 131071 terms whatever their order, so every kernel here gives the same bits.  x and w are rows of k: 16 bytes of a
 // row are a lane's operand of v_mfma_i32_16x16x64_i8 and v_mfma_i32_32x32x32_i8 as they lie.  w is the first operand: a lane then holds four
 // neighbouring channels of one token.
+#include <math.h>
+
 #include <type_traits>
 
 #include "token_types.h"
@@ -28,6 +30,8 @@ struct product_params {
     int N, K;
     long x_row, w_row, y_row;
     int tiles_m, tiles_n;
+    int *parts_at;           // [parts][M][N], where the reduction is cut
+    int part;                // bytes of a row that a part takes
 };
 
 // 16 bytes of a row from k on, wherever they begin; zeros past its end.
@@ -35,12 +39,29 @@ __device__ __forceinline__ intx4 row_word(const int8_t *row, int k, int K) {
     intx4 v = {0, 0, 0, 0};
     if (k + 16 <= K) {
         __builtin_memcpy(&v, row + k, 16);
+    } else if (k < K && K >= 16) {      // the row's last 16, moved down
+        unsigned __int128 last;
+        __builtin_memcpy(&last, row + K - 16, 16);
+        last >>= 8 * (k + 16 - K);
+        __builtin_memcpy(&v, &last, 16);
     } else if (k < K) {
         unsigned u[4] = {0, 0, 0, 0};
         for (int i = 0; i < K - k; i++) u[i >> 2] |= (unsigned)(uint8_t)row[k + i] << (8 * (i & 3));
         v = {(int)u[0], (int)u[1], (int)u[2], (int)u[3]};
     }
     return v;
+}
+
+// Four neighbours of a part's sums.
+__device__ __forceinline__ void put_part(const product_params &p, long m, int n, intx4 sum) {
+    int *to = p.parts_at + ((long)blockIdx.z * p.M + m) * p.N + n;
+    if (n + 4 <= p.N) {
+        __builtin_memcpy(to, &sum, 16);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (n + i < p.N) to[i] = sum[i];
 }
 
 // Four neighbouring channels, from n on, of token m.
@@ -72,40 +93,56 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_few_kernel(const p
     const int n0 = blockIdx.x * 16 * NF;
     const long m0 = (long)blockIdx.y * 16 * MF;
     const int8_t *w[NF], *x[MF];
+    const int k0 = blockIdx.z * p.part, K = p.K - k0 < p.part ? p.K - k0 : p.part;
 #pragma unroll
-    for (int f = 0; f < NF; f++) w[f] = p.w + (n0 + 16 * f + r < p.N ? n0 + 16 * f + r : p.N - 1) * p.w_row;
+    for (int f = 0; f < NF; f++) w[f] = p.w + k0 + (n0 + 16 * f + r < p.N ? n0 + 16 * f + r : p.N - 1) * p.w_row;
 #pragma unroll
-    for (int f = 0; f < MF; f++) x[f] = p.x + (m0 + 16 * f + r < p.M ? m0 + 16 * f + r : p.M - 1) * p.x_row;
+    for (int f = 0; f < MF; f++) x[f] = p.x + k0 + (m0 + 16 * f + r < p.M ? m0 + 16 * f + r : p.M - 1) * p.x_row;
     intx4 sum[MF][NF];
 #pragma unroll
     for (int i = 0; i < MF; i++)
 #pragma unroll
         for (int j = 0; j < NF; j++) sum[i][j] = intx4{0, 0, 0, 0};
-    int k = wave * kFewStage;
-    for (; k + kFewStage <= p.K; k += WAVES * kFewStage) {
-        intx4 a[2][NF], b[2][MF];
+    // two steps' operands in registers: one is on its way while the other is used
+    intx4 a[2][2][NF], b[2][2][MF];
+    auto read = [&](int k, int turn) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
-            for (int f = 0; f < NF; f++) __builtin_memcpy(&a[h][f], w[f] + k + 64 * h + 16 * q, 16);
+            for (int f = 0; f < NF; f++) __builtin_memcpy(&a[turn][h][f], w[f] + k + 64 * h + 16 * q, 16);
 #pragma unroll
-            for (int f = 0; f < MF; f++) __builtin_memcpy(&b[h][f], x[f] + k + 64 * h + 16 * q, 16);
+            for (int f = 0; f < MF; f++) __builtin_memcpy(&b[turn][h][f], x[f] + k + 64 * h + 16 * q, 16);
         }
+    };
+    auto use = [&](int turn) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int i = 0; i < MF; i++)
 #pragma unroll
-                for (int j = 0; j < NF; j++) sum[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h][j], b[h][i], sum[i][j], 0, 0, 0);
+                for (int j = 0; j < NF; j++) sum[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[turn][h][j], b[turn][h][i], sum[i][j], 0, 0, 0);
+    };
+    constexpr int STEP = WAVES * kFewStage;
+    int k = wave * kFewStage;
+    if (k + kFewStage <= K) read(k, 0);
+    for (; k + STEP + kFewStage <= K; k += 2 * STEP) {
+        read(k + STEP, 1);
+        use(0);
+        if (k + 2 * STEP + kFewStage <= K) read(k + 2 * STEP, 0);
+        use(1);
     }
-    if (k < p.K) {      // the last bytes
+    if (k + kFewStage <= K) {
+        use(0);
+        k += STEP;
+    }
+    if (k < K) {      // the last bytes
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             intx4 a[NF], b[MF];
 #pragma unroll
-            for (int f = 0; f < NF; f++) a[f] = row_word(w[f], k + 64 * h + 16 * q, p.K);
+            for (int f = 0; f < NF; f++) a[f] = row_word(w[f], k + 64 * h + 16 * q, K);
 #pragma unroll
-            for (int f = 0; f < MF; f++) b[f] = row_word(x[f], k + 64 * h + 16 * q, p.K);
+            for (int f = 0; f < MF; f++) b[f] = row_word(x[f], k + 64 * h + 16 * q, K);
 #pragma unroll
             for (int i = 0; i < MF; i++)
 #pragma unroll
@@ -124,7 +161,9 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_few_kernel(const p
         // column of the product: token; four rows: channels
         const long m = m0 + 16 * (f / NF) + r;
         const int n = n0 + 16 * (f % NF) + 4 * q, four[4] = {s[0], s[1], s[2], s[3]};
-        if (m < p.M && n < p.N) put<DT>(p, m, n, four, p.x_scale[m]);
+        if (m >= p.M || n >= p.N) continue;
+        if (p.parts_at) put_part(p, m, n, s);
+        else put<DT>(p, m, n, four, p.x_scale[m]);
     }
 }
 
@@ -147,7 +186,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
 
     // word i of a stage: row i / 4 (those of w first), place i % 4.  DIRECT: 32-bit offsets from where the tile begins, which moves on with the stages.
     const int k_of = ((lane & 3) ^ (lane >> 4 & 3)) * 16;      // rows of an access begin at a multiple of 16
-    const int8_t *const w_tile = p.w + n0 * p.w_row, *const x_tile = p.x + m0 * p.x_row;
+    const int k0 = blockIdx.z * p.part, K = p.K - k0 < p.part ? p.K - k0 : p.part;
+    const int8_t *const w_tile = p.w + n0 * p.w_row + k0, *const x_tile = p.x + m0 * p.x_row + k0;
     uint32_t off[DIRECT ? EACH : 1];
     const int8_t *from[DIRECT ? 1 : EACH];
 #pragma unroll
@@ -159,7 +199,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
         else from[e] = (of_w ? w_tile + at * p.w_row : x_tile + at * p.x_row) + k_of;
     }
     static_assert(BN % (16 * WAVES) == 0);
-    const int stages = (p.K + kStage - 1) / kStage;
+    const int stages = (K + kStage - 1) / kStage;
     intx4 held[DIRECT ? 1 : EACH];
     auto fetch = [&](int s, auto whole) __attribute__((always_inline)) {      // whole: the stage is known to be there, all of it
         const int k = s * kStage;
@@ -169,15 +209,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
                 const void *at = (e * WAVES * 16 < BN ? w : x) + off[e];
-                if (!whole && k + k_of >= p.K) at = &kZeroWord;
+                if (!whole && k + k_of >= K) at = &kZeroWord;
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at, (__attribute__((address_space(3))) void *)(to + e * THREADS),
                                                  16, 0, 0);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
-                if (whole || k + kStage <= p.K) __builtin_memcpy(&held[e], from[e] + k, 16);
-                else held[e] = row_word(from[e] - k_of, k + k_of, p.K);
+                if (whole || k + kStage <= K) __builtin_memcpy(&held[e], from[e] + k, 16);
+                else held[e] = row_word(from[e] - k_of, k + k_of, K);
             }
         }
     };
@@ -253,6 +293,21 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
     }
     // A lane has one token and, of every eight channels, four neighbours.  They are laid out as rows in LDS, 32 tokens of the wavefront at a time, and leave in
     // whole lines.
+    if (p.parts_at) {
+#pragma unroll
+        for (int i = 0; i < MI; i++) {
+            const long m = m0 + wm * (BM / WM) + 32 * i + r;
+#pragma unroll
+            for (int j = 0; j < NI; j++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int n = n0 + wn * (BN / WN) + 32 * j + 8 * g + 4 * half;
+                    const intx4 four = {sum[i][j][4 * g], sum[i][j][4 * g + 1], sum[i][j][4 * g + 2], sum[i][j][4 * g + 3]};
+                    if (m < p.M && n < p.N) put_part(p, m, n, four);
+                }
+        }
+        return;
+    }
     typedef typename fc_elem<DT>::type E;
     constexpr int VEC = 16 / (int)sizeof(E), COLS = BN / WN, PITCH = COLS * (int)sizeof(E) + 16, PER_ROW = COLS / VEC, AT_ONCE = 64 / PER_ROW;
     static_assert(WAVES * 32 * PITCH <= BUFFERS * WORDS * 16);
@@ -317,14 +372,104 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
     }
 }
 
+// The parts' sums added up, scaled and stored, four channels a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void fc_int8_product_join_kernel(const product_params p, int parts) {
+    const int quads = (p.N + 3) / 4;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+    const int n = (int)(i - m * quads) * 4;
+    if (m >= p.M) return;
+    int four[4] = {0, 0, 0, 0};
+    const int *from = p.parts_at + m * p.N + n;
+    const long part = p.M * p.N;
+    for (int first = 0; first < parts; first += 4) {      // four on their way at once
+        int v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int *at = from + (first + k < parts ? first + k : 0) * part;
+            if (n + 4 <= p.N) {
+                __builtin_memcpy(v[k], at, 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[k][j] = at[n + j < p.N ? j : 0];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) four[j] += first + k < parts ? v[k][j] : 0;
+    }
+    put<DT>(p, m, n, four, p.x_scale[m]);
+}
+
 int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
 
+// What the rows of a plan run on.
+struct product_form {
+    int tile;                // tokens and channels of a workgroup's tile; 0: few tokens
+    int mf, nf;              // few tokens: blocks of 16 of a workgroup
+    int parts;               // of the reduction
+    double us;               // expected
+};
+
+long ceil_div(long a, long b) { return (a + b - 1) / b; }
+
+constexpr int kFewTokens = 64;
+constexpr long kUnits = 256;      // compute units
+
+// Few tokens.  Wide workgroups read x seldom, many read w side by side: the widest of which there is one a unit.  8192 channels of 4096, 64 tokens:
+// 64x32 14.1 us, 32x32 17.8, 16x32 24.7; 2048 channels 13.9, 9.8 and 7.9; 16 tokens of 8192 channels 16x32 8.2 and 16x16 10.1, of 4096 channels 6.7 and 5.1.
+product_form few_form(long M, int N, int K) {
+    const int forms[4][2] = {{4, 2}, {2, 2}, {1, 2}, {1, 1}};
+    product_form f = {};
+    for (const auto &v : forms) {
+        f.mf = v[0];
+        f.nf = v[1];
+        if (f.mf > 1 && M <= 8 * f.mf) continue;
+        if (ceil_div(M, 16 * f.mf) * ceil_div(N, 16 * f.nf) >= kUnits) break;
+    }
+    f.parts = 1;
+    return f;
+}
+
+// Tiles.  Times of a call in us by tiles a compute unit, c, and 1024 bytes of the reduction, k, fitted to products of 256 to 12288 rows.
+double tile_time(int tile, long M, int N, int K) {
+    const double tiles = (double)(ceil_div(M, tile) * ceil_div(N, tile)), c = tiles / kUnits, k = K / 1024.0;
+    if (tile == 64) return 3 + 0.4 * c + k * (c < 0.9 ? 2.2 : 2.4 * c);
+    if (tile == 128) return 3 + 2.4 * c + k * (c < 0.8 ? 4.2 : 5.2 * c);
+    return c > 1 ? ceil(c) * (10 + 14.5 * k) : 8 + 2 * c + k * (10 + 5 * c);
+}
+
+product_form best_tile(long M, int N, int K) {
+    product_form f = {};
+    f.parts = 1;
+    for (int tile : {64, 128, 256}) {
+        const double us = tile_time(tile, M, N, K);
+        if (!f.tile || us < f.us) {
+            f.tile = tile;
+            f.us = us;
+        }
+    }
+    return f;
+}
+
+// Workgroups that leave most of the chip idle cut a reduction of `least` bytes and more; adding the parts up is a launch more.  With and without: 1 token, 512
+// channels of 16384 6.9 and 10.9 us, of 2048 channels of 4096 7.0 and 4.9; 300 tokens, 520 channels of 8192 12.7 and 20.4; 200 tokens, 1000 channels of 4096
+// 10.2 and 12.2, of 2048 10.4 and 8.1.
+void cut(product_form &f, long workgroups, int K, int least) {
+    if (workgroups > kUnits / 4 || K < least) return;
+    long parts = kUnits / workgroups;
+    if (parts > K / 1024) parts = K / 1024;
+    const long part = ceil_div(ceil_div(K, parts), 128) * 128;
+    f.parts = (int)ceil_div(K, part);
+}
+
 template <int DT, int BM, int BN, int WM, int WN, int BUFFERS>
-int run_tiles(fc_context *ctx, product_params p, bool direct) {
+int run_tiles(fc_context *ctx, product_params p, int parts, bool direct) {
     p.tiles_m = (int)((p.M + BM - 1) / BM);
     p.tiles_n = (p.N + BN - 1) / BN;
     constexpr size_t lds = BUFFERS * (BM + BN) * kStage;
-    const dim3 grid((unsigned)((long)p.tiles_m * p.tiles_n)), threads(64 * WM * WN);
+    const dim3 grid((unsigned)((long)p.tiles_m * p.tiles_n), 1, (unsigned)parts), threads(64 * WM * WN);
     const auto kernel = direct ? fc_int8_product_kernel<DT, BM, BN, WM, WN, BUFFERS, true> : fc_int8_product_kernel<DT, BM, BN, WM, WN, BUFFERS, false>;
     if (lds > 65536) FC_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     kernel<<<grid, threads, lds, ctx->stream>>>(p);
@@ -332,31 +477,49 @@ int run_tiles(fc_context *ctx, product_params p, bool direct) {
     return FC_OK;
 }
 
-template <int DT, int MF>
-int run_few(fc_context *ctx, const product_params &p) {
-    constexpr int NF = 1, WAVES = 8;
-    fc_int8_product_few_kernel<DT, MF, NF, WAVES><<<dim3((unsigned)((p.N + 16 * NF - 1) / (16 * NF)), (unsigned)((p.M + 16 * MF - 1) / (16 * MF))),
-                                                    dim3(64 * WAVES), 0, ctx->stream>>>(p);
+template <int DT, int MF, int NF>
+int run_few(fc_context *ctx, const product_params &p, int parts) {
+    constexpr int WAVES = 8;
+    fc_int8_product_few_kernel<DT, MF, NF, WAVES><<<dim3((unsigned)ceil_div(p.N, 16 * NF), (unsigned)ceil_div(p.M, 16 * MF), (unsigned)parts), dim3(64 * WAVES), 0,
+                                                    ctx->stream>>>(p);
     FC_LAUNCH_CHECK(ctx, "fc_int8_product_few_kernel");
     return FC_OK;
 }
 
 template <int DT>
-int run(fc_context *ctx, product_params &p, int tile, bool direct) {
-    if (tile == 0) {
-        if (p.M <= 16) return run_few<DT, 1>(ctx, p);
-        if (p.M <= 32) return run_few<DT, 2>(ctx, p);
-        return run_few<DT, 4>(ctx, p);
+int run_form(fc_context *ctx, product_params p, const product_form &f, bool direct, void *ws) {
+    p.part = (int)(ceil_div(ceil_div(p.K, f.parts), 128) * 128);
+    p.parts_at = f.parts > 1 ? (int *)ws : nullptr;
+    int rc;
+    if (f.tile == 0)
+        rc = f.mf == 4 ? run_few<DT, 4, 2>(ctx, p, f.parts) : f.mf == 2 ? run_few<DT, 2, 2>(ctx, p, f.parts) : f.nf == 2 ? run_few<DT, 1, 2>(ctx, p, f.parts) : run_few<DT, 1, 1>(ctx, p, f.parts);
+    else
+        rc = f.tile == 256   ? run_tiles<DT, 256, 256, 2, 4, 4>(ctx, p, f.parts, direct)
+             : f.tile == 128 ? run_tiles<DT, 128, 128, 2, 2, 4>(ctx, p, f.parts, direct)
+                             : run_tiles<DT, 64, 64, 2, 2, 4>(ctx, p, f.parts, direct);
+    if (rc || f.parts == 1) return rc;
+    fc_int8_product_join_kernel<DT><<<dim3((unsigned)ceil_div(p.M * ((p.N + 3) / 4), 256)), dim3(256), 0, ctx->stream>>>(p, f.parts);
+    FC_LAUNCH_CHECK(ctx, "fc_int8_product_join_kernel");
+    return FC_OK;
+}
+
+template <int DT>
+int run(fc_context *ctx, const product_params &p, const fc_int8_product_plan *plan, bool direct, void *ws) {
+    if (p.M <= kFewTokens) {
+        product_form f = few_form(p.M, p.N, p.K);
+        f.parts = plan->parts;
+        return run_form<DT>(ctx, p, f, direct, ws);
     }
-    if (tile == 256) return run_tiles<DT, 256, 256, 2, 4, 4>(ctx, p, direct);
-    if (tile == 128) return run_tiles<DT, 128, 128, 2, 2, 4>(ctx, p, direct);
-    return run_tiles<DT, 64, 64, 2, 2, 4>(ctx, p, direct);
+    product_form f = {};
+    f.tile = plan->tile;
+    f.parts = plan->parts;
+    return run_form<DT>(ctx, p, f, direct, ws);
 }
 
 bool same(const fc_int8_product_plan &a, const fc_int8_product_plan &b) {
     const fc_int8_product_shape &s = a.shape, &t = b.shape;
     return s.M == t.M && s.N == t.N && s.K == t.K && s.dtype == t.dtype && s.x_row == t.x_row && s.w_row == t.w_row && s.y_row == t.y_row &&
-           a.tile == b.tile && a.ws_bytes == b.ws_bytes;
+           a.tile == b.tile && a.parts == b.parts && a.ws_bytes == b.ws_bytes;
 }
 
 }  // namespace
@@ -366,8 +529,17 @@ extern "C" int fc_int8_product_make_plan(const fc_int8_product_shape *s, fc_int8
     if (s->K > kMostTerms || s->M >= (1l << 31) || fc_count(s->M, s->N) >= (1l << 36)) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    auto tiles = [&](long side) { return (s->M + side - 1) / side * ((s->N + side - 1) / side); };
-    plan->tile = s->M <= 64 ? 0 : tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 64;
+    product_form f;
+    if (s->M <= kFewTokens) {
+        f = few_form(s->M, s->N, s->K);
+        cut(f, ceil_div(s->M, 16 * f.mf) * ceil_div(s->N, 16 * f.nf), s->K, 8192);
+    } else {
+        f = best_tile(s->M, s->N, s->K);
+        cut(f, ceil_div(s->M, f.tile) * ceil_div(s->N, f.tile), s->K, 4096);
+    }
+    plan->tile = f.tile;
+    plan->parts = f.parts;
+    plan->ws_bytes = f.parts > 1 ? (size_t)f.parts * s->M * s->N * sizeof(int) : 0;
     return FC_OK;
 }
 
@@ -388,7 +560,7 @@ extern "C" int fc_int8_product(fc_context *ctx, const fc_int8_product_plan *plan
     // a tile's offsets are 32 bits
     const bool direct = ((s.K | s.x_row | s.w_row) & 15) == 0 && (((uint64_t)x_dev | (uint64_t)w_dev) & 15) == 0 && (s.x_row | s.w_row) < (1l << 23);
     const fc_device_scope on(ctx);
-    if (s.dtype == FC_F32) return run<FC_F32>(ctx, p, plan->tile, direct);
-    if (s.dtype == FC_BF16) return run<FC_BF16>(ctx, p, plan->tile, direct);
-    return run<FC_F16>(ctx, p, plan->tile, direct);
+    if (s.dtype == FC_F32) return run<FC_F32>(ctx, p, plan, direct, ws_dev);
+    if (s.dtype == FC_BF16) return run<FC_BF16>(ctx, p, plan, direct, ws_dev);
+    return run<FC_F16>(ctx, p, plan, direct, ws_dev);
 }

@@ -628,6 +628,7 @@ typedef struct {
 typedef struct {
     fc_int8_product_shape shape;
     int tile;                 /* tokens and channels that a workgroup takes; 0: few tokens, w read straight into registers */
+    int parts;                /* of the reduction, summed up afterwards */
     size_t ws_bytes;          /* workspace, 0 if none */
 } fc_int8_product_plan;
 
