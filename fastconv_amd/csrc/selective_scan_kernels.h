@@ -356,64 +356,93 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
     }
 }
 
-// A few tokens of many sequences, L lanes a channel without LDS.  Bound by the states, read and written once a call.
-template <int DT, int L, bool GATE>
-__global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_scan_run r) {
+// A few tokens of many sequences, L lanes a channel without LDS.  Bound by the states, read and written once a call; what belongs to a channel is read once for
+// SEQUENCES of them, whose loads are on their way together.
+template <int DT, int L, bool GATE, int SEQUENCES>
+__global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_scan_run r, unsigned across) {      // workgroups for all channels
     typedef typename fc_elem<DT>::type E;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x, row = i / L;
-    const int sg = threadIdx.x % L;
-    const long b = row / r.channels;
-    const int d = (int)(row - b * r.channels);
-    if (b >= r.B) return;
-    const int group = d / r.per_group, n0 = sg * kScanStates;
-    const long len = fc_scan_length(r, b);
-    float rate[kScanStates], h[kScanStates];
-    const bool wide = (r.N & 3) == 0 && (((uintptr_t)r.A | (uintptr_t)r.state_in | (uintptr_t)r.state_out) & 15) == 0;
-    const float *A = r.A + (long)d * r.N + n0, *from = r.state_in + row * r.N + n0;
-    float *to = r.state_out + row * r.N + n0;
-    if (wide) {
-        const bool some = n0 < r.N;
-        const float4 zeros = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = some ? *(const float4 *)A : zeros, s = some && r.state_in ? *(const float4 *)from : zeros;
-        rate[0] = a.x; rate[1] = a.y; rate[2] = a.z; rate[3] = a.w;
-        h[0] = s.x; h[1] = s.y; h[2] = s.z; h[3] = s.w;
-    } else {
+    typedef fc_vec<DT, kScanStates> V;
+    const long at = (long)(blockIdx.x % across) * 256 + threadIdx.x;
+    const int d = (int)(at / L), sg = threadIdx.x % L, n0 = sg * kScanStates;
+    if (d >= r.channels) return;
+    const int group = d / r.per_group;
+    // a lane's four states, or those that there are
+    const bool whole = n0 + kScanStates <= r.N;
+    float rate[kScanStates];
+    if (whole) __builtin_memcpy(rate, r.A + (long)d * r.N + n0, sizeof rate);
+    else
 #pragma unroll
-        for (int j = 0; j < kScanStates; j++) {
-            const bool some = n0 + j < r.N;
-            rate[j] = some ? A[j] : 0.f;
-            h[j] = some && r.state_in ? from[j] : 0.f;
-        }
-    }
+        for (int j = 0; j < kScanStates; j++) rate[j] = n0 + j < r.N ? r.A[(long)d * r.N + n0 + j] : 0.f;
 #pragma unroll
     for (int j = 0; j < kScanStates; j++) rate[j] = fc_scan_rate(rate[j]);
     const float bias = r.delta_bias ? r.delta_bias[d] : 0.f, skip = r.D ? r.D[d] : 0.f;
-    const E *pb = (const E *)r.b + b * r.b_batch + group * r.b_group + n0, *pc = (const E *)r.c + b * r.c_batch + group * r.c_group + n0;
-    E *y = (E *)r.y + b * r.y_batch + d;
-    for (long t = 0; t < len; t++) {
-        const float x = (float)((const E *)r.x)[b * r.x_batch + t * r.x_token + d];
-        const float dt = step_of<DT>(r, (float)((const E *)r.delta)[b * r.delta_batch + t * r.delta_token + d] + bias);
-        const float u = dt * x;
-        float s = 0.f;
+    const int first = (int)(blockIdx.x / across) * SEQUENCES;
+    float h[SEQUENCES][kScanStates];
+    long len[SEQUENCES];
 #pragma unroll
-        for (int j = 0; j < kScanStates; j++) {
-            if (n0 + j >= r.N) continue;
-            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * rate[j]), h[j], u * (float)pb[t * r.b_token + j]);
-            s = __builtin_fmaf((float)pc[t * r.c_token + j], h[j], s);
+    for (int s = 0; s < SEQUENCES; s++) {
+        const long b = first + s < r.B ? first + s : r.B - 1;
+        len[s] = first + s < r.B ? fc_scan_length(r, b) : 0;
+        const float *from = r.state_in + (b * r.channels + d) * r.N + n0;
+#pragma unroll
+        for (int j = 0; j < kScanStates; j++) h[s][j] = 0.f;
+        if (r.state_in && whole) {
+            __builtin_memcpy(h[s], from, sizeof h[s]);
+        } else if (r.state_in) {
+#pragma unroll
+            for (int j = 0; j < kScanStates; j++)
+                if (n0 + j < r.N) h[s][j] = from[j];
         }
-        s = __builtin_fmaf(skip, x, sum_states<L>(s));
-        if (GATE) s *= fc_silu((float)((const E *)r.z)[b * r.z_batch + t * r.z_token + d]);
-        if (sg == 0) y[t * r.y_token] = (E)s;
     }
-    if (sg == 0)
-        for (long t = len; t < r.T; t++) y[t * r.y_token] = (E)0.f;
-    if (!r.state_out) return;
-    if (wide) {
-        if (n0 < r.N) *(float4 *)to = make_float4(h[0], h[1], h[2], h[3]);
-    } else {
+    for (long t = 0; t < r.T; t++) {
+        E x[SEQUENCES], delta[SEQUENCES], z[SEQUENCES];
+        V B[SEQUENCES], C[SEQUENCES];
 #pragma unroll
-        for (int j = 0; j < kScanStates; j++)
-            if (n0 + j < r.N) to[j] = h[j];
+        for (int s = 0; s < SEQUENCES; s++) {      // a token past the end is read where the first lies, and moves nothing
+            const long b = first + s < r.B ? first + s : r.B - 1, u = t < len[s] ? t : 0;
+            x[s] = ((const E *)r.x)[b * r.x_batch + u * r.x_token + d];
+            delta[s] = ((const E *)r.delta)[b * r.delta_batch + u * r.delta_token + d];
+            if (GATE) z[s] = ((const E *)r.z)[b * r.z_batch + u * r.z_token + d];
+            const E *pb = (const E *)r.b + b * r.b_batch + u * r.b_token + group * r.b_group, *pc = (const E *)r.c + b * r.c_batch + u * r.c_token + group * r.c_group;
+            if (whole) {
+                __builtin_memcpy(&B[s], pb + n0, sizeof(V));
+                __builtin_memcpy(&C[s], pc + n0, sizeof(V));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kScanStates; j++) {
+                    B[s].v[j] = n0 + j < r.N ? pb[n0 + j] : (E)0.f;
+                    C[s].v[j] = n0 + j < r.N ? pc[n0 + j] : (E)0.f;
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < SEQUENCES; s++) {
+            const bool there = t < len[s];
+            const float v = (float)x[s], dt = step_of<DT>(r, (float)delta[s] + bias), u = dt * v;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < kScanStates; j++) {
+                const float now = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * rate[j]), h[s][j], u * B[s].get(j));
+                h[s][j] = there ? now : h[s][j];
+                sum = __builtin_fmaf(C[s].get(j), now, sum);
+            }
+            sum = __builtin_fmaf(skip, v, sum_states<L>(sum));
+            if (GATE) sum *= fc_silu((float)z[s]);
+            if (sg == 0 && first + s < r.B) ((E *)r.y)[(first + s) * r.y_batch + t * r.y_token + d] = (E)(there ? sum : 0.f);
+        }
+    }
+    if (!r.state_out) return;
+#pragma unroll
+    for (int s = 0; s < SEQUENCES; s++) {
+        if (first + s >= r.B) break;
+        float *to = r.state_out + ((long)(first + s) * r.channels + d) * r.N + n0;
+        if (whole) {
+            __builtin_memcpy(to, h[s], sizeof h[s]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kScanStates; j++)
+                if (n0 + j < r.N) to[j] = h[s][j];
+        }
     }
 }
 
@@ -646,12 +675,22 @@ int scan_ends(fc_context *ctx, const fc_scan_run &r) {
     return FC_OK;
 }
 
+// Lanes from which on several sequences share a channel's values.
+constexpr long kManyLanes = 1l << 18;
+
 template <int DT>
 int scan_step(fc_context *ctx, const fc_scan_run &r) {
     with_lanes(r.N, [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
-        const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true> : fc_selective_scan_step_kernel<DT, L, false>;
-        kernel<<<dim3((unsigned)(((long)r.B * r.channels * L + 255) / 256)), dim3(256), 0, ctx->stream>>>(r);
+        const unsigned across = (unsigned)(((long)r.channels * L + 255) / 256);
+        if ((long)r.channels * L * r.B >= kManyLanes) {
+            constexpr int S = 2;
+            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true, S> : fc_selective_scan_step_kernel<DT, L, false, S>;
+            kernel<<<dim3(across * (unsigned)((r.B + S - 1) / S)), dim3(256), 0, ctx->stream>>>(r, across);
+        } else {
+            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true, 1> : fc_selective_scan_step_kernel<DT, L, false, 1>;
+            kernel<<<dim3(across * (unsigned)r.B), dim3(256), 0, ctx->stream>>>(r, across);
+        }
     });
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_step_kernel");
     return FC_OK;
