@@ -8,9 +8,13 @@ constexpr long kMostThreads = 1l << 32;      // of a launch, not reached
 constexpr int kMostStates = 64;
 // Up to so many tokens run without tiles, L lanes a channel.
 constexpr long kMostSteps = 4;
-// A sequence is cut where its channels leave the chip idle, and then into as many segments as fill it: a cut forms every state twice.
-constexpr long kEnoughWavefronts = 1536, kWavefronts = 4096;
-constexpr long kWorkgroupsBackward = 1024;
+// A sequence is cut where its channels leave the chip idle, and then into as many segments as fill it: a cut forms every state twice.  2048 tokens of 2048
+// channels, 16 states, bf16: 8 sequences (1024 wavefronts) 282 us uncut and 238 in 8 segments, 12 of them 353 and 372 in 2.  One sequence of 12544 tokens: 228 us
+// in 56 segments (8192 wavefronts), 237 in 31, 269 in 16; 4 of 3136 tokens 205 in 14, 222 in 8, 252 in 4, 430 uncut.
+constexpr long kEnoughWavefronts = 1536, kWavefronts = 8192;
+// Workgroups of the gradients' kernel, each of which leaves sums of dA: 4 sequences of 3136 tokens, 2048 channels, 16 states 748 us with 512 of them, 766 with 1024,
+// 709 with 2048 and 722 with 4096; 8 of 2048 tokens, 1024 channels, 8 states, whose workgroups are half as large, 593, 355, 419 and 404.
+constexpr long kWorkgroupsBackward = 2048, kSmallWorkgroupsBackward = 1024;
 
 // What enters each segment, from what each adds to none.  Bound by the chain of segments, eight of which are read at once.  GRADS: from the last to the
 // first, and what leaves the first is the gradient of the state before it.
@@ -162,7 +166,8 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
         }
     }
     if (plan->segments > 1) plan->ws_bytes = (states_of(*s, plan->segments) + (size_t)s->B * plan->segments * s->D) * sizeof(float);
-    long walks = (kWorkgroupsBackward + workgroups - 1) / workgroups;
+    const long want = lanes < 4 ? kSmallWorkgroupsBackward : kWorkgroupsBackward;
+    long walks = (want + workgroups - 1) / workgroups;
     if (walks > tiles) walks = tiles;
     const long per_walk = (tiles + walks - 1) / walks;
     plan->walks_backward = (int)((tiles + per_walk - 1) / per_walk);

@@ -87,9 +87,12 @@ struct scan_offsets {
     }
 };
 
-template <int DT>
-__device__ __forceinline__ float step_of(const fc_scan_run &r, float raw) {
-    return r.softplus ? fc_softplus(raw) : raw;
+// One branch for all steps of a thread: their chains of dependent operations run side by side.
+template <int N>
+__device__ __forceinline__ void to_steps(const fc_scan_run &r, float (&v)[N]) {
+    if (!r.softplus) return;
+#pragma unroll
+    for (int k = 0; k < N; k++) v[k] = fc_softplus(v[k]);
 }
 
 // A tensor's tokens from t0 of a tile on, through a buffer resource: a thread has one 32-bit offset for all its tokens, whose distances are scalars, and an
@@ -221,14 +224,16 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_sele
     if (t0 < end) now.read(r, at, off, t0, end, true, true, true);
     for (long t = t0; t < end; t += kScanTile) {
         const int n = (int)(end - t < kScanTile ? end - t : kScanTile);
-        float x[F::EACH], z[GATE ? F::EACH : 1];
+        float x[F::EACH], z[GATE ? F::EACH : 1], dt[F::EACH];
 #pragma unroll
         for (int k = 0; k < F::EACH; k++) {
             x[k] = (float)now.x[k];
             if (GATE) z[k] = (float)now.z[k];
-            const float dt = step_of<DT>(r, (float)now.delta[k] + bias);
-            lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt, dt * x[k]);
+            dt[k] = (float)now.delta[k] + bias;
         }
+        to_steps(r, dt);
+#pragma unroll
+        for (int k = 0; k < F::EACH; k++) lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt[k], dt[k] * x[k]);
         lay_out<L>(lds.b, now.b);
         lay_out<L>(lds.c, now.c);
         __syncthreads();
@@ -303,10 +308,13 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
             }
         }
         if (n > 0) {
+            float dt[F::EACH];
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) dt[k] = (float)now.delta[k] + bias;
+            to_steps(r, dt);
 #pragma unroll
             for (int k = 0; k < F::EACH; k++) {
-                const float dt = step_of<DT>(r, (float)now.delta[k] + bias);
-                lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt, dt * (float)now.x[k]);
+                lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt[k], dt[k] * (float)now.x[k]);
                 if constexpr (GRADS) {
                     float g = (float)now.dy[k];
                     if (GATE) g *= fc_silu((float)now.z[k]);
@@ -415,10 +423,14 @@ __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_sc
                 }
             }
         }
+        float steps[SEQUENCES];
+#pragma unroll
+        for (int s = 0; s < SEQUENCES; s++) steps[s] = (float)delta[s] + bias;
+        to_steps(r, steps);
 #pragma unroll
         for (int s = 0; s < SEQUENCES; s++) {
             const bool there = t < len[s];
-            const float v = (float)x[s], dt = step_of<DT>(r, (float)delta[s] + bias), u = dt * v;
+            const float v = (float)x[s], dt = steps[s], u = dt * v;
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < kScanStates; j++) {
@@ -495,11 +507,14 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gr
         if (n > 0) {
             float steps[F::EACH];
 #pragma unroll
+            for (int k = 0; k < F::EACH; k++) steps[k] = (float)now.delta[k] + bias;
+            to_steps(r, steps);
+#pragma unroll
             for (int k = 0; k < F::EACH; k++) {
                 const int i = at.row + k * F::ROWS;
                 const bool in = i < n && at.d >= 0;      // a token past the last moves nothing
                 const float x = in ? (float)now.x[k] : 0.f;
-                steps[k] = in ? step_of<DT>(r, (float)now.delta[k] + bias) : 0.f;
+                steps[k] = in ? steps[k] : 0.f;
                 float g = in ? (float)now.dy[k] : 0.f;
                 if (GATE && in) g *= fc_silu((float)now.z[k]);
                 lds.du[i][at.c] = make_float2(steps[k], steps[k] * x);
@@ -590,14 +605,19 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gr
             if (seg + 1 < last && t + kScanTile < at.len) now.read(r, at, off, t + kScanTile, at.len, true, true, true);
             const scan_window<DT> dx(r.dx, at.b * r.x_batch + t * r.x_token + at.first), dd(r.ddelta, at.b * r.delta_batch + t * r.delta_token + at.first);
             const scan_window<DT> dz(r.dz, at.b * r.z_batch + t * r.z_token + at.first);
+            float slope[F::EACH];      // of the step
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) slope[k] = 1.f;
+            if (r.softplus)
+#pragma unroll
+                for (int k = 0; k < F::EACH; k++) slope[k] = fc_sigmoid((float)here.delta[k] + bias);
 #pragma unroll
             for (int k = 0; k < F::EACH; k++) {
                 const int i = at.row + k * F::ROWS;
                 const bool in = i < n;      // channels past the last are zeros and nowhere
                 const float2 s = lds.du[i][at.c];
                 const float x = (float)here.x[k], g = gs[i][at.c];
-                float dstep = __builtin_fmaf(x, s.x, 0.693147181f * s.y);
-                if (r.softplus) dstep *= fc_sigmoid((float)here.delta[k] + bias);
+                const float dstep = __builtin_fmaf(x, s.x, 0.693147181f * s.y) * slope[k];
                 auto put = [&](const scan_window<DT> &w, float v, uint32_t lane, uint32_t token) __attribute__((always_inline)) {
                     if (n == kScanTile) w.put(v, lane, k * F::ROWS * token);
                     else w.put(v, in ? lane + k * F::ROWS * token : kNowhere, 0);
