@@ -82,6 +82,13 @@ __device__ __forceinline__ void read_before(V (&to)[N], const E *first, const E 
     }
 }
 
+// The window moves on by the N rows of `now`.
+template <int N, int W, class V>
+__device__ __forceinline__ void move_on(V (&window)[W], const V (&now)[N]) {
+#pragma unroll
+    for (int i = 0; i < W; i++) window[i] = i + N < W ? window[i + N < W ? i + N : 0] : now[i + N < W ? 0 : i + N - W];
+}
+
 template <class V, class E>
 __device__ __forceinline__ void store(E *to, const V &v, int skip) {
     if (!skip) {
@@ -140,8 +147,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
         if (t + kAhead <= (at.len < at.t1 ? at.len : at.t1)) results(std::false_type());
         else results(std::true_type());
         to += kAhead * p.y_token;
-#pragma unroll
-        for (int i = 0; i < TAPS - 1; i++) window[i] = now[kAhead - (TAPS - 1) + i];
+        move_on(window, now);
     }
     // The last rows, by whoever read the first: the state may be written over the one before.  Row i lies at or before what it is read from.
     if (at.walk == 0 && p.state_out) {
@@ -239,11 +245,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
         if (t + AHEAD <= inside && t - (TAPS - 1) >= at.t0) results(std::false_type());
         else results(std::true_type());
         to += AHEAD * p.x_token;
-#pragma unroll
-        for (int i = 0; i < TAPS - 1; i++) {
-            if constexpr (TAPS - 1 <= AHEAD) window[i] = now[AHEAD - (TAPS - 1) + i];
-            else window[i] = i + AHEAD < TAPS - 1 ? window[i + AHEAD < TAPS - 1 ? i + AHEAD : 0] : now[i + AHEAD < TAPS - 1 ? 0 : i + AHEAD - (TAPS - 1)];
-        }
+        move_on(window, now);
     }
     if (!p.part) return;
     float *part = p.part + (at.b * p.walks + at.walk) * (taps + 1) * p.C + at.c;
@@ -288,8 +290,9 @@ int check_plan(fc_context *ctx, const fc_causal_conv_plan *plan, const char *wha
 int channels_of(const fc_causal_conv_shape &s) { return s.C < kChannels ? 1 : kChannels; }
 int columns_of(const fc_causal_conv_shape &s) { return (s.C + channels_of(s) - 1) / channels_of(s); }
 
+// Walks of `least` tokens or more.  They hold a window at least: only the first reads the state, which it may write over.
 long walks_of(const fc_causal_conv_shape *s, int least) {
-    const long rows = (long)columns_of(*s) * s->B, most = (s->T + least - 1) / least;
+    const long rows = (long)columns_of(*s) * s->B, most = s->T > least ? s->T / least : 1;
     long walks = (kFill + rows - 1) / rows;
     if (walks > most) walks = most;
     const long walk = (s->T + walks - 1) / walks;
@@ -332,10 +335,11 @@ extern "C" int fc_causal_conv_make_plan(const fc_causal_conv_shape *s, fc_causal
     if (!plan || !s || s->B < 1 || s->T < 1 || s->C < 1 || s->taps < 2 || !fc_dtype_ok(s->dtype)) return FC_ERR_INVALID;
     if (s->act != FC_ACT_NONE && s->act != FC_ACT_SILU) return s->act < FC_ACT_NONE || s->act > FC_ACT_GELU ? FC_ERR_INVALID : FC_ERR_UNSUPPORTED;
     if (s->x_batch < 0 || s->x_token < 0 || s->y_batch < 0 || s->y_token < 0) return FC_ERR_INVALID;
-    if (s->taps > kMostTaps || s->T >= (1l << 31) || fc_count(s->B, s->C) < 0 || fc_count(s->B, s->C) >= (1l << 30)) return FC_ERR_UNSUPPORTED;
+    // tokens are counted in 32 bits, past the last; the sums of dw and dbias take 32 threads for each of (taps + 1) * C
+    if (s->taps > kMostTaps || s->T > (1l << 30) || s->C > (1 << 23) || fc_count(s->B, s->C) < 0 || fc_count(s->B, s->C) >= (1l << 30)) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    plan->walks = (int)walks_of(s, kAhead);
+    plan->walks = (int)walks_of(s, s->taps - 1 > kAhead ? s->taps - 1 : kAhead);
     plan->walks_backward = (int)walks_of(s, 4 * s->taps);
     plan->ws_backward_bytes = (size_t)s->B * plan->walks_backward * (s->taps + 1) * s->C * sizeof(float);
     return FC_OK;

@@ -643,7 +643,7 @@ int fc_int8_product(fc_context *ctx, const fc_int8_product_plan *plan, const int
  * Token t of sequence b begins at b*x_batch + t*x_token, and so for y; dy as y, dx as x.  w is fp32 [C][taps], the last tap the token's own.  The inputs before
  * the first token are a state of taps - 1 rows, packed [B][taps - 1][C] in the tensors' type, the oldest first.
  * lengths as above: later tokens are not read, their outputs and gradients are zeros, and the state after a sequence holds its own last rows.
- * Limits: 2 <= taps <= 8, B*C < 2^30, T < 2^31. */
+ * Limits: 2 <= taps <= 8, C <= 2^23, B*C < 2^30, T <= 2^30. */
 typedef struct {
     int B;
     long T;

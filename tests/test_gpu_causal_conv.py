@@ -215,3 +215,42 @@ def test_refusals(lib):
         with pytest.raises(F.FastConvError) as e:
             call()
         assert e.value.status == -1, i
+
+
+@pytest.mark.parametrize("taps", [5, 6, 7, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_taps_over_long_walks(lib, taps, dtype):
+    """A walk of many steps whose window reaches further back than the rows that are read at once, and the state over the one before."""
+    B, T, C = 64, 45, 2 * 4096 + 1
+    rng = np.random.default_rng(taps)
+    mark = lib.mark()
+    try:
+        print("causal conv, many taps", taps, dtype, flush=True)
+        plan = lib.causal_conv_plan(F.CausalConvShape.packed(B, T, C, taps, K.TYPES[dtype]))
+        assert plan.walks == 1
+        x, state = K.Dev(lib, (B, T, C), dtype, None, rng.standard_normal((B, T, C))), K.Dev(lib, (B, taps - 1, C), dtype, None, rng.standard_normal((B, taps - 1, C)))
+        w, bias = (rng.standard_normal((C, taps)) / np.sqrt(taps)).astype(np.float32), (0.3 * rng.standard_normal(C)).astype(np.float32)
+        y, first = K.Dev(lib, (B, T, C), dtype), state.values
+        lib.causal_conv(plan, x.ptr, K.floats(lib, w), K.floats(lib, bias), y.ptr, state.ptr, state.ptr)
+        want, last, z, tz = S.causal_conv(x.values, w.astype(np.float64), bias.astype(np.float64), True, first, None)
+        S.close(y.get(), want, K.ROUND[dtype] * np.abs(want) + 1.1 * tz + (8 + 2 * np.abs(z)) * K.EPS * np.abs(want) + K.TINY[dtype], "y")
+        assert np.array_equal(state.get(), last)
+    finally:
+        lib.release(mark)
+
+
+@pytest.mark.parametrize("taps", [3, 5, 8])
+def test_state_over_the_one_before_in_many_walks(lib, taps):
+    """However a sequence is cut, the walks read the state before it is written over."""
+    rng = np.random.default_rng(taps)
+    for T in (taps - 1, 9, 13, 64, 1225):
+        for C in (1, 33):
+            print("causal conv, state in place", taps, T, C, flush=True)
+            x, given = rng.standard_normal((2, T, C)), rng.standard_normal((2, taps - 1, C))
+            plan = lib.causal_conv_plan(F.CausalConvShape.packed(2, T, C, taps, K.TYPES["f32"]))
+            dx, w = K.Dev(lib, (2, T, C), "f32", None, x), K.floats(lib, rng.standard_normal((C, taps)))
+            apart, same = K.Dev(lib, (2, taps - 1, C), "f32", None, given), K.Dev(lib, (2, taps - 1, C), "f32", None, given)
+            after, one, two = K.Dev(lib, (2, taps - 1, C), "f32"), K.Dev(lib, (2, T, C), "f32"), K.Dev(lib, (2, T, C), "f32")
+            lib.causal_conv(plan, dx.ptr, w, None, one.ptr, apart.ptr, after.ptr)
+            lib.causal_conv(plan, dx.ptr, w, None, two.ptr, same.ptr, same.ptr)
+            assert np.array_equal(one.get(), two.get()) and np.array_equal(after.get(), same.get())

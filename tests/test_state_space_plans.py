@@ -101,3 +101,17 @@ def test_every_part_has_work():
         for parts in (p.segments, p.walks_backward):
             per = -(-tiles // parts)
             assert (parts - 1) * per < tiles
+
+
+def test_only_the_first_walk_of_a_convolution_reaches_the_state():
+    """The state after a sequence may be written over the one before it: the walks after the first begin a window or more behind its start."""
+    for taps in range(2, 9):
+        for t in list(range(1, 70)) + [1225, 12544]:
+            for c in (1, 2, 65, 2048):
+                rc, p = make("conv", T=t, C=c, taps=taps, x_token=c, y_token=c, x_batch=t * c, y_batch=t * c)
+                assert rc == 0 and (p.walks == 1 or -(-t // p.walks) >= taps - 1), (taps, t, c)
+
+
+@pytest.mark.parametrize("field,value,status", [("T", 1 << 30, 0), ("T", (1 << 30) + 1, -6), ("T", (1 << 31) - 1, -6), ("C", 1 << 23, 0), ("C", (1 << 23) + 1, -6)])
+def test_convolutions_whose_counts_pass_32_bits(field, value, status):
+    assert make("conv", **{field: value})[0] == status
