@@ -528,7 +528,6 @@ extern "C" int fc_int8_product_make_plan(const fc_int8_product_shape *s, fc_int8
     if (!plan || !s || s->M < 1 || s->N < 1 || s->K < 1 || !fc_dtype_ok(s->dtype) || s->x_row < 0 || s->w_row < 0 || s->y_row < 0) return FC_ERR_INVALID;
     if (s->K > kMostTerms || s->M >= (1l << 31) || fc_count(s->M, s->N) >= (1l << 36)) return FC_ERR_UNSUPPORTED;
     *plan = {};
-    plan->shape = *s;
     product_form f;
     if (s->M <= kFewTokens) {
         f = few_form(s->M, s->N, s->K);
@@ -537,6 +536,11 @@ extern "C" int fc_int8_product_make_plan(const fc_int8_product_shape *s, fc_int8
         f = best_tile(s->M, s->N, s->K);
         cut(f, ceil_div(s->M, f.tile) * ceil_div(s->N, f.tile), s->K, 4096);
     }
+    // a launch has fewer than 2^32 threads
+    const long threads = f.tile == 256 || !f.tile ? 512 : 256;
+    const long workgroups = f.tile ? ceil_div(s->M, f.tile) * ceil_div(s->N, f.tile) : ceil_div(s->M, 16 * f.mf) * ceil_div(s->N, 16 * f.nf);
+    if (workgroups * f.parts >= (1l << 32) / threads) return FC_ERR_UNSUPPORTED;
+    plan->shape = *s;
     plan->tile = f.tile;
     plan->parts = f.parts;
     plan->ws_bytes = f.parts > 1 ? (size_t)f.parts * s->M * s->N * sizeof(int) : 0;

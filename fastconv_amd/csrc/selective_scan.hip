@@ -148,9 +148,11 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     if (fc_count(workgroups, tiles) < 0 || workgroups * tiles >= kMostThreads / kThreads || fc_count(s->B, s->D) >= kMostThreads / kMostStates ||
         fc_count(s->B * tiles, s->D, kScanTile * kMostStates) < 0)
         return FC_ERR_UNSUPPORTED;
+    // the sums of the gradients of A, D and delta_bias take 32 threads for each
+    if (fc_count(s->D, s->N + 2) >= kMostThreads / 32) return FC_ERR_UNSUPPORTED;
     // a tile's offsets are 31 bits
     const long far = s->x_token | s->delta_token | s->z_token | s->b_token | s->c_token | s->y_token;
-    if (s->T > kMostSteps && far >= (1l << 24)) return FC_ERR_UNSUPPORTED;
+    if (s->T > 1 && far >= (1l << 24)) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
     plan->tiles = s->T > kMostSteps ? (int)tiles : 0;

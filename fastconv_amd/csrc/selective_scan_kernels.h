@@ -484,7 +484,7 @@ __device__ __forceinline__ float2 sum_channels(float (&v)[8]) {
 
 // Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.
 template <int DT, int L, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS, 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
+__global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
     typedef typename fc_elem<DT>::type E;
     __shared__ scan_shared<L> lds;

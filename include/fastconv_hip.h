@@ -617,7 +617,8 @@ int fc_quantize_rows(fc_context *ctx, long rows, int C, int dtype, const void *x
 /* Product of 8-bit rows with scales for each token and channel:
  *   y[m][n] = (sum over k of x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]
  * Rows of x, w (bytes) and y (of `dtype`) begin x_row, w_row and y_row apart; w holds a row for each output channel.  Sums are exact, in 32-bit integers.
- * Rows of x and w that begin on 16 bytes and have sizes that are multiples of 16 are read fastest.  Limits: K <= 131071, M < 2^31, M*N < 2^36. */
+ * Rows of x and w that begin on 16 bytes and have sizes that are multiples of 16 are read fastest.  Limits: K <= 131071, M < 2^31, M*N < 2^36,
+ * and fewer than 2^24 tiles of 64 or 128 tokens and channels (2^23 of 256; 2^23 workgroups of up to 32 channels where tokens are few). */
 typedef struct {
     long M;
     int N, K;
@@ -677,7 +678,8 @@ int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_plan *plan, co
  * group: N values from b*b_batch + t*b_token + group*b_group on.  A is fp32 [D][N], not its logarithm; a rate above 0 is not checked for (the state
  * grows), one of minus infinity is a decay of 0 after a step above 0.  States are packed fp32 [B][D][N].
  * lengths as above: later tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
- * Limits: N <= 64, T < 2^31, B*D < 2^26, fewer than 2^24 workgroups, of which 32 tokens of 64 channels (N > 16: 32; N > 32: 16) are one. */
+ * Limits: N <= 64, B*D < 2^26, D*(N+2) < 2^27, fewer than 2^24 workgroups, of which 32 tokens of 64 channels (N > 16: 32; N > 32: 16) are one; more
+ * than one token: distances of tokens below 2^24 values. */
 typedef struct {
     int B;
     long T;

@@ -115,3 +115,17 @@ def test_only_the_first_walk_of_a_convolution_reaches_the_state():
 @pytest.mark.parametrize("field,value,status", [("T", 1 << 30, 0), ("T", (1 << 30) + 1, -6), ("T", (1 << 31) - 1, -6), ("C", 1 << 23, 0), ("C", (1 << 23) + 1, -6)])
 def test_convolutions_whose_counts_pass_32_bits(field, value, status):
     assert make("conv", **{field: value})[0] == status
+
+
+@pytest.mark.parametrize("M,N,status", [(1, 1 << 26, 0), (1, 1 << 28, -6), (1, (1 << 31) - 1, -6), (64, 1 << 27, 0), (64, 1 << 29, -6), ((1 << 31) - 1, 1, -6),
+                                        (1 << 28, 1, 0), (1 << 20, 1 << 15, 0)])
+def test_products_whose_launch_passes_32_bits(M, N, status):
+    assert make("product", M=M, N=N, K=16, x_row=16, w_row=16, y_row=N)[0] == status
+
+
+def test_scans_whose_launch_or_tiles_pass_32_bits():
+    for t, token, status in ((1, 1 << 40, 0), (2, (1 << 24) - 1, 0), (2, 1 << 24, -6), (4, 1 << 24, -6), (5, 1 << 24, -6), (100, (1 << 24) - 1, 0)):
+        for field in ("x_token", "delta_token", "z_token", "b_token", "c_token", "y_token"):
+            assert make("scan", T=t, **{field: token})[0] == status, (t, token, field)
+    for d, n, status in ((1 << 20, 64, 0), (1 << 21, 64, -6), (1 << 23, 14, -6), (1 << 23, 13, 0)):
+        assert make("scan", B=1, T=1, D=d, N=n, G=1)[0] == status, (d, n)
