@@ -266,13 +266,18 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_sele
         }
         __syncthreads();
         const scan_window<DT> y(r.y, at.b * r.y_batch + t * r.y_token + at.first);
+        float out[F::EACH];
 #pragma unroll
         for (int k = 0; k < F::EACH; k++) {
-            const int i = at.row + k * F::ROWS;
-            float v = __builtin_fmaf(skip, x[k], ys[i][at.c]);
-            if (GATE) v *= fc_silu(z[k]);
-            if (n == kScanTile) y.put(v, off.y, k * F::ROWS * off.y_token);
-            else y.put(v, i < n ? off.y + k * F::ROWS * off.y_token : kNowhere, 0);
+            out[k] = __builtin_fmaf(skip, x[k], ys[at.row + k * F::ROWS][at.c]);
+            if (GATE) out[k] *= fc_silu(z[k]);
+        }
+        if (n == kScanTile) {
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) y.put(out[k], off.y, k * F::ROWS * off.y_token);
+        } else {
+#pragma unroll
+            for (int k = 0; k < F::EACH; k++) y.put(out[k], at.row + k * F::ROWS < n ? off.y + k * F::ROWS * off.y_token : kNowhere, 0);
         }
     }
     // tokens past the end of a shorter sequence
