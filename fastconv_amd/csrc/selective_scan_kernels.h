@@ -491,6 +491,11 @@ __device__ __forceinline__ float2 sum_channels(float (&v)[8]) {
 template <int DT, int L, bool GATE>
 __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
+    // Tokens whose states are in registers at a time, and whether their decays are too, by what the other lanes' values leave.  2048 channels of 4 x 3136 tokens
+    // and 16 states: 709 us with 8 and decays, 903 with 16 and decays, 732 with 16 and decays formed again; 1024 channels of 8 x 2048 tokens and 8 states: 449, 712
+    // and 342; 4 states: 363, 363 and, with 32, 369 without decays and 518 with them.
+    constexpr int PART = L == 1 ? 32 : L == 4 || L == 8 ? 8 : 16;
+    constexpr bool KEEP = L > 2;
     typedef typename fc_elem<DT>::type E;
     __shared__ scan_shared<L> lds;
     __shared__ float gs[kScanTile][F::CH], ys[GATE ? kScanTile : 1][GATE ? F::CH : 1];
@@ -531,41 +536,52 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
             read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
             read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
             __syncthreads();
-            // Half a tile's states are kept at a time: with all of them there are no registers left for what comes next.
-            constexpr int HALF = kScanTile / 2;
-            float mid[kScanStates] = {start[0], start[1], start[2], start[3]};
-#pragma unroll 8
-            for (int i = 0; i < HALF; i++) {
-                const float2 du = lds.du[i][at.chan];
-                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
-                const float bs[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-                for (int j = 0; j < kScanStates; j++) mid[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), mid[j], du.y * bs[j]);
-            }
+            // Some tokens' states and decays are kept at a time: with all of them there are no registers left for what comes next.  First the states that enter each
+            // part but the first; they wait where the sums of the part before theirs will lie.
+            static_assert(PART == kScanTile || sizeof(waves[0][0]) * PART >= 64 * sizeof(float4));
+            auto mid = [&](int part) __attribute__((always_inline)) { return (float4 *)&waves[wave][part - PART][0] + lane; };
+            float h[kScanStates] = {start[0], start[1], start[2], start[3]};
 #pragma unroll 1
-            for (int half = HALF; half >= 0; half -= HALF) {
-                float hs[HALF][kScanStates], enters[kScanStates];
+            for (int part = PART; part < kScanTile; part += PART) {
 #pragma unroll
-                for (int j = 0; j < kScanStates; j++) enters[j] = half ? mid[j] : start[j];
-#pragma unroll
-                for (int i = 0; i < HALF; i++) {
-                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);      // else all reads move to the front, and registers spill
-                    const float2 du = lds.du[half + i][at.chan];
-                    const float4 b = *(const float4 *)&lds.b[half + i][at.sg * kScanStates];
+                for (int i = 0; i < PART; i++) {
+                    const float2 du = lds.du[part - PART + i][at.chan];
+                    const float4 b = *(const float4 *)&lds.b[part - PART + i][at.sg * kScanStates];
                     const float bs[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int j = 0; j < kScanStates; j++)
-                        hs[i][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), i ? hs[i ? i - 1 : 0][j] : enters[j], du.y * bs[j]);
+                    for (int j = 0; j < kScanStates; j++) h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), h[j], du.y * bs[j]);
                 }
-                fc_wave_sync();      // steps and exponentials are formed again: kept, they would need twice the registers
+                *mid(part) = make_float4(h[0], h[1], h[2], h[3]);
+            }
+#pragma unroll 1
+            for (int part = kScanTile - PART; part >= 0; part -= PART) {
+                float hs[PART][kScanStates], as[KEEP ? PART : 1][kScanStates], enters[kScanStates] = {start[0], start[1], start[2], start[3]};
+                if (part) {
+                    const float4 from = *mid(part);
+                    enters[0] = from.x; enters[1] = from.y; enters[2] = from.z; enters[3] = from.w;
+                }
+#pragma unroll
+                for (int i = 0; i < PART; i++) {
+                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);      // else all reads move to the front, and registers spill
+                    const float2 du = lds.du[part + i][at.chan];
+                    const float4 b = *(const float4 *)&lds.b[part + i][at.sg * kScanStates];
+                    const float bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int j = 0; j < kScanStates; j++) {
+                        const float decay = __builtin_amdgcn_exp2f(du.x * rate[j]);
+                        if (KEEP) as[KEEP ? i : 0][j] = decay;
+                        hs[i][j] = __builtin_fmaf(decay, i ? hs[i ? i - 1 : 0][j] : enters[j], du.y * bs[j]);
+                    }
+                }
+                fc_wave_sync();
                 float2 kept = make_float2(0.f, 0.f);
                 float mine = 0.f;
 #pragma unroll
-                for (int i = HALF - 1; i >= 0; i--) {
+                for (int i = PART - 1; i >= 0; i--) {
                     if (i % 2) __builtin_amdgcn_sched_barrier(0);
-                    const float2 du = lds.du[half + i][at.chan];
-                    const float g = gs[half + i][at.chan];
-                    const float4 b = *(const float4 *)&lds.b[half + i][at.sg * kScanStates], c = *(const float4 *)&lds.c[half + i][at.sg * kScanStates];
+                    const float2 du = lds.du[part + i][at.chan];
+                    const float g = gs[part + i][at.chan];
+                    const float4 b = *(const float4 *)&lds.b[part + i][at.sg * kScanStates], c = *(const float4 *)&lds.c[part + i][at.sg * kScanStates];
                     const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
                     float v[8], du_sum = 0.f, dt_sum = 0.f, y = 0.f;
 #pragma unroll
@@ -575,7 +591,7 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
                         v[4 + j] = g * hs[i][j];
                         if (GATE) y = __builtin_fmaf(cs[j], hs[i][j], y);
                         du_sum = __builtin_fmaf(G[j], bs[j], du_sum);
-                        G[j] *= __builtin_amdgcn_exp2f(du.x * rate[j]);
+                        G[j] *= KEEP ? as[KEEP ? i : 0][j] : __builtin_amdgcn_exp2f(du.x * rate[j]);
                         const float k = G[j] * (i ? hs[i ? i - 1 : 0][j] : enters[j]);
                         dt_sum = __builtin_fmaf(k, rate[j], dt_sum);
                         dA[j] = __builtin_fmaf(k, du.x, dA[j]);
@@ -584,14 +600,14 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
                     dt_sum = sum_states<L>(dt_sum);
                     const float2 s = sum_channels<L>(v);
                     if (L == 16 || (lane & 15) < L)
-                        *(float2 *)&waves[wave][half + i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
+                        *(float2 *)&waves[wave][part + i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
                     // each lane keeps one of L tokens
                     if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
-                    if (i % L == 0) lds.du[half + i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
+                    if (i % L == 0) lds.du[part + i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
                     if constexpr (GATE) {
                         y = sum_states<L>(y);
                         mine = i % L == at.sg ? y : mine;
-                        if (i % L == 0) ys[half + i + at.sg][at.chan] = mine;
+                        if (i % L == 0) ys[part + i + at.sg][at.chan] = mine;
                     }
                 }
             }
