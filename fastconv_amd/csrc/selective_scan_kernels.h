@@ -515,6 +515,9 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
         const int n = (int)(at.len - t < 0 ? 0 : at.len - t < kScanTile ? at.len - t : kScanTile);
         float *shared = r.shared + ((at.block * (long)r.B + at.b) * r.T + t) * 2 * r.N;
         if (n > 0) {
+            float start[kScanStates], G[kScanStates];
+            read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
+            read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
             float steps[F::EACH];
 #pragma unroll
             for (int k = 0; k < F::EACH; k++) steps[k] = (float)now.delta[k] + bias;
@@ -532,9 +535,6 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
             }
             lay_out<L>(lds.b, now.b);
             lay_out<L>(lds.c, now.c);
-            float start[kScanStates], G[kScanStates];
-            read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
-            read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
             __syncthreads();
             // Some tokens' states and decays are kept at a time: with all of them there are no registers left for what comes next.  First the states that enter each
             // part but the first; they wait where the sums of the part before theirs will lie.
