@@ -84,6 +84,15 @@ __device__ __forceinline__ void put(const product_params &p, long m, int n, cons
         if (n + i < p.N) y[i] = (E)(p.bias ? __builtin_fmaf((float)sum[i] * xs, p.w_scale[n + i], p.bias[n + i]) : (float)sum[i] * xs * p.w_scale[n + i]);
 }
 
+// What a lane has of a product of 16 tokens and 16 channels: column, a token; four rows, channels.
+template <int DT>
+__device__ __forceinline__ void put_few(const product_params &p, long m, int n, intx4 s) {
+    const int four[4] = {s[0], s[1], s[2], s[3]};
+    if (m >= p.M || n >= p.N) return;
+    if (p.parts_at) put_part(p, m, n, s);
+    else put<DT>(p, m, n, four, p.x_scale[m]);
+}
+
 // Few tokens.  Bound by w, read once: a workgroup takes 16 * NF channels and up to 16 * MF tokens, its wavefronts take 128 bytes of the rows
 // in turn, operands from memory straight into registers, and add up through LDS.
 template <int DT, int MF, int NF, int WAVES>
@@ -158,12 +167,88 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_few_kernel(const p
         intx4 s = part[0][f][lane];
 #pragma unroll
         for (int v = 1; v < WAVES; v++) s += part[v][f][lane];
-        // column of the product: token; four rows: channels
-        const long m = m0 + 16 * (f / NF) + r;
-        const int n = n0 + 16 * (f % NF) + 4 * q, four[4] = {s[0], s[1], s[2], s[3]};
-        if (m >= p.M || n >= p.N) continue;
-        if (p.parts_at) put_part(p, m, n, s);
-        else put<DT>(p, m, n, four, p.x_scale[m]);
+        put_few<DT>(p, m0 + 16 * (f / NF) + r, n0 + 16 * (f % NF) + 4 * q, s);
+    }
+}
+
+// The same where rows begin on and are multiples of 16 bytes.  Eight neighbouring lanes read 128 bytes of a row, which go to LDS without passing registers: an
+// operand's own lanes lie in 16 rows each, and a load of them takes the L1 four times as long.  A wavefront has a ring of its own and waits for nobody.
+template <int DT, int MF, int NF, int WAVES, int BUFFERS>
+__global__ __launch_bounds__(64 * WAVES) void fc_int8_product_ring_kernel(const product_params p) {
+    static_assert(BUFFERS <= 2);
+    constexpr int LOADS = 2 * (NF + MF), WORDS = LOADS * 64;
+    extern __shared__ intx4 lds[];      // [WAVES][BUFFERS][16 * (NF + MF) rows][8]; then the wavefronts' sums
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NF;
+    const long m0 = (long)blockIdx.y * 16 * MF;
+    const int k0 = blockIdx.z * p.part, K = p.K - k0 < p.part ? p.K - k0 : p.part;
+    // load e: eight rows of the stage, those of w first; word c of a row lies at place c ^ (row % 8)
+    const int k_of = ((lane & 7) ^ (lane >> 3)) * 16;
+    const int8_t *const w = p.w + n0 * p.w_row + k0, *const x = p.x + m0 * p.x_row + k0;
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int e = 0; e < LOADS; e++) {
+        const int row = 8 * (e < 2 * NF ? e : e - 2 * NF) + (lane >> 3);
+        const long at = e < 2 * NF ? (n0 + row < p.N ? row : p.N - 1 - n0) * p.w_row : (m0 + row < p.M ? row : p.M - 1 - m0) * p.x_row;
+        off[e] = (uint32_t)at + k_of;
+    }
+    const int all = (K + kFewStage - 1) / kFewStage, steps = all > wave ? (all - wave - 1) / WAVES + 1 : 0;
+    // Workgroups begin at steps of their own: rows a power of two apart have their bytes of one step in few of the L2's channels.
+    unsigned turn = steps ? (blockIdx.x / 8) % steps : 0;
+    intx4 *const ring = lds + wave * BUFFERS * WORDS;
+    auto fetch = [&](int s) __attribute__((always_inline)) {
+        const int k = (wave + (int)turn * WAVES) * kFewStage;
+        turn = turn + 1 < (unsigned)steps ? turn + 1 : 0;
+        const int8_t *wk = uniform_ptr(w + k), *xk = uniform_ptr(x + k);
+        intx4 *to = ring + s % BUFFERS * WORDS;
+#pragma unroll
+        for (int e = 0; e < LOADS; e++) {
+            const void *at = (e < 2 * NF ? wk : xk) + off[e];
+            if (k + kFewStage > K && k + k_of >= K) at = &kZeroWord;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at, (__attribute__((address_space(3))) void *)(to + e * 64), 16, 0, 0);
+        }
+    };
+    intx4 sum[MF][NF];
+#pragma unroll
+    for (int i = 0; i < MF; i++)
+#pragma unroll
+        for (int j = 0; j < NF; j++) sum[i][j] = intx4{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < BUFFERS; s++)
+        if (s < steps) fetch(s);
+    for (int s = 0; s < steps; s++) {
+        // all but the next step's loads have arrived
+        if (BUFFERS > 1 && s + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BUFFERS > 1 ? LOADS : 0) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const intx4 *at = ring + s % BUFFERS * WORDS + r * 8;
+        intx4 a[2][NF], b[2][MF];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int f = 0; f < NF; f++) a[h][f] = at[f * 128 + ((4 * h + q) ^ (r & 7))];
+#pragma unroll
+            for (int f = 0; f < MF; f++) b[h][f] = at[(NF + f) * 128 + ((4 * h + q) ^ (r & 7))];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // read, before they are written over
+        if (s + BUFFERS < steps) fetch(s + BUFFERS);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < MF; i++)
+#pragma unroll
+                for (int j = 0; j < NF; j++) sum[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h][j], b[h][i], sum[i][j], 0, 0, 0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MF; i++)
+#pragma unroll
+        for (int j = 0; j < NF; j++) lds[(wave * MF * NF + i * NF + j) * 64 + lane] = sum[i][j];
+    __syncthreads();
+    for (int f = wave; f < MF * NF; f += WAVES) {
+        intx4 s = lds[f * 64 + lane];
+#pragma unroll
+        for (int v = 1; v < WAVES; v++) s += lds[(v * MF * NF + f) * 64 + lane];
+        put_few<DT>(p, m0 + 16 * (f / NF) + r, n0 + 16 * (f % NF) + 4 * q, s);
     }
 }
 
@@ -478,10 +563,20 @@ int run_tiles(fc_context *ctx, product_params p, int parts, bool direct) {
 }
 
 template <int DT, int MF, int NF>
-int run_few(fc_context *ctx, const product_params &p, int parts) {
+int run_few(fc_context *ctx, const product_params &p, int parts, bool direct) {
+    const dim3 grid((unsigned)ceil_div(p.N, 16 * NF), (unsigned)ceil_div(p.M, 16 * MF), (unsigned)parts);
+    if (direct) {
+        constexpr int WAVES = 8, BUFFERS = MF == 4 ? 1 : 2;
+        constexpr size_t lds = (size_t)WAVES * BUFFERS * 2 * (NF + MF) * 1024;
+        static_assert(lds <= 160 * 1024 && lds >= (size_t)WAVES * MF * NF * 1024);
+        const auto kernel = fc_int8_product_ring_kernel<DT, MF, NF, WAVES, BUFFERS>;
+        if (lds > 65536) FC_HIP_CHECK(ctx, hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        kernel<<<grid, dim3(64 * WAVES), lds, ctx->stream>>>(p);
+        FC_LAUNCH_CHECK(ctx, "fc_int8_product_ring_kernel");
+        return FC_OK;
+    }
     constexpr int WAVES = 8;
-    fc_int8_product_few_kernel<DT, MF, NF, WAVES><<<dim3((unsigned)ceil_div(p.N, 16 * NF), (unsigned)ceil_div(p.M, 16 * MF), (unsigned)parts), dim3(64 * WAVES), 0,
-                                                    ctx->stream>>>(p);
+    fc_int8_product_few_kernel<DT, MF, NF, WAVES><<<grid, dim3(64 * WAVES), 0, ctx->stream>>>(p);
     FC_LAUNCH_CHECK(ctx, "fc_int8_product_few_kernel");
     return FC_OK;
 }
@@ -492,7 +587,7 @@ int run_form(fc_context *ctx, product_params p, const product_form &f, bool dire
     p.parts_at = f.parts > 1 ? (int *)ws : nullptr;
     int rc;
     if (f.tile == 0)
-        rc = f.mf == 4 ? run_few<DT, 4, 2>(ctx, p, f.parts) : f.mf == 2 ? run_few<DT, 2, 2>(ctx, p, f.parts) : f.nf == 2 ? run_few<DT, 1, 2>(ctx, p, f.parts) : run_few<DT, 1, 1>(ctx, p, f.parts);
+        rc = f.mf == 4 ? run_few<DT, 4, 2>(ctx, p, f.parts, direct) : f.mf == 2 ? run_few<DT, 2, 2>(ctx, p, f.parts, direct) : f.nf == 2 ? run_few<DT, 1, 2>(ctx, p, f.parts, direct) : run_few<DT, 1, 1>(ctx, p, f.parts, direct);
     else
         rc = f.tile == 256   ? run_tiles<DT, 256, 256, 2, 4, 4>(ctx, p, f.parts, direct)
              : f.tile == 128 ? run_tiles<DT, 128, 128, 2, 2, 4>(ctx, p, f.parts, direct)
