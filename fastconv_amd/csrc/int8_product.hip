@@ -502,8 +502,9 @@ long ceil_div(long a, long b) { return (a + b - 1) / b; }
 constexpr int kFewTokens = 64;
 constexpr long kUnits = 256;      // compute units
 
-// Few tokens.  Wide workgroups read x seldom, many read w side by side: the widest of which there is one a unit.  8192 channels of 4096, 64 tokens:
-// 64x32 14.1 us, 32x32 17.8, 16x32 24.7; 2048 channels 13.9, 9.8 and 7.9; 16 tokens of 8192 channels 16x32 8.2 and 16x16 10.1, of 4096 channels 6.7 and 5.1.
+// Few tokens.  Wide workgroups read x seldom, many read w side by side: the widest of which there is one a unit.  8192 channels of 4096, 64 tokens: 64x32 8.4 us,
+// 32x32 11.5, 16x32 16.5; 4096 channels 7.8, 6.3 and 8.6; 2048 channels 6.9, 5.4 and 5.0; 32 tokens of 8192 channels 7.3, 6.6 and 8.8; 16 tokens of 8192 channels
+// 16x32 5.3 and 16x16 6.0.
 product_form few_form(long M, int N, int K) {
     const int forms[4][2] = {{4, 2}, {2, 2}, {1, 2}, {1, 1}};
     product_form f = {};
@@ -538,9 +539,9 @@ product_form best_tile(long M, int N, int K) {
     return f;
 }
 
-// Workgroups that leave most of the chip idle cut a reduction of `least` bytes and more; adding the parts up is a launch more.  With and without: 1 token, 512
-// channels of 16384 6.9 and 10.9 us, of 2048 channels of 4096 7.0 and 4.9; 300 tokens, 520 channels of 8192 12.7 and 20.4; 200 tokens, 1000 channels of 4096
-// 10.2 and 12.2, of 2048 10.4 and 8.1.
+// Workgroups that leave most of the chip idle cut a reduction of `least` bytes and more; adding the parts up is a launch more.  With and without: 1 token, 64
+// channels of 65536 11.5 and 18.6 us, 512 channels of 16384 6.8 and 6.8, of 8192 8.0 and 4.7; 300 tokens, 520 channels of 8192 12.7 and 20.4; 200 tokens, 1000
+// channels of 4096 10.2 and 12.2, of 2048 10.4 and 8.1.
 void cut(product_form &f, long workgroups, int K, int least) {
     if (workgroups > kUnits / 4 || K < least) return;
     long parts = kUnits / workgroups;
@@ -626,7 +627,7 @@ extern "C" int fc_int8_product_make_plan(const fc_int8_product_shape *s, fc_int8
     product_form f;
     if (s->M <= kFewTokens) {
         f = few_form(s->M, s->N, s->K);
-        cut(f, ceil_div(s->M, 16 * f.mf) * ceil_div(s->N, 16 * f.nf), s->K, 8192);
+        cut(f, ceil_div(s->M, 16 * f.mf) * ceil_div(s->N, 16 * f.nf), s->K, 32768);
     } else {
         f = best_tile(s->M, s->N, s->K);
         cut(f, ceil_div(s->M, f.tile) * ceil_div(s->N, f.tile), s->K, 4096);
