@@ -360,34 +360,39 @@ __global__ __launch_bounds__(kPartThreads) void fc_rms_norm_dgamma_kernel(const 
 
 int fail(fc_context *ctx, int status, const char *what) { return fc_set_error(ctx, status, what, hipSuccess); }
 
-// Wavefronts of a row: one, four or sixteen, and whether the row stays in their registers.
+// Workgroups; each of the gradients' leaves a part of dgamma.  12544 rows of 2048, bf16: 33.8, 32.5 and 33.9 us with 1024, 2048 and 8192, gradients 32.2, 34.2, 36.0
+// and 38.2 with 256, 512, 768 and 1024; 4000 rows of 2048, fp32: gradients 28.1, 20.8, 20.7 and 23.0.  Rows of one access a thread need few registers, so that more
+// workgroups are on their way at once: 100000 rows of 256, bf16, gradients 48.4, 35.3 and 38.7 with 512, 1024 and 2048, the norm 35.7, 34.6 and 35.0 with 2048,
+// 4096 and 8192 (133 and 65 where four accesses are kept).
+constexpr long kBlocks = 2048, kBlocksBackward = 512, kNarrow = 2;
+// Wavefronts of a row: one, four or sixteen, and the accesses that each of their threads keeps in registers: one, four or, where that is too few, none.
 struct row_form {
-    int waves;
-    bool kept;
+    int waves, kept;
     // workgroups, each of which takes rows until there are none
     long blocks(long rows, long most) const {
         const long want = waves > 1 ? rows : (rows + 3) / 4;
         if (waves > 4) most /= 4;
+        if (kept == 1) most *= kNarrow;
         return want < most ? want : most;
     }
 };
 
-constexpr long kBlocks = 2048, kBlocksBackward = 768;
 constexpr int kAccesses = 4;      // of a thread
-row_form form_of(long rows, int C, int dtype) {
+// As few wavefronts as hold the row: nobody waits for another.  12544 rows of 2048, bf16: 32.5 us by one wavefront and 46.4 by four, gradients 35.8 and 78.8.
+row_form form_of(int C, int dtype) {
     const int vec = dtype == FC_F32 ? 4 : 8, accesses = (C + vec - 1) / vec;
-    // few rows: as many wavefronts as there are accesses for, a wait for one access each; many: as few as hold the row
-    const int least = rows < 1024 ? 1 : kAccesses;
-    if (accesses <= 64 * least) return {1, true};
-    if (accesses <= 256 * kAccesses) return {4, true};
-    return {16, accesses <= 1024 * kAccesses};
+    if (accesses <= 64) return {1, 1};
+    if (accesses <= 64 * kAccesses) return {1, kAccesses};
+    if (accesses <= 256 * kAccesses) return {4, kAccesses};
+    return {16, accesses <= 1024 * kAccesses ? kAccesses : 0};
 }
 
 template <int DT, class F>
 void with_rows(const row_form &f, F launch) {
     using std::integral_constant;
     typedef integral_constant<int, DT> dt;
-    if (f.waves == 1) launch(dt(), integral_constant<int, 1>(), integral_constant<int, kAccesses>());
+    if (f.kept == 1) launch(dt(), integral_constant<int, 1>(), integral_constant<int, 1>());
+    else if (f.waves == 1) launch(dt(), integral_constant<int, 1>(), integral_constant<int, kAccesses>());
     else if (f.waves == 4) launch(dt(), integral_constant<int, 4>(), integral_constant<int, kAccesses>());
     else if (f.kept) launch(dt(), integral_constant<int, 16>(), integral_constant<int, kAccesses>());
     else launch(dt(), integral_constant<int, 16>(), integral_constant<int, 0>());
@@ -402,7 +407,7 @@ void with_kernel(int dtype, const row_form &f, F launch) {
 
 template <int TO>
 int run(fc_context *ctx, const rms_params &p, int dtype, const char *name) {
-    const row_form f = form_of(p.rows, p.C, dtype);
+    const row_form f = form_of(p.C, dtype);
     const fc_device_scope on(ctx);
     with_kernel(dtype, f, [&](auto dt, auto waves, auto r) {
         constexpr int W = decltype(waves)::value;
@@ -446,7 +451,7 @@ extern "C" int fc_rms_norm_make_plan(const fc_rms_norm_shape *s, fc_rms_norm_pla
     if (s->rows > kMostRows || s->C > kMostChannels) return FC_ERR_UNSUPPORTED;
     *plan = {};
     plan->shape = *s;
-    plan->parts = (int)form_of(s->rows, s->C, s->dtype).blocks(s->rows, kBlocksBackward);
+    plan->parts = (int)form_of(s->C, s->dtype).blocks(s->rows, kBlocksBackward);
     plan->ws_backward_bytes = (size_t)plan->parts * s->C * sizeof(float);
     return FC_OK;
 }
@@ -513,7 +518,7 @@ extern "C" int fc_rms_norm_backward(fc_context *ctx, const fc_rms_norm_plan *pla
     p.part = dgamma_dev ? (float *)ws_dev : nullptr;
     p.rows = s.rows; p.C = s.C;
     p.x_row = s.x_row; p.sum_row = s.sum_row; p.dy_row = s.y_row;
-    const row_form f = form_of(s.rows, s.C, s.dtype);
+    const row_form f = form_of(s.C, s.dtype);
     const fc_device_scope on(ctx);
     with_kernel(s.dtype, f, [&](auto dt, auto waves, auto r) {
         constexpr int W = decltype(waves)::value;

@@ -205,7 +205,9 @@ __device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_pl
     }
 }
 
-// Answers.  Bound by the vector ALUs: an exponential (four cycles' worth) and four operations a state, 16 states a value.
+// Answers.  Bound by the vector ALUs, which are busy 99 % of the time: an exponential (two instructions' time) and four instructions a state, and for each token of a
+// lane about 15 more, 4 of which sum the lanes' parts, 5 form the step and 3 the gate.  12544 tokens of 2048 channels, 16 states, bf16: 114 us, of which 62 are the
+// states' own.  u B through 4x4x1 matrix instructions takes 12 cycles of 157 off the vector ALUs and leaves the time as it is (118 to 122 us).
 template <int DT, int L, bool GATE>
 __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_selective_scan_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
@@ -286,7 +288,9 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_sele
     if (r.state_out && at.walk == r.segments - 1) write_states<L>(r, at, r.state_out, at.b, h);
 }
 
-// What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient.
+// What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient: the gradient of a state is the sum of what each later token
+// adds, decayed on its way, and the product of the decays from the segment's begin on is at hand.  Bound as the answers are: 87 us there, with GRADS 159 (4 x 3136
+// tokens).
 template <int DT, int L, bool GRADS, bool GATE>
 __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
@@ -369,8 +373,8 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
     }
 }
 
-// A few tokens of many sequences, L lanes a channel without LDS.  Bound by the states, read and written once a call; what belongs to a channel is read once for
-// SEQUENCES of them, whose loads are on their way together.
+// A few tokens, L lanes a channel without LDS.  Bound by the states, read and written once a call (64 sequences of 4096 channels and 16 states: 33.5 MB in 11 us);
+// what belongs to a channel is read once for SEQUENCES of them, whose loads are on their way together.
 template <int DT, int L, bool GATE, int SEQUENCES>
 __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_scan_run r, unsigned across) {      // workgroups for all channels
     typedef typename fc_elem<DT>::type E;
@@ -487,7 +491,10 @@ __device__ __forceinline__ float2 sum_channels(float (&v)[8]) {
     return make_float2(o[0], o[1]);
 }
 
-// Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.
+// Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.  Bound by the vector ALUs, busy
+// 77 % of the time with two wavefronts a SIMD (256 registers): 121 instructions for each token of a lane, 64 of them the states' own.  dB and dC are sums over
+// channels, of a wavefront's by lane swaps, of a workgroup's through LDS, of all by a launch of their own, so that their order is always the same.  4 x 3136 tokens of
+// 2048 channels, 16 states, bf16: 507 us.
 template <int DT, int L, bool GATE>
 __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
     typedef scan_form<L> F;
@@ -716,7 +723,8 @@ int scan_ends(fc_context *ctx, const fc_scan_run &r) {
     return FC_OK;
 }
 
-// Lanes from which on several sequences share a channel's values.
+// Lanes from which on two sequences share a channel's values, where a token is all there is: 64 sequences of 4096 channels, 16 states, bf16 11.8 us and 12.1, 16
+// sequences 5.8 and 5.8; four tokens of 64 sequences 19.6 and 18.4.
 constexpr long kManyLanes = 1l << 18;
 
 template <int DT>
@@ -724,7 +732,7 @@ int scan_step(fc_context *ctx, const fc_scan_run &r) {
     with_lanes(r.N, [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
         const unsigned across = (unsigned)(((long)r.channels * L + 255) / 256);
-        if ((long)r.channels * L * r.B >= kManyLanes) {
+        if (r.T == 1 && (long)r.channels * L * r.B >= kManyLanes) {
             constexpr int S = 2;
             const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true, S> : fc_selective_scan_step_kernel<DT, L, false, S>;
             kernel<<<dim3(across * (unsigned)((r.B + S - 1) / S)), dim3(256), 0, ctx->stream>>>(r, across);

@@ -190,3 +190,49 @@ def test_refusals(lib):
         with pytest.raises(F.FastConvError) as e:
             call()
         assert e.value.status == -1, i
+
+
+@pytest.mark.parametrize("case", [  # M, N, K, gap, in parts
+    (1, 40, 16, 0, False),
+    (1, 8193, 48, 16, False),
+    (5, 4100, 144, 0, False),            # 16 channels a workgroup
+    (16, 8200, 1040, 0, False),          # 32 channels, 16 tokens
+    (30, 8200, 2064, 32, False),         # 32 tokens
+    (50, 8200, 1168, 0, False),          # 64 tokens
+    (64, 8192, 4096, 0, False),
+    (3, 70, 32784, 0, True),           # a reduction in parts
+    (64, 96, 33024, 16, True),
+    (3, 70, 32787, 0, True),           # the same from rows that begin anywhere
+    (40, 96, 33025, 3, True),
+], ids=lambda c: "-".join(map(str, c)))
+def test_few_tokens(lib, case):
+    M, N, K_, gap, parts = case
+    rng = np.random.default_rng(M + N + K_)
+    mark = lib.mark()
+    try:
+        print("int8 product, few tokens", case, flush=True)
+        plan = lib.int8_product_plan(F.Int8ProductShape(M, N, K_, K.TYPES["bf16"], K_ + gap, K_ + gap, N))
+        assert plan.tile == 0 and (plan.parts > 1) == parts and plan.ws_bytes == (4 * plan.parts * M * N if parts else 0)
+        x, w = rng.integers(-127, 128, (M, K_)).astype(np.int8), rng.integers(-127, 128, (N, K_)).astype(np.int8)
+        xs, ws = (rng.uniform(0.001, 0.02, n).astype(np.float32) for n in (M, N))
+        check(lib, x, w, xs, ws, rng.standard_normal(N).astype(np.float32), "bf16", gap=gap)
+    finally:
+        lib.release(mark)
+
+
+@pytest.mark.parametrize("M,N,K_", [(5, 48, 208), (64, 8192, 272), (20, 8192, 400), (16, 8192, 1040)])
+def test_single_elements_of_few_tokens(lib, M, N, K_):
+    """One value of x and of w at a time, in rows that begin on 16 bytes."""
+    rng = np.random.default_rng(K_)
+    one = np.ones(max(M, N), np.float32)
+    for _ in range(8):
+        mark = lib.mark()
+        m, n, k = rng.integers(M), rng.integers(N), rng.integers(K_)
+        print("int8 product, single element of few tokens", m, n, k, flush=True)
+        x, w = np.zeros((M, K_), np.int8), np.zeros((N, K_), np.int8)
+        x[m, k], w[n, k] = 3, -7
+        got = run(lib, x, w, one[:M], one[:N], None, "f32")
+        want = np.zeros((M, N))
+        want[m, n] = -21
+        assert np.array_equal(got, want)
+        lib.release(mark)
