@@ -273,3 +273,10 @@ def test_refusals(lib):
     with pytest.raises(F.FastConvError) as e:
         lib.quantize_rows(1, (1 << 20) + 1, F.F32, p[0], p[1], p[2])
     assert e.value.status == -6
+
+
+@pytest.mark.parametrize("case", [  # widths on both sides of where another number of accesses is kept, more rows than there are workgroups for
+    (17000, 72, "bf16", True, 0, 0), (4500, 256, "f32", True, 0, 0), (4500, 257, "f32", True, 3, 1), (9000, 512, "f16", True, 0, 0), (9000, 513, "bf16", True, 0, 0),
+    (2100, 1024, "bf16", False, 0, 0), (2100, 1025, "bf16", True, 0, 0), (2100, 516, "f32", True, 0, 0)], ids=lambda c: "-".join(map(str, c)))
+def test_widths_of_each_form(lib, case):
+    test_forward_and_backward(lib, case)
