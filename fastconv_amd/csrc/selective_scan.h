@@ -9,14 +9,14 @@
 //   dD = sum of g x,   dz = dy (C h + D x) silu'(z)
 //
 // A workgroup takes 64 channels (32 or 16 where there are more than 16 states) and walks over their tokens in tiles of 32.  Each channel has L lanes of
-// 4 states: what all its states need of a token (dt, dt x, the gate) is formed once, by threads that lie along the channels, and reaches the
-// lanes through LDS, as B and C do; so the inner loop is four states' exponentials and multiply-adds.
+// S states: what all its states need of a token (dt, dt x, the gate) is formed once, by threads that lie along the channels, and reaches the lanes through LDS, as
+// B and C do; so the inner loop is S states' exponentials and multiply-adds.
 #pragma once
 
 #include "token_math.h"
 
 constexpr int kScanTile = 32;      // tokens
-constexpr int kScanStates = 4;     // of a lane
+constexpr int kScanThreads = 256;
 
 struct fc_scan_run {
     const void *x, *delta, *b, *c, *z, *dy;
@@ -39,8 +39,7 @@ struct fc_scan_run {
     long b_batch, b_token, b_group, c_batch, c_token, c_group;
 };
 
-static inline int fc_scan_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-static inline int fc_scan_width(int lanes) { return lanes <= 4 ? 64 : 256 / lanes; }      // channels of a workgroup
+static inline int fc_scan_channels(int N) { return kScanThreads / (N <= 16 ? 4 : N <= 32 ? 8 : 16); }      // of a workgroup, each with so many lanes
 
 // selective_scan_<type>.hip.  ends: parts, steps and, if dy is there, grads of each segment.  answers: y and the last state, each segment from what
 // enters it.  step: the same for a few tokens.  gradients: of each segment, from what enters it on both sides.

@@ -13,9 +13,9 @@ constexpr long kMostSteps = 4;
 // channels, 16 states, bf16: 8 sequences (1024 wavefronts) 282 us uncut and 238 in 8 segments, 12 of them 353 and 372 in 2.  One sequence of 12544 tokens: 228 us
 // in 56 segments (8192 wavefronts), 237 in 31, 269 in 16; 4 of 3136 tokens 205 in 14, 222 in 8, 252 in 4, 430 uncut.
 constexpr long kEnoughWavefronts = 1536, kWavefronts = 8192;
-// Workgroups of the gradients' kernel, each of which leaves sums of dA: 4 sequences of 3136 tokens, 2048 channels, 16 states 748 us with 512 of them, 766 with 1024,
-// 709 with 2048 and 722 with 4096; 8 of 2048 tokens, 1024 channels, 8 states, whose workgroups are half as large, 593, 355, 419 and 404.
-constexpr long kWorkgroupsBackward = 2048, kSmallWorkgroupsBackward = 1024;
+// Workgroups of the gradients' kernel, each of which leaves sums of dA: 4 sequences of 3136 tokens, 2048 channels, 16 states 733 us with 1024 of them, 682 with 2048
+// and 693 with 4096; 8 of 2048 tokens, 1024 channels, 8 states 333, 329 and 336.
+constexpr long kWorkgroupsBackward = 2048;
 
 // What enters each segment, from what each adds to none.  Bound by the chain of segments, eight of which are read at once.  GRADS: from the last to the
 // first, and what leaves the first is the gradient of the state before it.
@@ -113,7 +113,7 @@ int check_plan(fc_context *ctx, const fc_selective_scan_plan *plan, const char *
 }
 
 int blocks_of(const fc_selective_scan_shape &s) {
-    const int width = fc_scan_width(fc_scan_lanes(s.N)), per_group = s.D / s.G;
+    const int width = fc_scan_channels(s.N), per_group = s.D / s.G;
     return s.G * ((per_group + width - 1) / width);
 }
 
@@ -158,8 +158,7 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     plan->shape = *s;
     plan->tiles = s->T > kMostSteps ? (int)tiles : 0;
     plan->segments = 1;
-    const int lanes = fc_scan_lanes(s->N);
-    const long wavefronts = workgroups * (fc_scan_width(lanes) * lanes / 64);
+    const long wavefronts = workgroups * (kScanThreads / 64);
     if (plan->tiles && wavefronts < kEnoughWavefronts) {
         long segments = kWavefronts / wavefronts;
         if (segments > tiles / 2) segments = tiles / 2;
@@ -169,8 +168,7 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
         }
     }
     if (plan->segments > 1) plan->ws_bytes = (states_of(*s, plan->segments) + (size_t)s->B * plan->segments * s->D) * sizeof(float);
-    const long want = lanes < 4 ? kSmallWorkgroupsBackward : kWorkgroupsBackward;
-    long walks = (want + workgroups - 1) / workgroups;
+    long walks = (kWorkgroupsBackward + workgroups - 1) / workgroups;
     if (walks > tiles) walks = tiles;
     const long per_walk = (tiles + walks - 1) / walks;
     plan->walks_backward = (int)((tiles + per_walk - 1) / per_walk);

@@ -23,23 +23,24 @@ __device__ __forceinline__ float sum_states(float v) {
     return v;
 }
 
-template <int L>
+// Channels have L lanes of S states each.
+template <int L, int S>
 struct scan_form {
-    static constexpr int CH = L <= 4 ? 64 : 256 / L, THREADS = CH * L, WAVES = THREADS / 64, NP = L * kScanStates;
+    static constexpr int THREADS = kScanThreads, CH = THREADS / L, WAVES = THREADS / 64, NP = L * S;
     static constexpr int ROWS = THREADS / CH, EACH = kScanTile / ROWS;      // tokens at once, and of a thread, where threads lie along the channels
     static constexpr int SHARED = (kScanTile * NP + THREADS - 1) / THREADS;      // values of B of a thread
 };
 
 // Where a workgroup is, and its threads in both of their arrangements.
-template <int L>
+template <int L, int S>
 struct scan_place {
-    typedef scan_form<L> F;
+    typedef scan_form<L, S> F;
     long b, len;
     int walk, group, block;
     long first;              // channel of the tensors that the workgroup begins with
     int c, row;              // channel and first token of a tile, along the channels
     int d, ds;               // channel along the channels and along the states; -1 past the last
-    int chan, sg;            // along the states: channel of the workgroup, four states of it
+    int chan, sg;            // along the states: channel of the workgroup, which S states of it
     __device__ __forceinline__ scan_place(const fc_scan_run &r) {
         unsigned i = blockIdx.x;
         block = i % r.blocks;
@@ -66,9 +67,9 @@ constexpr uint32_t kNowhere = 0x80000000u;
 struct scan_offsets {
     uint32_t x, delta, z, y, b, c;
     uint32_t x_token, delta_token, z_token, y_token, b_token, c_token;
-    template <int L>
-    __device__ __forceinline__ scan_offsets(const fc_scan_run &r, const scan_place<L> &at, uint32_t es) {
-        typedef scan_form<L> F;
+    template <int L, int S>
+    __device__ __forceinline__ scan_offsets(const fc_scan_run &r, const scan_place<L, S> &at, uint32_t es) {
+        typedef scan_form<L, S> F;
         x_token = (uint32_t)r.x_token * es;
         delta_token = (uint32_t)r.delta_token * es;
         z_token = (uint32_t)r.z_token * es;
@@ -116,15 +117,15 @@ struct scan_window {
 };
 
 // What a thread has of a tile before it is laid out for the states: values of its channel, one every ROWS tokens.  `n` tokens are there, the others zeros.
-template <int DT, int L, bool GATE, bool DY>
+template <int DT, int L, int S, bool GATE, bool DY>
 struct scan_tile {
-    typedef scan_form<L> F;
+    typedef scan_form<L, S> F;
     typedef typename fc_elem<DT>::type E;
     typedef scan_window<DT> W;
     E x[F::EACH], delta[F::EACH], z[GATE ? F::EACH : 1], dy[DY ? F::EACH : 1], b[F::SHARED], c[F::SHARED];
 
     // channels: x, delta, z, dy; states: B, and C if asked for
-    __device__ __forceinline__ void read(const fc_scan_run &r, const scan_place<L> &at, const scan_offsets &off, long t0, long end, bool channels, bool states,
+    __device__ __forceinline__ void read(const fc_scan_run &r, const scan_place<L, S> &at, const scan_offsets &off, long t0, long end, bool channels, bool states,
                                          bool with_c) {
         const int n = (int)(end - t0 < kScanTile ? end - t0 : kScanTile);
         const W wx(r.x, at.b * r.x_batch + t0 * r.x_token + at.first), wd(r.delta, at.b * r.delta_batch + t0 * r.delta_token + at.first);
@@ -161,16 +162,15 @@ struct scan_tile {
 };
 
 // The same laid out for the states.
-template <int L>
+template <int L, int S>
 struct alignas(16) scan_shared {
-    typedef scan_form<L> F;
+    typedef scan_form<L, S> F;
     float2 du[kScanTile][F::CH];      // dt and dt x
     float b[kScanTile][F::NP], c[kScanTile][F::NP];
 };
 
-template <int L, class E>
-__device__ __forceinline__ void lay_out(float (*to)[scan_form<L>::NP], const E (&v)[scan_form<L>::SHARED]) {
-    typedef scan_form<L> F;
+template <class F, class E>
+__device__ __forceinline__ void lay_out(float (*to)[F::NP], const E (&v)[F::SHARED]) {
 #pragma unroll
     for (int k = 0; k < F::SHARED; k++) {
         const int i = threadIdx.x + k * F::THREADS;
@@ -178,29 +178,35 @@ __device__ __forceinline__ void lay_out(float (*to)[scan_form<L>::NP], const E (
     }
 }
 
-template <int L>
-__device__ __forceinline__ void read_rates(const fc_scan_run &r, const scan_place<L> &at, float (&rate)[kScanStates]) {
+// A lane's S values of a row in LDS, in one access.
+template <int S>
+__device__ __forceinline__ void take(float (&to)[S], const float *from) {
+    __builtin_memcpy(to, __builtin_assume_aligned(from, S * sizeof(float)), sizeof to);
+}
+
+template <int L, int S>
+__device__ __forceinline__ void read_rates(const fc_scan_run &r, const scan_place<L, S> &at, float (&rate)[S]) {
 #pragma unroll
-    for (int j = 0; j < kScanStates; j++) {
-        const int n = at.sg * kScanStates + j;
+    for (int j = 0; j < S; j++) {
+        const int n = at.sg * S + j;
         rate[j] = at.ds >= 0 && n < r.N ? fc_scan_rate(r.A[(long)at.ds * r.N + n]) : 0.f;
     }
 }
 
-template <int L>
-__device__ __forceinline__ void read_states(const fc_scan_run &r, const scan_place<L> &at, const float *from, long row, float (&h)[kScanStates]) {
+template <int L, int S>
+__device__ __forceinline__ void read_states(const fc_scan_run &r, const scan_place<L, S> &at, const float *from, long row, float (&h)[S]) {
 #pragma unroll
-    for (int j = 0; j < kScanStates; j++) {
-        const int n = at.sg * kScanStates + j;
+    for (int j = 0; j < S; j++) {
+        const int n = at.sg * S + j;
         h[j] = from && at.ds >= 0 && n < r.N ? from[(row * r.channels + at.ds) * r.N + n] : 0.f;
     }
 }
 
-template <int L>
-__device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_place<L> &at, float *to, long row, const float (&h)[kScanStates]) {
+template <int L, int S>
+__device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_place<L, S> &at, float *to, long row, const float (&h)[S]) {
 #pragma unroll
-    for (int j = 0; j < kScanStates; j++) {
-        const int n = at.sg * kScanStates + j;
+    for (int j = 0; j < S; j++) {
+        const int n = at.sg * S + j;
         if (at.ds >= 0 && n < r.N) to[(row * r.channels + at.ds) * r.N + n] = h[j];
     }
 }
@@ -208,21 +214,21 @@ __device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_pl
 // Answers.  Bound by the vector ALUs, which are busy 99 % of the time: an exponential (two instructions' time) and four instructions a state, and for each token of a
 // lane about 15 more, 4 of which sum the lanes' parts, 5 form the step and 3 the gate.  12544 tokens of 2048 channels, 16 states, bf16: 114 us, of which 62 are the
 // states' own.  u B through 4x4x1 matrix instructions takes 12 cycles of 157 off the vector ALUs and leaves the time as it is (118 to 122 us).
-template <int DT, int L, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_selective_scan_kernel(const fc_scan_run r) {
-    typedef scan_form<L> F;
+template <int DT, int L, int S, bool GATE>
+__global__ __launch_bounds__(kScanThreads, 4) void fc_selective_scan_kernel(const fc_scan_run r) {
+    typedef scan_form<L, S> F;
     typedef typename fc_elem<DT>::type E;
-    __shared__ scan_shared<L> lds;
+    __shared__ scan_shared<L, S> lds;
     __shared__ float ys[kScanTile][F::CH];
-    const scan_place<L> at(r);
+    const scan_place<L, S> at(r);
     const long t0 = at.walk * r.segment, t1 = t0 + r.segment < r.T ? t0 + r.segment : r.T, end = t1 < at.len ? t1 : at.len;
-    float rate[kScanStates], h[kScanStates];
-    read_rates<L>(r, at, rate);
-    if (r.segments > 1) read_states<L>(r, at, r.parts, at.b * r.segments + at.walk, h);
-    else read_states<L>(r, at, r.state_in, at.b, h);
+    float rate[S], h[S];
+    read_rates<L, S>(r, at, rate);
+    if (r.segments > 1) read_states<L, S>(r, at, r.parts, at.b * r.segments + at.walk, h);
+    else read_states<L, S>(r, at, r.state_in, at.b, h);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
     const scan_offsets off(r, at, sizeof(E));
-    scan_tile<DT, L, GATE, false> now;
+    scan_tile<DT, L, S, GATE, false> now;
     if (t0 < end) now.read(r, at, off, t0, end, true, true, true);
     for (long t = t0; t < end; t += kScanTile) {
         const int n = (int)(end - t < kScanTile ? end - t : kScanTile);
@@ -236,18 +242,19 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_sele
         to_steps(r, dt);
 #pragma unroll
         for (int k = 0; k < F::EACH; k++) lds.du[at.row + k * F::ROWS][at.c] = make_float2(dt[k], dt[k] * x[k]);
-        lay_out<L>(lds.b, now.b);
-        lay_out<L>(lds.c, now.c);
+        lay_out<F>(lds.b, now.b);
+        lay_out<F>(lds.c, now.c);
         __syncthreads();
         if (t + kScanTile < end) now.read(r, at, off, t + kScanTile, end, true, true, true);
         float mine = 0.f;
         auto token = [&](int i) __attribute__((always_inline)) {
             const float2 du = lds.du[i][at.chan];
-            const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates], c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
-            const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
+            float bs[S], cs[S];
+            take(bs, &lds.b[i][at.sg * S]);
+            take(cs, &lds.c[i][at.sg * S]);
             float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < kScanStates; j++) {
+            for (int j = 0; j < S; j++) {
                 h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), h[j], du.y * bs[j]);
                 s = __builtin_fmaf(cs[j], h[j], s);
             }
@@ -285,25 +292,25 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? 4 : 2) void fc_sele
     // tokens past the end of a shorter sequence
     if (at.d >= 0)
         for (long t = (end > t0 ? end : t0) + at.row; t < t1; t += F::ROWS) ((E *)r.y)[at.b * r.y_batch + t * r.y_token + at.d] = (E)0.f;
-    if (r.state_out && at.walk == r.segments - 1) write_states<L>(r, at, r.state_out, at.b, h);
+    if (r.state_out && at.walk == r.segments - 1) write_states<L, S>(r, at, r.state_out, at.b, h);
 }
 
 // What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient: the gradient of a state is the sum of what each later token
 // adds, decayed on its way, and the product of the decays from the segment's begin on is at hand.  Bound as the answers are: 87 us there, with GRADS 159 (4 x 3136
 // tokens).
-template <int DT, int L, bool GRADS, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
-    typedef scan_form<L> F;
-    __shared__ scan_shared<L> lds;
+template <int DT, int L, int S, bool GRADS, bool GATE>
+__global__ __launch_bounds__(kScanThreads, GRADS ? 3 : 4) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
+    typedef scan_form<L, S> F;
+    __shared__ scan_shared<L, S> lds;
     __shared__ float gs[GRADS ? kScanTile : 1][GRADS ? F::CH : 1];
-    const scan_place<L> at(r);
+    const scan_place<L, S> at(r);
     const long first = (long)at.walk * r.per_walk * r.segment, last = first + r.per_walk * r.segment < r.T ? first + r.per_walk * r.segment : r.T;
     const long end = last < at.len ? last : at.len;
-    float rate[kScanStates], h[kScanStates], decay[kScanStates], grad[kScanStates], steps = 0.f;
-    read_rates<L>(r, at, rate);
+    float rate[S], h[S], decay[S], grad[S], steps = 0.f;
+    read_rates<L, S>(r, at, rate);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f;
     const scan_offsets off(r, at, sizeof(typename fc_elem<DT>::type));
-    scan_tile<DT, L, GATE && GRADS, GRADS> now;
+    scan_tile<DT, L, S, GATE && GRADS, GRADS> now;
     if (first < end) now.read(r, at, off, first, end, true, true, GRADS);
     long segment = at.b * r.segments + (long)at.walk * r.per_walk;
     for (long t = first; t < last; t += kScanTile) {
@@ -311,7 +318,7 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
         if ((t - first) % r.segment == 0) {
             steps = 0.f;
 #pragma unroll
-            for (int j = 0; j < kScanStates; j++) {
+            for (int j = 0; j < S; j++) {
                 h[j] = grad[j] = 0.f;
                 decay[j] = 1.f;
             }
@@ -330,23 +337,22 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
                     gs[at.row + k * F::ROWS][at.c] = g;
                 }
             }
-            lay_out<L>(lds.b, now.b);
-            if (GRADS) lay_out<L>(lds.c, now.c);
+            lay_out<F>(lds.b, now.b);
+            if (GRADS) lay_out<F>(lds.c, now.c);
             __syncthreads();
             if (t + kScanTile < end) now.read(r, at, off, t + kScanTile, end, true, true, GRADS);
             auto token = [&](int i) __attribute__((always_inline)) {
                 const float2 du = lds.du[i][at.chan];
-                const float4 b = *(const float4 *)&lds.b[i][at.sg * kScanStates];
-                const float bs[4] = {b.x, b.y, b.z, b.w};
-                float cs[4] = {0.f, 0.f, 0.f, 0.f}, g = 0.f;
+                float bs[S];
+                take(bs, &lds.b[i][at.sg * S]);
+                float cs[S] = {}, g = 0.f;
                 if constexpr (GRADS) {
-                    const float4 c = *(const float4 *)&lds.c[i][at.sg * kScanStates];
-                    cs[0] = c.x; cs[1] = c.y; cs[2] = c.z; cs[3] = c.w;
+                    take(cs, &lds.c[i][at.sg * S]);
                     g = gs[i][at.chan];
                 }
                 steps += du.x;
 #pragma unroll
-                for (int j = 0; j < kScanStates; j++) {
+                for (int j = 0; j < S; j++) {
                     const float a = __builtin_amdgcn_exp2f(du.x * rate[j]);
                     h[j] = __builtin_fmaf(a, h[j], du.y * bs[j]);
                     if (GRADS) {
@@ -365,8 +371,8 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
         }
         const long next = t + kScanTile;
         if ((next - first) % r.segment == 0 || next >= last) {
-            write_states<L>(r, at, r.parts, segment, h);
-            if (GRADS) write_states<L>(r, at, r.grads, segment, grad);
+            write_states<L, S>(r, at, r.parts, segment, h);
+            if (GRADS) write_states<L, S>(r, at, r.grads, segment, grad);
             if (at.sg == 0 && at.ds >= 0) r.steps[segment * r.channels + at.ds] = steps;
             segment++;
         }
@@ -375,26 +381,26 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L >= 4 ? GRADS ? 3 : 4 : 2) 
 
 // A few tokens, L lanes a channel without LDS.  Bound by the states, read and written once a call (64 sequences of 4096 channels and 16 states: 33.5 MB in 11 us);
 // what belongs to a channel is read once for SEQUENCES of them, whose loads are on their way together.
-template <int DT, int L, bool GATE, int SEQUENCES>
+template <int DT, int L, int S, bool GATE, int SEQUENCES>
 __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_scan_run r, unsigned across) {      // workgroups for all channels
     typedef typename fc_elem<DT>::type E;
-    typedef fc_vec<DT, kScanStates> V;
+    typedef fc_vec<DT, S> V;
     const long at = (long)(blockIdx.x % across) * 256 + threadIdx.x;
-    const int d = (int)(at / L), sg = threadIdx.x % L, n0 = sg * kScanStates;
+    const int d = (int)(at / L), sg = threadIdx.x % L, n0 = sg * S;
     if (d >= r.channels) return;
     const int group = d / r.per_group;
     // a lane's four states, or those that there are
-    const bool whole = n0 + kScanStates <= r.N;
-    float rate[kScanStates];
+    const bool whole = n0 + S <= r.N;
+    float rate[S];
     if (whole) __builtin_memcpy(rate, r.A + (long)d * r.N + n0, sizeof rate);
     else
 #pragma unroll
-        for (int j = 0; j < kScanStates; j++) rate[j] = n0 + j < r.N ? r.A[(long)d * r.N + n0 + j] : 0.f;
+        for (int j = 0; j < S; j++) rate[j] = n0 + j < r.N ? r.A[(long)d * r.N + n0 + j] : 0.f;
 #pragma unroll
-    for (int j = 0; j < kScanStates; j++) rate[j] = fc_scan_rate(rate[j]);
+    for (int j = 0; j < S; j++) rate[j] = fc_scan_rate(rate[j]);
     const float bias = r.delta_bias ? r.delta_bias[d] : 0.f, skip = r.D ? r.D[d] : 0.f;
     const int first = (int)(blockIdx.x / across) * SEQUENCES;
-    float h[SEQUENCES][kScanStates];
+    float h[SEQUENCES][S];
     long len[SEQUENCES];
 #pragma unroll
     for (int s = 0; s < SEQUENCES; s++) {
@@ -402,12 +408,12 @@ __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_sc
         len[s] = first + s < r.B ? fc_scan_length(r, b) : 0;
         const float *from = r.state_in + (b * r.channels + d) * r.N + n0;
 #pragma unroll
-        for (int j = 0; j < kScanStates; j++) h[s][j] = 0.f;
+        for (int j = 0; j < S; j++) h[s][j] = 0.f;
         if (r.state_in && whole) {
             __builtin_memcpy(h[s], from, sizeof h[s]);
         } else if (r.state_in) {
 #pragma unroll
-            for (int j = 0; j < kScanStates; j++)
+            for (int j = 0; j < S; j++)
                 if (n0 + j < r.N) h[s][j] = from[j];
         }
     }
@@ -426,7 +432,7 @@ __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_sc
                 __builtin_memcpy(&C[s], pc + n0, sizeof(V));
             } else {
 #pragma unroll
-                for (int j = 0; j < kScanStates; j++) {
+                for (int j = 0; j < S; j++) {
                     B[s].v[j] = n0 + j < r.N ? pb[n0 + j] : (E)0.f;
                     C[s].v[j] = n0 + j < r.N ? pc[n0 + j] : (E)0.f;
                 }
@@ -442,7 +448,7 @@ __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_sc
             const float v = (float)x[s], dt = steps[s], u = dt * v;
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < kScanStates; j++) {
+            for (int j = 0; j < S; j++) {
                 const float now = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * rate[j]), h[s][j], u * B[s].get(j));
                 h[s][j] = there ? now : h[s][j];
                 sum = __builtin_fmaf(C[s].get(j), now, sum);
@@ -461,70 +467,69 @@ __global__ __launch_bounds__(256) void fc_selective_scan_step_kernel(const fc_sc
             __builtin_memcpy(to, h[s], sizeof h[s]);
         } else {
 #pragma unroll
-            for (int j = 0; j < kScanStates; j++)
+            for (int j = 0; j < S; j++)
                 if (n0 + j < r.N) to[j] = h[s][j];
         }
     }
 }
 
-// Sums over the channels of a wavefront (lanes with the same lane % L) of eight values a lane, v[0..3] and v[4..7]: 16 lanes are left with two
-// each.  Lanes of rows 0 and 1 (16 lanes a row) get sums of v[0..1] and v[2..3], rows 2 and 3 of v[4..5] and v[6..7].
-template <int L>
-__device__ __forceinline__ float2 sum_channels(float (&v)[8]) {
-    float w[4], o[2];
+// The sum of two values over lanes that lie 32 (ROWS: 16) apart: the first where the lane's bit is 0, the second where it is 1.
+template <bool ROWS>
+__device__ __forceinline__ float sum_two(float a, float b) {
+    const unsigned x = __builtin_bit_cast(unsigned, a), y = __builtin_bit_cast(unsigned, b);
+    const auto s = ROWS ? __builtin_amdgcn_permlane16_swap(x, y, false, false) : __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    const unsigned u = s[0], v = s[1];
+    return __builtin_bit_cast(float, u) + __builtin_bit_cast(float, v);
+}
+
+// Sums over the channels of a wavefront (lanes with the same lane % L) of 2 S values a lane, spread over its four rows of 16 lanes: rows 0 and 1 get the first S values'
+// sums, half of them each (S = 1: both the same), rows 2 and 3 the others'.
+template <int L, int S2, int O>
+__device__ __forceinline__ void sum_channels(float (&o)[O], float (&v)[S2]) {
+    constexpr int S = S2 / 2;
+    float w[S];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]), __builtin_bit_cast(unsigned, v[i + 4]), false, false);
-        const unsigned a = s[0], b = s[1];
-        w[i] = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
-    }
+    for (int i = 0; i < S; i++) w[i] = sum_two<false>(v[i], v[i + S]);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, w[i]), __builtin_bit_cast(unsigned, w[i + 2]), false, false);
-        const unsigned a = s[0], b = s[1];
-        o[i] = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+    for (int i = 0; i < O; i++) {
+        o[i] = sum_two<true>(w[i], w[S > 1 ? i + O : i]);
         if (L <= 8) o[i] += dpp<0x128>(o[i]);      // lanes turned by 8 of 16
         if (L <= 4) o[i] += dpp<0x124>(o[i]);
-        if (L <= 2) o[i] += dpp<0x122>(o[i]);
-        if (L <= 1) o[i] += dpp<0x121>(o[i]);
     }
-    return make_float2(o[0], o[1]);
 }
 
 // Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.  Bound by the vector ALUs, busy
 // 77 % of the time with two wavefronts a SIMD (256 registers): 121 instructions for each token of a lane, 64 of them the states' own.  dB and dC are sums over
 // channels, of a wavefront's by lane swaps, of a workgroup's through LDS, of all by a launch of their own, so that their order is always the same.  4 x 3136 tokens of
 // 2048 channels, 16 states, bf16: 507 us.
-template <int DT, int L, bool GATE>
-__global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
-    typedef scan_form<L> F;
-    // Tokens whose states are in registers at a time, and whether their decays are too, by what the other lanes' values leave.  2048 channels of 4 x 3136 tokens
-    // and 16 states: 709 us with 8 and decays, 903 with 16 and decays, 732 with 16 and decays formed again; 1024 channels of 8 x 2048 tokens and 8 states: 449, 712
-    // and 342; 4 states: 363, 363 and, with 32, 369 without decays and 518 with them.
-    constexpr int PART = L == 1 ? 32 : L == 4 || L == 8 ? 8 : 16;
-    constexpr bool KEEP = L > 2;
+template <int DT, int L, int S, bool GATE>
+__global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
+    typedef scan_form<L, S> F;
+    // Tokens whose states and decays are in registers at a time.  2048 channels of 4 x 3136 tokens and 16 states: 709 us with 8, 903 with 16, and 732 with 16 whose
+    // decays are formed again.
+    constexpr int PART = L < 16 ? 8 : 16;
     typedef typename fc_elem<DT>::type E;
-    __shared__ scan_shared<L> lds;
+    __shared__ scan_shared<L, S> lds;
     __shared__ float gs[kScanTile][F::CH], ys[GATE ? kScanTile : 1][GATE ? F::CH : 1];
     __shared__ alignas(16) float waves[F::WAVES][kScanTile][2 * F::NP];      // dB and dC of each wavefront's channels
     __shared__ float2 rows[F::ROWS][F::CH];
-    const scan_place<L> at(r);
+    const scan_place<L, S> at(r);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    float rate[kScanStates], dA[kScanStates] = {0.f, 0.f, 0.f, 0.f}, dD = 0.f, dbias = 0.f;
-    read_rates<L>(r, at, rate);
+    float rate[S], dA[S] = {}, dD = 0.f, dbias = 0.f;
+    read_rates<L, S>(r, at, rate);
     const float bias = r.delta_bias && at.d >= 0 ? r.delta_bias[at.d] : 0.f, skip = r.D && at.d >= 0 ? r.D[at.d] : 0.f;
     const long first = (long)at.walk * r.per_walk, last = first + r.per_walk < r.segments ? first + r.per_walk : r.segments;
     const scan_offsets off(r, at, sizeof(E));
-    scan_tile<DT, L, GATE, true> now;
+    scan_tile<DT, L, S, GATE, true> now;
     if (first * kScanTile < at.len) now.read(r, at, off, first * kScanTile, at.len, true, true, true);
     for (long seg = first; seg < last; seg++) {
         const long t = seg * kScanTile, end = t + kScanTile < r.T ? t + kScanTile : r.T;
         const int n = (int)(at.len - t < 0 ? 0 : at.len - t < kScanTile ? at.len - t : kScanTile);
         float *shared = r.shared + ((at.block * (long)r.B + at.b) * r.T + t) * 2 * r.N;
         if (n > 0) {
-            float start[kScanStates], G[kScanStates];
-            read_states<L>(r, at, r.parts, at.b * r.segments + seg, start);
-            read_states<L>(r, at, r.grads, at.b * r.segments + seg, G);
+            float start[S], G[S];
+            read_states<L, S>(r, at, r.parts, at.b * r.segments + seg, start);
+            read_states<L, S>(r, at, r.grads, at.b * r.segments + seg, G);
             float steps[F::EACH];
 #pragma unroll
             for (int k = 0; k < F::EACH; k++) steps[k] = (float)now.delta[k] + bias;
@@ -540,44 +545,44 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
                 lds.du[i][at.c] = make_float2(steps[k], steps[k] * x);
                 gs[i][at.c] = g;
             }
-            lay_out<L>(lds.b, now.b);
-            lay_out<L>(lds.c, now.c);
+            lay_out<F>(lds.b, now.b);
+            lay_out<F>(lds.c, now.c);
             __syncthreads();
             // Some tokens' states and decays are kept at a time: with all of them there are no registers left for what comes next.  First the states that enter each
             // part but the first; they wait where the sums of the part before theirs will lie.
-            static_assert(PART == kScanTile || sizeof(waves[0][0]) * PART >= 64 * sizeof(float4));
-            auto mid = [&](int part) __attribute__((always_inline)) { return (float4 *)&waves[wave][part - PART][0] + lane; };
-            float h[kScanStates] = {start[0], start[1], start[2], start[3]};
+            static_assert(PART == kScanTile || sizeof(waves[0][0]) * PART >= 64 * S * sizeof(float));
+            auto mid = [&](int part) __attribute__((always_inline)) { return &waves[wave][part - PART][0] + lane * S; };
+            float h[S];
+#pragma unroll
+            for (int j = 0; j < S; j++) h[j] = start[j];
 #pragma unroll 1
             for (int part = PART; part < kScanTile; part += PART) {
 #pragma unroll
                 for (int i = 0; i < PART; i++) {
                     const float2 du = lds.du[part - PART + i][at.chan];
-                    const float4 b = *(const float4 *)&lds.b[part - PART + i][at.sg * kScanStates];
-                    const float bs[4] = {b.x, b.y, b.z, b.w};
+                    float bs[S];
+                    take(bs, &lds.b[part - PART + i][at.sg * S]);
 #pragma unroll
-                    for (int j = 0; j < kScanStates; j++) h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), h[j], du.y * bs[j]);
+                    for (int j = 0; j < S; j++) h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(du.x * rate[j]), h[j], du.y * bs[j]);
                 }
-                *mid(part) = make_float4(h[0], h[1], h[2], h[3]);
+                __builtin_memcpy(__builtin_assume_aligned(mid(part), S * sizeof(float)), h, sizeof h);
             }
 #pragma unroll 1
             for (int part = kScanTile - PART; part >= 0; part -= PART) {
-                float hs[PART][kScanStates], as[KEEP ? PART : 1][kScanStates], enters[kScanStates] = {start[0], start[1], start[2], start[3]};
-                if (part) {
-                    const float4 from = *mid(part);
-                    enters[0] = from.x; enters[1] = from.y; enters[2] = from.z; enters[3] = from.w;
-                }
+                float hs[PART][S], as[PART][S], enters[S];
+#pragma unroll
+                for (int j = 0; j < S; j++) enters[j] = start[j];
+                if (part) take(enters, mid(part));
 #pragma unroll
                 for (int i = 0; i < PART; i++) {
                     if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);      // else all reads move to the front, and registers spill
                     const float2 du = lds.du[part + i][at.chan];
-                    const float4 b = *(const float4 *)&lds.b[part + i][at.sg * kScanStates];
-                    const float bs[4] = {b.x, b.y, b.z, b.w};
+                    float bs[S];
+                    take(bs, &lds.b[part + i][at.sg * S]);
 #pragma unroll
-                    for (int j = 0; j < kScanStates; j++) {
-                        const float decay = __builtin_amdgcn_exp2f(du.x * rate[j]);
-                        if (KEEP) as[KEEP ? i : 0][j] = decay;
-                        hs[i][j] = __builtin_fmaf(decay, i ? hs[i ? i - 1 : 0][j] : enters[j], du.y * bs[j]);
+                    for (int j = 0; j < S; j++) {
+                        as[i][j] = __builtin_amdgcn_exp2f(du.x * rate[j]);
+                        hs[i][j] = __builtin_fmaf(as[i][j], i ? hs[i ? i - 1 : 0][j] : enters[j], du.y * bs[j]);
                     }
                 }
                 fc_wave_sync();
@@ -588,26 +593,28 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
                     if (i % 2) __builtin_amdgcn_sched_barrier(0);
                     const float2 du = lds.du[part + i][at.chan];
                     const float g = gs[part + i][at.chan];
-                    const float4 b = *(const float4 *)&lds.b[part + i][at.sg * kScanStates], c = *(const float4 *)&lds.c[part + i][at.sg * kScanStates];
-                    const float bs[4] = {b.x, b.y, b.z, b.w}, cs[4] = {c.x, c.y, c.z, c.w};
-                    float v[8], du_sum = 0.f, dt_sum = 0.f, y = 0.f;
+                    float bs[S], cs[S];
+                    take(bs, &lds.b[part + i][at.sg * S]);
+                    take(cs, &lds.c[part + i][at.sg * S]);
+                    float v[2 * S], du_sum = 0.f, dt_sum = 0.f, y = 0.f;
 #pragma unroll
-                    for (int j = 0; j < kScanStates; j++) {
+                    for (int j = 0; j < S; j++) {
                         G[j] = __builtin_fmaf(cs[j], g, G[j]);
                         v[j] = G[j] * du.y;
-                        v[4 + j] = g * hs[i][j];
+                        v[S + j] = g * hs[i][j];
                         if (GATE) y = __builtin_fmaf(cs[j], hs[i][j], y);
                         du_sum = __builtin_fmaf(G[j], bs[j], du_sum);
-                        G[j] *= KEEP ? as[KEEP ? i : 0][j] : __builtin_amdgcn_exp2f(du.x * rate[j]);
+                        G[j] *= as[i][j];
                         const float k = G[j] * (i ? hs[i ? i - 1 : 0][j] : enters[j]);
                         dt_sum = __builtin_fmaf(k, rate[j], dt_sum);
                         dA[j] = __builtin_fmaf(k, du.x, dA[j]);
                     }
                     du_sum = sum_states<L>(du_sum);
                     dt_sum = sum_states<L>(dt_sum);
-                    const float2 s = sum_channels<L>(v);
-                    if (L == 16 || (lane & 15) < L)
-                        *(float2 *)&waves[wave][part + i][(lane >> 5) * F::NP + (lane & 15) * kScanStates + (lane >> 4 & 1) * 2] = s;
+                    float s[S < 4 ? 1 : 2];
+                    sum_channels<L>(s, v);
+                    if ((L == 16 || (lane & 15) < L) && (S > 1 || (lane & 16) == 0))
+                        __builtin_memcpy(__builtin_assume_aligned(&waves[wave][part + i][(lane >> 5) * F::NP + (lane & 15) * S + (lane >> 4 & 1) * (S / 2)], sizeof s), s, sizeof s);
                     // each lane keeps one of L tokens
                     if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
                     if (i % L == 0) lds.du[part + i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
                     }
                 }
             }
-            scan_tile<DT, L, GATE, true> here;
+            scan_tile<DT, L, S, GATE, true> here;
             // this tile's values once more: kept, they would leave the states no registers
             here.read(r, at, off, t, at.len, true, false, false);
             __syncthreads();
@@ -670,8 +677,8 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
     // what this walk adds to the gradients of its channels
     float *sums = r.sums + ((at.b * r.walks + at.walk) * r.channels) * (r.N + 2);
 #pragma unroll
-    for (int j = 0; j < kScanStates; j++) {
-        const int s = at.sg * kScanStates + j;
+    for (int j = 0; j < S; j++) {
+        const int s = at.sg * S + j;
         if (at.ds >= 0 && s < r.N) sums[(long)at.ds * (r.N + 2) + s] = dA[j];
     }
     rows[at.row][at.c] = make_float2(dD, dbias);
@@ -688,23 +695,40 @@ __global__ __launch_bounds__(scan_form<L>::THREADS, L == 1 || L == 16 ? 1 : 2) v
     }
 }
 
+// Lanes of a channel and states of a lane for more than 8 states.
+template <class F>
+void with_many_states(int N, F launch) {
+    using std::integral_constant;
+    if (N <= 16) launch(integral_constant<int, 4>(), integral_constant<int, 4>());
+    else if (N <= 32) launch(integral_constant<int, 8>(), integral_constant<int, 4>());
+    else launch(integral_constant<int, 16>(), integral_constant<int, 4>());
+}
+
+// Of tiles: four lanes at least, so that a thread has few tokens along the channels.  4 states, bf16, 22 x 4031 tokens of 192 channels 102 us with four lanes, 108 with
+// two and 192 with one; 2 x 157 of 196 23.1, 31.0 and 54.3; 8 states, 2 x 14926 of 2432 444 with four and 434 with two, 8 x 2048 of 1024 107 and 116.
 template <class F>
 void with_lanes(int N, F launch) {
-    switch (fc_scan_lanes(N)) {
-        case 1: return launch(std::integral_constant<int, 1>());
-        case 2: return launch(std::integral_constant<int, 2>());
-        case 4: return launch(std::integral_constant<int, 4>());
-        case 8: return launch(std::integral_constant<int, 8>());
-        default: return launch(std::integral_constant<int, 16>());
-    }
+    using std::integral_constant;
+    if (N <= 4) launch(integral_constant<int, 4>(), integral_constant<int, 1>());
+    else if (N <= 8) launch(integral_constant<int, 4>(), integral_constant<int, 2>());
+    else with_many_states(N, launch);
+}
+
+// Of single tokens: whole accesses of states.
+template <class F>
+void with_step_lanes(int N, F launch) {
+    using std::integral_constant;
+    if (N <= 4) launch(integral_constant<int, 1>(), integral_constant<int, 4>());
+    else if (N <= 8) launch(integral_constant<int, 2>(), integral_constant<int, 4>());
+    else with_many_states(N, launch);
 }
 
 template <int DT>
 int scan_answers(fc_context *ctx, const fc_scan_run &r) {
-    with_lanes(r.N, [&](auto lanes) {
-        constexpr int L = decltype(lanes)::value;
-        const auto kernel = r.z ? fc_selective_scan_kernel<DT, L, true> : fc_selective_scan_kernel<DT, L, false>;
-        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    with_lanes(r.N, [&](auto lanes, auto states) {
+        constexpr int L = decltype(lanes)::value, S = decltype(states)::value;
+        const auto kernel = r.z ? fc_selective_scan_kernel<DT, L, S, true> : fc_selective_scan_kernel<DT, L, S, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(kScanThreads), 0, ctx->stream>>>(r);
     });
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_kernel");
     return FC_OK;
@@ -712,12 +736,12 @@ int scan_answers(fc_context *ctx, const fc_scan_run &r) {
 
 template <int DT>
 int scan_ends(fc_context *ctx, const fc_scan_run &r) {
-    with_lanes(r.N, [&](auto lanes) {
-        constexpr int L = decltype(lanes)::value;
-        const auto kernel = !r.dy  ? fc_selective_scan_ends_kernel<DT, L, false, false>
-                            : r.z ? fc_selective_scan_ends_kernel<DT, L, true, true>
-                                  : fc_selective_scan_ends_kernel<DT, L, true, false>;
-        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    with_lanes(r.N, [&](auto lanes, auto states) {
+        constexpr int L = decltype(lanes)::value, S = decltype(states)::value;
+        const auto kernel = !r.dy  ? fc_selective_scan_ends_kernel<DT, L, S, false, false>
+                            : r.z ? fc_selective_scan_ends_kernel<DT, L, S, true, true>
+                                  : fc_selective_scan_ends_kernel<DT, L, S, true, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(kScanThreads), 0, ctx->stream>>>(r);
     });
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_ends_kernel");
     return FC_OK;
@@ -729,15 +753,15 @@ constexpr long kManyLanes = 1l << 18;
 
 template <int DT>
 int scan_step(fc_context *ctx, const fc_scan_run &r) {
-    with_lanes(r.N, [&](auto lanes) {
-        constexpr int L = decltype(lanes)::value;
+    with_step_lanes(r.N, [&](auto lanes, auto states) {
+        constexpr int L = decltype(lanes)::value, S = decltype(states)::value;
         const unsigned across = (unsigned)(((long)r.channels * L + 255) / 256);
         if (r.T == 1 && (long)r.channels * L * r.B >= kManyLanes) {
-            constexpr int S = 2;
-            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true, S> : fc_selective_scan_step_kernel<DT, L, false, S>;
-            kernel<<<dim3(across * (unsigned)((r.B + S - 1) / S)), dim3(256), 0, ctx->stream>>>(r, across);
+            constexpr int Q = 2;
+            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, S, true, Q> : fc_selective_scan_step_kernel<DT, L, S, false, Q>;
+            kernel<<<dim3(across * (unsigned)((r.B + Q - 1) / Q)), dim3(256), 0, ctx->stream>>>(r, across);
         } else {
-            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, true, 1> : fc_selective_scan_step_kernel<DT, L, false, 1>;
+            const auto kernel = r.z ? fc_selective_scan_step_kernel<DT, L, S, true, 1> : fc_selective_scan_step_kernel<DT, L, S, false, 1>;
             kernel<<<dim3(across * (unsigned)r.B), dim3(256), 0, ctx->stream>>>(r, across);
         }
     });
@@ -747,10 +771,10 @@ int scan_step(fc_context *ctx, const fc_scan_run &r) {
 
 template <int DT>
 int scan_gradients(fc_context *ctx, const fc_scan_run &r) {
-    with_lanes(r.N, [&](auto lanes) {
-        constexpr int L = decltype(lanes)::value;
-        const auto kernel = r.z ? fc_selective_scan_gradient_kernel<DT, L, true> : fc_selective_scan_gradient_kernel<DT, L, false>;
-        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(scan_form<L>::THREADS), 0, ctx->stream>>>(r);
+    with_lanes(r.N, [&](auto lanes, auto states) {
+        constexpr int L = decltype(lanes)::value, S = decltype(states)::value;
+        const auto kernel = r.z ? fc_selective_scan_gradient_kernel<DT, L, S, true> : fc_selective_scan_gradient_kernel<DT, L, S, false>;
+        kernel<<<dim3((unsigned)((long)r.blocks * r.walks * r.B)), dim3(kScanThreads), 0, ctx->stream>>>(r);
     });
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_gradient_kernel");
     return FC_OK;
