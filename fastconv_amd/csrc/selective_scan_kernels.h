@@ -503,15 +503,16 @@ __device__ __forceinline__ void sum_channels(float (&o)[O], float (&v)[S2]) {
 // channels, of a wavefront's by lane swaps, of a workgroup's through LDS, of all by a launch of their own, so that their order is always the same.  4 x 3136 tokens of
 // 2048 channels, 16 states, bf16: 507 us.
 template <int DT, int L, int S, bool GATE>
-__global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
+__global__ __launch_bounds__(kScanThreads, 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
     typedef scan_form<L, S> F;
+    typedef typename fc_elem<DT>::type E;
     // Tokens whose states and decays are in registers at a time.  2048 channels of 4 x 3136 tokens and 16 states: 709 us with 8, 903 with 16, and 732 with 16 whose
     // decays are formed again.
     constexpr int PART = L < 16 ? 8 : 16;
-    typedef typename fc_elem<DT>::type E;
     __shared__ scan_shared<L, S> lds;
     __shared__ float gs[kScanTile][F::CH], ys[GATE ? kScanTile : 1][GATE ? F::CH : 1];
-    __shared__ alignas(16) float waves[F::WAVES][kScanTile][2 * F::NP];      // dB and dC of each wavefront's channels
+    constexpr int HELD = L < 16 ? kScanTile : PART;      // tokens: with 16 lanes a whole tile of them would leave room for one workgroup a unit
+    __shared__ alignas(16) float waves[F::WAVES][HELD][2 * F::NP];      // dB and dC of each wavefront's channels
     __shared__ float2 rows[F::ROWS][F::CH];
     const scan_place<L, S> at(r);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_sc
             // Some tokens' states and decays are kept at a time: with all of them there are no registers left for what comes next.  First the states that enter each
             // part but the first; they wait where the sums of the part before theirs will lie.
             static_assert(PART == kScanTile || sizeof(waves[0][0]) * PART >= 64 * S * sizeof(float));
-            auto mid = [&](int part) __attribute__((always_inline)) { return &waves[wave][part - PART][0] + lane * S; };
+            auto mid = [&](int part) __attribute__((always_inline)) { return &waves[wave][HELD == PART ? 0 : part - PART][0] + lane * S; };
             float h[S];
 #pragma unroll
             for (int j = 0; j < S; j++) h[j] = start[j];
@@ -567,6 +568,17 @@ __global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_sc
                 }
                 __builtin_memcpy(__builtin_assume_aligned(mid(part), S * sizeof(float)), h, sizeof h);
             }
+            // the workgroup's sums of dB and dC of `count` tokens from `from` on
+            auto add_up = [&](int from, int count) __attribute__((always_inline)) {
+                for (int i = threadIdx.x; i < count * 2 * F::NP; i += F::THREADS) {
+                    const int token = i / (2 * F::NP), k = i % (2 * F::NP), half = k / F::NP, state = k % F::NP;
+                    if (state >= r.N) continue;
+                    float s = waves[0][token][k];
+#pragma unroll
+                    for (int w = 1; w < F::WAVES; w++) s += waves[w][token][k];
+                    shared[((long)(from + token) * 2 + half) * r.N + state] = s;
+                }
+            };
 #pragma unroll 1
             for (int part = kScanTile - PART; part >= 0; part -= PART) {
                 float hs[PART][S], as[PART][S], enters[S];
@@ -614,7 +626,7 @@ __global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_sc
                     float s[S < 4 ? 1 : 2];
                     sum_channels<L>(s, v);
                     if ((L == 16 || (lane & 15) < L) && (S > 1 || (lane & 16) == 0))
-                        __builtin_memcpy(__builtin_assume_aligned(&waves[wave][part + i][(lane >> 5) * F::NP + (lane & 15) * S + (lane >> 4 & 1) * (S / 2)], sizeof s), s, sizeof s);
+                        __builtin_memcpy(__builtin_assume_aligned(&waves[wave][HELD == PART ? i : part + i][(lane >> 5) * F::NP + (lane & 15) * S + (lane >> 4 & 1) * (S / 2)], sizeof s), s, sizeof s);
                     // each lane keeps one of L tokens
                     if (i % L == at.sg) kept = make_float2(du_sum, dt_sum);
                     if (i % L == 0) lds.du[part + i + at.sg][at.chan] = kept;      // these tokens' steps are not needed any more
@@ -624,19 +636,17 @@ __global__ __launch_bounds__(kScanThreads, L == 16 ? 1 : 2) void fc_selective_sc
                         if (i % L == 0) ys[part + i + at.sg][at.chan] = mine;
                     }
                 }
+                if (HELD < kScanTile) {
+                    __syncthreads();
+                    add_up(part, n - part < 0 ? 0 : n - part < PART ? n - part : PART);
+                    if (part) __syncthreads();
+                }
             }
             scan_tile<DT, L, S, GATE, true> here;
             // this tile's values once more: kept, they would leave the states no registers
             here.read(r, at, off, t, at.len, true, false, false);
             __syncthreads();
-            for (int i = threadIdx.x; i < n * 2 * F::NP; i += F::THREADS) {
-                const int token = i / (2 * F::NP), k = i % (2 * F::NP), half = k / F::NP, state = k % F::NP;
-                if (state >= r.N) continue;
-                float s = waves[0][token][k];
-#pragma unroll
-                for (int w = 1; w < F::WAVES; w++) s += waves[w][token][k];
-                shared[((long)token * 2 + half) * r.N + state] = s;
-            }
+            if (HELD == kScanTile) add_up(0, n);
             if (seg + 1 < last && t + kScanTile < at.len) now.read(r, at, off, t + kScanTile, at.len, true, true, true);
             const scan_window<DT> dx(r.dx, at.b * r.x_batch + t * r.x_token + at.first), dd(r.ddelta, at.b * r.delta_batch + t * r.delta_token + at.first);
             const scan_window<DT> dz(r.dz, at.b * r.z_batch + t * r.z_token + at.first);
