@@ -105,26 +105,24 @@ __device__ __forceinline__ void store(E *to, const V &v, int skip) {
         if (i >= skip) to[i] = v.v[i];
 }
 
-// Weights by distance: back[m] belongs to the row m tokens back, so that the loops are the same for every number of taps up to TAPS (2, 3, 4 or 8); those that
-// a convolution lacks are left out, not multiplied by zero.
+// Weights by distance: back[m] belongs to the row m tokens back.
 template <int DT, int VEC, int TAPS>
 __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_params p, int columns) {
     typedef fc_vec<DT, VEC> V;
     typedef typename fc_elem<DT>::type E;
     const conv_place at(p, columns, VEC);
     if (at.none) return;
-    const int taps = TAPS < 8 ? TAPS : p.taps;
-    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (taps - 1) * p.C + at.c;
+    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (TAPS - 1) * p.C + at.c;
     E *y = (E *)p.y + at.b * p.y_batch + at.c;
     float back[VEC][TAPS], bias[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
         bias[v] = p.bias ? p.bias[at.c + v] : 0.f;
 #pragma unroll
-        for (int m = 0; m < TAPS; m++) back[v][m] = m < taps ? p.w[(long)(at.c + v) * taps + taps - 1 - m] : 0.f;
+        for (int m = 0; m < TAPS; m++) back[v][m] = p.w[(long)(at.c + v) * TAPS + TAPS - 1 - m];
     }
     V window[TAPS - 1], now[kAhead], next[kAhead];
-    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.t0, at.len);
+    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.t0, at.len);
     const E *row = x + at.t0 * p.x_token;
     E *to = y + at.t0 * p.y_token;
     read_rows(next, x, row, p.x_token, at.t0, at.len);
@@ -142,7 +140,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
                     float z = bias[v];
 #pragma unroll
                     for (int m = TAPS - 1; m >= 0; m--)
-                        if (m < taps) z = __builtin_fmaf(back[v][m], u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v), z);
+                        z = __builtin_fmaf(back[v][m], u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v), z);
                     if (p.act == FC_ACT_SILU) z = fc_silu(z);
                     out.set(v, edge && t + u >= at.len ? 0.f : z);
                 }
@@ -156,25 +154,25 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
     }
     // The last rows, by whoever read the first: the state may be written over the one before.  Row i lies at or before what it is read from.
     if (at.walk == 0 && p.state_out) {
-        E *after = (E *)p.state_out + at.b * (taps - 1) * p.C + at.c;
-        for (int i = 0; i < taps - 1; i++) {
+        E *after = (E *)p.state_out + at.b * (TAPS - 1) * p.C + at.c;
+        for (int i = 0; i < TAPS - 1; i++) {
             V last[1];
-            read_before(last, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.len - (taps - 1) + i + 1, at.len);
+            read_before(last, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.len - (TAPS - 1) + i + 1, at.len);
             store(after + (long)i * p.C, last[0], at.skip);
         }
     }
 }
 
+// Four wavefronts a SIMD: three, which 133 registers at four taps would leave, take 50 us for 41.  More taps spill there: seven 65 us with what they need, 244 with 128.
 template <int DT, int VEC, int TAPS>
-__global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const conv_params p, int columns) {
+__global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gradient_kernel(const conv_params p, int columns) {
     typedef fc_vec<DT, VEC> V;
     typedef typename fc_elem<DT>::type E;
     const conv_place at(p, columns, VEC);
     if (at.none) return;
-    const int taps = TAPS < 8 ? TAPS : p.taps;
-    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (taps - 1) * p.C + at.c;
-    const E *dy = (const E *)p.dy + at.b * p.y_batch + at.c, *dlast = (const E *)p.dstate_out + at.b * (taps - 1) * p.C + at.c;
-    E *dx = (E *)p.y + at.b * p.x_batch + at.c, *dfirst = (E *)p.dstate_in + at.b * (taps - 1) * p.C + at.c;
+    const E *x = (const E *)p.x + at.b * p.x_batch + at.c, *before = (const E *)p.state_in + at.b * (TAPS - 1) * p.C + at.c;
+    const E *dy = (const E *)p.dy + at.b * p.y_batch + at.c, *dlast = (const E *)p.dstate_out + at.b * (TAPS - 1) * p.C + at.c;
+    E *dx = (E *)p.y + at.b * p.x_batch + at.c, *dfirst = (E *)p.dstate_in + at.b * (TAPS - 1) * p.C + at.c;
     float back[VEC][TAPS], bias[VEC], dback[VEC][TAPS], dbias[VEC], dz[VEC][TAPS];      // dz: of the last tokens, the newest last
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
@@ -182,14 +180,14 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
         dbias[v] = 0.f;
 #pragma unroll
         for (int m = 0; m < TAPS; m++) {
-            back[v][m] = m < taps ? p.w[(long)(at.c + v) * taps + taps - 1 - m] : 0.f;
+            back[v][m] = p.w[(long)(at.c + v) * TAPS + TAPS - 1 - m];
             dback[v][m] = dz[v][m] = 0.f;
         }
     }
     constexpr int AHEAD = kAheadBackward;
     V window[TAPS - 1], now[AHEAD], grads[AHEAD], next[AHEAD], more_grads[AHEAD];
     const V zeros = {};
-    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, taps, at.t0, at.len);
+    read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.t0, at.len);
     const E *row = x + at.t0 * p.x_token, *from = dy + at.t0 * p.y_token;
     E *to = dx + ((long)at.t0 - (TAPS - 1)) * p.x_token;      // of row t - (TAPS - 1), whose gradient is whole once dz_t is there:
     const int end = at.t1 + TAPS - 1;                         // TAPS - 1 tokens past the walk's own
@@ -211,10 +209,10 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 const bool there = !edge || t + u < at.len, mine = !edge || (there && t + u < at.t1);
-                const int r = t + u - (TAPS - 1), last = r - (at.len - (taps - 1));      // last: row of the state after the last token
+                const int r = t + u - (TAPS - 1), last = r - (at.len - (TAPS - 1));      // last: row of the state after the last token
                 V more = zeros, out;
-                const bool wanted = !edge || r >= at.t0 || (at.walk == 0 && r >= 1 - taps && p.dstate_in);
-                if (edge && p.dstate_out && wanted && last >= 0 && last < taps - 1) __builtin_memcpy(&more, dlast + (long)last * p.C, sizeof more);
+                const bool wanted = !edge || r >= at.t0 || (at.walk == 0 && r >= 1 - TAPS && p.dstate_in);
+                if (edge && p.dstate_out && wanted && last >= 0 && last < TAPS - 1) __builtin_memcpy(&more, dlast + (long)last * p.C, sizeof more);
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
                     auto x_back = [&](int m) __attribute__((always_inline)) { return u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v); };
@@ -225,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
                         float z = bias[v];
 #pragma unroll
                         for (int m = TAPS - 1; m >= 0; m--)
-                            if (m < taps) z = __builtin_fmaf(back[v][m], x_back(m), z);
+                            z = __builtin_fmaf(back[v][m], x_back(m), z);
                         g *= fc_silu_slope(z);
                     }
                     if (!there) g = 0.f;      // what was read in place of rows that are not there may be anything
@@ -234,16 +232,16 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
                         dbias[v] += g;
 #pragma unroll
                         for (int m = 0; m < TAPS; m++)
-                            if (m < taps) dback[v][m] = __builtin_fmaf(g, x_back(m), dback[v][m]);
+                            dback[v][m] = __builtin_fmaf(g, x_back(m), dback[v][m]);
                     }
                     float s = edge ? more.get(v) : 0.f;
 #pragma unroll
                     for (int m = 0; m < TAPS; m++)
-                        if (m < taps) s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz of row r + m
+                        s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz of row r + m
                     out.set(v, edge && r >= at.len ? 0.f : s);
                 }
                 if (!edge || (t + u < end && r >= at.t0)) store(to + u * p.x_token, out, at.skip);
-                else if (t + u < end && r < 0 && wanted) store(dfirst + (long)(r + taps - 1) * p.C, out, at.skip);
+                else if (t + u < end && r < 0 && wanted) store(dfirst + (long)(r + TAPS - 1) * p.C, out, at.skip);
             }
         };
         const int inside = at.len < at.t1 ? at.len : at.t1;      // rows of the state after the last token come later
@@ -253,14 +251,14 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_gradient_kernel(const
         move_on(window, now);
     }
     if (!p.part) return;
-    float *part = p.part + (at.b * p.walks + at.walk) * (taps + 1) * p.C + at.c;
+    float *part = p.part + (at.b * p.walks + at.walk) * (TAPS + 1) * p.C + at.c;
 #pragma unroll
     for (int v = 0; v < VEC; v++) {
         if (v < at.skip) continue;
 #pragma unroll
         for (int m = 0; m < TAPS; m++)
-            if (m < taps) part[(long)(taps - 1 - m) * p.C + v] = dback[v][m];
-        part[(long)taps * p.C + v] = dbias[v];
+            part[(long)(TAPS - 1 - m) * p.C + v] = dback[v][m];
+        part[(long)TAPS * p.C + v] = dbias[v];
     }
 }
 
@@ -312,6 +310,9 @@ void with_taps(int taps, F launch) {
     if (taps == 2) launch(dt(), vec(), integral_constant<int, 2>());
     else if (taps == 3) launch(dt(), vec(), integral_constant<int, 3>());
     else if (taps == 4) launch(dt(), vec(), integral_constant<int, 4>());
+    else if (taps == 5) launch(dt(), vec(), integral_constant<int, 5>());
+    else if (taps == 6) launch(dt(), vec(), integral_constant<int, 6>());
+    else if (taps == 7) launch(dt(), vec(), integral_constant<int, 7>());
     else launch(dt(), vec(), integral_constant<int, 8>());
 }
 
