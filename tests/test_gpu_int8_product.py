@@ -236,3 +236,32 @@ def test_single_elements_of_few_tokens(lib, M, N, K_):
         want[m, n] = -21
         assert np.array_equal(got, want)
         lib.release(mark)
+
+
+@pytest.mark.parametrize("M,N,K_,tile,cut", [(64, 8192, 400, 0, False), (3, 70, 33024, 0, True), (300, 300, 8192, 64, True), (4096, 4096, 4096, 256, False)])
+def test_each_way_in_a_graph(lib, M, N, K_, tile, cut):
+    """Captured before anything else has run it: what a kernel needs besides its launch is no part of the capture."""
+    rng = np.random.default_rng(M)
+    mark = lib.mark()
+    try:
+        plan = lib.int8_product_plan(F.Int8ProductShape.packed(M, N, K_, F.F16))
+        assert plan.tile == tile and (plan.parts > 1) == cut
+        x, w, y = lib.alloc(M * K_), lib.upload_raw(rng.integers(-127, 128, (N, K_)).astype(np.int8)), K.Dev(lib, (M, N), "f16")
+        xs, ws = K.floats(lib, np.full(M, 1 / 64)), K.floats(lib, np.full(N, 1 / 64))
+        space = lib.alloc(plan.ws_bytes) if cut else None
+        print("int8 product captured first", M, N, K_, flush=True)
+        lib.graph_begin()
+        lib.int8_product(plan, x, xs, w, ws, y.ptr, None, space)
+        g = lib.graph_end()
+        for turn in range(3):
+            lib.device_copy(x, lib.upload_raw(rng.integers(-127, 128, (M, K_)).astype(np.int8)), M * K_)
+            print("replay", turn, flush=True)
+            lib.graph_launch(g)
+            lib.sync()
+            got = y.get()
+            lib.int8_product(plan, x, xs, w, ws, y.ptr, None, space)
+            lib.sync()
+            assert np.isfinite(got).all() and got.any() and np.array_equal(got, y.get())
+        lib.graph_destroy(g)
+    finally:
+        lib.release(mark)
