@@ -6,6 +6,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr long kMostThreads = 1l << 32;      // of a launch, not reached
 constexpr int kMostStates = 64;
+constexpr long kMostShared = 16384;      // workgroups of the sums of dB and dC
 // Up to so many tokens run without tiles.  16 states, bf16, without and with: 64 sequences of 4096 channels, 1 token 11.8 us and 28.0, 4 tokens 18.4 and 29.1, 8
 // tokens 33.1 and 31.7; one of 2048 channels, 4 tokens 5.4 and 5.9, 8 tokens 7.3 and 6.3.
 constexpr long kMostSteps = 4;
@@ -20,7 +21,7 @@ constexpr long kWorkgroupsBackward = 2048;
 // What enters each segment, from what each adds to none.  Bound by the chain of segments, eight of which are read at once.  GRADS: from the last to the
 // first, and what leaves the first is the gradient of the state before it.
 template <bool GRADS>
-__global__ __launch_bounds__(kThreads) void fc_selective_scan_join_kernel(const fc_scan_run r) {
+__device__ __forceinline__ void join_segments(const fc_scan_run &r) {
     constexpr int AHEAD = 8;
     const long i = (long)blockIdx.x * kThreads + threadIdx.x, size = (long)r.channels * r.N, b = i / size, dn = i - b * size;
     if (b >= r.B) return;
@@ -51,38 +52,53 @@ __global__ __launch_bounds__(kThreads) void fc_selective_scan_join_kernel(const 
     if (GRADS && r.dstate_in) r.dstate_in[i] = s;
 }
 
-// dB and dC of a group from those of its workgroups, always in the same order.
+// States, and in the second row of workgroups gradients.
+__global__ __launch_bounds__(kThreads) void fc_selective_scan_join_kernel(const fc_scan_run r) {
+    if (blockIdx.y == 0) join_segments<false>(r);
+    else join_segments<true>(r);
+}
+
+// Always in the same order: in the first workgroups dA, dD and the gradient of delta_bias from those of each walk, [D][N + 2] each; in the others dB and dC of a group from
+// those of its workgroups.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void fc_selective_scan_shared_kernel(const fc_scan_run r, void *db, void *dc, long values) {
+__global__ __launch_bounds__(kPartThreads) void fc_selective_scan_sums_kernel(const fc_scan_run r, float *dA, float *dD, float *dbias, unsigned first, void *db, void *dc,
+                                                                              long values) {
     typedef typename fc_elem<DT>::type E;
+    if (blockIdx.x < first) {
+        long i;
+        float s;
+        if (!fc_sum_parts(r.sums, (long)r.B * r.walks, (long)r.channels * (r.N + 2), i, s)) return;
+        const long d = i / (r.N + 2);
+        const int n = (int)(i - d * (r.N + 2));
+        if (n < r.N) {
+            if (dA) dA[d * r.N + n] = s;
+        } else if (n == r.N) {
+            if (dD) dD[d] = s;
+        } else if (dbias) {
+            dbias[d] = s;
+        }
+        return;
+    }
     const int per = r.blocks / r.G;
     const long block = (long)r.B * r.T * 2 * r.N;
-    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < values; i += (long)gridDim.x * kThreads) {      // [B][T][G][2][N]
+    for (long i = (long)(blockIdx.x - first) * kPartThreads + threadIdx.x; i < values; i += (long)(gridDim.x - first) * kPartThreads) {      // [B][T][G][2][N]
         long rest = i / r.N;
         const int n = (int)(i - rest * r.N), half = (int)(rest & 1);
         rest >>= 1;
         const long bt = rest / r.G, g = rest - bt * r.G, b = bt / r.T, t = bt - b * r.T;
         const float *p = r.shared + g * per * block + (bt * 2 + half) * r.N + n;
         float s = 0.f;
-        for (int k = 0; k < per; k++) s += p[k * block];
+        int k = 0;
+        for (; k + 8 <= per; k += 8) {      // eight on their way at once
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = p[(k + u) * block];
+#pragma unroll
+            for (int u = 0; u < 8; u++) s += v[u];
+        }
+        for (; k < per; k++) s += p[k * block];
         if (half) ((E *)dc)[b * r.c_batch + t * r.c_token + g * r.c_group + n] = (E)s;
         else ((E *)db)[b * r.b_batch + t * r.b_token + g * r.b_group + n] = (E)s;
-    }
-}
-
-// dA, dD and the gradient of delta_bias from those of each walk, [D][N + 2] each.
-__global__ __launch_bounds__(kPartThreads) void fc_selective_scan_sums_kernel(const fc_scan_run r, float *dA, float *dD, float *dbias) {
-    long i;
-    float s;
-    if (!fc_sum_parts(r.sums, (long)r.B * r.walks, (long)r.channels * (r.N + 2), i, s)) return;
-    const long d = i / (r.N + 2);
-    const int n = (int)(i - d * (r.N + 2));
-    if (n < r.N) {
-        if (dA) dA[d * r.N + n] = s;
-    } else if (n == r.N) {
-        if (dD) dD[d] = s;
-    } else if (dbias) {
-        dbias[d] = s;
     }
 }
 
@@ -129,9 +145,8 @@ fc_scan_run run_of(const fc_selective_scan_shape &s) {
 }
 
 int join(fc_context *ctx, const fc_scan_run &r, bool grads) {
-    const dim3 grid((unsigned)(((long)r.B * r.channels * r.N + kThreads - 1) / kThreads));
-    if (grads) fc_selective_scan_join_kernel<true><<<grid, dim3(kThreads), 0, ctx->stream>>>(r);
-    else fc_selective_scan_join_kernel<false><<<grid, dim3(kThreads), 0, ctx->stream>>>(r);
+    const dim3 grid((unsigned)(((long)r.B * r.channels * r.N + kThreads - 1) / kThreads), grads ? 2 : 1);
+    fc_selective_scan_join_kernel<<<grid, dim3(kThreads), 0, ctx->stream>>>(r);
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_join_kernel");
     return FC_OK;
 }
@@ -149,8 +164,8 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     if (fc_count(workgroups, tiles) < 0 || workgroups * tiles >= kMostThreads / kThreads || fc_count(s->B, s->D) >= kMostThreads / kMostStates ||
         fc_count(s->B * tiles, s->D, kScanTile * kMostStates) < 0)
         return FC_ERR_UNSUPPORTED;
-    // the sums of the gradients of A, D and delta_bias take 32 threads for each
-    if (fc_count(s->D, s->N + 2) >= kMostThreads / 32) return FC_ERR_UNSUPPORTED;
+    // the sums of the gradients of A, D and delta_bias take 32 threads for each, beside which there are workgroups for dB and dC
+    if (fc_count(s->D, s->N + 2) >= kMostThreads / 32 - kMostShared * kPartThreads / 32) return FC_ERR_UNSUPPORTED;
     // a tile's offsets are 31 bits
     const long far = s->x_token | s->delta_token | s->z_token | s->b_token | s->c_token | s->y_token;
     if (s->T > 1 && far >= (1l << 24)) return FC_ERR_UNSUPPORTED;
@@ -245,18 +260,15 @@ extern "C" int fc_selective_scan_backward(fc_context *ctx, const fc_selective_sc
     r.sums = r.shared + (size_t)r.blocks * s.B * s.T * 2 * s.N;
     const fc_device_scope on(ctx);
     int rc = FC_SCAN_CALL(ends, s.dtype, ctx, r);
-    if (rc || (rc = join(ctx, r, false)) || (rc = join(ctx, r, true))) return rc;
+    if (rc || (rc = join(ctx, r, true))) return rc;
     rc = FC_SCAN_CALL(gradients, s.dtype, ctx, r);
     if (rc) return rc;
-    const long values = (long)s.B * s.T * s.G * 2 * s.N, want = (values + kThreads - 1) / kThreads;
-    const auto sum = s.dtype == FC_F32    ? fc_selective_scan_shared_kernel<FC_F32>
-                     : s.dtype == FC_BF16 ? fc_selective_scan_shared_kernel<FC_BF16>
-                                          : fc_selective_scan_shared_kernel<FC_F16>;
-    sum<<<dim3((unsigned)(want < 65536 ? want : 65536)), dim3(kThreads), 0, ctx->stream>>>(r, dB_dev, dC_dev, values);
-    FC_LAUNCH_CHECK(ctx, "fc_selective_scan_shared_kernel");
-    if (!dA_dev && !dD_dev && !ddelta_bias_dev) return FC_OK;
-    fc_selective_scan_sums_kernel<<<dim3((unsigned)(((long)s.D * (s.N + 2) + kPartValues - 1) / kPartValues)), dim3(kPartThreads), 0, ctx->stream>>>(r, dA_dev, dD_dev,
-                                                                                                                                           ddelta_bias_dev);
+    const long values = (long)s.B * s.T * s.G * 2 * s.N, want = (values + kPartThreads - 1) / kPartThreads;
+    const unsigned first = dA_dev || dD_dev || ddelta_bias_dev ? (unsigned)(((long)s.D * (s.N + 2) + kPartValues - 1) / kPartValues) : 0;
+    const auto sums = s.dtype == FC_F32    ? fc_selective_scan_sums_kernel<FC_F32>
+                      : s.dtype == FC_BF16 ? fc_selective_scan_sums_kernel<FC_BF16>
+                                           : fc_selective_scan_sums_kernel<FC_F16>;
+    sums<<<dim3(first + (unsigned)(want < kMostShared ? want : kMostShared)), dim3(kPartThreads), 0, ctx->stream>>>(r, dA_dev, dD_dev, ddelta_bias_dev, first, dB_dev, dC_dev, values);
     FC_LAUNCH_CHECK(ctx, "fc_selective_scan_sums_kernel");
     return FC_OK;
 }

@@ -678,7 +678,7 @@ int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_plan *plan, co
  * group: N values from b*b_batch + t*b_token + group*b_group on.  A is fp32 [D][N], not its logarithm; a rate above 0 is not checked for (the state
  * grows), one of minus infinity is a decay of 0 after a step above 0.  States are packed fp32 [B][D][N].
  * lengths as above: later tokens are not read, their outputs and gradients are zeros, and a state passes an empty sequence unchanged.
- * Limits: N <= 64, B*D < 2^26, D*(N+2) < 2^27, fewer than 2^24 workgroups, of which 32 tokens of 64 channels (N > 16: 32; N > 32: 16) are one; more
+ * Limits: N <= 64, B*D < 2^26, D*(N+2) < 2^27 - 2^19, fewer than 2^24 workgroups, of which 32 tokens of 64 channels (N > 16: 32; N > 32: 16) are one; more
  * than one token: distances of tokens below 2^24 values. */
 typedef struct {
     int B;
