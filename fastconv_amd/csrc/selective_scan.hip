@@ -14,6 +14,9 @@ constexpr long kMostSteps = 4;
 // channels, 16 states, bf16: 8 sequences (1024 wavefronts) 282 us uncut and 238 in 8 segments, 12 of them 353 and 372 in 2.  One sequence of 12544 tokens: 228 us
 // in 56 segments (8192 wavefronts), 237 in 31, 269 in 16; 4 of 3136 tokens 205 in 14, 222 in 8, 252 in 4, 430 uncut.
 constexpr long kEnoughWavefronts = 1536, kWavefronts = 8192;
+// A tile takes a lone workgroup about 4 us, two launches more about 8: 6 sequences of 288 channels, 16 states, tiles of one segment each and uncut: 4 tiles 17.6 and 20.4
+// us, 7 tiles 18.9 and 32.7, 13 tiles 22.4 and 55.9 (32.7 in segments of three).
+constexpr long kLeastTiles = 4;
 // Workgroups of the gradients' kernel, each of which leaves sums of dA: 4 sequences of 3136 tokens, 2048 channels, 16 states 733 us with 1024 of them, 682 with 2048
 // and 693 with 4096; 8 of 2048 tokens, 1024 channels, 8 states 333, 329 and 336.
 constexpr long kWorkgroupsBackward = 2048;
@@ -174,9 +177,9 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     plan->tiles = s->T > kMostSteps ? (int)tiles : 0;
     plan->segments = 1;
     const long wavefronts = workgroups * (kScanThreads / 64);
-    if (plan->tiles && wavefronts < kEnoughWavefronts) {
+    if (tiles >= kLeastTiles && wavefronts < kEnoughWavefronts) {
         long segments = kWavefronts / wavefronts;
-        if (segments > tiles / 2) segments = tiles / 2;
+        if (segments > tiles) segments = tiles;
         if (segments > 1) {
             const long per = (tiles + segments - 1) / segments;
             plan->segments = (int)((tiles + per - 1) / per);

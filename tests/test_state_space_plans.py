@@ -82,7 +82,7 @@ def test_workspaces_hold_what_the_plans_say():
                     rc, p = make("scan", B=b, T=t, D=d, N=n, G=1, **strides)
                     assert rc == 0
                     tiles = -(-t // 32)
-                    assert p.tiles == (tiles if t > 4 else 0) and 1 <= p.segments <= max(1, tiles // 2) and 1 <= p.walks_backward <= tiles
+                    assert p.tiles == (tiles if t > 4 else 0) and 1 <= p.segments <= tiles and 1 <= p.walks_backward <= tiles
                     assert p.ws_bytes == (4 * b * p.segments * d * (n + 1) if p.segments > 1 else 0)
                     assert p.ws_backward_bytes >= 4 * b * tiles * d * (2 * n + 1)
 
