@@ -265,3 +265,16 @@ def test_each_way_in_a_graph(lib, M, N, K_, tile, cut):
         lib.graph_destroy(g)
     finally:
         lib.release(mark)
+
+
+@pytest.mark.parametrize("K_", [1, 3, 12, 15, 16, 17, 31, 67, 130])
+@pytest.mark.parametrize("M,N", [(1, 3), (40, 50), (70, 90), (300, 200)])
+def test_ends_of_rows_of_every_kind(lib, M, N, K_):
+    """Rows without a gap, with one, and with one that is not 16 bytes: what lies behind a row, the next one or nothing, is no part of it."""
+    rng = np.random.default_rng(M + K_)
+    for gap in (0, 5, 40):
+        mark = lib.mark()
+        print("int8 product, ends of rows", M, N, K_, gap, flush=True)
+        x, w = rng.integers(-127, 128, (M, K_)).astype(np.int8), rng.integers(-127, 128, (N, K_)).astype(np.int8)
+        check(lib, x, w, np.ones(M, np.float32), np.ones(N, np.float32), None, "f32", gap=gap, offset=gap % 3)
+        lib.release(mark)
