@@ -17,6 +17,9 @@ constexpr long kEnoughWavefronts = 1536, kWavefronts = 8192;
 // A tile takes a lone workgroup about 4 us, two launches more about 8: 6 sequences of 288 channels, 16 states, tiles of one segment each and uncut: 4 tiles 17.6 and 20.4
 // us, 7 tiles 18.9 and 32.7, 13 tiles 22.4 and 55.9 (32.7 in segments of three).
 constexpr long kLeastTiles = 4;
+// The join goes through the segments one after another, about 0.05 us each against 4 of a tile twice, so that a segment has about the square root of a 160th of the
+// tiles at least.  One sequence of 64 channels, 16 states: 12544 tokens 43.8 us in 196 segments, 58.5 in 392 and 48.8 in 98; 100000 tokens 138, 221 (in 1563) and 127 (391).
+constexpr long kTilesSquared = 160;
 // Workgroups of the gradients' kernel, each of which leaves sums of dA: 4 sequences of 3136 tokens, 2048 channels, 16 states 733 us with 1024 of them, 682 with 2048
 // and 693 with 4096; 8 of 2048 tokens, 1024 channels, 8 states 333, 329 and 336.
 constexpr long kWorkgroupsBackward = 2048;
@@ -178,12 +181,11 @@ extern "C" int fc_selective_scan_make_plan(const fc_selective_scan_shape *s, fc_
     plan->segments = 1;
     const long wavefronts = workgroups * (kScanThreads / 64);
     if (tiles >= kLeastTiles && wavefronts < kEnoughWavefronts) {
-        long segments = kWavefronts / wavefronts;
-        if (segments > tiles) segments = tiles;
-        if (segments > 1) {
-            const long per = (tiles + segments - 1) / segments;
-            plan->segments = (int)((tiles + per - 1) / per);
-        }
+        long least = 1;
+        while (least * least * kTilesSquared < tiles) least++;
+        const long segments = kWavefronts / wavefronts < tiles ? kWavefronts / wavefronts : tiles, even = (tiles + segments - 1) / segments;
+        const long per = even > least ? even : least;
+        plan->segments = (int)((tiles + per - 1) / per);
     }
     if (plan->segments > 1) plan->ws_bytes = (states_of(*s, plan->segments) + (size_t)s->B * plan->segments * s->D) * sizeof(float);
     long walks = (kWorkgroupsBackward + workgroups - 1) / workgroups;

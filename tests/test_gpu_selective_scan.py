@@ -325,3 +325,13 @@ def test_refusals(lib):
         with pytest.raises(F.FastConvError) as e:
             call()
         assert e.value.status == -1, i
+
+
+@pytest.mark.parametrize("case", [(1, 5201, 20, 5, dict()), (2, 5500, 8, 16, dict(dtype="bf16", lengths=[5500, 3003])), (1, 130, 64, 4, dict(dtype="f16", lengths=[97])),
+                                  (3, 257, 130, 2, dict(dtype="bf16", G=2))], ids=lambda c: "-".join(map(str, c[:4])))
+def test_segments_of_one_tile_and_of_several(lib, case):
+    """Every tile a segment, and a join over many segments of several, the last one shorter."""
+    B, T, D, N, how = case
+    plan = lib.selective_scan_plan(F.SelectiveScanShape.packed(B, T, D, N, how.get("G", 1), K.TYPES[how.get("dtype", "f32")]))
+    assert plan.segments == (82 if T == 5201 else 86 if T == 5500 else plan.tiles)
+    test_forward_and_backward(lib, case)
