@@ -11,8 +11,8 @@ constexpr long kMostShared = 16384;      // workgroups of the sums of dB and dC
 // tokens 33.1 and 31.7; one of 2048 channels, 4 tokens 5.4 and 5.9, 8 tokens 7.3 and 6.3.
 constexpr long kMostSteps = 4;
 // A sequence is cut where its channels leave the chip idle, and then into as many segments as fill it: a cut forms every state twice.  2048 tokens of 2048
-// channels, 16 states, bf16: 8 sequences (1024 wavefronts) 282 us uncut and 238 in 8 segments, 12 of them 353 and 372 in 2.  One sequence of 12544 tokens: 228 us
-// in 56 segments (8192 wavefronts), 237 in 31, 269 in 16; 4 of 3136 tokens 205 in 14, 222 in 8, 252 in 4, 430 uncut.
+// channels, 16 states, bf16: 8 sequences (1024 wavefronts) 268 us uncut and 236 in 8 segments, 11 of them 337 and 315 in 5, 12 of them 335 and 336.  One sequence of
+// 12544 tokens: 219 us in 56 segments (8192 wavefronts), 229 in 31, 259 in 16; 4 of 3136 tokens 203 in 14, 216 in 8, 246 in 4, 405 uncut.
 constexpr long kEnoughWavefronts = 1536, kWavefronts = 8192;
 // A tile takes a lone workgroup about 4 us, two launches more about 8: 6 sequences of 288 channels, 16 states, tiles of one segment each and uncut: 4 tiles 17.6 and 20.4
 // us, 7 tiles 18.9 and 32.7, 13 tiles 22.4 and 55.9 (32.7 in segments of three).
