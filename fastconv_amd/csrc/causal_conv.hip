@@ -95,8 +95,8 @@ __device__ __forceinline__ void move_on(V (&window)[W], const V (&now)[N]) {
 }
 
 template <class V, class E>
-__device__ __forceinline__ void store(E *to, const V &v, int skip) {
-    if (!skip) {
+__device__ __forceinline__ void store(E *to, const V &v, int skip, bool whole) {      // whole: no thread of the launch leaves anything out
+    if (whole || !skip) {
         __builtin_memcpy(to, &v, sizeof v);
         return;
     }
@@ -122,6 +122,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
         for (int m = 0; m < TAPS; m++) back[v][m] = p.w[(long)(at.c + v) * TAPS + TAPS - 1 - m];
     }
     V window[TAPS - 1], now[kAhead], next[kAhead];
+    const bool whole = p.C % VEC == 0;
     read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.t0, at.len);
     const E *row = x + at.t0 * p.x_token;
     E *to = y + at.t0 * p.y_token;
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
                     if (p.act == FC_ACT_SILU) z = fc_silu(z);
                     out.set(v, edge && t + u >= at.len ? 0.f : z);
                 }
-                if (!edge || t + u < at.t1) store(to + u * p.y_token, out, at.skip);
+                if (!edge || t + u < at.t1) store(to + u * p.y_token, out, at.skip, whole);
             }
         };
         if (t + kAhead <= (at.len < at.t1 ? at.len : at.t1)) results(std::false_type());
@@ -158,12 +159,12 @@ __global__ __launch_bounds__(kThreads) void fc_causal_conv_kernel(const conv_par
         for (int i = 0; i < TAPS - 1; i++) {
             V last[1];
             read_before(last, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.len - (TAPS - 1) + i + 1, at.len);
-            store(after + (long)i * p.C, last[0], at.skip);
+            store(after + (long)i * p.C, last[0], at.skip, whole);
         }
     }
 }
 
-// Four wavefronts a SIMD: three, which 133 registers at four taps would leave, take 50 us for 41.  More taps spill there: seven 65 us with what they need, 244 with 128.
+// Four wavefronts a SIMD: three, which 133 registers at four taps would leave, take 50 us for 41.  More taps spill there: seven 60 us with the registers that they need, 244 with 128.
 template <int DT, int VEC, int TAPS>
 __global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gradient_kernel(const conv_params p, int columns) {
     typedef fc_vec<DT, VEC> V;
@@ -186,6 +187,7 @@ __global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gr
     }
     constexpr int AHEAD = kAheadBackward;
     V window[TAPS - 1], now[AHEAD], grads[AHEAD], next[AHEAD], more_grads[AHEAD];
+    const bool whole = p.C % VEC == 0;
     const V zeros = {};
     read_before(window, x, p.state_in ? before : nullptr, p.x_token, p.C, TAPS, at.t0, at.len);
     const E *row = x + at.t0 * p.x_token, *from = dy + at.t0 * p.y_token;
@@ -206,6 +208,22 @@ __global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gr
             read_rows(more_grads, dy, from, p.y_token, t + AHEAD, at.len);
         }
         auto results = [&](auto edge) __attribute__((always_inline)) {      // edge: some of the tokens or rows are not there, or another walk's, or in the state
+            auto x_back = [&](int u, int m, int v) __attribute__((always_inline)) { return u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v); };
+            float gs[AHEAD][VEC];
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) gs[u][v] = grads[u].get(v);
+            if (p.act == FC_ACT_SILU)      // one branch for all of them
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) {
+                        float z = bias[v];
+#pragma unroll
+                        for (int m = TAPS - 1; m >= 0; m--) z = __builtin_fmaf(back[v][m], x_back(u, m, v), z);
+                        gs[u][v] *= fc_silu_slope(z);
+                    }
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 const bool there = !edge || t + u < at.len, mine = !edge || (there && t + u < at.t1);
@@ -215,24 +233,16 @@ __global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gr
                 if (edge && p.dstate_out && wanted && last >= 0 && last < TAPS - 1) __builtin_memcpy(&more, dlast + (long)last * p.C, sizeof more);
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
-                    auto x_back = [&](int m) __attribute__((always_inline)) { return u >= m ? now[u >= m ? u - m : 0].get(v) : window[u >= m ? 0 : TAPS - 1 + u - m].get(v); };
 #pragma unroll
                     for (int j = 0; j < TAPS - 1; j++) dz[v][j] = dz[v][j + 1];
-                    float g = grads[u].get(v);
-                    if (p.act == FC_ACT_SILU) {
-                        float z = bias[v];
-#pragma unroll
-                        for (int m = TAPS - 1; m >= 0; m--)
-                            z = __builtin_fmaf(back[v][m], x_back(m), z);
-                        g *= fc_silu_slope(z);
-                    }
+                    float g = gs[u][v];
                     if (!there) g = 0.f;      // what was read in place of rows that are not there may be anything
                     dz[v][TAPS - 1] = g;
                     if (mine) {
                         dbias[v] += g;
 #pragma unroll
                         for (int m = 0; m < TAPS; m++)
-                            dback[v][m] = __builtin_fmaf(g, x_back(m), dback[v][m]);
+                            dback[v][m] = __builtin_fmaf(g, x_back(u, m, v), dback[v][m]);
                     }
                     float s = edge ? more.get(v) : 0.f;
 #pragma unroll
@@ -240,8 +250,8 @@ __global__ __launch_bounds__(kThreads, TAPS <= 4 ? 4 : 2) void fc_causal_conv_gr
                         s = __builtin_fmaf(back[v][m], dz[v][m], s);      // dz of row r + m
                     out.set(v, edge && r >= at.len ? 0.f : s);
                 }
-                if (!edge || (t + u < end && r >= at.t0)) store(to + u * p.x_token, out, at.skip);
-                else if (t + u < end && r < 0 && wanted) store(dfirst + (long)(r + TAPS - 1) * p.C, out, at.skip);
+                if (!edge || (t + u < end && r >= at.t0)) store(to + u * p.x_token, out, at.skip, whole);
+                else if (t + u < end && r < 0 && wanted) store(dfirst + (long)(r + TAPS - 1) * p.C, out, at.skip, whole);
             }
         };
         const int inside = at.len < at.t1 ? at.len : at.t1;      // rows of the state after the last token come later
