@@ -1,13 +1,13 @@
 // RMS norm over rows of channels, after the addition of a residual, with a result in the rows' type or in 8 bits with a scale for each row:
 //
 //   h = x + residual, rounded to the rows' type,   rstd = 1/sqrt(mean of h^2 + eps),   y = h * rstd * gamma
-//   8 bits: scale = max |y| / 127,  q = y / scale rounded to nearest, ties to even
+//   8 bits: scale = max |y| / 127,  q = y / scale rounded to nearest, ties to even, of y in fp32
 //   dh = rstd * (gamma dy - xhat * mean of (gamma dy xhat)) + dsum,   dgamma = sum over rows of dy xhat,   xhat = h * rstd
 //
 // Bound by memory: about 10 operations a value against 8 bytes in 16-bit types.  A row stays in the registers of its wavefronts between its
 // two uses, gamma from row to row.  12544 rows of 2048, bf16, with residual and sum: 32 us in the kernel (206 MB, some of them from the last cache; 41 us where they
-// come from memory, 5.0 TB/s); 9800 rows of 771, fp32: 19.0 us, gradients 17.8 and 4.1 for the sums of dgamma.  rstd is no part of q: y / scale is 127 h gamma / max |h gamma|, so that the sum of squares and the largest
-// value are found together, with one wait.
+// come from memory, 5.0 TB/s); 9800 rows of 771, fp32: 19.0 us, gradients 17.8 and 4.1 for the sums of dgamma.  In 8 bits every step is one fp32 operation, as it is
+// written: a value on the border between two steps goes where it goes for whoever rounds y to fp32 and divides.
 #include <type_traits>
 
 #include "token_types.h"
@@ -17,7 +17,8 @@ namespace {
 constexpr long kMostRows = 1l << 40;
 constexpr int kMostChannels = 1 << 20;
 // Rows whose largest value is smaller are zeros in 8 bits, with a scale of 0: their scale would leave the normal numbers.
-constexpr float kLeastTop = 7.7037197775489434e-34f;      // 2^-110
+constexpr float kLeastTop = 0x1p-110f;
+constexpr float kLeastDivisor = 0x1p-100f;      // a remainder of half a step by it has its last place at 2^-147
 
 enum { TO_TYPE = 0, TO_INT8 = 1, ONLY_INT8 = 2 };      // ONLY_INT8: no norm
 
@@ -180,73 +181,92 @@ __global__ __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) void fc_rms_norm_kern
                 }
             }
         };
-        // the sum of squares and the largest |h gamma|, of h times unit
-        auto measure = [&](bool again, float unit) __attribute__((always_inline)) {
-            float2 m = make_float2(0.f, 0.f);
-            bool bad = false;
-            visit(again, [&](const auto &t, const float *gamma, auto n, int, bool) __attribute__((always_inline)) {
+        // the sum of squares of h times unit
+        auto squares = [&](bool again, float unit) __attribute__((always_inline)) {
+            float sum = 0.f;
+            visit(again, [&](const auto &t, const float *, auto n, int, bool) __attribute__((always_inline)) {
 #pragma unroll
                 for (int v = 0; v < n; v++) {
                     const float s = t.get(v) * unit;
-                    if (TO != ONLY_INT8) m.x = __builtin_fmaf(s, s, m.x);
-                    if (TO != TO_TYPE) {
-                        const float w = TO == ONLY_INT8 ? s : s * gamma[v];
-                        m.y = fmaxf(m.y, __builtin_fabsf(w));
-                        bad |= !(__builtin_fabsf(w) < __builtin_inff());
-                    }
+                    sum = __builtin_fmaf(s, s, sum);
                 }
             });
-            if (TO != TO_TYPE && bad) m.y = __builtin_inff();      // also where it is NaN, which fmaxf drops
-            return join<WAVES>(m, slots, turn++);
+            return join<WAVES>(make_float2(sum, 0.f), slots, turn++).x;
         };
-        float2 m = measure(false, 1.f);
         row_scale s = {1.f, 1.f};
         if constexpr (TO != ONLY_INT8) {
-            float eps = p.eps;
+            float sum = squares(false, 1.f), eps = p.eps;
             // Squares that overflow, or vanish beside no eps to speak of: again, of values near 1.
-            if (!(m.x < 1e36f) || !(m.y < 1e36f) || (m.x < 1e-20f && eps < 1e-20f)) {
-                float2 top = make_float2(0.f, 0.f);
+            if (!(sum < 1e36f) || (sum < 1e-20f && eps < 1e-20f)) {
+                float top = 0.f;
                 visit(true, [&](const auto &t, const float *, auto n, int, bool) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int v = 0; v < n; v++) top.y = fmaxf(top.y, __builtin_fabsf(t.get(v)));
+                    for (int v = 0; v < n; v++) top = fmaxf(top, __builtin_fabsf(t.get(v)));
                 });
-                top = join<WAVES>(top, slots, turn++);
-                if (top.y > 0.f && top.y < __builtin_inff()) {
-                    int e = ilogbf(top.y);
+                top = join<WAVES>(make_float2(0.f, top), slots, turn++).y;
+                if (top > 0.f && top < __builtin_inff()) {
+                    int e = ilogbf(top);
                     if (eps > 0.f && ilogbf(eps) / 2 > e) e = ilogbf(eps) / 2;
                     e = e < -120 ? -120 : e > 120 ? 120 : e;
                     s.unit = ldexpf(1.f, -e);
                     eps = ldexpf(eps, -2 * e);
-                    m = measure(true, s.unit);
+                    sum = squares(true, s.unit);
                 }
             }
-            s.rstd = 1.f / sqrtf(m.x / (float)p.C + eps);
+            s.rstd = 1.f / sqrtf(sum / (float)p.C + eps);
             if (p.rstd && of.me == 0) p.rstd[row] = s.whole();
         }
-        float inv = 0.f;
+        auto result = [&](float h, float gamma) __attribute__((always_inline)) { return TO == ONLY_INT8 ? h : h * s.unit * s.rstd * gamma; };
+        float scale = 0.f, inv = 0.f;
         if constexpr (TO != TO_TYPE) {
-            // y = h unit gamma rstd; q is the same of max |h unit gamma|
-            const float top = m.y * s.rstd;
-            const bool number = top < __builtin_inff();
-            if (top >= kLeastTop && number) inv = 127.f / m.y;
-            if (of.me == 0) p.scale[row] = !number ? __builtin_nanf("") : top >= kLeastTop ? top / 127.f : 0.f;
-        }
-        visit(true, [&](const auto &t, const float *gamma, auto n, int at, bool there) __attribute__((always_inline)) {
-            if constexpr (TO == TO_TYPE) {
-                auto y = t;
-#pragma unroll
-                for (int v = 0; v < n; v++) y.set(v, t.get(v) * s.unit * s.rstd * gamma[v]);
-                if (there) __builtin_memcpy((E *)p.y + row * p.y_row + at, &y, sizeof y);
-            } else {
-                int8_t q[n];
+            float top = 0.f;
+            bool bad = false;
+            visit(TO != ONLY_INT8, [&](const auto &t, const float *gamma, auto n, int, bool) __attribute__((always_inline)) {
 #pragma unroll
                 for (int v = 0; v < n; v++) {
-                    const float w = TO == ONLY_INT8 ? t.get(v) : t.get(v) * s.unit * gamma[v];
-                    q[v] = inv > 0.f ? (int8_t)(int)rintf(w * inv) : (int8_t)0;
+                    const float y = __builtin_fabsf(result(t.get(v), gamma[v]));
+                    top = fmaxf(top, y);
+                    bad |= !(y < __builtin_inff());
                 }
-                if (there) __builtin_memcpy((int8_t *)p.y + row * p.y_row + at, q, n);
+            });
+            if (bad) top = __builtin_inff();      // also where it is NaN, which fmaxf drops
+            top = join<WAVES>(make_float2(0.f, top), slots, turn++).y;
+            const bool number = top < __builtin_inff();
+            if (top >= kLeastTop && number) {
+                scale = top / 127.f;
+                inv = 1.f / scale;
             }
-        });
+            if (of.me == 0) p.scale[row] = number ? scale : __builtin_nanf("");
+        }
+        // y / scale, rounded as a division rounds it: y times 1 / scale, which is off by less than two last places, takes what is left of y twice, the second time from
+        // a last place off at most, so that the remainder is exact and what it adds is off by less than any quotient lies from the middle of two floats (Markstein,
+        // Computation of elementary functions on the IBM RISC System/6000 processor, 1990).  Rows to 8 bits, 12544 of 2048, bf16: 15.3 us, 21.5 where a division decides
+        // next to a border, 13.5 with the first product alone.
+        auto quotient = [&](float y) __attribute__((always_inline)) {
+            float q = y * inv;
+            q = __builtin_fmaf(__builtin_fmaf(-q, scale, y), inv, q);
+            return __builtin_fmaf(__builtin_fmaf(-q, scale, y), inv, q);
+        };
+        auto write = [&](auto smallest) __attribute__((always_inline)) {
+            visit(true, [&](const auto &t, const float *gamma, auto n, int at, bool there) __attribute__((always_inline)) {
+                if constexpr (TO == TO_TYPE) {
+                    auto y = t;
+#pragma unroll
+                    for (int v = 0; v < n; v++) y.set(v, result(t.get(v), gamma[v]));
+                    if (there) __builtin_memcpy((E *)p.y + row * p.y_row + at, &y, sizeof y);
+                } else {
+                    int8_t q[n];
+#pragma unroll
+                    for (int v = 0; v < n; v++) {
+                        const float y = result(t.get(v), gamma[v]);
+                        q[v] = smallest ? scale > 0.f ? (int8_t)(int)rintf(y / scale) : (int8_t)0 : (int8_t)(int)rintf(quotient(y));
+                    }
+                    if (there) __builtin_memcpy((int8_t *)p.y + row * p.y_row + at, q, n);
+                }
+            });
+        };
+        if (TO == TO_TYPE || scale >= kLeastDivisor) write(std::false_type());
+        else write(std::true_type());
     }
 }
 

@@ -600,8 +600,9 @@ int fc_rms_norm_make_plan(const fc_rms_norm_shape *shape, fc_rms_norm_plan *plan
 int fc_rms_norm(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x_dev, const void *residual_dev, const float *gamma_dev,
                 void *sum_dev, void *y_dev, float *rstd_dev);
 
-/* The same in 8 bits with a scale for each row: scale = max |y| / 127, q = y / scale rounded to nearest, ties to even.  A row whose largest value is below
- * 2^-110 is zeros with a scale of 0; one with a value that is not finite is zeros with a scale of NaN, so that a product of it is NaN. */
+/* The same in 8 bits with a scale for each row: scale = max |y| / 127, q = y / scale rounded to nearest, ties to even.  y is in fp32 here, whatever the
+ * tensors' type, and every product and quotient is one fp32 operation: fc_quantize_rows makes the same bits of the same rows of y.  A row whose largest value
+ * is below 2^-110 is zeros with a scale of 0; one with a value that is not finite is zeros with a scale of NaN, so that a product of it is NaN. */
 int fc_rms_norm_int8(fc_context *ctx, const fc_rms_norm_plan *plan, const void *x_dev, const void *residual_dev, const float *gamma_dev,
                      void *sum_dev, int8_t *q_dev, float *scale_dev);
 
