@@ -70,3 +70,26 @@ def test_values_on_the_border_between_two_steps(lib, rows, C, dtype):
         assert np.array_equal(scale.get(), want_scale) and np.array_equal(lib.download(q, (rows, C), np.int8), want)
     finally:
         lib.release(mark)
+
+
+@pytest.mark.parametrize("C", [40, 2048, 9001, 40001])
+@pytest.mark.parametrize("size,eps", [(2.0 ** -122, 1e-8), (1e-36, 1e-8), (2e-38, 1e-12), (1e-40, 1e-19), (3e-32, 1e-5), (2e-36, 3e-7)])
+def test_small_rows_beside_a_small_eps(lib, C, size, eps):
+    """Rows far below the root of eps, whose results are still numbers: the norm multiplies them by up to 1 / sqrt(eps), and 127 over their own largest
+    value would be infinite.  y errs by its two products and rstd's rounding, which its scale shares: 8 last places of up to 127 as elsewhere, and
+    subnormal values of x are exact."""
+    rng = np.random.default_rng(C)
+    mark = lib.mark()
+    try:
+        print("small rows", C, size, eps, flush=True)
+        h = K.to_type(size * rng.uniform(0.5, 2, (3, C)) * rng.choice((-1, 1), (3, C)), "f32")[1]
+        gamma = (1 + 0.2 * rng.standard_normal(C)).astype(f32)
+        x, scale, q = K.Dev(lib, (3, C), "f32", None, h), K.Dev(lib, (3,), "f32"), lib.alloc(3 * C)
+        lib.rms_norm_int8(lib.rms_norm_plan(F.RmsNormShape.packed(3, C, F.F32, eps)), x.ptr, K.floats(lib, gamma), q, scale.ptr)
+        want, _ = S.rms_norm(h, gamma.astype(np.float64), np.float64(f32(eps)))
+        top = np.abs(want).max(axis=1)
+        assert (top > 2.0 ** -109).all()      # rows that the interface promises to round
+        S.close(scale.get(), top / 127, 56 * K.EPS * top / 127, "scale")
+        S.close(lib.download(q, (3, C), np.int8).astype(np.float64), want * (127 / top)[:, None], 0.5 + 127 * 8 * K.EPS, "q")
+    finally:
+        lib.release(mark)
