@@ -13,10 +13,8 @@
 // B and C do; so the inner loop is S states' exponentials and multiply-adds.
 #pragma once
 
+#include "selective_scan_forms.h"
 #include "token_math.h"
-
-constexpr int kScanTile = 32;      // tokens
-constexpr int kScanThreads = 256;
 
 struct fc_scan_run {
     const void *x, *delta, *b, *c, *z, *dy;
@@ -38,8 +36,6 @@ struct fc_scan_run {
     long x_batch, x_token, delta_batch, delta_token, z_batch, z_token, y_batch, y_token;
     long b_batch, b_token, b_group, c_batch, c_token, c_group;
 };
-
-static inline int fc_scan_channels(int N) { return kScanThreads / (N <= 16 ? 4 : N <= 32 ? 8 : 16); }      // of a workgroup, each with so many lanes
 
 // selective_scan_<type>.hip.  ends: parts, steps and, if dy is there, grads of each segment.  answers: y and the last state, each segment from what
 // enters it.  step: the same for a few tokens.  gradients: of each segment, from what enters it on both sides.

@@ -23,14 +23,6 @@ __device__ __forceinline__ float sum_states(float v) {
     return v;
 }
 
-// Channels have L lanes of S states each.
-template <int L, int S>
-struct scan_form {
-    static constexpr int THREADS = kScanThreads, CH = THREADS / L, WAVES = THREADS / 64, NP = L * S;
-    static constexpr int ROWS = THREADS / CH, EACH = kScanTile / ROWS;      // tokens at once, and of a thread, where threads lie along the channels
-    static constexpr int SHARED = (kScanTile * NP + THREADS - 1) / THREADS;      // values of B of a thread
-};
-
 // Where a workgroup is, and its threads in both of their arrangements.
 template <int L, int S>
 struct scan_place {
@@ -52,16 +44,14 @@ struct scan_place {
         group = block / per;
         const int from = (block - group * per) * F::CH, tid = threadIdx.x;
         first = group * (long)r.per_group + from;
-        c = tid % F::CH;
-        row = tid / F::CH;
+        c = F::channel(tid);
+        row = F::row(tid);
         chan = tid / L;
         sg = tid % L;
         d = from + c < r.per_group ? group * r.per_group + from + c : -1;
         ds = from + chan < r.per_group ? group * r.per_group + from + chan : -1;
     }
 };
-
-constexpr uint32_t kNowhere = 0x80000000u;
 
 // A thread's offsets in bytes into tiles of the tensors, and the tokens' distances.
 struct scan_offsets {
@@ -76,15 +66,13 @@ struct scan_offsets {
         y_token = (uint32_t)r.y_token * es;
         b_token = (uint32_t)r.b_token * es;
         c_token = (uint32_t)r.c_token * es;
-        const uint32_t none = at.d >= 0 ? 0 : kNowhere, lane = at.c * es | none, row = at.row;
-        x = lane + row * x_token;
-        delta = lane + row * delta_token;
-        z = lane + row * z_token;
-        y = lane + row * y_token;
-        const int n = threadIdx.x % F::NP;
-        const uint32_t state = n < r.N ? n * es : kNowhere, token = threadIdx.x / F::NP;
-        b = state + token * b_token;
-        c = state + token * c_token;
+        const bool there = at.d >= 0;
+        x = F::channel_offset(threadIdx.x, there, es, x_token);
+        delta = F::channel_offset(threadIdx.x, there, es, delta_token);
+        z = F::channel_offset(threadIdx.x, there, es, z_token);
+        y = F::channel_offset(threadIdx.x, there, es, y_token);
+        b = F::shared_offset(threadIdx.x, r.N, es, b_token);
+        c = F::shared_offset(threadIdx.x, r.N, es, c_token);
     }
 };
 
@@ -131,7 +119,6 @@ struct scan_tile {
         const W wx(r.x, at.b * r.x_batch + t0 * r.x_token + at.first), wd(r.delta, at.b * r.delta_batch + t0 * r.delta_token + at.first);
         const W wz(r.z, at.b * r.z_batch + t0 * r.z_token + at.first), wy(r.dy, at.b * r.y_batch + t0 * r.y_token + at.first);
         const W wb(r.b, at.b * r.b_batch + t0 * r.b_token + at.group * r.b_group), wc(r.c, at.b * r.c_batch + t0 * r.c_token + at.group * r.c_group);
-        constexpr int BC = F::THREADS / F::NP;      // tokens of B and C at once
         auto all = [&](auto each, auto several) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < F::EACH && channels; k++) {
@@ -148,14 +135,14 @@ struct scan_tile {
         };
         if (n == kScanTile) {
             all([&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) { return w.get(lane, k * F::ROWS * token); },
-                [&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) { return w.get(lane, k * BC * token); });
+                [&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) { return w.get(lane, k * F::BC * token); });
         } else {
-            const int row = threadIdx.x / F::NP;
+            const int row = F::shared_token(threadIdx.x);
             all([&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) {
                     return w.get(at.row + k * F::ROWS < n ? lane + k * F::ROWS * token : kNowhere, 0);
                 },
                 [&](const W &w, uint32_t lane, uint32_t token, int k) __attribute__((always_inline)) {
-                    return w.get(row + k * BC < n ? lane + k * BC * token : kNowhere, 0);
+                    return w.get(row + k * F::BC < n ? lane + k * F::BC * token : kNowhere, 0);
                 });
         }
     }
@@ -703,34 +690,6 @@ __global__ __launch_bounds__(kScanThreads, 2) void fc_selective_scan_gradient_ke
         sums[(long)at.d * (r.N + 2) + r.N] = s.x;
         sums[(long)at.d * (r.N + 2) + r.N + 1] = s.y;
     }
-}
-
-// Lanes of a channel and states of a lane for more than 8 states.
-template <class F>
-void with_many_states(int N, F launch) {
-    using std::integral_constant;
-    if (N <= 16) launch(integral_constant<int, 4>(), integral_constant<int, 4>());
-    else if (N <= 32) launch(integral_constant<int, 8>(), integral_constant<int, 4>());
-    else launch(integral_constant<int, 16>(), integral_constant<int, 4>());
-}
-
-// Of tiles: four lanes at least, so that a thread has few tokens along the channels.  4 states, bf16, 22 x 4031 tokens of 192 channels 102 us with four lanes, 108 with
-// two and 192 with one; 2 x 157 of 196 23.1, 31.0 and 54.3; 8 states, 2 x 14926 of 2432 444 with four and 434 with two, 8 x 2048 of 1024 107 and 116.
-template <class F>
-void with_lanes(int N, F launch) {
-    using std::integral_constant;
-    if (N <= 4) launch(integral_constant<int, 4>(), integral_constant<int, 1>());
-    else if (N <= 8) launch(integral_constant<int, 4>(), integral_constant<int, 2>());
-    else with_many_states(N, launch);
-}
-
-// Of single tokens: whole accesses of states.
-template <class F>
-void with_step_lanes(int N, F launch) {
-    using std::integral_constant;
-    if (N <= 4) launch(integral_constant<int, 1>(), integral_constant<int, 4>());
-    else if (N <= 8) launch(integral_constant<int, 2>(), integral_constant<int, 4>());
-    else with_many_states(N, launch);
 }
 
 template <int DT>
