@@ -370,7 +370,7 @@ extern "C" int fc_causal_conv(fc_context *ctx, const fc_causal_conv_plan *plan, 
     const uint64_t addr = (uint64_t)x_dev | (uint64_t)y_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev;
     if ((addr & (fc_elem_size(s.dtype) - 1)) || (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)lengths_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: unaligned pointer");
-    if (!fc_apart(s.B, s.y_batch, s.C) || !fc_apart(s.T, s.y_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: tokens of y overlap");
+    if (!fc_apart({{s.B, s.y_batch}, {s.T, s.y_token}}, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv: tokens of y overlap");
     const int columns = columns_of(s);
     conv_params p = params_of(s, plan->walks);
     p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = y_dev; p.state_in = state_in_dev; p.state_out = state_out_dev; p.lengths = lengths_dev;
@@ -395,7 +395,7 @@ extern "C" int fc_causal_conv_backward(fc_context *ctx, const fc_causal_conv_pla
     if ((addr & (fc_elem_size(s.dtype) - 1)) ||
         (((uint64_t)w_dev | (uint64_t)bias_dev | (uint64_t)dw_dev | (uint64_t)dbias_dev | (uint64_t)lengths_dev | (uint64_t)ws_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: unaligned pointer");
-    if (!fc_apart(s.B, s.x_batch, s.C) || !fc_apart(s.T, s.x_token, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: tokens of dx overlap");
+    if (!fc_apart({{s.B, s.x_batch}, {s.T, s.x_token}}, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_causal_conv_backward: tokens of dx overlap");
     const int columns = columns_of(s);
     conv_params p = params_of(s, plan->walks_backward);
     p.dy = dy_dev; p.x = x_dev; p.w = w_dev; p.bias = bias_dev; p.y = dx_dev; p.state_in = state_in_dev; p.dstate_out = dstate_out_dev;

@@ -209,7 +209,7 @@ extern "C" int fc_selective_scan(fc_context *ctx, const fc_selective_scan_plan *
         (((uint64_t)A_dev | (uint64_t)D_dev | (uint64_t)delta_bias_dev | (uint64_t)state_in_dev | (uint64_t)state_out_dev | (uint64_t)lengths_dev |
           (uint64_t)ws_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: unaligned pointer");
-    if (!fc_apart(s.B, s.y_batch, s.D) || !fc_apart(s.T, s.y_token, s.D)) return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: tokens of y overlap");
+    if (!fc_apart({{s.B, s.y_batch}, {s.T, s.y_token}}, s.D)) return fail(ctx, FC_ERR_INVALID, "fc_selective_scan: tokens of y overlap");
     fc_scan_run r = run_of(s);
     r.x = x_dev; r.delta = delta_dev; r.A = A_dev; r.b = B_dev; r.c = C_dev; r.D = D_dev; r.z = z_dev; r.delta_bias = delta_bias_dev; r.y = y_dev;
     r.state_in = state_in_dev; r.state_out = state_out_dev; r.lengths = lengths_dev;
@@ -245,9 +245,9 @@ extern "C" int fc_selective_scan_backward(fc_context *ctx, const fc_selective_sc
     const uint64_t floats = (uint64_t)A_dev | (uint64_t)D_dev | (uint64_t)delta_bias_dev | (uint64_t)dA_dev | (uint64_t)dD_dev | (uint64_t)ddelta_bias_dev |
                             (uint64_t)state_in_dev | (uint64_t)dstate_out_dev | (uint64_t)dstate_in_dev | (uint64_t)lengths_dev | (uint64_t)ws_dev;
     if ((addr & (fc_elem_size(s.dtype) - 1)) || (floats & 3)) return fail(ctx, FC_ERR_INVALID, "fc_selective_scan_backward: unaligned pointer");
-    if (!fc_apart(s.B, s.x_batch, s.D) || !fc_apart(s.T, s.x_token, s.D) || !fc_apart(s.B, s.delta_batch, s.D) || !fc_apart(s.T, s.delta_token, s.D) ||
-        (z_dev && (!fc_apart(s.B, s.z_batch, s.D) || !fc_apart(s.T, s.z_token, s.D))) || !fc_apart(s.B, s.b_batch, s.N) || !fc_apart(s.T, s.b_token, s.N) ||
-        !fc_apart(s.G, s.b_group, s.N) || !fc_apart(s.B, s.c_batch, s.N) || !fc_apart(s.T, s.c_token, s.N) || !fc_apart(s.G, s.c_group, s.N))
+    if (!fc_apart({{s.B, s.x_batch}, {s.T, s.x_token}}, s.D) || !fc_apart({{s.B, s.delta_batch}, {s.T, s.delta_token}}, s.D) ||
+        (z_dev && !fc_apart({{s.B, s.z_batch}, {s.T, s.z_token}}, s.D)) || !fc_apart({{s.B, s.b_batch}, {s.T, s.b_token}, {s.G, s.b_group}}, s.N) ||
+        !fc_apart({{s.B, s.c_batch}, {s.T, s.c_token}, {s.G, s.c_group}}, s.N))
         return fail(ctx, FC_ERR_INVALID, "fc_selective_scan_backward: tokens of a gradient overlap");
     fc_scan_run r = run_of(s);
     r.dy = dy_dev; r.x = x_dev; r.delta = delta_dev; r.A = A_dev; r.b = B_dev; r.c = C_dev; r.D = D_dev; r.z = z_dev; r.delta_bias = delta_bias_dev;

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include "fc_internal.h"
+#include "token_layout.h"
 
 template <int DT>
 struct fc_elem;
@@ -87,9 +88,6 @@ static inline long fc_count(long a, long b, long c = 1) {
     const __int128 p = (__int128)a * b * c;
     return p < 0 || p > ((__int128)1 << 62) ? -1 : (long)p;
 }
-
-// Rows of so many elements, n of them a stride apart, share none.
-static inline bool fc_apart(long n, long stride, long row) { return n < 2 || stride >= row; }
 
 // The context's device, for as long as a call launches on it: a stream takes launches of its own device only.
 struct fc_device_scope {

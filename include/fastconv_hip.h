@@ -640,7 +640,10 @@ int fc_int8_product_make_plan(const fc_int8_product_shape *shape, fc_int8_produc
 int fc_int8_product(fc_context *ctx, const fc_int8_product_plan *plan, const int8_t *x_dev, const float *x_scale_dev, const int8_t *w_dev,
                     const float *w_scale_dev, const float *bias_dev, void *y_dev, void *ws_dev);
 
-/* Short causal convolution of each channel over the tokens of a sequence, with its activation (FC_ACT_NONE or FC_ACT_SILU):
+/* What the calls below write shares nothing: answers or gradients of which two tokens, sequences or groups have an element in common are refused.  Inputs may lie
+ * anyhow.
+ *
+ * Short causal convolution of each channel over the tokens of a sequence, with its activation (FC_ACT_NONE or FC_ACT_SILU):
  *   y_t = act(bias + sum over j < taps of w[c][j] x_(t - taps + 1 + j))
  * Token t of sequence b begins at b*x_batch + t*x_token, and so for y; dy as y, dx as x.  w is fp32 [C][taps], the last tap the token's own.  The inputs before
  * the first token are a state of taps - 1 rows, packed [B][taps - 1][C] in the tensors' type, the oldest first.
