@@ -64,6 +64,16 @@ __device__ __forceinline__ void put_part(const product_params &p, long m, int n,
         if (n + i < p.N) to[i] = sum[i];
 }
 
+// sum * xs * ws, and a bias: a sum below 2^31 times a scale above 2^96 may leave fp32's numbers although the other scale brings it back, so that one goes first then.
+__device__ __forceinline__ float scaled(int sum, float xs, float ws) {
+    const bool far = __builtin_fabsf(xs) > 0x1p96f;
+    return (float)sum * (far ? ws : xs) * (far ? xs : ws);
+}
+__device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
+    const bool far = __builtin_fabsf(xs) > 0x1p96f;
+    return __builtin_fmaf((float)sum * (far ? ws : xs), far ? xs : ws, bias);
+}
+
 // Four neighbouring channels, from n on, of token m.
 template <int DT>
 __device__ __forceinline__ void put(const product_params &p, long m, int n, const int (&sum)[4], float xs) {
@@ -75,13 +85,13 @@ __device__ __forceinline__ void put(const product_params &p, long m, int n, cons
         if (p.bias) __builtin_memcpy(bias, p.bias + n, sizeof bias);
         fc_vec<DT, 4> out;
 #pragma unroll
-        for (int i = 0; i < 4; i++) out.set(i, p.bias ? __builtin_fmaf((float)sum[i] * xs, ws[i], bias[i]) : (float)sum[i] * xs * ws[i]);
+        for (int i = 0; i < 4; i++) out.set(i, p.bias ? scaled(sum[i], xs, ws[i], bias[i]) : scaled(sum[i], xs, ws[i]));
         __builtin_memcpy(y, &out, sizeof out);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (n + i < p.N) y[i] = (E)(p.bias ? __builtin_fmaf((float)sum[i] * xs, p.w_scale[n + i], p.bias[n + i]) : (float)sum[i] * xs * p.w_scale[n + i]);
+        if (n + i < p.N) y[i] = (E)(p.bias ? scaled(sum[i], xs, p.w_scale[n + i], p.bias[n + i]) : scaled(sum[i], xs, p.w_scale[n + i]));
 }
 
 // What a lane has of a product of 16 tokens and 16 channels: column, a token; four rows, channels.
@@ -436,8 +446,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) v
                 fc_vec<DT, 4> out;
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    const float product = (float)sum[i][j][4 * g + v] * xs[i];
-                    out.set(v, p.bias ? __builtin_fmaf(product, ws[j][g][v], bias[j][g][v]) : product * ws[j][g][v]);
+                    const int whole = sum[i][j][4 * g + v];
+                    out.set(v, p.bias ? scaled(whole, xs[i], ws[j][g][v], bias[j][g][v]) : scaled(whole, xs[i], ws[j][g][v]));
                 }
                 *(fc_vec<DT, 4> *)(mine + r * PITCH + (32 * j + 8 * g + 4 * half) * sizeof(E)) = out;
             }
