@@ -31,7 +31,7 @@ struct conv_params {
     float *part;             // backward: [B * walks][taps + 1][C], the sums of dw and, last, dbias
     const int32_t *lengths;
     long T, walk;            // tokens of a sequence and of a walk
-    int B, C, taps, walks, act;
+    int B, C, walks, act;
     fc_fastdiv by_columns, by_walks;
     long x_batch, x_token, y_batch, y_token;
 
@@ -336,7 +336,7 @@ void with_kernel(const fc_causal_conv_shape &s, F launch) {
 
 conv_params params_of(const fc_causal_conv_shape &s, int walks) {
     conv_params p = {};
-    p.B = s.B; p.T = s.T; p.C = s.C; p.taps = s.taps; p.act = s.act;
+    p.B = s.B; p.T = s.T; p.C = s.C; p.act = s.act;
     p.walks = walks;
     p.walk = (s.T + walks - 1) / walks;
     p.by_columns = fc_make_fastdiv((uint32_t)columns_of(s));

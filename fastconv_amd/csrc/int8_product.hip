@@ -518,7 +518,7 @@ constexpr long kUnits = 256;      // compute units
 // Few tokens.  Wide workgroups read x seldom, many read w side by side: the widest of which there is one a unit.  8192 channels of 4096, 64 tokens: 64x32 8.4 us,
 // 32x32 11.5, 16x32 16.5; 4096 channels 7.8, 6.3 and 8.6; 2048 channels 6.9, 5.4 and 5.0; 32 tokens of 8192 channels 7.3, 6.6 and 8.8; 16 tokens of 8192 channels
 // 16x32 5.3 and 16x16 6.0.
-product_form few_form(long M, int N, int K) {
+product_form few_form(long M, int N) {
     const int forms[4][2] = {{4, 2}, {2, 2}, {1, 2}, {1, 1}};
     product_form f = {};
     for (const auto &v : forms) {
@@ -615,7 +615,7 @@ int run_form(fc_context *ctx, product_params p, const product_form &f, bool dire
 template <int DT>
 int run(fc_context *ctx, const product_params &p, const fc_int8_product_plan *plan, bool direct, void *ws) {
     if (p.M <= kFewTokens) {
-        product_form f = few_form(p.M, p.N, p.K);
+        product_form f = few_form(p.M, p.N);
         f.parts = plan->parts;
         return run_form<DT>(ctx, p, f, direct, ws);
     }
@@ -639,7 +639,7 @@ extern "C" int fc_int8_product_make_plan(const fc_int8_product_shape *s, fc_int8
     *plan = {};
     product_form f;
     if (s->M <= kFewTokens) {
-        f = few_form(s->M, s->N, s->K);
+        f = few_form(s->M, s->N);
         cut(f, ceil_div(s->M, 16 * f.mf) * ceil_div(s->N, 16 * f.nf), s->K, 32768);
     } else {
         f = best_tile(s->M, s->N, s->K);
