@@ -5,8 +5,8 @@
 //
 // Bound by memory: 2 * taps operations a value against 4 bytes read and written in 16-bit types.  A thread walks down the tokens of a few
 // neighbouring channels with the last rows in registers, so that every row is read once; sequences are cut into walks to fill the chip, each of
-// which reads the taps - 1 rows before its own (backward: and after) once more.  4 x 3136 tokens of 2048 channels, four taps, bf16: 23.8 us (103 MB, 4.3 TB/s),
-// gradients 36.8 us (154 MB, 4.2 TB/s) and 4.2 for the sums of the walks' parts.
+// which reads the taps - 1 rows before its own (backward: and after) once more.  4 x 3136 tokens of 2048 channels, four taps, bf16: 24 to 28 us (103 MB, about
+// 4 TB/s), gradients 37 to 41 us (154 MB) and 4.2 for the sums of the walks' parts.
 #include <type_traits>
 
 #include "token_math.h"

@@ -267,8 +267,8 @@ __global__ __launch_bounds__(64 * WAVES) void fc_int8_product_ring_kernel(const 
 // Many tokens: tiles of BM tokens x BN channels, WM x WN wavefronts, stages of 64 bytes of the rows in LDS, read two stages before they are ready and one
 // more before they are used, so that a wavefront's first operands of a stage arrive under the products of the one before.  Word c of a stage's row lies
 // at place c ^ (row / 4 % 4): 16 neighbouring rows' words of one k cover all banks.  DIRECT: rows begin on and are multiples of 16 bytes, which go to
-// LDS without passing registers.  12544 x 8192 of 4096, bf16: 445 us, 1.89e15 operations a second; 8192 x 8192 of 8192 2.19e15.  Bound by power and LDS: the same with
-// zeros for values takes 349 us, 12288 rows (six tiles a unit instead of 49 / 8) 411; four wavefronts of 128 x 128 479, stages begun in turn by the workgroups 446 to 461.
+// LDS without passing registers.  12544 x 8192 of 4096, bf16: 435 to 453 us, 1.86 to 1.94e15 operations a second; 8192 x 8192 of 8192 2.19e15.  The clock gives way to
+// power: the same with zeros for values takes 349 us; 12288 rows (six tiles a unit instead of 49 / 8) 411; four wavefronts of 128 x 128 479, stages begun in turn by the workgroups 446 to 461.
 template <int DT, int BM, int BN, int WM, int WN, int BUFFERS, bool DIRECT>
 __global__ __launch_bounds__(64 * WM * WN, BM / WM * (BN / WN) > 8192 ? 1 : 2) void fc_int8_product_kernel(const product_params p) {
     constexpr int WAVES = WM * WN, THREADS = 64 * WAVES, MI = BM / WM / 32, NI = BN / WN / 32, WORDS = (BM + BN) * 4, EACH = WORDS / THREADS;

@@ -199,8 +199,8 @@ __device__ __forceinline__ void write_states(const fc_scan_run &r, const scan_pl
 }
 
 // Answers.  Bound by the vector ALUs, which are busy 99 % of the time: an exponential (two instructions' time) and four instructions a state, and for each token of a
-// lane about 15 more, 4 of which sum the lanes' parts, 5 form the step and 3 the gate.  12544 tokens of 2048 channels, 16 states, bf16: 114 us, of which 62 are the
-// states' own.  u B through 4x4x1 matrix instructions takes 12 cycles of 157 off the vector ALUs and leaves the time as it is (118 to 122 us).
+// lane about 15 more, 4 of which sum the lanes' parts, 5 form the step and 3 the gate.  12544 tokens of 2048 channels, 16 states, bf16: 114 to 124 us, of
+// which 62 are the states' own.  u B through 4x4x1 matrix instructions takes 12 cycles of 157 off the vector ALUs and leaves the time as it is (118 to 122 us).
 template <int DT, int L, int S, bool GATE>
 __global__ __launch_bounds__(kScanThreads, 4) void fc_selective_scan_kernel(const fc_scan_run r) {
     typedef scan_form<L, S> F;
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kScanThreads, 4) void fc_selective_scan_kernel(cons
 }
 
 // What each segment adds to no state, the sum of its steps and, with GRADS, what it adds to no gradient: the gradient of a state is the sum of what each later token
-// adds, decayed on its way, and the product of the decays from the segment's begin on is at hand.  Bound as the answers are: 87 us there, with GRADS 159 (4 x 3136
+// adds, decayed on its way, and the product of the decays from the segment's begin on is at hand.  Bound as the answers are: 87 to 93 us there, with GRADS 147 to 159 (4 x 3136
 // tokens).
 template <int DT, int L, int S, bool GRADS, bool GATE>
 __global__ __launch_bounds__(kScanThreads, GRADS ? 3 : 4) void fc_selective_scan_ends_kernel(const fc_scan_run r) {
@@ -488,7 +488,7 @@ __device__ __forceinline__ void sum_channels(float (&o)[O], float (&v)[S2]) {
 // Gradients of each segment, which is a tile: forwards through it from the state that enters, states in registers, then backwards.  Bound by the vector ALUs, busy
 // 77 % of the time with two wavefronts a SIMD (256 registers): 121 instructions for each token of a lane, 64 of them the states' own.  dB and dC are sums over
 // channels, of a wavefront's by lane swaps, of a workgroup's through LDS, of all by a launch of their own, so that their order is always the same.  4 x 3136 tokens of
-// 2048 channels, 16 states, bf16: 470 to 495 us.
+// 2048 channels, 16 states, bf16: 462 to 495 us.
 template <int DT, int L, int S, bool GATE>
 __global__ __launch_bounds__(kScanThreads, 2) void fc_selective_scan_gradient_kernel(const fc_scan_run r) {
     typedef scan_form<L, S> F;
