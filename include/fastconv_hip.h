@@ -578,7 +578,8 @@ int fc_linear_attention_backward(fc_context *ctx, const fc_linear_attention_plan
 /* RMS norm over rows of channels, after the addition of a residual:
  *   h = x + residual, rounded to the tensors' type;   rstd = 1/sqrt(mean of h^2 + eps);   y = h * rstd * gamma
  * Row i of x begins at i*x_row, and so for the residual, the sum h and y (in 8 bits: strides of bytes); dy as y, dsum as the sum, dx as x.  A row whose
- * squares overflow fp32 is normed like any other.  Limits: C <= 2^20, rows <= 2^40. */
+ * squares overflow fp32 is normed like any other.  One whose root is below 2^-128 (subnormal rows, no eps) is too, but its rstd is infinite and its gradients are
+ * no numbers.  Limits: C <= 2^20, rows <= 2^40. */
 typedef struct {
     long rows;
     int C;
