@@ -1065,7 +1065,7 @@ extern "C" int fc_group_norm(fc_context *ctx, const fc_group_norm_plan *plan, co
         (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_group_norm: unaligned pointer");
     const fc_group_norm_shape &s = plan->shape;
-    if (!fc_apart(s.N, s.y_image, s.C) || !fc_apart(s.P, s.y_pixel, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm: pixels of y overlap");
+    if (!fc_apart({{s.N, s.y_image}, {s.P, s.y_pixel}}, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm: pixels of y overlap");
     norm_params p = params_of(plan);
     p.x = x_dev; p.y = y_dev; p.gamma = gamma_dev; p.beta = beta_dev; p.mean = mean_dev; p.rstd = rstd_dev;
     p.part = (float2 *)ws_dev;
@@ -1094,7 +1094,7 @@ extern "C" int fc_group_norm_backward(fc_context *ctx, const fc_group_norm_plan 
         (((uint64_t)gamma_dev | (uint64_t)beta_dev | (uint64_t)mean_dev | (uint64_t)rstd_dev | (uint64_t)dgamma_dev | (uint64_t)dbeta_dev) & 3))
         return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: unaligned pointer");
     const fc_group_norm_shape &s = plan->shape;
-    if (!fc_apart(s.N, s.x_image, s.C) || !fc_apart(s.P, s.x_pixel, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: pixels of dx overlap");
+    if (!fc_apart({{s.N, s.x_image}, {s.P, s.x_pixel}}, s.C)) return fail(ctx, FC_ERR_INVALID, "fc_group_norm_backward: pixels of dx overlap");
     norm_params p = params_of(plan);
     p.x = x_dev; p.dy = dy_dev; p.y = dx_dev; p.gamma = gamma_dev; p.beta = beta_dev;
     p.mean = const_cast<float *>(mean_dev); p.rstd = const_cast<float *>(rstd_dev);      // only read

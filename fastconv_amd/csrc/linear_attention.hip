@@ -369,7 +369,7 @@ extern "C" int fc_linear_attention_make_plan(const fc_linear_attention_shape *s,
 }
 
 static bool apart(const fc_linear_attention_shape &s, long heads, long batch, long token, long head, int row) {
-    return fc_apart(s.B, batch, row) && fc_apart(s.T, token, row) && fc_apart(heads, head, row);
+    return fc_apart({{s.B, batch}, {s.T, token}, {heads, head}}, row);
 }
 
 static int check_plan(fc_context *ctx, const fc_linear_attention_plan *plan, const char *what) {

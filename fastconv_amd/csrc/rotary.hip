@@ -182,8 +182,8 @@ extern "C" int fc_rotary(fc_context *ctx, const fc_rotary_shape *s, const void *
     // a last workgroup may have one token of two: 2^25 - 2 tokens are the most
     if (s->D > 1024 || heads > 65536 || tokens < 0 || (tokens + group - 1) / group >= kMostThreads / kThreads)
         return fail(ctx, FC_ERR_UNSUPPORTED, "fc_rotary: more than 1024 channels, 65536 heads or 2^25 - 2 tokens");
-    if (!fc_apart(s->B, s->qo_batch, s->D) || !fc_apart(s->T, s->qo_token, s->D) || !fc_apart(s->Hq, s->qo_head, s->D) ||
-        (s->Hk > 0 && (!fc_apart(s->B, s->ko_batch, s->D) || !fc_apart(s->T, s->ko_token, s->D) || !fc_apart(s->Hk, s->ko_head, s->D))))
+    if (!fc_apart({{s->B, s->qo_batch}, {s->T, s->qo_token}, {s->Hq, s->qo_head}}, s->D) ||
+        (s->Hk > 0 && !fc_apart({{s->B, s->ko_batch}, {s->T, s->ko_token}, {s->Hk, s->ko_head}}, s->D)))
         return fail(ctx, FC_ERR_INVALID, "fc_rotary: heads of an output overlap");
     const int vec = fc_widest(s->dtype, bits | (uint64_t)s->D | (uint64_t)(s->interleaved ? 2 * R : R), addr);
     rotary_params p;
